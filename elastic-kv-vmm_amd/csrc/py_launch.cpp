@@ -3,8 +3,9 @@
 // (ekv_gather_rows), the plane gather / scatter / move (ekv_gather_kv,
 // ekv_scatter_kv, ekv_move_kv), the residency summary
 // (ekv_residency_summary), the batch-token swap-in (ekv_swap_in*), the
-// per-layer SGLang-convention swap-in (ekv_hisparse_swap_in) and the one-call
-// decode step (ekv_decode_step). Their GPU work can be a few microseconds at
+// per-layer SGLang-convention swap-in (ekv_hisparse_swap_in), the one-call
+// decode step (ekv_decode_step), the block tables (ekv_extend_block_tables) and
+// both attentions (ekv_shared_prefix_attention, ekv_topk_attention). Their GPU work can be a few microseconds at
 // small shapes, so
 // describing the tensors for the C ABI from Python (attribute reads and
 // struct packing, about 1 us per tensor) set the call rate. Here the
@@ -703,6 +704,168 @@ PyObject* swap_in(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     }
 }
 
+// The device of a KVPlanes object must be the tensors'. False with a Python
+// exception set.
+bool planes_on(PyObject* object, int device) {
+    PyObject* value = PyObject_GetAttrString(object, "device");
+    if (value == nullptr) {
+        return false;
+    }
+    const long long pool_device = PyLong_AsLongLong(value);
+    Py_DECREF(value);
+    if (pool_device == -1 && PyErr_Occurred()) {
+        return false;
+    }
+    if (pool_device != device) {
+        PyErr_SetString(PyExc_ValueError, "the tensors and the pool live on different devices");
+        return false;
+    }
+    return true;
+}
+
+bool read_scale(PyObject* object, double& value) {
+    value = PyFloat_AsDouble(object);
+    return !(value == -1.0 && PyErr_Occurred());
+}
+
+// extend_tables(entry, block_tables, rows, lengths, added, free_pages,
+//               free_head, page_size, slots, positions, starts, new_lengths,
+//               new_head, status) -> status of ekv_extend_block_tables
+PyObject* extend_tables(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+    if (argc != 14) {
+        PyErr_SetString(PyExc_TypeError, "extend_tables takes 14 arguments");
+        return nullptr;
+    }
+    int64_t entry = 0, page_size = 0;
+    if (!read_int(argv[0], "entry", entry) || !read_int(argv[7], "page_size", page_size)) {
+        return nullptr;
+    }
+    Arg args[] = {{argv[1], "block_tables"}, {argv[2], "rows"},          {argv[3], "lengths"},
+                  {argv[4], "added"},        {argv[5], "free_pages"},    {argv[6], "free_head"},
+                  {argv[8], "slots"},        {argv[9], "positions"},     {argv[10], "starts"},
+                  {argv[11], "new_lengths"}, {argv[12], "new_head"},     {argv[13], "status"}};
+    try {
+        const int device = describe_all(args);
+        if (device < 0) {
+            return nullptr;
+        }
+        CurrentDevice current(device);
+        void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+        int status = 0;
+        Py_BEGIN_ALLOW_THREADS
+        status = reinterpret_cast<decltype(&ekv_extend_block_tables)>(entry)(
+            args[0].pointer(), args[1].pointer(), args[2].pointer(), args[3].pointer(), args[4].pointer(),
+            args[5].pointer(), page_size, args[6].pointer(), args[7].pointer(), args[8].pointer(), args[9].pointer(),
+            args[10].pointer(), args[11].pointer(), stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(status);
+    } catch (const std::exception& error) {
+        PyErr_SetString(PyExc_RuntimeError, error.what());
+        return nullptr;
+    }
+}
+
+// prefix_attention(entry, query, planes, layer, kv_heads, page_size,
+//                  block_tables, rows, lengths, prefix_tables, prefix_lengths,
+//                  group_starts, query_starts, max_query, scale, output, lse,
+//                  workspace) -> status of ekv_shared_prefix_attention
+PyObject* prefix_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+    if (argc != 18) {
+        PyErr_SetString(PyExc_TypeError, "prefix_attention takes 18 arguments");
+        return nullptr;
+    }
+    ekv_prefix_attention_args call{};
+    int64_t entry = 0;
+    if (!read_int(argv[0], "entry", entry) || !read_int(argv[3], "layer", call.layer) ||
+        !read_int(argv[4], "kv_heads", call.kv_heads) || !read_int(argv[5], "page_size", call.page_size) ||
+        !read_int(argv[13], "max_query", call.max_query) || !read_scale(argv[14], call.scale)) {
+        return nullptr;
+    }
+    Arg args[] = {{argv[1], "query"},           {argv[6], "block_tables"},  {argv[7], "rows"},
+                  {argv[8], "lengths"},         {argv[9], "prefix_tables"}, {argv[10], "prefix_lengths"},
+                  {argv[11], "group_starts"},   {argv[12], "query_starts"}, {argv[15], "output"},
+                  {argv[16], "lse"},            {argv[17], "workspace", false}};
+    try {
+        const int device = describe_all(args);
+        if (device < 0) {
+            return nullptr;
+        }
+        ekv_planes planes{};
+        if (!read_planes(argv[2], planes) || !planes_on(argv[2], device)) {
+            return nullptr;
+        }
+        call.query = args[0].pointer();
+        call.planes = &planes;
+        call.block_tables = args[1].pointer();
+        call.rows = args[2].pointer();
+        call.lengths = args[3].pointer();
+        call.prefix_tables = args[4].pointer();
+        call.prefix_lengths = args[5].pointer();
+        call.group_starts = args[6].pointer();
+        call.query_starts = args[7].pointer();
+        call.output = args[8].pointer();
+        call.lse = args[9].pointer();
+        const at::Tensor* workspace = args[10].tensor;
+        void* data = workspace != nullptr ? workspace->data_ptr() : nullptr;
+        const uint64_t bytes =
+            workspace != nullptr ? static_cast<uint64_t>(workspace->numel()) * workspace->element_size() : 0;
+        CurrentDevice current(device);
+        void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+        int status = 0;
+        Py_BEGIN_ALLOW_THREADS
+        status = reinterpret_cast<decltype(&ekv_shared_prefix_attention)>(entry)(&call, data, bytes, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(status);
+    } catch (const std::exception& error) {
+        PyErr_SetString(PyExc_RuntimeError, error.what());
+        return nullptr;
+    }
+}
+
+// topk_attention(entry, query, planes, layer, kv_heads, slots, zero_below,
+//                scale, output, lse, workspace) -> status of ekv_topk_attention
+PyObject* topk_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+    if (argc != 11) {
+        PyErr_SetString(PyExc_TypeError, "topk_attention takes 11 arguments");
+        return nullptr;
+    }
+    int64_t entry = 0, layer = 0, kv_heads = 0, zero_below = 0;
+    double scale = 0;
+    if (!read_int(argv[0], "entry", entry) || !read_int(argv[3], "layer", layer) ||
+        !read_int(argv[4], "kv_heads", kv_heads) || !read_int(argv[6], "zero_below", zero_below) ||
+        !read_scale(argv[7], scale)) {
+        return nullptr;
+    }
+    Arg args[] = {{argv[1], "query"}, {argv[5], "slots"}, {argv[8], "output"}, {argv[9], "lse"},
+                  {argv[10], "workspace", false}};
+    try {
+        const int device = describe_all(args);
+        if (device < 0) {
+            return nullptr;
+        }
+        ekv_planes planes{};
+        if (!read_planes(argv[2], planes) || !planes_on(argv[2], device)) {
+            return nullptr;
+        }
+        const at::Tensor* workspace = args[4].tensor;
+        void* data = workspace != nullptr ? workspace->data_ptr() : nullptr;
+        const uint64_t bytes =
+            workspace != nullptr ? static_cast<uint64_t>(workspace->numel()) * workspace->element_size() : 0;
+        CurrentDevice current(device);
+        void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+        int status = 0;
+        Py_BEGIN_ALLOW_THREADS
+        status = reinterpret_cast<decltype(&ekv_topk_attention)>(entry)(
+            args[0].pointer(), &planes, layer, kv_heads, args[1].pointer(), zero_below, scale, args[2].pointer(),
+            args[3].pointer(), data, bytes, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(status);
+    } catch (const std::exception& error) {
+        PyErr_SetString(PyExc_RuntimeError, error.what());
+        return nullptr;
+    }
+}
+
 PyObject* abi_version(PyObject*, PyObject*) { return PyLong_FromLong(EKV_ABI_VERSION); }
 
 PyObject* source_hash(PyObject*, PyObject*) { return PyUnicode_FromString(EKV_STRINGIFY(EKV_SOURCE_HASH)); }
@@ -724,6 +887,12 @@ PyMethodDef methods[] = {
      "Describe a table, its residency summary and group counts and call ekv_residency_summary."},
     {"swap_in", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(swap_in)), METH_FASTCALL,
      "Describe the batch-token LRU swap-in's tensors and call ekv_swap_in / ekv_swap_in_counted."},
+    {"extend_tables", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(extend_tables)), METH_FASTCALL,
+     "Describe a step's block tables, lengths and free pages and call ekv_extend_block_tables."},
+    {"prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(prefix_attention)),
+     METH_FASTCALL, "Describe the queries, tables and planes and call ekv_shared_prefix_attention."},
+    {"topk_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(topk_attention)), METH_FASTCALL,
+     "Describe the queries, slots and planes and call ekv_topk_attention."},
     {"abi_version", abi_version, METH_NOARGS, "EKV_ABI_VERSION this module was built against."},
     {"source_hash", source_hash, METH_NOARGS, "Fingerprint of the native sources this module was built from."},
     {nullptr, nullptr, 0, nullptr}};

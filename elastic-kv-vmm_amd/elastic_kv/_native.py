@@ -105,6 +105,12 @@ _SIGNATURES = {
     "ekv_decode_step_workspace_bytes": ([ct.c_int64, ct.c_int64, ct.c_int64], ct.c_uint64),
     "ekv_decode_step": ([ct.c_void_p, ct.c_void_p, ct.c_uint64, ct.c_void_p], ct.c_int),
     "ekv_decode_step_static": ([ct.c_void_p, ct.c_void_p], ct.c_int),
+    "ekv_extend_block_tables": ([_P_TENSOR] * 6 + [ct.c_int64] + [_P_TENSOR] * 6 + [ct.c_void_p], ct.c_int),
+    "ekv_shared_prefix_workspace_bytes": ([ct.c_int64] * 7, ct.c_uint64),
+    "ekv_shared_prefix_attention": ([ct.c_void_p, ct.c_void_p, ct.c_uint64, ct.c_void_p], ct.c_int),
+    "ekv_topk_workspace_bytes": ([ct.c_int64] * 5, ct.c_uint64),
+    "ekv_topk_attention": ([_P_TENSOR, ct.POINTER(EkvPlanes), ct.c_int64, ct.c_int64, _P_TENSOR, ct.c_int64,
+                            ct.c_double, _P_TENSOR, _P_TENSOR, ct.c_void_p, ct.c_uint64, ct.c_void_p], ct.c_int),
 }
 KERNEL_SYMBOLS = tuple(_SIGNATURES)
 
@@ -155,7 +161,8 @@ _LAUNCH = {}   # ELASTIC_VMM_LIBRARY key -> (launch helper module, {entry name: 
 _LAUNCH_ENTRIES = ("ekv_resolve_resident", "ekv_resolve_resident_bits", "ekv_resolve_resident_local",
                    "ekv_residency_summary", "ekv_gather_rows", "ekv_gather_kv", "ekv_scatter_kv", "ekv_move_kv",
                    "ekv_swap_in", "ekv_swap_in_counted", "ekv_hisparse_swap_in", "ekv_host_device_pointer",
-                   "ekv_decode_step")
+                   "ekv_decode_step", "ekv_extend_block_tables", "ekv_shared_prefix_attention",
+                   "ekv_topk_attention")
 
 
 _DEFAULT = object()   # _LAUNCH key of the helper bound on the first call without a library argument

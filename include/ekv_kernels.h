@@ -448,6 +448,111 @@ int ekv_decode_step(const ekv_step_args* args, void* workspace, uint64_t workspa
  */
 int ekv_decode_step_static(const ekv_step_args* args, void* stream);
 
+/* Bits that ekv_extend_block_tables ORs into its status word. */
+#define EKV_TABLES_BAD_ROW 1    /* a request outside the table, a negative length or count, or a length past the table */
+#define EKV_TABLES_ROW_FULL 2   /* a row's new tokens pass its table's columns: the ones that do not fit are left out */
+#define EKV_TABLES_NO_PAGES 4   /* the free list ran out: entry 0 (the sink) was written, those tokens' slots are -1 */
+#define EKV_TABLES_MAP_FULL 8   /* more new tokens than the slot map holds: the ones past it are left out */
+#define EKV_TABLES_SLOT_RANGE 16 /* a slot does not fit the int32 slot map: -1 */
+
+/*
+ * Block tables and slot maps of a step, from request lengths: every batch row
+ * b of request r = rows[b] (NULL: r = b) holds lengths[b] tokens in pages of
+ * page_size and gets added[b] more. With have = ceil(lengths[b] / page_size),
+ * need = ceil((lengths[b] + added[b]) / page_size), base = the pages and
+ * start = the tokens that earlier batch rows take:
+ *   block_tables[r, j] = free_pages[free_head[0] + base + j - have], have <= j < need
+ *   starts[b] = start, starts[B] = their sum
+ *   positions[start + i] = p = lengths[b] + i, i < added[b]        (NULL: not written)
+ *   slots[start + i] = block_tables[r, p / page_size] * page_size + p % page_size
+ *   new_lengths[b] = lengths[b] + added[b]
+ *   new_head[0] = free_head[0] + the pages taken
+ * slots and positions past the last token are -1, and a token whose page id is
+ * below 1 (0 is the sink) gets slot -1. Other table entries are left as they are.
+ *   block_tables [R, M]; rows, lengths, added, new_lengths [B]; starts [B + 1];
+ *   free_pages [F]; free_head, new_head [1]; slots, positions [N]: int32 or
+ *   int64 each; status NULL or [1] int32. M * page_size < 2^30.
+ * What does not fit is left out and sets EKV_TABLES_* bits: a row that names no
+ * request, or whose length is negative or past its columns, gets no tokens.
+ * Batch rows must name distinct requests; new_lengths and new_head must not
+ * share memory with lengths and free_head. One launch.
+ * No reference counterpart: the reference extends its tables on the host
+ * (adaptive_sparse/request_residency.py:739-790).
+ */
+int ekv_extend_block_tables(const ekv_tensor* block_tables, const ekv_tensor* rows, const ekv_tensor* lengths,
+                            const ekv_tensor* added, const ekv_tensor* free_pages, const ekv_tensor* free_head,
+                            int64_t page_size, const ekv_tensor* slots, const ekv_tensor* positions,
+                            const ekv_tensor* starts, const ekv_tensor* new_lengths, const ekv_tensor* new_head,
+                            const ekv_tensor* status, void* stream);
+
+/* The arguments of ekv_shared_prefix_attention. */
+typedef struct ekv_prefix_attention_args {
+    const ekv_tensor* query;          /* [N, Hq, D] bfloat16 or float16 */
+    const ekv_planes* planes;         /* the pool (kv 2); a plane row is a token or a whole page */
+    int64_t layer;
+    int64_t kv_heads;                 /* Hkv, a divisor of Hq: query head h reads KV head h / (Hq / Hkv) */
+    int64_t page_size;
+    const ekv_tensor* block_tables;   /* [R, M] own pages of each request */
+    const ekv_tensor* rows;           /* NULL (r = b) or [B] request of each batch row */
+    const ekv_tensor* lengths;        /* [B] own tokens of each batch row, its query tokens among them */
+    const ekv_tensor* prefix_tables;  /* NULL (no prefix) or [G, P] pages of each group's prefix */
+    const ekv_tensor* prefix_lengths; /* [G] */
+    const ekv_tensor* group_starts;   /* NULL (one group of all rows) or [G + 1] first batch row of each group */
+    const ekv_tensor* query_starts;   /* NULL (one query token a row) or [B + 1] first query token of each row */
+    int64_t max_query;                /* the most query tokens of a row, or about: picks kernels, never results */
+    double scale;                     /* of the scores, e.g. D^-0.5 */
+    const ekv_tensor* output;         /* [N, Hq, D], the query's type */
+    const ekv_tensor* lse;            /* NULL or [N, Hq] float32 */
+} ekv_prefix_attention_args;
+
+/*
+ * Workspace bytes of ekv_shared_prefix_attention over N query tokens of B
+ * batch rows in G groups. UINT64_MAX on error.
+ */
+uint64_t ekv_shared_prefix_workspace_bytes(int64_t tokens, int64_t batch, int64_t groups, int64_t query_heads,
+                                           int64_t kv_heads, int64_t head_dim, int64_t max_query);
+
+/*
+ * Attention of a batch whose groups of consecutive batch rows share a prefix:
+ * query token i of the n of batch row b, in group g, sees the prefix's tokens
+ * 0 .. prefix_lengths[g] - 1 and its request's own tokens
+ * 0 .. lengths[b] - n + i. Over the tokens it sees, per query head h:
+ *   output = sum_j softmax_j(scale q . k_j) v_j,  lse = log sum_j exp(scale q . k_j)
+ * The prefix's K and V are read once for all rows of a group. Token t of a
+ * table row lies in page table[t / page_size]; page ids below 1 or past the
+ * pool, and tokens past the table's columns, are not seen, and their memory is
+ * not read. A query token that sees nothing, or that belongs to no batch row,
+ * gets zeros and lse -inf. Rows outside every group have no prefix, rows that
+ * name no request no own tokens; starts are taken as non-decreasing.
+ * D is a multiple of 8 up to 256; addresses and strides of planes, query and
+ * output are multiples of 16 bytes. workspace: 256-byte aligned device memory
+ * of ekv_shared_prefix_workspace_bytes, its contents of no account; calls that
+ * overlap need one each. Records no memset, so it can be captured in a HIP graph.
+ * Replaces: what the reference routes to its engine's attention after
+ * resolving a shared prefix's blocks (adaptive_sparse/shared_prefix.py:122-204).
+ */
+int ekv_shared_prefix_attention(const ekv_prefix_attention_args* args, void* workspace, uint64_t workspace_bytes,
+                                void* stream);
+
+/* Workspace bytes of ekv_topk_attention. UINT64_MAX on error. */
+uint64_t ekv_topk_workspace_bytes(int64_t tokens, int64_t lanes, int64_t query_heads, int64_t kv_heads,
+                                  int64_t head_dim);
+
+/*
+ * Decode attention over the slots that a lookup returned, one layer: query
+ * token t sees the rows slots[t, k] with zero_below <= slot < planes->rows
+ * (slot 0 = not resident and -1 = padding are not seen and not read). A slot
+ * listed twice counts twice. Otherwise as ekv_shared_prefix_attention: query and
+ * output [N, Hq, D], lse NULL or [N, Hq] float32, slots [N, K] int32/int64 of
+ * any strides, plane rows of one token.
+ * Replaces: ekv_gather_kv and the attention that would read its output (the
+ * reference hands the slots to its engine's sparse attention,
+ * adaptive_sparse/logical_shadow.py:243-256).
+ */
+int ekv_topk_attention(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64_t kv_heads,
+                       const ekv_tensor* slots, int64_t zero_below, double scale, const ekv_tensor* output,
+                       const ekv_tensor* lse, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* Modes of ekv_stream_probe. */
 #define EKV_PROBE_READ 0   /* read src (fold, no stores)       */
 #define EKV_PROBE_WRITE 1  /* write zeros to dst                */
