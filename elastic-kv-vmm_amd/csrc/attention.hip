@@ -6,182 +6,140 @@
 // over the keys that a query token sees. With the running largest score m, the sum l = sum exp(s_j - m) and the
 // weighted values a = sum exp(s_j - m) v_j, two parts of the keys join as m = max(m1, m2),
 // l = l1 e^(m1 - m) + l2 e^(m2 - m), a likewise, and o = a / l; statistics and sums are held in 32 bits.
-#include "../../include/ekv_kernels.h"
-#include "ekv_common.h"
-#include "ekv_tensor_util.h"
-#include "ekv_vec.h"
-
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
+//
+// The kernels that read K and V are in attention_narrow.hip; here are the checks, the choice of a launch, and the merge
+// of the parts that a launch's workgroups leave of one item (ekv_attention.h).
+#include "ekv_attention.h"
+#include "ekv_mfma.h"
 
 #include <algorithm>
-#include <cmath>
 
 namespace ekv {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-// Token offset o of page p of one KV head: k + p * page_stride + o * token_stride (bytes), V likewise.
-struct Cache {
-    const char* k;
-    const char* v;
-    int64_t page_stride, token_stride, head_stride;
-    int64_t pages;      // page ids 1 .. pages - 1 (or zero_below ..) name pages
-    int64_t page_size;
-    int64_t zero_below;
+// The workgroups that hold a token's parts of one phase, and where.
+struct Parts {
+    const float* base;          // first part's row of values
+    const float* stats;         // first part's largest score of the row; its sum is row_tile later
+    int64_t step;               // to the next part
+    int32_t row_tile;
+    int32_t count;
 };
 
-struct Args {
-    const char* query;
-    int64_t q_token, q_head;      // bytes
-    char* out;
-    int64_t o_token, o_head;
-    float* lse;
-    int64_t l_token, l_head;      // elements
-    Cache cache;
-    const void* tables;           // [R, M] own pages of each request (or the slots of each query token)
-    int64_t table_row, table_col;
-    int32_t table64;
-    int64_t requests, columns;
-    IndexRef rows, lengths, query_starts;
-    const void* prefix_tables;    // [G, P]
-    int64_t prefix_row, prefix_col;
-    int32_t prefix64;
-    int64_t prefix_columns;
-    IndexRef prefix_lengths, group_starts;
-    int64_t tokens, batch, groups, heads, kv_heads, dim;
-    float scale;                  // times log2 e
-};
+// The parts of row `row` (of one KV head) of sequence s: none when the sequence was nobody's work.
+__device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p, int32_t s, int32_t head, int32_t row) {
+    int64_t begin, total;
+    int32_t item, tiles, row_tiles;
+    if (p.mode == kSlots) {
+        const Sequence any = sequence_of(a, kSlots, 0);
+        tiles = tiles_of(any, p), row_tiles = row_tiles_of(a, any, p);
+        item = s * a.kv_heads * row_tiles;
+        begin = static_cast<int64_t>(item) * tiles;
+        total = static_cast<int64_t>(p.sequences) * a.kv_heads * row_tiles * tiles;
+    } else {
+        begin = p.tile_starts[s];
+        item = p.item_starts[s];
+        total = p.tile_starts[p.sequences];
+        const int32_t items = p.item_starts[s + 1] - item;
+        if (items == 0) {
+            return Parts{};
+        }
+        tiles = static_cast<int32_t>((p.tile_starts[s + 1] - begin) / items);
+        row_tiles = items / a.kv_heads;
+    }
+    const int32_t local = head * row_tiles + row / p.row_tile;
+    begin += static_cast<int64_t>(local) * tiles;
+    const int32_t active = active_workgroups(p, total);
+    const int32_t first = line_owner(total, begin, active), last = line_owner(total, begin + tiles - 1, active);
+    Parts r;
+    r.row_tile = p.row_tile;
+    r.step = static_cast<int64_t>(p.row_tile) * (p.dim_pad + 2);
+    const int64_t slot = first + item + local;
+    const float* part = p.parts + slot * r.step;
+    r.base = part + static_cast<int64_t>(row % p.row_tile) * p.dim_pad;
+    r.stats = part + static_cast<int64_t>(p.row_tile) * p.dim_pad + row % p.row_tile;
+    r.count = last - first + 1;
+    if (p.direct != 0 && r.count == 1) {
+        r.count = -1;           // written to the output by the one that had it whole
+    }
+    if (slot + r.count > p.slots) {
+        r.count = 0;            // only if the starts were not in order
+    }
+    return r;
+}
 
-__device__ __forceinline__ float to_float(__hip_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ void from_float(__hip_bfloat16& y, float x) { y = __float2bfloat16(x); }
-__device__ __forceinline__ void from_float(__half& y, float x) { y = __float2half(x); }
-
-// One wave per (query token, query head); each key is read by kLanes lanes of 8 elements, 64 / kLanes keys at a time.
-template <typename T, int kLanes>
-__global__ __launch_bounds__(kThreads) void attend_kernel(const Args a) {
-    constexpr int kKeys = 64 / kLanes;
-    const int lane = threadIdx.x & 63;
-    const int64_t item = int64_t{blockIdx.x} * kWaves + (threadIdx.x >> 6);
-    if (item >= a.tokens * a.heads) {
-        return;
-    }
-    const int64_t token = item / a.heads, head = item % a.heads;
-    const int64_t kv_head = head / (a.heads / a.kv_heads);
-    const int part = lane % kLanes, sub = lane / kLanes;
-    const bool live = part * 8 < a.dim;
-    float q[8], acc[8] = {}, m = -INFINITY, l = 0;
-    const T* q_at = reinterpret_cast<const T*>(a.query + token * a.q_token + head * a.q_head) + part * 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        q[e] = live ? to_float(q_at[e]) : 0.0f;
-    }
-    // The batch row that the token belongs to, and its place there.
-    int64_t b = token, at = 0, count = 1;
-    if (a.query_starts.data != nullptr) {
-        b = -1;
-        for (int64_t i = 0; i < a.batch; ++i) {
-            const int64_t begin = a.query_starts[i], end = a.query_starts[i + 1];
-            if (begin <= token && token < end) {
-                b = i, at = token - begin, count = end - begin;
-                break;
+// One workgroup per (query token, KV head): a thread joins four elements of one row over all parts, own first, then the
+// prefix's, each in the order of the workgroups.
+template <typename T>
+__global__ __launch_bounds__(kAttentionThreads) void merge_kernel(const AttentionArgs a, const Phase own,
+                                                                  const Phase prefix) {
+    const int32_t token = blockIdx.x, head = blockIdx.y;
+    int32_t b = token;
+    if (own.mode != kSlots && a.query_starts.data != nullptr) {
+        int32_t low = 0, high = a.batch;
+        while (high - low > 1) {
+            const int32_t mid = (low + high) >> 1;
+            if (first_token(a, mid) <= token) {
+                low = mid;
+            } else {
+                high = mid;
             }
         }
-    } else if (token >= a.batch) {
-        b = -1;
+        b = a.batch > 0 && first_token(a, low) <= token && token < first_token(a, low + 1) ? low : -1;
     }
-    int64_t group = -1;
-    for (int64_t g = 0; g < a.groups && b >= 0; ++g) {
-        const int64_t begin = a.group_starts.data != nullptr ? a.group_starts[g] : 0;
-        const int64_t end = a.group_starts.data != nullptr ? a.group_starts[g + 1] : a.batch;
-        if (begin <= b && b < end) {
-            group = g;
-            break;
+    const int32_t group = b >= 0 && prefix.sequences > 0 ? group_of(a, b) : -1;
+    const int32_t own_first = b >= 0 && own.mode != kSlots ? first_token(a, b) : token;
+    const int32_t prefix_first = group >= 0 ? first_token(a, first_row(a, group)) : 0;
+    const int32_t quads = (a.dim + 3) >> 2;
+    for (int32_t unit = threadIdx.x; unit < a.share * quads; unit += kAttentionThreads) {
+        const int32_t sub = unit / quads, element = (unit % quads) * 4;
+        Parts part[2] = {};
+        if (b >= 0) {
+            part[0] = parts_of(a, own, b, head, (token - own_first) * a.share + sub);
         }
-    }
-    for (int side = 0; side < 2; ++side) {
-        int64_t keys = 0, page_base = 0, page_col = 0;
-        const void* table = nullptr;
-        int32_t is64 = 0;
-        if (side == 0 && group >= 0) {
-            keys = min(a.prefix_lengths[group], a.prefix_columns * a.cache.page_size);
-            table = a.prefix_tables, is64 = a.prefix64;
-            page_base = group * a.prefix_row, page_col = a.prefix_col;
-        } else if (side == 1 && b >= 0) {
-            const int64_t row = a.rows.data != nullptr ? a.rows[b] : b;
-            if (row >= 0 && row < a.requests) {
-                const int64_t length = a.lengths.data != nullptr ? a.lengths[b] : a.columns;
-                keys = min(a.lengths.data != nullptr ? length - count + at + 1 : length,
-                           a.columns * a.cache.page_size);
-                table = a.tables, is64 = a.table64;
-                page_base = row * a.table_row, page_col = a.table_col;
+        if (group >= 0) {
+            part[1] = parts_of(a, prefix, group, head, (token - prefix_first) * a.share + sub);
+        }
+        if (part[0].count < 0) {
+            continue;
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+#pragma unroll 4
+            for (int32_t i = 0; i < part[side].count; ++i) {
+                most = fmaxf(most, part[side].stats[i * part[side].step]);
             }
         }
-        for (int64_t j0 = 0; j0 < keys; j0 += kKeys) {
-            const int64_t j = j0 + sub;
-            int64_t page = -1;
-            if (j < keys) {
-                const int64_t entry = page_base + j / a.cache.page_size * page_col;
-                page = is64 ? static_cast<const int64_t*>(table)[entry] : static_cast<const int32_t*>(table)[entry];
-            }
-            const bool seen = page >= a.cache.zero_below && page < a.cache.pages;
-            float k[8], v[8], s = 0;
-            const int64_t offset = page * a.cache.page_stride + j % a.cache.page_size * a.cache.token_stride +
-                                   kv_head * a.cache.head_stride + part * 16;
+        const float safe = most == -INFINITY ? 0.0f : most;
+        float total = 0;
+        f32x4 value = {0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                k[e] = seen && live ? to_float(reinterpret_cast<const T*>(a.cache.k + offset)[e]) : 0.0f;
-                v[e] = seen && live ? to_float(reinterpret_cast<const T*>(a.cache.v + offset)[e]) : 0.0f;
-                s += q[e] * k[e];
-            }
-#pragma unroll
-            for (int d = 1; d < kLanes; d <<= 1) {
-                s += __shfl_xor(s, d);
-            }
-            s = seen ? s * a.scale : -INFINITY;
-            const float top = fmaxf(m, s);
-            const float safe = top == -INFINITY ? 0.0f : top;
-            const float keep = exp2f(m - safe), p = exp2f(s - safe);
-            m = top;
-            l = l * keep + p;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                acc[e] = acc[e] * keep + p * v[e];
+        for (int side = 0; side < 2; ++side) {
+#pragma unroll 4
+            for (int32_t i = 0; i < part[side].count; ++i) {
+                const float* stats = part[side].stats + i * part[side].step;
+                const float keep = exp2f(stats[0] - safe);
+                total += stats[part[side].row_tile] * keep;
+                value += *reinterpret_cast<const f32x4*>(part[side].base + i * part[side].step + element) * keep;
             }
         }
-    }
-#pragma unroll
-    for (int d = kLanes; d < 64; d <<= 1) {
-        const float other = __shfl_xor(m, d);
-        const float top = fmaxf(m, other);
-        const float safe = top == -INFINITY ? 0.0f : top;
-        const float mine = exp2f(m - safe), theirs = exp2f(other - safe);
-        l = l * mine + __shfl_xor(l, d) * theirs;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            acc[e] = acc[e] * mine + __shfl_xor(acc[e], d) * theirs;
+        const int32_t row_head = head * a.share + sub;
+        const float inverse = total == 0 ? 0.0f : 1.0f / total;
+        *reinterpret_cast<words2*>(a.out + token * a.o_token + row_head * a.o_head + element * 2) =
+            words2{T::pack(value[0] * inverse, value[1] * inverse), T::pack(value[2] * inverse, value[3] * inverse)};
+        if (element == 0 && a.lse != nullptr) {
+            a.lse[token * a.l_token + row_head * a.l_head] =
+                total == 0 ? -INFINITY : (most - T::kShift + log2f(total)) * kLn2;
         }
-        m = top;
-    }
-    if (sub == 0 && live) {
-        T* to = reinterpret_cast<T*>(a.out + token * a.o_token + head * a.o_head) + part * 8;
-        const float inverse = l > 0 ? 1.0f / l : (l == 0 ? 0.0f : l);   // a NaN sum stays one
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            from_float(to[e], acc[e] * inverse);
-        }
-    }
-    if (lane == 0 && a.lse != nullptr) {
-        a.lse[token * a.l_token + head * a.l_head] = l == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
     }
 }
 
 // ---------------------------------------------------------------- host
+
+constexpr int64_t kMostHeads = 65535, kMostTokens = 1 << 23, kMostRows = int64_t{1} << 30,
+                  kMostBatch = 1 << 20;
+constexpr int32_t kComputeUnits = 256;
 
 void need_aligned(int64_t value, const char* what) {
     if (value % 16 != 0) {
@@ -218,7 +176,7 @@ const ekv_tensor& need_list(const ekv_tensor* p, int64_t extent, const char* nam
 }
 
 // Query, output, statistics and cache: what both entry points share.
-Args common_args(const ekv_tensor* query_p, const ekv_planes* planes, int64_t layer, int64_t kv_heads,
+AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, int64_t layer, int64_t kv_heads,
                  int64_t page_size, double scale, const ekv_tensor* out_p, const ekv_tensor* lse_p) {
     const ekv_tensor& query = need_rows(query_p, "query");
     const ekv_tensor& out = need_rows(out_p, "output");
@@ -228,18 +186,21 @@ Args common_args(const ekv_tensor* query_p, const ekv_planes* planes, int64_t la
     if (out.dtype != query.dtype) {
         throw std::invalid_argument("output must have the query's type");
     }
-    Args a{};
-    a.tokens = query.shape[0], a.heads = query.shape[1], a.dim = query.shape[2];
-    a.kv_heads = kv_heads;
-    if (kv_heads < 1 || a.heads < 1 || a.heads % kv_heads != 0) {
+    AttentionArgs a{};
+    const int64_t tokens = query.shape[0], heads = query.shape[1], dim = query.shape[2];
+    if (kv_heads < 1 || heads < 1 || heads % kv_heads != 0) {
         throw std::invalid_argument("kv_heads must divide the query's heads");
     }
-    if (a.dim < 8 || a.dim > 256 || a.dim % 8 != 0) {
+    if (dim < 8 || dim > 256 || dim % 8 != 0) {
         throw std::invalid_argument("the head size must be a multiple of 8 from 8 to 256");
     }
-    if (a.tokens > (int64_t{1} << 30) / a.heads) {
-        throw std::invalid_argument("more than 2^30 query rows");
+    if (heads > kMostHeads || tokens > kMostTokens || tokens > kMostRows / heads) {
+        throw std::invalid_argument("more than 65535 heads, 2^23 query tokens or 2^30 query rows");
     }
+    a.tokens = static_cast<int32_t>(tokens), a.heads = static_cast<int32_t>(heads), a.dim = static_cast<int32_t>(dim);
+    a.kv_heads = static_cast<int32_t>(kv_heads);
+    a.share = a.heads / a.kv_heads;
+    a.share_div = FastDiv(static_cast<uint32_t>(a.share));
     if (!std::isfinite(scale)) {
         throw std::invalid_argument("scale must be finite");
     }
@@ -274,10 +235,10 @@ Args common_args(const ekv_tensor* query_p, const ekv_planes* planes, int64_t la
         throw std::invalid_argument("null plane base");
     }
     c.head_stride = a.dim * 2;
-    c.page_size = page_size;
+    c.page = FastDiv(static_cast<uint32_t>(page_size));
     c.zero_below = 1;
     c.k = static_cast<const char*>(planes->base) + layer * planes->layer_stride;
-    c.v = c.k + planes->kv_stride;
+    c.kv_stride = planes->kv_stride;
     need_aligned(reinterpret_cast<int64_t>(c.k), "plane address");
     need_aligned(planes->kv_stride, "kv stride");
     need_aligned(planes->row_stride, "plane row stride");
@@ -297,63 +258,136 @@ Args common_args(const ekv_tensor* query_p, const ekv_planes* planes, int64_t la
         a.lse = static_cast<float*>(lse.data);
         a.l_token = lse.stride[0], a.l_head = lse.stride[1];
     }
-    a.scale = static_cast<float>(scale * 1.4426950408889634);
+    a.scale = static_cast<float>(scale * 1.4426950408889634);   // log2 e: the kernels' exponentials have base two
     return a;
 }
 
-template <typename T>
-void launch_attend(const Args& a, hipStream_t stream) {
-    const int64_t groups = (a.tokens * a.heads + kWaves - 1) / kWaves;
-    const dim3 grid(static_cast<uint32_t>(groups)), block(kThreads);
-    if (a.dim <= 64) {
-        attend_kernel<T, 8><<<grid, block, 0, stream>>>(a);
-    } else if (a.dim <= 128) {
-        attend_kernel<T, 16><<<grid, block, 0, stream>>>(a);
-    } else {
-        attend_kernel<T, 32><<<grid, block, 0, stream>>>(a);
+uint64_t aligned(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// The launches of a call and the workspace they use.
+struct Plan {
+    int tiles16 = 0, prefix_tiles16 = 0;   // 16-row tiles of each launch (0: no such launch)
+    Phase own{}, prefix{};
+    uint64_t bytes = 0;
+};
+
+int32_t padded_dim(int64_t dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : (dim <= 128 ? 128 : 256)); }
+
+// 16-row tiles that hold `rows` rows, as far as the kernel's registers go.
+int tiles_for(int64_t rows, int32_t dim_pad) {
+    return rows <= 16 ? 1 : (rows <= 32 || dim_pad > 128 ? 2 : 4);
+}
+
+void take(Plan& plan, Phase& p, int64_t rows) {
+    // Row tiles of all sequences: every sequence's last may be part-filled.
+    p.slots = p.workgroups + rows;
+    p.parts = reinterpret_cast<float*>(plan.bytes);
+    plan.bytes += aligned(static_cast<uint64_t>(p.slots) * p.row_tile * (p.dim_pad + 2) * sizeof(float));
+    if (p.mode != kSlots) {
+        p.tile_starts = reinterpret_cast<int64_t*>(plan.bytes);
+        plan.bytes += aligned((static_cast<uint64_t>(p.sequences) + 1) * sizeof(int64_t));
+        p.item_starts = reinterpret_cast<int32_t*>(plan.bytes);
+        plan.bytes += aligned((static_cast<uint64_t>(p.sequences) + 1) * sizeof(int32_t));
     }
 }
 
-int launch(const Args& a, int32_t dtype, void* stream) {
+void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, int64_t tokens, int64_t share,
+         int64_t kv_heads, int32_t dim_pad, bool direct) {
+    p.mode = mode;
+    p.sequences = static_cast<int32_t>(sequences);
+    p.row_tile = 16 * tiles16;
+    p.key_tile = 32;
+    p.dim_pad = dim_pad;
+    p.workgroups = kComputeUnits * (tiles16 == 1 && dim_pad <= 128 ? 2 : 1);
+    p.direct = direct;
+    take(plan, p, kv_heads * (tokens * share / p.row_tile + sequences));
+}
+
+void need_sizes(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim) {
+    if (tokens < 0 || sequences < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dim < 8 || dim > 256) {
+        throw std::invalid_argument("attention sizes must be positive, kv_heads a divisor of the heads and the head "
+                                    "size from 8 to 256");
+    }
+    if (heads > kMostHeads || tokens > kMostTokens || tokens > kMostRows / heads || sequences > kMostBatch) {
+        throw std::invalid_argument("more than 65535 heads, 2^23 query tokens, 2^30 query rows or 2^20 batch rows");
+    }
+}
+
+Plan prefix_plan(int64_t tokens, int64_t batch, int64_t groups, int64_t heads, int64_t kv_heads, int64_t dim,
+                 int64_t max_query) {
+    need_sizes(tokens, std::max(batch, groups), heads, kv_heads, dim);
+    if (groups < 0 || max_query < 1) {
+        throw std::invalid_argument("max_query must be positive");
+    }
+    Plan plan;
+    const int64_t share = heads / kv_heads, row_rows = std::min(max_query, tokens) * share;
+    const int32_t dim_pad = padded_dim(dim);
+    // Rows of a group fill tiles that a batch row's alone leave part-empty: then the prefix is a launch of its own.
+    const int64_t group_rows = groups > 0 ? tokens * share / groups : 0;
+    if (groups > 0 && group_rows > row_rows && row_rows < 64) {
+        plan.prefix_tiles16 = tiles_for(group_rows, dim_pad);
+        cut(plan, plan.prefix, kPrefixes, groups, plan.prefix_tiles16, tokens, share, kv_heads, dim_pad, false);
+        plan.tiles16 = tiles_for(row_rows, dim_pad);
+        cut(plan, plan.own, kOwn, batch, plan.tiles16, tokens, share, kv_heads, dim_pad, false);
+    } else {
+        plan.tiles16 = tiles_for(row_rows, dim_pad);
+        cut(plan, plan.own, groups > 0 ? kWhole : kOwn, batch, plan.tiles16, tokens, share, kv_heads, dim_pad, true);
+    }
+    return plan;
+}
+
+Plan topk_plan(int64_t tokens, int64_t lanes, int64_t heads, int64_t kv_heads, int64_t dim) {
+    if (lanes < 0) {
+        throw std::invalid_argument("the number of lanes is negative");
+    }
+    need_sizes(tokens, 0, heads, kv_heads, dim);
+    Plan plan;
+    plan.tiles16 = tiles_for(heads / kv_heads, padded_dim(dim));
+    cut(plan, plan.own, kSlots, tokens, plan.tiles16, tokens, heads / kv_heads, kv_heads, padded_dim(dim), true);
+    return plan;
+}
+
+void place(Phase& p, void* workspace) {
+    const auto at = [&](auto*& pointer) {
+        pointer = reinterpret_cast<std::remove_reference_t<decltype(pointer)>>(static_cast<char*>(workspace) +
+                                                                              reinterpret_cast<uintptr_t>(pointer));
+    };
+    at(p.parts);
+    if (p.mode != kSlots) {
+        at(p.tile_starts);
+        at(p.item_starts);
+    }
+}
+
+int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, uint64_t bytes, void* stream) {
+    if (bytes < plan.bytes) {
+        throw std::invalid_argument("the attention needs " + std::to_string(plan.bytes) + " workspace bytes, got " +
+                                    std::to_string(bytes));
+    }
+    if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) {
+        throw std::invalid_argument("the workspace must be a 256-byte aligned device buffer");
+    }
     if (a.tokens == 0) {
         return 0;
     }
+    place(plan.own, workspace);
+    if (plan.prefix_tiles16 != 0) {
+        place(plan.prefix, workspace);
+        launch_narrow(a, plan.prefix, dtype, plan.prefix_tiles16, stream);
+    }
+    launch_narrow(a, plan.own, dtype, plan.tiles16, stream);
+    const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.kv_heads));
     if (dtype == EKV_BFLOAT16) {
-        launch_attend<__hip_bfloat16>(a, static_cast<hipStream_t>(stream));
+        merge_kernel<Bf16><<<grid, kAttentionThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);
     } else {
-        launch_attend<__half>(a, static_cast<hipStream_t>(stream));
+        merge_kernel<F16><<<grid, kAttentionThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);
     }
-    check_hip(hipGetLastError(), "launch attention");
-    return 0;
-}
-
-void need_workspace(uint64_t needed, const void* workspace, uint64_t bytes) {
-    if (bytes < needed) {
-        throw std::invalid_argument("the attention needs " + std::to_string(needed) + " workspace bytes, got " +
-                                    std::to_string(bytes));
-    }
-    if (needed > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)) {
-        throw std::invalid_argument("the workspace must be a 256-byte aligned device buffer");
-    }
-}
-
-uint64_t prefix_workspace(int64_t tokens, int64_t batch, int64_t groups, int64_t heads, int64_t kv_heads, int64_t dim,
-                          int64_t max_query) {
-    if (tokens < 0 || batch < 0 || groups < 0 || heads < 1 || kv_heads < 1 || dim < 1 || max_query < 1) {
-        throw std::invalid_argument("attention sizes must be positive");
-    }
-    return 0;
-}
-
-uint64_t topk_workspace(int64_t tokens, int64_t lanes, int64_t heads, int64_t kv_heads, int64_t dim) {
-    if (tokens < 0 || lanes < 0 || heads < 1 || kv_heads < 1 || dim < 1) {
-        throw std::invalid_argument("attention sizes must be positive");
-    }
+    check_hip(hipGetLastError(), "launch attention merge");
     return 0;
 }
 
 int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t workspace_bytes, void* stream) {
-    Args a = common_args(s.query, s.planes, s.layer, s.kv_heads, s.page_size, s.scale, s.output, s.lse);
+    AttentionArgs a = common_args(s.query, s.planes, s.layer, s.kv_heads, s.page_size, s.scale, s.output, s.lse);
     const auto need_table = [&](const ekv_tensor* p, const char* name) -> const ekv_tensor& {
         const ekv_tensor& t = need(p, name);
         need_ndim(t, 2, name);
@@ -369,10 +403,10 @@ int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t 
     need_ndim(lengths, 1, "lengths");
     need_index(lengths, "lengths");
     need_data(lengths, "lengths");
-    a.batch = lengths.shape[0];
-    if (a.batch > (int64_t{1} << 24)) {
-        throw std::invalid_argument("more than 2^24 batch rows");
+    if (lengths.shape[0] > kMostBatch) {
+        throw std::invalid_argument("more than 2^20 batch rows");
     }
+    a.batch = static_cast<int32_t>(lengths.shape[0]);
     a.lengths = index_ref(lengths, 0);
     a.tables = tables.data;
     a.table_row = tables.stride[0], a.table_col = tables.stride[1], a.table64 = tables.dtype == EKV_INT64;
@@ -394,7 +428,10 @@ int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t 
     }
     if (s.prefix_tables != nullptr) {
         const ekv_tensor& prefix = need_table(s.prefix_tables, "prefix_tables");
-        a.groups = prefix.shape[0];
+        if (prefix.shape[0] > kMostBatch) {
+            throw std::invalid_argument("more than 2^20 prefixes");
+        }
+        a.groups = static_cast<int32_t>(prefix.shape[0]);
         a.prefix_tables = prefix.data;
         a.prefix_row = prefix.stride[0], a.prefix_col = prefix.stride[1], a.prefix64 = prefix.dtype == EKV_INT64;
         a.prefix_columns = prefix.shape[1];
@@ -407,15 +444,14 @@ int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t 
     } else if (s.group_starts != nullptr) {
         throw std::invalid_argument("group_starts without prefix_tables");
     }
-    need_workspace(prefix_workspace(a.tokens, a.batch, a.groups, a.heads, a.kv_heads, a.dim, s.max_query), workspace,
-                   workspace_bytes);
-    return launch(a, s.query->dtype, stream);
+    Plan plan = prefix_plan(a.tokens, a.batch, a.groups, a.heads, a.kv_heads, a.dim, s.max_query);
+    return launch(a, plan, s.query->dtype, workspace, workspace_bytes, stream);
 }
 
 int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64_t kv_heads, const ekv_tensor* slots_p,
          int64_t zero_below, double scale, const ekv_tensor* out, const ekv_tensor* lse, void* workspace,
          uint64_t workspace_bytes, void* stream) {
-    Args a = common_args(query, planes, layer, kv_heads, 1, scale, out, lse);
+    AttentionArgs a = common_args(query, planes, layer, kv_heads, 1, scale, out, lse);
     const ekv_tensor& slots = need(slots_p, "slots");
     need_ndim(slots, 2, "slots");
     need_index(slots, "slots");
@@ -432,8 +468,8 @@ int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64
     a.tables = slots.data;
     a.table_row = slots.stride[0], a.table_col = slots.stride[1], a.table64 = slots.dtype == EKV_INT64;
     a.requests = a.tokens, a.columns = slots.shape[1];
-    need_workspace(topk_workspace(a.tokens, a.columns, a.heads, a.kv_heads, a.dim), workspace, workspace_bytes);
-    return launch(a, query->dtype, stream);
+    Plan plan = topk_plan(a.tokens, a.columns, a.heads, a.kv_heads, a.dim);
+    return launch(a, plan, query->dtype, workspace, workspace_bytes, stream);
 }
 
 }  // namespace
@@ -442,7 +478,7 @@ int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64
 extern "C" uint64_t ekv_shared_prefix_workspace_bytes(int64_t tokens, int64_t batch, int64_t groups, int64_t heads,
                                                       int64_t kv_heads, int64_t head_dim, int64_t max_query) {
     return ekv::guarded(~uint64_t{0}, [&] {
-        return ekv::prefix_workspace(tokens, batch, groups, heads, kv_heads, head_dim, max_query);
+        return ekv::prefix_plan(tokens, batch, groups, heads, kv_heads, head_dim, max_query).bytes;
     });
 }
 
@@ -458,7 +494,7 @@ extern "C" int ekv_shared_prefix_attention(const ekv_prefix_attention_args* args
 
 extern "C" uint64_t ekv_topk_workspace_bytes(int64_t tokens, int64_t lanes, int64_t heads, int64_t kv_heads,
                                              int64_t head_dim) {
-    return ekv::guarded(~uint64_t{0}, [&] { return ekv::topk_workspace(tokens, lanes, heads, kv_heads, head_dim); });
+    return ekv::guarded(~uint64_t{0}, [&] { return ekv::topk_plan(tokens, lanes, heads, kv_heads, head_dim).bytes; });
 }
 
 extern "C" int ekv_topk_attention(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64_t kv_heads,
