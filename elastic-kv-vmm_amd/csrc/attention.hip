@@ -17,52 +17,52 @@
 namespace ekv {
 namespace {
 
+constexpr int kMergeThreads = 256;
+
 // The workgroups that hold a token's parts of one phase, and where.
 struct Parts {
     const float* base;          // first part's row of values
     const float* stats;         // first part's largest score of the row; its sum is row_tile later
     int64_t step;               // to the next part
     int32_t row_tile;
-    int32_t count;
+    int32_t count;              // -1: the output is written already
 };
 
 // The parts of row `row` (of one KV head) of sequence s: none when the sequence was nobody's work.
 __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p, int32_t s, int32_t head, int32_t row) {
-    int64_t begin, total;
-    int32_t item, tiles, row_tiles;
+    uint32_t begin, total, item, units, row_tiles;
     if (p.mode == kSlots) {
         const Sequence any = sequence_of(a, kSlots, 0);
-        tiles = tiles_of(any, p), row_tiles = row_tiles_of(a, any, p);
+        units = units_of(any, p), row_tiles = row_tiles_of(a, any, p);
         item = s * a.kv_heads * row_tiles;
-        begin = static_cast<int64_t>(item) * tiles;
-        total = static_cast<int64_t>(p.sequences) * a.kv_heads * row_tiles * tiles;
+        begin = item * units;
+        total = p.sequences * a.kv_heads * row_tiles * units;
     } else {
-        begin = p.tile_starts[s];
+        begin = p.unit_starts[s];
         item = p.item_starts[s];
-        total = p.tile_starts[p.sequences];
-        const int32_t items = p.item_starts[s + 1] - item;
+        total = p.unit_starts[p.sequences];
+        const uint32_t items = p.item_starts[s + 1] - item;
         if (items == 0) {
             return Parts{};
         }
-        tiles = static_cast<int32_t>((p.tile_starts[s + 1] - begin) / items);
+        units = (p.unit_starts[s + 1] - begin) / items;
         row_tiles = items / a.kv_heads;
     }
-    const int32_t local = head * row_tiles + row / p.row_tile;
-    begin += static_cast<int64_t>(local) * tiles;
-    const int32_t active = active_workgroups(p, total);
-    const int32_t first = line_owner(total, begin, active), last = line_owner(total, begin + tiles - 1, active);
+    const uint32_t local = head * row_tiles + (row >> p.row_shift);
+    begin += local * units;
+    const uint32_t quota = quota_of(p, total);
+    const uint32_t first = begin / quota, last = (begin + units - 1) / quota;
     Parts r;
-    r.row_tile = p.row_tile;
-    r.step = static_cast<int64_t>(p.row_tile) * (p.dim_pad + 2);
-    const int64_t slot = first + item + local;
+    r.row_tile = 1 << p.row_shift;
+    r.step = static_cast<int64_t>(r.row_tile) * (p.dim_pad + 2);
+    const uint32_t slot = first + item + local, inside = row & (r.row_tile - 1);
     const float* part = p.parts + slot * r.step;
-    r.base = part + static_cast<int64_t>(row % p.row_tile) * p.dim_pad;
-    r.stats = part + static_cast<int64_t>(p.row_tile) * p.dim_pad + row % p.row_tile;
-    r.count = last - first + 1;
+    r.base = part + inside * p.dim_pad;
+    r.stats = part + r.row_tile * p.dim_pad + inside;
+    r.count = static_cast<int32_t>(last - first + 1);
     if (p.direct != 0 && r.count == 1) {
-        r.count = -1;           // written to the output by the one that had it whole
-    }
-    if (slot + r.count > p.slots) {
+        r.count = -1;
+    } else if (slot + r.count > static_cast<uint32_t>(p.slots)) {
         r.count = 0;            // only if the starts were not in order
     }
     return r;
@@ -71,7 +71,7 @@ __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p
 // One workgroup per (query token, KV head): a thread joins four elements of one row over all parts, own first, then the
 // prefix's, each in the order of the workgroups.
 template <typename T>
-__global__ __launch_bounds__(kAttentionThreads) void merge_kernel(const AttentionArgs a, const Phase own,
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArgs a, const Phase own,
                                                                   const Phase prefix) {
     const int32_t token = blockIdx.x, head = blockIdx.y;
     int32_t b = token;
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kAttentionThreads) void merge_kernel(const Attentio
     const int32_t own_first = b >= 0 && own.mode != kSlots ? first_token(a, b) : token;
     const int32_t prefix_first = group >= 0 ? first_token(a, first_row(a, group)) : 0;
     const int32_t quads = (a.dim + 3) >> 2;
-    for (int32_t unit = threadIdx.x; unit < a.share * quads; unit += kAttentionThreads) {
+    for (int32_t unit = threadIdx.x; unit < a.share * quads; unit += kMergeThreads) {
         const int32_t sub = unit / quads, element = (unit % quads) * 4;
         Parts part[2] = {};
         if (b >= 0) {
@@ -175,6 +175,15 @@ const ekv_tensor& need_list(const ekv_tensor* p, int64_t extent, const char* nam
     return t;
 }
 
+// Bytes between the columns of a table of page ids.
+uint32_t column_step(const ekv_tensor& t, const char* name) {
+    const int64_t step = t.shape[1] > 1 ? t.stride[1] * itemsize(t.dtype) : 0;
+    if (step < 0 || step > 0x7fffffff) {
+        throw std::invalid_argument(std::string(name) + ": columns more than 2 GiB apart");
+    }
+    return static_cast<uint32_t>(step);
+}
+
 // Query, output, statistics and cache: what both entry points share.
 AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, int64_t layer, int64_t kv_heads,
                  int64_t page_size, double scale, const ekv_tensor* out_p, const ekv_tensor* lse_p) {
@@ -218,15 +227,19 @@ AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, i
         throw std::invalid_argument("page_size must be from 1 to 2^30");
     }
     const int64_t row = kv_heads * a.dim * 2;
-    Cache& c = a.cache;
+    int64_t token_stride, page_stride, pages;
+    constexpr int64_t kMostStride = 0xffffffff;
+    if (planes->row_stride < 0 || planes->row_stride > kMostStride) {
+        throw std::invalid_argument("the plane row stride must be below 4 GiB");
+    }
     if (planes->row_bytes == row) {                       // a plane row is a token
-        c.token_stride = planes->row_stride;
-        c.page_stride = planes->row_stride * page_size;
-        c.pages = planes->rows / page_size;
+        token_stride = planes->row_stride;
+        page_stride = planes->row_stride * page_size;
+        pages = planes->rows / page_size;
     } else if (planes->row_bytes == row * page_size) {    // a plane row is a page
-        c.token_stride = row;
-        c.page_stride = planes->row_stride;
-        c.pages = planes->rows;
+        token_stride = row;
+        page_stride = planes->row_stride;
+        pages = planes->rows;
     } else {
         throw std::invalid_argument("plane rows hold " + std::to_string(planes->row_bytes) + " bytes: neither a token's " +
                                     std::to_string(row) + " nor a page's " + std::to_string(row * page_size));
@@ -234,7 +247,14 @@ AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, i
     if (planes->base == nullptr && planes->rows > 0) {
         throw std::invalid_argument("null plane base");
     }
-    c.head_stride = a.dim * 2;
+    if (page_stride > kMostStride || pages > 0x7fffffff) {
+        throw std::invalid_argument("a page must lie within 4 GiB, and a plane hold fewer than 2^31 pages");
+    }
+    Cache& c = a.cache;
+    c.token_stride = static_cast<uint32_t>(token_stride);
+    c.page_stride = static_cast<uint32_t>(page_stride);
+    c.pages = static_cast<uint32_t>(pages);
+    c.head_stride = static_cast<uint32_t>(dim * 2);
     c.page = FastDiv(static_cast<uint32_t>(page_size));
     c.zero_below = 1;
     c.k = static_cast<const char*>(planes->base) + layer * planes->layer_stride;
@@ -278,29 +298,38 @@ int tiles_for(int64_t rows, int32_t dim_pad) {
     return rows <= 16 ? 1 : (rows <= 32 || dim_pad > 128 ? 2 : 4);
 }
 
-void take(Plan& plan, Phase& p, int64_t rows) {
-    // Row tiles of all sequences: every sequence's last may be part-filled.
-    p.slots = p.workgroups + rows;
-    p.parts = reinterpret_cast<float*>(plan.bytes);
-    plan.bytes += aligned(static_cast<uint64_t>(p.slots) * p.row_tile * (p.dim_pad + 2) * sizeof(float));
-    if (p.mode != kSlots) {
-        p.tile_starts = reinterpret_cast<int64_t*>(plan.bytes);
-        plan.bytes += aligned((static_cast<uint64_t>(p.sequences) + 1) * sizeof(int64_t));
-        p.item_starts = reinterpret_cast<int32_t*>(plan.bytes);
-        plan.bytes += aligned((static_cast<uint64_t>(p.sequences) + 1) * sizeof(int32_t));
-    }
-}
-
+// A phase's cut and its place in the workspace.
 void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, int64_t tokens, int64_t share,
          int64_t kv_heads, int32_t dim_pad, bool direct) {
     p.mode = mode;
     p.sequences = static_cast<int32_t>(sequences);
-    p.row_tile = 16 * tiles16;
-    p.key_tile = 32;
+    p.row_shift = tiles16 == 1 ? 4 : (tiles16 == 2 ? 5 : 6);
+    p.unit_shift = narrow_unit_shift(tiles16, dim_pad);
     p.dim_pad = dim_pad;
-    p.workgroups = kComputeUnits * (tiles16 == 1 && dim_pad <= 128 ? 2 : 1);
+    p.workgroups = kComputeUnits;
     p.direct = direct;
-    take(plan, p, kv_heads * (tokens * share / p.row_tile + sequences));
+    // Row tiles of all sequences: every sequence's last may be part-filled.
+    const int64_t items = kv_heads * ((tokens * share >> p.row_shift) + std::min(sequences, tokens));
+    if (items > (int64_t{1} << 30)) {
+        throw std::invalid_argument("more than 2^30 row tiles");
+    }
+    p.slots = static_cast<int32_t>(p.workgroups + items);
+    p.parts = reinterpret_cast<float*>(plan.bytes);
+    plan.bytes += aligned((static_cast<uint64_t>(p.slots) << p.row_shift) * (dim_pad + 2) * sizeof(float));
+    if (mode != kSlots) {
+        p.unit_starts = reinterpret_cast<uint32_t*>(plan.bytes);
+        plan.bytes += aligned((static_cast<uint64_t>(sequences) + 1) * sizeof(uint32_t));
+        p.item_starts = reinterpret_cast<uint32_t*>(plan.bytes);
+        plan.bytes += aligned((static_cast<uint64_t>(sequences) + 1) * sizeof(uint32_t));
+    }
+}
+
+// Makes the unit so large that the line's places fit 31 bits, whatever the lengths on the device are.
+void fit_units(Phase& p, int64_t keys) {
+    const int64_t items = p.slots - p.workgroups;
+    while (items > 0 && (keys >> p.unit_shift) + 2 > 0x7fffffff / items) {
+        ++p.unit_shift;
+    }
 }
 
 void need_sizes(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim) {
@@ -354,7 +383,7 @@ void place(Phase& p, void* workspace) {
     };
     at(p.parts);
     if (p.mode != kSlots) {
-        at(p.tile_starts);
+        at(p.unit_starts);
         at(p.item_starts);
     }
 }
@@ -371,16 +400,18 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
         return 0;
     }
     place(plan.own, workspace);
+    fit_units(plan.own, int64_t{a.own_most} + a.prefix_most);
     if (plan.prefix_tiles16 != 0) {
         place(plan.prefix, workspace);
+        fit_units(plan.prefix, a.prefix_most);
         launch_narrow(a, plan.prefix, dtype, plan.prefix_tiles16, stream);
     }
     launch_narrow(a, plan.own, dtype, plan.tiles16, stream);
     const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.kv_heads));
     if (dtype == EKV_BFLOAT16) {
-        merge_kernel<Bf16><<<grid, kAttentionThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);
+        merge_kernel<Bf16><<<grid, kMergeThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);
     } else {
-        merge_kernel<F16><<<grid, kAttentionThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);
+        merge_kernel<F16><<<grid, kMergeThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);
     }
     check_hip(hipGetLastError(), "launch attention merge");
     return 0;
@@ -408,9 +439,12 @@ int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t 
     }
     a.batch = static_cast<int32_t>(lengths.shape[0]);
     a.lengths = index_ref(lengths, 0);
-    a.tables = tables.data;
-    a.table_row = tables.stride[0], a.table_col = tables.stride[1], a.table64 = tables.dtype == EKV_INT64;
-    a.requests = tables.shape[0], a.columns = tables.shape[1];
+    a.tables = static_cast<const char*>(tables.data);
+    a.table_row = tables.stride[0] * itemsize(tables.dtype);
+    a.table_col = column_step(tables, "block_tables");
+    a.table64 = tables.dtype == EKV_INT64;
+    a.requests = static_cast<int32_t>(std::min<int64_t>(tables.shape[0], 0x7fffffff));
+    a.own_most = static_cast<int32_t>(tables.shape[1] * s.page_size);
     if (s.rows != nullptr) {
         a.rows = index_ref(need_list(s.rows, a.batch, "rows"), 0);
     }
@@ -432,9 +466,11 @@ int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t 
             throw std::invalid_argument("more than 2^20 prefixes");
         }
         a.groups = static_cast<int32_t>(prefix.shape[0]);
-        a.prefix_tables = prefix.data;
-        a.prefix_row = prefix.stride[0], a.prefix_col = prefix.stride[1], a.prefix64 = prefix.dtype == EKV_INT64;
-        a.prefix_columns = prefix.shape[1];
+        a.prefix_tables = static_cast<const char*>(prefix.data);
+        a.prefix_row = prefix.stride[0] * itemsize(prefix.dtype);
+        a.prefix_col = column_step(prefix, "prefix_tables");
+        a.prefix64 = prefix.dtype == EKV_INT64;
+        a.prefix_most = static_cast<int32_t>(prefix.shape[1] * s.page_size);
         a.prefix_lengths = index_ref(need_list(s.prefix_lengths, a.groups, "prefix_lengths"), 0);
         if (s.group_starts != nullptr) {
             a.group_starts = index_ref(need_list(s.group_starts, a.groups + 1, "group_starts"), 0);
@@ -460,15 +496,18 @@ int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64
     if (slots.shape[1] > (int64_t{1} << 30) - 1) {
         throw std::invalid_argument("more than 2^30 - 1 lanes");
     }
-    if (zero_below < 0) {
-        throw std::invalid_argument("zero_below must not be negative");
+    if (zero_below < 0 || zero_below > 0x7fffffff) {
+        throw std::invalid_argument("zero_below must be from 0 to 2^31 - 1");
     }
-    a.cache.zero_below = zero_below;
+    a.cache.zero_below = static_cast<uint32_t>(zero_below);
     a.batch = a.tokens;
-    a.tables = slots.data;
-    a.table_row = slots.stride[0], a.table_col = slots.stride[1], a.table64 = slots.dtype == EKV_INT64;
-    a.requests = a.tokens, a.columns = slots.shape[1];
-    Plan plan = topk_plan(a.tokens, a.columns, a.heads, a.kv_heads, a.dim);
+    a.tables = static_cast<const char*>(slots.data);
+    a.table_row = slots.stride[0] * itemsize(slots.dtype);
+    a.table_col = column_step(slots, "slots");
+    a.table64 = slots.dtype == EKV_INT64;
+    a.requests = a.tokens;
+    a.own_most = static_cast<int32_t>(slots.shape[1]);
+    Plan plan = topk_plan(a.tokens, a.own_most, a.heads, a.kv_heads, a.dim);
     return launch(a, plan, query->dtype, workspace, workspace_bytes, stream);
 }
 

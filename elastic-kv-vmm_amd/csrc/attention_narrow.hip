@@ -7,10 +7,11 @@
 // to the second product when its keys are taken in that order, so P never leaves its registers; V^T comes from a
 // transposed read of LDS in the same order of keys.
 //
-// What bounds it: the K and V rows from HBM. Every wave reads its own keys (four waves a workgroup, each every
-// fourth tile), K straight into the registers of the first product, V by way of LDS, with the next tile's rows in
-// flight while a tile is worked on and the one after's page ids before them: 16 KB a wave in flight at a head size
-// of 128. Each row of 16 * kTiles rows is held by every wave and joined at the end of an item in a fixed order.
+// What bounds it: the K and V rows from HBM. Every wave reads its own keys (each every kWaves-th tile of the segment), K
+// straight into the registers of the first product, V by way of LDS. A tile's registers are free once the first
+// product and the LDS write have taken them, so the next tile's rows are in flight during the rest of a tile, and the
+// page ids of the one after before them: 16 KB a wave at a head size of 128. Each row of 16 * kTiles rows is held by
+// every wave and joined at the end of an item in a fixed order.
 #include "ekv_attention.h"
 #include "ekv_mfma.h"
 
@@ -33,10 +34,16 @@ struct Rows {
     }
 };
 
+// Waves of a workgroup: as many as share a compute unit at the registers that the row tiles take.
+template <int kDim, int kTiles>
+constexpr int waves_of() {
+    return kTiles == 1 && kDim <= 128 ? 8 : 4;
+}
+
 template <int kDim, int kTiles>
 constexpr int lds_bytes() {
-    const int values = kAttentionWaves * kKeys * Rows<kDim>::kBytes;      // V of each wave's tile
-    const int join = kAttentionWaves * 4 * kTiles * 64 * 16;              // four 16-column pieces of each wave's sums
+    const int values = waves_of<kDim, kTiles>() * kKeys * Rows<kDim>::kBytes;       // V of each wave's tile
+    const int join = waves_of<kDim, kTiles>() * (kDim / 16) * kTiles * 64 * 16;     // each wave's weighted values
     return values > join ? values : join;
 }
 
@@ -54,26 +61,31 @@ __device__ __forceinline__ float over_groups_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// A tile of keys: where it lies, and the page id of each of the lane's two keys (l % 16 and 16 + l % 16 of the tile).
-struct Pages {
-    int32_t low[2], high[2];
+// One of the two sources of an item's keys.
+struct Source {
+    const char* table;        // its row of the page table
+    uint32_t step;            // bytes between columns
+    uint32_t wide;            // 4 for int64 ids: the high word's place
+    int32_t keys;
 };
 
-// K and V rows of a tile, in the lane order of the first product: key l % 16 (+ 16), pieces l / 16 + 4 c.
-template <int kSteps>
-struct Held {
-    words4 k[2][kSteps], v[2][kSteps];
-    uint32_t seen;            // bit per key
+// Page ids of the lane's two keys of a tile (l % 16 and 16 + l % 16), as words: int64 ids whose high word is not zero
+// name no page.
+struct Ids {
+    uint32_t low[2], high[2];
 };
 
 template <typename T, int kDim, int kTiles>
-__global__ __launch_bounds__(kAttentionThreads, kTiles == 1 && kDim <= 128 ? 2 : 1) void narrow_kernel(
+__global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kTiles>() / 4)) void narrow_kernel(
     const AttentionArgs a, const Phase p) {
+    constexpr int kWaves = waves_of<kDim, kTiles>();
     constexpr int kSteps = kDim / 32;      // matrix steps of the first product
     constexpr int kCols = kDim / 16;       // 16-column pieces of the output
+    // Head sizes between kDim and the next smaller class end in one of the last steps.
+    constexpr int kWholeSteps = kDim == 64 ? 0 : (kDim == 96 ? 2 : (kDim == 128 ? 3 : 4));
     __shared__ __align__(16) char s_data[lds_bytes<kDim, kTiles>()];
-    __shared__ float s_max[kAttentionWaves][kTiles * 16], s_sum[kAttentionWaves][kTiles * 16];
-    __shared__ LineCells s_line;
+    __shared__ float s_max[kWaves][kTiles * 16], s_sum[kWaves][kTiles * 16];
+    __shared__ LineCells<kWaves> s_line;
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     char* const values = s_data + wave * (kKeys * Rows<kDim>::kBytes);
@@ -92,63 +104,12 @@ __global__ __launch_bounds__(kAttentionThreads, kTiles == 1 && kDim <= 128 ? 2 :
 #pragma unroll
             for (int c = 0; c < kSteps; ++c) {
                 const int piece = c * 4 + quad;
-                const bool live = row < g.rows && piece < pieces;
+                const bool live = row < g.rows && (c < kWholeSteps || piece < pieces);
                 q[m][c] = *reinterpret_cast<const words4*>(live ? at + piece * 16 : zeros);
             }
-            visible[m] = clamped(g.q.length - g.q.count + token + 1, 0, g.q.own);
+            visible[m] = seen_by(g.q, token);
         }
-        const int32_t first_visible =
-            __builtin_amdgcn_readfirstlane(clamped(g.q.length - g.q.count + g.row_begin / a.share + 1, 0, g.q.own));
-        const int32_t prefix_tiles = (g.q.prefix + kKeys - 1) / kKeys;
-        const bool prefix64 = a.prefix64, own64 = a.table64;
-
-        const auto pages_of = [&](int32_t t) {
-            Pages e;
-            const bool own = t >= prefix_tiles;
-            const int32_t base = (own ? t - prefix_tiles : t) * kKeys;
-            const int32_t keys = t < g.end ? (own ? g.q.own : g.q.prefix) : 0;
-            const bool wide = own ? own64 : prefix64;
-            const char* table = static_cast<const char*>(own ? a.tables : a.prefix_tables);
-            const int64_t start = own ? g.q.request * a.table_row : g.q.group * a.prefix_row;
-            const int64_t step = own ? a.table_col : a.prefix_col;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int32_t key = base + h * 16 + col;
-                const int64_t at = (start + a.cache.page.div(key) * step) * (wide ? 8 : 4);
-                const char* from = key < keys ? table + at : zeros;
-                e.low[h] = *reinterpret_cast<const int32_t*>(from);
-                e.high[h] = *reinterpret_cast<const int32_t*>(from + (wide ? 4 : 0));
-            }
-            return e;
-        };
-        const auto rows_of = [&](int32_t t, const Pages& e) {
-            Held<kSteps> d;
-            const bool own = t >= prefix_tiles;
-            const int32_t base = (own ? t - prefix_tiles : t) * kKeys;
-            const int32_t keys = t < g.end ? (own ? g.q.own : g.q.prefix) : 0;
-            const bool wide = own ? own64 : prefix64;
-            d.seen = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int32_t key = base + h * 16 + col;
-                const int32_t high = wide ? e.high[h] : e.low[h] >> 31;
-                const int64_t page = static_cast<int64_t>(
-                    (static_cast<uint64_t>(static_cast<uint32_t>(high)) << 32) | static_cast<uint32_t>(e.low[h]));
-                const bool seen = key < keys && page >= a.cache.zero_below && page < a.cache.pages;
-                const uint32_t inside = key - a.cache.page.div(key) * a.cache.page.divisor;
-                const char* at = a.cache.k + page * a.cache.page_stride + inside * a.cache.token_stride +
-                                 g.head * a.cache.head_stride;
-#pragma unroll
-                for (int c = 0; c < kSteps; ++c) {
-                    const int piece = c * 4 + quad;
-                    const bool live = seen && piece < pieces;
-                    d.k[h][c] = *reinterpret_cast<const words4*>(live ? at + piece * 16 : zeros);
-                    d.v[h][c] = *reinterpret_cast<const words4*>(live ? at + a.cache.kv_stride + piece * 16 : zeros);
-                }
-                d.seen |= (static_cast<uint32_t>(__ballot(seen)) & 0xffffu) << (16 * h);
-            }
-            return d;
-        };
+        const int32_t first_visible = seen_by(g.q, g.row_begin / a.share);
 
         f32x4 o[kTiles][kCols];
         float top[kTiles], sum[kTiles];
@@ -160,133 +121,204 @@ __global__ __launch_bounds__(kAttentionThreads, kTiles == 1 && kDim <= 128 ? 2 :
                 o[m][c] = f32x4{0, 0, 0, 0};
             }
         }
-        int32_t t = g.begin + wave;
-        Pages ahead = pages_of(t);
-        Held<kSteps> next = rows_of(t, ahead);
-        ahead = pages_of(t + kAttentionWaves);
-        for (; t < g.end; t += kAttentionWaves) {
-            const Held<kSteps> now = next;
-            const Pages later = pages_of(t + 2 * kAttentionWaves);
-            next = rows_of(t + kAttentionWaves, ahead);
-            ahead = later;
-            const bool own = t >= prefix_tiles;
-            const int32_t base = (own ? t - prefix_tiles : t) * kKeys;
-            // Whether some row sees fewer keys of this tile than it holds.
-            const bool ragged = own && base + kKeys > first_visible;
-            f32x4 s[kTiles][2];
-#pragma unroll
-            for (int m = 0; m < kTiles; ++m) {
+
+        const int32_t prefix_end = prefix_units(g.q, p);
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side) {
+            // Tiles [first, last) of this source; a wave takes every kWaves-th.
+            const bool own = side == 1;
+            const int32_t from = own ? max(g.begin - prefix_end, 0) : g.begin;
+            const int32_t to = own ? g.end - prefix_end : min(g.end, prefix_end);
+            if (to <= from) {
+                continue;
+            }
+            Source src;
+            src.table = own ? a.tables + g.q.request * a.table_row : a.prefix_tables + g.q.group * a.prefix_row;
+            src.step = own ? a.table_col : a.prefix_col;
+            src.wide = (own ? a.table64 : a.prefix64) != 0 ? 4 : 0;
+            src.keys = min(own ? g.q.own : g.q.prefix, to << p.unit_shift);
+            const char* const k_head = a.cache.k + static_cast<uint64_t>(a.cache.head_stride) * g.head + quad * 16;
+            const char* const v_head = k_head + a.cache.kv_stride;
+
+            const auto ids_of = [&](int32_t base) {
+                Ids e;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    s[m][h] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int c = 0; c < kSteps; ++c) {
-                        s[m][h] = T::mfma16(now.k[h][c], q[m][c], s[m][h]);
-                    }
+                    const int32_t key = base + h * 16 + col;
+                    const char* at = src.table + static_cast<uint64_t>(a.cache.page.div(key)) * src.step;
+                    at = key < src.keys ? at : zeros;
+                    e.low[h] = *reinterpret_cast<const uint32_t*>(at);
+                    e.high[h] = *reinterpret_cast<const uint32_t*>(at + src.wide);
                 }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int c = 0; c < kSteps; ++c) {
-                    *reinterpret_cast<words4*>(values + Rows<kDim>::place(h * 16 + col, c * 4 + quad)) = now.v[h][c];
-                }
-            }
-            words4 weights[kTiles];
-#pragma unroll
-            for (int m = 0; m < kTiles; ++m) {
-                float x[8], most = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[j] = s[m][j >> 2][j & 3] * a.scale;
-                }
-                if (ragged || now.seen != 0xffffffffu) {
-                    const int32_t left = own ? visible[m] - base : kKeys;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int key = (j >> 2) * 16 + quad * 4 + (j & 3);
-                        x[j] = ((now.seen >> key) & 1) != 0 && key < left ? x[j] : -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    most = fmaxf(most, x[j]);
-                }
-                most = fmaxf(top[m], over_groups_max(most));
-                const float safe = most == -INFINITY ? 0.0f : most;
-                if (__ballot(most > top[m]) != 0) {
-                    const float keep = exp2f(top[m] - safe);
-                    sum[m] *= keep;
-#pragma unroll
-                    for (int c = 0; c < kCols; ++c) {
-                        o[m][c] *= keep;
-                    }
-                    top[m] = most;
-                }
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    w[j] = __builtin_amdgcn_exp2f(x[j] - safe + T::kShift);
-                    sum[m] += w[j];
-                }
-                weights[m] = words4{T::pack(w[0], w[1]), T::pack(w[2], w[3]), T::pack(w[4], w[5]), T::pack(w[6], w[7])};
-            }
-            const auto column = [&](int c) {
-                // Row quad * 4 + col / 4 of each 16 keys, the (col % 4)-th 8 bytes of the 32-byte column piece.
-                const int key = quad * 4 + (col >> 2), piece = c * 2 + ((col & 3) >> 1), half = (col & 1) * 8;
-                const words2 low = read_transposed(values + Rows<kDim>::place(key, piece) + half);
-                const words2 high = read_transposed(values + Rows<kDim>::place(16 + key, piece) + half);
-                return words4{low[0], low[1], high[0], high[1]};
+                return e;
             };
-            bool spoiled = false;
-            if (ragged) {
-                // A key that only some rows see has weight 0 for the others, and 0 * infinity is not 0.
+            words4 k[2][kSteps], v[2][kSteps];
+            uint32_t seen = 0;                // bit per key of the tile
+            const auto fetch = [&](int32_t base, const Ids& e) {
+                seen = 0;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    const int32_t key = base + h * 16 + col;
+                    const uint32_t id = e.low[h];
+                    const bool good = key < src.keys && id >= a.cache.zero_below && id < a.cache.pages &&
+                                      (src.wide == 0 || e.high[h] == 0);
+                    const uint32_t inside = key - a.cache.page.div(key) * a.cache.page.divisor;
+                    const uint64_t offset = static_cast<uint64_t>(id) * a.cache.page_stride +
+                                            static_cast<uint64_t>(inside) * a.cache.token_stride;
+                    const char* k_at = good ? k_head + offset : zeros;
+                    const char* v_at = good ? v_head + offset : zeros;
 #pragma unroll
                     for (int c = 0; c < kSteps; ++c) {
+                        // Past the head size: any piece of the row; K meets zeros of q once it is cleared, V's columns
+                        // are not stored.
+                        const int piece = c < kWholeSteps || c * 4 + quad < pieces ? c * 64 : -quad * 16;
+                        k[h][c] = *reinterpret_cast<const words4*>(k_at + (good || c < kWholeSteps ? piece : 0));
+                        v[h][c] = *reinterpret_cast<const words4*>(v_at + (good || c < kWholeSteps ? piece : 0));
+                    }
+                    seen |= (static_cast<uint32_t>(__ballot(good)) & 0xffffu) << (16 * h);
+                }
+            };
+
+            constexpr int kStride = kWaves * kKeys;
+            int32_t base = (from << p.unit_shift) + wave * kKeys;
+            Ids ids = ids_of(base);
+            fetch(base, ids);
+            ids = ids_of(base + kStride);
+#pragma unroll 1
+            for (; base < src.keys; base += kStride) {
+                const Ids later = ids_of(base + 2 * kStride);
+                const uint32_t now = seen;
+                // Whether some row sees fewer keys of this tile than it holds.
+                const bool ragged = own && base + kKeys > first_visible;
+                f32x4 s[kTiles][2];
+                if (kWholeSteps < kSteps && a.dim != kDim) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            spoiled |= not_finite<T>(now.v[h][c][e]);
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int c = kWholeSteps; c < kSteps; ++c) {
+                            k[h][c] = c * 4 + quad < pieces ? k[h][c] : words4{0, 0, 0, 0};
                         }
                     }
                 }
-                spoiled = __ballot(spoiled) != 0;
-            }
-            if (!spoiled) {
 #pragma unroll
-                for (int c = 0; c < kCols; ++c) {
-                    const words4 v = column(c);
+                for (int m = 0; m < kTiles; ++m) {
 #pragma unroll
-                    for (int m = 0; m < kTiles; ++m) {
-                        o[m][c] = T::mfma16(v, weights[m], o[m][c]);
+                    for (int h = 0; h < 2; ++h) {
+                        s[m][h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                        for (int c = 0; c < kSteps; ++c) {
+                            s[m][h] = T::mfma16(k[h][c], q[m][c], s[m][h]);
+                        }
                     }
                 }
-            } else {
-                // One query token at a time: its rows take the product with the values that it sees.
-                const int32_t last = min(g.row_begin + 16 * kTiles, g.rows) - 1;
-                for (int32_t token = g.row_begin / a.share; token <= last / a.share; ++token) {
-                    const int32_t left = clamped(g.q.length - g.q.count + token + 1, 0, g.q.own) - base;
+                bool spoiled = false;
+                if (ragged) {
+                    // A key that only some rows see has weight 0 for the others, and 0 * infinity is not 0.
 #pragma unroll
-                    for (int c = 0; c < kCols; ++c) {
-                        words4 v = column(c);
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int c = 0; c < kSteps; ++c) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                spoiled |= not_finite<T>(v[h][c][e]);
+                            }
+                        }
+                    }
+                    spoiled = __ballot(spoiled) != 0;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int c = 0; c < kSteps; ++c) {
+                        *reinterpret_cast<words4*>(values + Rows<kDim>::place(h * 16 + col, c * 4 + quad)) = v[h][c];
+                    }
+                }
+                fetch(base + kStride, ids);
+                ids = later;
+                words4 weights[kTiles];
+#pragma unroll
+                for (int m = 0; m < kTiles; ++m) {
+                    float x[8], most = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        x[j] = s[m][j >> 2][j & 3] * a.scale;
+                    }
+                    if (ragged || now != 0xffffffffu) {
+                        const int32_t left = own ? visible[m] - base : kKeys;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const int key = (j >> 2) * 16 + quad * 4 + (j & 3);
-                            v[j >> 1] &= key < left ? 0xffffffffu : ((j & 1) != 0 ? 0x0000ffffu : 0xffff0000u);
+                            x[j] = ((now >> key) & 1) != 0 && key < left ? x[j] : -INFINITY;
                         }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        most = fmaxf(most, x[j]);
+                    }
+                    most = fmaxf(top[m], over_groups_max(most));
+                    const float safe = most == -INFINITY ? 0.0f : most;
+                    if (__ballot(most > top[m]) != 0) {
+                        const float keep = __builtin_amdgcn_exp2f(top[m] - safe);
+                        sum[m] *= keep;
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) {
+                            o[m][c] *= keep;
+                        }
+                        top[m] = most;
+                    }
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        w[j] = __builtin_amdgcn_exp2f(x[j] - safe + T::kShift);
+                        sum[m] += w[j];
+                    }
+                    weights[m] =
+                        words4{T::pack(w[0], w[1]), T::pack(w[2], w[3]), T::pack(w[4], w[5]), T::pack(w[6], w[7])};
+                }
+                const auto column = [&](int c) {
+                    // Row quad * 4 + col / 4 of each 16 keys, the (col % 4)-th 8 bytes of the 32-byte column piece.
+                    const int key = quad * 4 + (col >> 2), piece = c * 2 + ((col & 3) >> 1), half = (col & 1) * 8;
+                    const words2 low = read_transposed(values + Rows<kDim>::place(key, piece) + half);
+                    const words2 high = read_transposed(values + Rows<kDim>::place(16 + key, piece) + half);
+                    return words4{low[0], low[1], high[0], high[1]};
+                };
+                if (!spoiled) {
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        const words4 column_c = column(c);
 #pragma unroll
                         for (int m = 0; m < kTiles; ++m) {
-                            const f32x4 x = T::mfma16(v, weights[m], o[m][c]);
-                            const int32_t row = g.row_begin + m * 16 + col;
-                            o[m][c] = static_cast<int32_t>(a.share_div.div(row)) == token ? x : o[m][c];
+                            o[m][c] = T::mfma16(column_c, weights[m], o[m][c]);
+                        }
+                    }
+                } else {
+                    // One query token at a time: its rows take the product with the values that it sees.
+                    const int32_t last = min(g.row_begin + 16 * kTiles, g.rows) - 1;
+#pragma unroll 1
+                    for (int32_t token = g.row_begin / a.share; token <= last / a.share; ++token) {
+                        const int32_t left = seen_by(g.q, token) - base;
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) {
+                            words4 column_c = column(c);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const int key = (j >> 2) * 16 + quad * 4 + (j & 3);
+                                column_c[j >> 1] &= key < left ? 0xffffffffu : ((j & 1) != 0 ? 0x0000ffffu : 0xffff0000u);
+                            }
+#pragma unroll
+                            for (int m = 0; m < kTiles; ++m) {
+                                const f32x4 x = T::mfma16(column_c, weights[m], o[m][c]);
+                                const int32_t row = g.row_begin + m * 16 + col;
+                                o[m][c] = static_cast<int32_t>(a.share_div.div(row)) == token ? x : o[m][c];
+                            }
                         }
                     }
                 }
             }
         }
 
-        // The waves' parts, joined in the order of the waves.
+        // The waves' parts, joined in the order of the waves: each wave scales its values to the largest score of all,
+        // then sums its columns of everybody's.
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) {
             sum[m] = over_groups_sum(sum[m]);
@@ -296,96 +328,83 @@ __global__ __launch_bounds__(kAttentionThreads, kTiles == 1 && kDim <= 128 ? 2 :
             }
         }
         __syncthreads();
-        const bool whole = p.direct != 0 && g.begin == 0 && g.end == g.tiles;
-        float* const part = p.parts + static_cast<int64_t>(g.slot) * p.row_tile * (p.dim_pad + 2);
+        const bool whole = p.direct != 0 && g.begin == 0 && g.end == g.units;
+        const int32_t row_tile = 16 * kTiles;
+        float* const part = p.parts + static_cast<int64_t>(g.slot) * row_tile * (kDim + 2);
         const bool room = g.slot < p.slots;
-        float all_sum[kTiles];
+        f32x4* const cells = reinterpret_cast<f32x4*>(s_data);   // [wave][column][row tile][lane]
+        float factor[kTiles];
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) {
             float most = -INFINITY, total = 0;
 #pragma unroll
-            for (int w = 0; w < kAttentionWaves; ++w) {
+            for (int w = 0; w < kWaves; ++w) {
                 most = fmaxf(most, s_max[w][m * 16 + col]);
             }
             const float safe = most == -INFINITY ? 0.0f : most;
 #pragma unroll
-            for (int w = 0; w < kAttentionWaves; ++w) {
-                total += s_sum[w][m * 16 + col] * exp2f(s_max[w][m * 16 + col] - safe);
+            for (int w = 0; w < kWaves; ++w) {
+                total += s_sum[w][m * 16 + col] * __builtin_amdgcn_exp2f(s_max[w][m * 16 + col] - safe);
             }
-            const float mine = exp2f(top[m] - safe);
+            const float mine = __builtin_amdgcn_exp2f(top[m] - safe);
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
-                o[m][c] *= mine;
+                cells[((wave * kCols + c) * kTiles + m) * 64 + lane] = o[m][c] * mine;
             }
-            all_sum[m] = total;
+            factor[m] = !whole ? 1.0f : (total == 0 ? 0.0f : 1.0f / total);
             const int32_t row = g.row_begin + m * 16 + col;
             if (wave == 0 && quad == 0 && row < g.rows) {
                 if (!whole) {
                     if (room) {
-                        part[p.row_tile * p.dim_pad + m * 16 + col] = most;
-                        part[p.row_tile * p.dim_pad + p.row_tile + m * 16 + col] = total;
+                        part[row_tile * kDim + m * 16 + col] = most;
+                        part[row_tile * kDim + row_tile + m * 16 + col] = total;
                     }
                 } else if (a.lse != nullptr) {
-                    const int32_t place = a.share_div.div(row);
-                    const int32_t token = g.q.first + place, head = (g.head - place) * a.share + row;
-                    a.lse[token * a.l_token + head * a.l_head] =
+                    const int32_t token = a.share_div.div(row);
+                    a.lse[(g.q.first + token) * a.l_token + ((g.head - token) * a.share + row) * a.l_head] =
                         total == 0 ? -INFINITY : (most - T::kShift + log2f(total)) * kLn2;
                 }
             }
         }
-        f32x4* const cells = reinterpret_cast<f32x4*>(s_data);   // [wave][column of the round][row tile][lane]
+        __syncthreads();
 #pragma unroll
-        for (int round = 0; round < (kCols + 3) / 4; ++round) {
+        for (int c = wave; c < kCols; c += kWaves) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (round * 4 + c < kCols) {
+            for (int m = 0; m < kTiles; ++m) {
+                f32x4 x = cells[(c * kTiles + m) * 64 + lane];
 #pragma unroll
-                    for (int m = 0; m < kTiles; ++m) {
-                        cells[((wave * 4 + c) * kTiles + m) * 64 + lane] = o[m][round * 4 + c];
-                    }
+                for (int w = 1; w < kWaves; ++w) {
+                    x += cells[((w * kCols + c) * kTiles + m) * 64 + lane];
                 }
-            }
-            __syncthreads();
-            const int piece = round * 4 + wave;
-            if (piece < kCols) {
-#pragma unroll
-                for (int m = 0; m < kTiles; ++m) {
-                    f32x4 x = cells[(wave * kTiles + m) * 64 + lane];
-#pragma unroll
-                    for (int w = 1; w < kAttentionWaves; ++w) {
-                        x += cells[((w * 4 + wave) * kTiles + m) * 64 + lane];
-                    }
-                    const int32_t row = g.row_begin + m * 16 + col;
-                    const int32_t element = piece * 16 + quad * 4;
-                    if (row < g.rows) {
-                        if (!whole) {
-                            if (room) {
-                                *reinterpret_cast<f32x4*>(part + (m * 16 + col) * p.dim_pad + element) = x;
-                            }
-                        } else if (element < a.dim) {
-                            const float inverse = all_sum[m] == 0 ? 0.0f : 1.0f / all_sum[m];
-                            const int32_t place = a.share_div.div(row);
-                            const int32_t token = g.q.first + place, head = (g.head - place) * a.share + row;
-                            *reinterpret_cast<words2*>(a.out + token * a.o_token + head * a.o_head + element * 2) =
-                                words2{T::pack(x[0] * inverse, x[1] * inverse), T::pack(x[2] * inverse, x[3] * inverse)};
+                x *= factor[m];
+                const int32_t row = g.row_begin + m * 16 + col;
+                const int32_t element = c * 16 + quad * 4;
+                if (row < g.rows) {
+                    if (!whole) {
+                        if (room) {
+                            *reinterpret_cast<f32x4*>(part + (m * 16 + col) * kDim + element) = x;
                         }
+                    } else if (element < a.dim) {
+                        const int32_t token = a.share_div.div(row), head = (g.head - token) * a.share + row;
+                        *reinterpret_cast<words2*>(a.out + (g.q.first + token) * a.o_token + head * a.o_head +
+                                                   element * 2) = words2{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
                     }
                 }
             }
-            __syncthreads();
         }
+        __syncthreads();
     });
 }
 
 template <typename T, int kDim>
 void launch_dim(const AttentionArgs& a, const Phase& p, int tiles16, hipStream_t stream) {
-    const dim3 grid(static_cast<uint32_t>(p.workgroups)), block(kAttentionThreads);
+    const dim3 grid(static_cast<uint32_t>(p.workgroups));
     if (tiles16 == 1) {
-        narrow_kernel<T, kDim, 1><<<grid, block, 0, stream>>>(a, p);
+        narrow_kernel<T, kDim, 1><<<grid, waves_of<kDim, 1>() * 64, 0, stream>>>(a, p);
     } else if (tiles16 == 2) {
-        narrow_kernel<T, kDim, 2><<<grid, block, 0, stream>>>(a, p);
+        narrow_kernel<T, kDim, 2><<<grid, waves_of<kDim, 2>() * 64, 0, stream>>>(a, p);
     } else if constexpr (kDim <= 128) {
-        narrow_kernel<T, kDim, 4><<<grid, block, 0, stream>>>(a, p);
+        narrow_kernel<T, kDim, 4><<<grid, waves_of<kDim, 4>() * 64, 0, stream>>>(a, p);
     }
     check_hip(hipGetLastError(), "launch attention");
 }
@@ -401,6 +420,8 @@ void launch_type(const AttentionArgs& a, const Phase& p, int tiles16, hipStream_
 }
 
 }  // namespace
+
+int narrow_unit_shift(int tiles16, int32_t dim_pad) { return tiles16 == 1 && dim_pad <= 128 ? 8 : 7; }
 
 void launch_narrow(const AttentionArgs& a, const Phase& p, int32_t dtype, int tiles16, void* stream) {
     if (dtype == EKV_BFLOAT16) {

@@ -2,10 +2,11 @@
 //
 // A launch attends for sequences: a group's query tokens to its prefix, a batch row's to its own tokens or to both, or
 // one query token's to its slots. A sequence has `rows` rows (query tokens x query heads of one KV head) in tiles of
-// row_tile, and keys in tiles of key_tile; an item is one (sequence, KV head, row tile), and its key tiles are counted in
-// one line over all items. Workgroup w of W takes places [w * total / W, (w + 1) * total / W) of that line, whatever the
-// lengths are, so every workgroup has the same number of key tiles to read; an item cut between workgroups is joined by
-// the merge kernel from the parts that each left (weighted values, largest score, sum).
+// row_tile, and keys in units of unit; an item is one (sequence, KV head, row tile), and its key units are counted in one
+// line over all items. Workgroup w takes places [w * quota, (w + 1) * quota) of that line, whatever the lengths are, so
+// every workgroup has as many keys to read; an item cut between workgroups is joined by the merge kernel from the parts
+// that each left (weighted values, largest score, sum). Places fit 31 bits: the host makes the unit larger where the
+// tables' widths could pass them.
 #pragma once
 
 #include "../../include/ekv_kernels.h"
@@ -20,14 +21,14 @@
 
 namespace ekv {
 
-// Token offset o of page p of one KV head: k + p * page_stride + o * token_stride (bytes), V at + kv_stride.
+// Token offset o of page p of KV head h: k + p * page_stride + o * token_stride + h * head_stride (bytes), V at
+// + kv_stride.
 struct Cache {
     const char* k;
     int64_t kv_stride;
-    int64_t page_stride, token_stride, head_stride;
-    int64_t pages;        // ids zero_below .. pages - 1 name pages
-    int64_t zero_below;
-    FastDiv page;         // tokens per page
+    uint32_t page_stride, token_stride, head_stride;
+    uint32_t pages, zero_below;   // ids zero_below .. pages - 1 name pages
+    FastDiv page;                 // tokens per page
 };
 
 struct AttentionArgs {
@@ -38,12 +39,13 @@ struct AttentionArgs {
     float* lse;
     int64_t l_token, l_head;      // elements
     Cache cache;
-    const void* tables;           // [R, M] own pages of each request, or the slots of each query token
-    int64_t table_row, table_col;
-    int64_t requests, columns;
-    const void* prefix_tables;    // [G, P]
-    int64_t prefix_row, prefix_col;
-    int64_t prefix_columns;
+    const char* tables;           // [R, M] own pages of each request, or the slots of each query token
+    int64_t table_row;            // bytes, as the columns' step
+    const char* prefix_tables;    // [G, P]
+    int64_t prefix_row;
+    uint32_t table_col, prefix_col;
+    int32_t requests;
+    int32_t own_most, prefix_most;   // tokens that a table row covers
     IndexRef rows, lengths, query_starts, prefix_lengths, group_starts;
     int32_t table64, prefix64;
     int32_t tokens, batch, groups;
@@ -63,21 +65,17 @@ enum PhaseMode : int32_t {
 struct Phase {
     PhaseMode mode;
     int32_t sequences;
-    int32_t row_tile, key_tile;
-    int32_t workgroups;           // the most that take part
-    int32_t direct;               // an item that one workgroup has whole is written to the output
-    float* parts;                 // slots of row_tile x dim_pad values, then row_tile largest scores and sums
+    int32_t row_shift, unit_shift;   // row_tile and unit as powers of two
+    int32_t workgroups;              // the most that take part
+    int32_t direct;                  // an item that one workgroup has whole is written to the output
     int32_t dim_pad;
-    int64_t slots;
-    int64_t* tile_starts;         // [sequences + 1] of the line, written for the merge
-    int32_t* item_starts;         // [sequences + 1]
+    int32_t slots;
+    float* parts;                    // slots of row_tile x dim_pad values, then row_tile largest scores and sums
+    uint32_t* unit_starts;           // [sequences + 1] of the line, written for the merge
+    uint32_t* item_starts;           // [sequences + 1]
 };
 
-constexpr int kAttentionThreads = 256;
-constexpr int kAttentionWaves = kAttentionThreads / 64;
-constexpr int kSeqPer = 4;
-constexpr int kSeqChunk = kAttentionThreads * kSeqPer;   // sequences whose sums a workgroup holds at a time
-constexpr int kFewestTiles = 4;                          // a workgroup takes no fewer key tiles: one a wave
+constexpr int kSeqChunk = 1024;      // sequences whose sums a workgroup holds at a time
 constexpr float kLn2 = 0.6931471805599453f;
 
 #if defined(__HIPCC__)
@@ -85,7 +83,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct Sequence {
     int32_t first, count;       // query tokens
     int32_t prefix, own;        // keys of each kind
-    int64_t length;             // own tokens as given (the last query token's position is length - 1)
+    int32_t newest;             // position of the last query token among the own tokens
     int32_t group, request;     // table rows (-1: none)
 };
 
@@ -102,7 +100,7 @@ __device__ __forceinline__ int32_t first_row(const AttentionArgs& a, int32_t g) 
 }
 
 __device__ __forceinline__ int32_t prefix_keys(const AttentionArgs& a, int32_t g) {
-    return clamped(a.prefix_lengths.fetch(g), 0, a.prefix_columns * a.cache.page.divisor);
+    return clamped(a.prefix_lengths.fetch(g), 0, a.prefix_most);
 }
 
 // The group that batch row b belongs to, or -1: the last whose first row is not past b, if it reaches b.
@@ -126,8 +124,8 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, PhaseMod
     Sequence q{};
     if (mode == kSlots) {
         q.first = s, q.count = 1;
-        q.own = static_cast<int32_t>(a.columns);
-        q.length = a.columns;
+        q.own = a.own_most;
+        q.newest = a.own_most;
         q.group = -1, q.request = s;
     } else if (mode == kPrefixes) {
         const int32_t begin = first_row(a, s), end = first_row(a, s + 1);
@@ -138,100 +136,95 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, PhaseMod
     } else {
         q.first = first_token(a, s);
         q.count = a.query_starts.data != nullptr ? max(first_token(a, s + 1) - q.first, 0) : 1;
-        q.length = a.lengths.fetch(s);
+        const int64_t length = a.lengths.fetch(s);
         const int64_t request = a.rows.data != nullptr ? a.rows.fetch(s) : s;
         q.request = request >= 0 && request < a.requests ? static_cast<int32_t>(request) : -1;
-        q.own = q.request >= 0 ? clamped(q.length, 0, a.columns * a.cache.page.divisor) : 0;
+        q.own = q.request >= 0 ? clamped(length, 0, a.own_most) : 0;
+        q.newest = clamped(length - 1, -1, 0x7ffffffe);
         q.group = mode == kWhole ? group_of(a, s) : -1;
         q.prefix = q.group >= 0 ? prefix_keys(a, q.group) : 0;
     }
     return q;
 }
 
-// Key tiles of a row tile: at least one, so that every row of a sequence is somebody's work.
-__device__ __forceinline__ int32_t tiles_of(const Sequence& q, const Phase& p) {
-    const int32_t k = p.key_tile;
-    return max((q.prefix + k - 1) / k + (q.own + k - 1) / k, 1);
+// Key units of a row tile: the prefix's, then the own tokens'. At least one, so that every row is somebody's work.
+__device__ __forceinline__ int32_t prefix_units(const Sequence& q, const Phase& p) {
+    return (q.prefix + (1 << p.unit_shift) - 1) >> p.unit_shift;
+}
+
+__device__ __forceinline__ int32_t units_of(const Sequence& q, const Phase& p) {
+    return max(prefix_units(q, p) + ((q.own + (1 << p.unit_shift) - 1) >> p.unit_shift), 1);
 }
 
 __device__ __forceinline__ int32_t row_tiles_of(const AttentionArgs& a, const Sequence& q, const Phase& p) {
-    return (q.count * a.share + p.row_tile - 1) / p.row_tile;
+    return (q.count * a.share + (1 << p.row_shift) - 1) >> p.row_shift;
 }
 
-// How many workgroups take part in a line of `total` key tiles, and the place where workgroup w begins.
-__device__ __forceinline__ int32_t active_workgroups(const Phase& p, int64_t total) {
-    return clamped(total / kFewestTiles, 1, p.workgroups);
+// Places of the line per workgroup.
+__device__ __forceinline__ uint32_t quota_of(const Phase& p, uint32_t total) {
+    return max((total + p.workgroups - 1) / p.workgroups, 1u);
 }
 
-__device__ __forceinline__ int64_t line_begin(int64_t total, int32_t w, int32_t active) {
-    return total * w / active;
+// How many own tokens a row of query token i (of the sequence's count) sees.
+__device__ __forceinline__ int32_t seen_by(const Sequence& q, int32_t i) {
+    return min(max(q.newest - q.count + i + 2, 0), q.own);
 }
 
-// The workgroup that has place t: the last w with total * w / active <= t.
-__device__ __forceinline__ int32_t line_owner(int64_t total, int64_t t, int32_t active) {
-    return static_cast<int32_t>(((t + 1) * active - 1) / total);
-}
-
+template <int kWaves>
 struct LineCells {
-    int64_t tiles[kSeqChunk + 1];     // first place of each sequence of the chunk
-    int32_t items[kSeqChunk + 1];
-    uint32_t sums[3][kAttentionWaves];
+    uint32_t units[kSeqChunk + 1];     // first place of each sequence of the chunk
+    uint32_t items[kSeqChunk + 1];
+    uint32_t sums[2][kWaves];
 };
 
 // The places and items of the sequences of one chunk, given what lies before it. All threads call it.
-__device__ __forceinline__ void line_chunk(const AttentionArgs& a, const Phase& p, int32_t chunk, int64_t tiles_before,
-                                           int32_t items_before, LineCells& cells) {
+template <int kWaves>
+__device__ __forceinline__ void line_chunk(const AttentionArgs& a, const Phase& p, int32_t chunk, uint32_t units_before,
+                                           uint32_t items_before, LineCells<kWaves>& cells) {
+    constexpr int kThreads = kWaves * 64;
     const int tid = threadIdx.x, wave = tid >> 6;
     const int32_t count = min(kSeqChunk, p.sequences - chunk);
-    int64_t tiles = 0;
-    uint32_t items = 0;
+    const int32_t per = (count + kThreads - 1) / kThreads;
+    const int32_t first = min(tid * per, count), last = min(first + per, count);
+    uint32_t units = 0, items = 0;
     __syncthreads();   // the cells' last use
 #pragma unroll 1
-    for (int k = 0; k < kSeqPer && tid * kSeqPer + k < count; ++k) {
-        const int at = tid * kSeqPer + k;
+    for (int32_t at = first; at < last; ++at) {
         const Sequence q = sequence_of(a, p.mode, chunk + at);
-        const int32_t mine = a.kv_heads * row_tiles_of(a, q, p);
-        cells.tiles[at] = static_cast<int64_t>(mine) * tiles_of(q, p);
+        const uint32_t mine = a.kv_heads * row_tiles_of(a, q, p);
+        cells.units[at] = mine * units_of(q, p);
         cells.items[at] = mine;
-        tiles += cells.tiles[at];
+        units += cells.units[at];
         items += mine;
     }
-    // A thread's tiles stay below 2^40; 20 bits of them at a time keep the sums of 256 threads in 32 bits.
-    const uint32_t low = static_cast<uint32_t>(tiles) & 0xfffffu;
-    const uint32_t high = static_cast<uint32_t>(tiles >> 20);
-    const uint32_t low_sum = wave_scan<kAdd>(low), high_sum = wave_scan<kAdd>(high), item_sum = wave_scan<kAdd>(items);
+    const uint32_t unit_sum = wave_scan<kAdd>(units), item_sum = wave_scan<kAdd>(items);
     if ((tid & 63) == 63) {
-        cells.sums[0][wave] = low_sum, cells.sums[1][wave] = high_sum, cells.sums[2][wave] = item_sum;
+        cells.sums[0][wave] = unit_sum, cells.sums[1][wave] = item_sum;
     }
     __syncthreads();
-    int64_t tile_at = tiles_before + static_cast<int64_t>(low_sum - low) + (static_cast<int64_t>(high_sum - high) << 20);
-    int32_t item_at = items_before + static_cast<int32_t>(item_sum - items);
+    uint32_t unit_at = units_before + unit_sum - units, item_at = items_before + item_sum - items;
 #pragma unroll
-    for (int w = 0; w < kAttentionWaves - 1; ++w) {
-        if (w < wave) {
-            tile_at += static_cast<int64_t>(cells.sums[0][w]) + (static_cast<int64_t>(cells.sums[1][w]) << 20);
-            item_at += static_cast<int32_t>(cells.sums[2][w]);
-        }
+    for (int w = 0; w < kWaves - 1; ++w) {
+        unit_at += w < wave ? cells.sums[0][w] : 0;
+        item_at += w < wave ? cells.sums[1][w] : 0;
     }
-    const bool publish = blockIdx.x == 0 && p.tile_starts != nullptr;
+    const bool publish = blockIdx.x == 0 && p.unit_starts != nullptr;
 #pragma unroll 1
-    for (int k = 0; k < kSeqPer && tid * kSeqPer + k < count; ++k) {
-        const int at = tid * kSeqPer + k;
-        const int64_t mine = cells.tiles[at];
-        const int32_t my_items = cells.items[at];
-        cells.tiles[at] = tile_at;
+    for (int32_t at = first; at < last; ++at) {
+        const uint32_t my_units = cells.units[at], my_items = cells.items[at];
+        cells.units[at] = unit_at;
         cells.items[at] = item_at;
         if (publish) {
-            p.tile_starts[chunk + at] = tile_at;
+            p.unit_starts[chunk + at] = unit_at;
             p.item_starts[chunk + at] = item_at;
         }
-        tile_at += mine;
+        unit_at += my_units;
         item_at += my_items;
         if (at == count - 1) {
-            cells.tiles[count] = tile_at;
+            cells.units[count] = unit_at;
             cells.items[count] = item_at;
             if (publish && chunk + count == p.sequences) {
-                p.tile_starts[p.sequences] = tile_at;
+                p.unit_starts[p.sequences] = unit_at;
                 p.item_starts[p.sequences] = item_at;
             }
         }
@@ -239,90 +232,84 @@ __device__ __forceinline__ void line_chunk(const AttentionArgs& a, const Phase& 
     __syncthreads();
 }
 
-// What a workgroup does next: key tiles [begin, end) of one item.
+// What a workgroup does next: key units [begin, end) of the `units` of one item.
 struct Segment {
     Sequence q;
     int32_t head, row_begin, rows;      // KV head; first row of the tile; rows of the whole sequence
-    int32_t begin, end, tiles;
+    int32_t begin, end, units;
     int32_t slot;
 };
 
 // Calls body(segment) for every segment of this workgroup, in order; all threads take part.
-template <typename Body>
-__device__ __forceinline__ void for_segments(const AttentionArgs& a, const Phase& p, LineCells& cells, Body&& body) {
-    const int32_t w = blockIdx.x;
+template <int kWaves, typename Body>
+__device__ __forceinline__ void for_segments(const AttentionArgs& a, const Phase& p, LineCells<kWaves>& cells,
+                                             Body&& body) {
+    const uint32_t w = blockIdx.x;
     const bool alike = p.mode == kSlots;   // every sequence is as long: places are divided, not searched
-    int64_t total = 0;
-    int32_t alike_items = 0, alike_tiles = 1;
+    uint32_t total = 0, alike_items = 0, alike_units = 1;
     if (alike) {
         const Sequence any = sequence_of(a, kSlots, 0);
-        alike_tiles = tiles_of(any, p);
+        alike_units = units_of(any, p);
         alike_items = a.kv_heads * row_tiles_of(a, any, p);
-        total = static_cast<int64_t>(p.sequences) * alike_items * alike_tiles;
+        total = p.sequences * alike_items * alike_units;
     } else {
-        int32_t items = 0;
+        uint32_t items = 0;
         for (int32_t chunk = 0; chunk < p.sequences; chunk += kSeqChunk) {
             line_chunk(a, p, chunk, total, items, cells);
             const int32_t count = min(kSeqChunk, p.sequences - chunk);
-            total = cells.tiles[count];
+            total = cells.units[count];
             items = cells.items[count];
         }
+        total = __builtin_amdgcn_readfirstlane(total);
     }
-    const int32_t active = active_workgroups(p, total);
-    if (total == 0 || w >= active) {
+    const uint32_t quota = quota_of(p, total);
+    uint32_t at = w * quota;
+    const uint32_t end = min(at + quota, total);
+    if (at >= end) {
         return;
     }
-    int64_t at = line_begin(total, w, active);
-    const int64_t end = line_begin(total, w + 1, active);
     int32_t chunk = 0, count = min(kSeqChunk, p.sequences);
     if (!alike && p.sequences > kSeqChunk) {
         line_chunk(a, p, 0, 0, 0, cells);
     }
+#pragma unroll 1
     while (at < end) {
-        int32_t s, item, before = 0;      // sequence, item within it, items before it
-        int64_t local;
+        int32_t s;
+        uint32_t local, before;           // place within the sequence; items before it
         if (alike) {
-            const int64_t place = at / alike_tiles;
-            s = static_cast<int32_t>(place / alike_items);
-            item = static_cast<int32_t>(place % alike_items);
+            s = at / (alike_items * alike_units);
+            local = at - s * (alike_items * alike_units);
             before = s * alike_items;
-            local = at - place * alike_tiles;
         } else {
-            while (cells.tiles[count] <= at) {
-                const int64_t tiles_before = cells.tiles[count];
-                const int32_t items_before = cells.items[count];
+            while (cells.units[count] <= at) {
+                const uint32_t units_before = cells.units[count], items_before = cells.items[count];
                 chunk += kSeqChunk;
                 count = min(kSeqChunk, p.sequences - chunk);
-                line_chunk(a, p, chunk, tiles_before, items_before, cells);
+                line_chunk(a, p, chunk, units_before, items_before, cells);
             }
             int32_t low = 0, high = count;
             while (high - low > 1) {
                 const int32_t mid = (low + high) >> 1;
-                if (cells.tiles[mid] <= at) {
+                if (cells.units[mid] <= at) {
                     low = mid;
                 } else {
                     high = mid;
                 }
             }
-            low = __builtin_amdgcn_readfirstlane(low);
-            s = chunk + low;
-            before = cells.items[low];
-            local = at - cells.tiles[low];
-            item = 0;
+            s = __builtin_amdgcn_readfirstlane(chunk + low);
+            local = __builtin_amdgcn_readfirstlane(at - cells.units[low]);
+            before = __builtin_amdgcn_readfirstlane(cells.items[low]);
         }
         Segment g;
         g.q = sequence_of(a, p.mode, s);
-        g.tiles = tiles_of(g.q, p);
-        if (!alike) {
-            item = static_cast<int32_t>(local / g.tiles);
-            local -= static_cast<int64_t>(item) * g.tiles;
-        }
-        const int32_t row_tiles = row_tiles_of(a, g.q, p);
+        g.units = units_of(g.q, p);
+        const uint32_t item = local / g.units;
+        const uint32_t row_tiles = row_tiles_of(a, g.q, p);
         g.head = item / row_tiles;
-        g.row_begin = item % row_tiles * p.row_tile;
+        g.row_begin = (item - g.head * row_tiles) << p.row_shift;
         g.rows = g.q.count * a.share;
-        g.begin = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(local));
-        g.end = static_cast<int32_t>(min(static_cast<int64_t>(g.tiles), g.begin + (end - at)));
+        g.begin = local - item * g.units;
+        g.end = min(static_cast<uint32_t>(g.units), g.begin + (end - at));
         g.slot = w + before + item;
         body(g);
         at += g.end - g.begin;
@@ -331,7 +318,8 @@ __device__ __forceinline__ void for_segments(const AttentionArgs& a, const Phase
 
 #endif
 
-// The launches of attention_narrow.hip and attention.hip's merge; the row tiles are 16 * tiles16.
+// attention_narrow.hip: row tiles of 16 * tiles16 rows, units of at least narrow_unit_shift's size.
+int narrow_unit_shift(int tiles16, int32_t dim_pad);
 void launch_narrow(const AttentionArgs& a, const Phase& p, int32_t dtype, int tiles16, void* stream);
 
 }  // namespace ekv
