@@ -293,9 +293,16 @@ struct Plan {
 
 int32_t padded_dim(int64_t dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : (dim <= 128 ? 128 : 256)); }
 
-// 16-row tiles that hold `rows` rows, as far as the kernel's registers go.
+// 16-row tiles that hold `rows` rows: 1, 2 or 4 of the kernel for few rows (2 at most at 256 columns, whose registers
+// hold no more), 8 or 16 of the one for many.
 int tiles_for(int64_t rows, int32_t dim_pad) {
-    return rows <= 16 ? 1 : (rows <= 32 || dim_pad > 128 ? 2 : 4);
+    if (rows <= 32) {
+        return rows <= 16 ? 1 : 2;
+    }
+    if (rows <= 64 && dim_pad <= 128) {
+        return 4;
+    }
+    return rows <= 128 ? 8 : 16;
 }
 
 // A phase's cut and its place in the workspace.
@@ -303,10 +310,13 @@ void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, i
          int64_t kv_heads, int32_t dim_pad, bool direct) {
     p.mode = mode;
     p.sequences = static_cast<int32_t>(sequences);
-    p.row_shift = tiles16 == 1 ? 4 : (tiles16 == 2 ? 5 : 6);
-    p.unit_shift = narrow_unit_shift(tiles16, dim_pad);
+    p.row_shift = 4;
+    while ((1 << p.row_shift) < 16 * tiles16) {
+        ++p.row_shift;
+    }
+    p.unit_shift = tiles16 < 8 ? narrow_unit_shift(tiles16, dim_pad) : 6;
     p.dim_pad = dim_pad;
-    p.workgroups = kComputeUnits;
+    p.workgroups = kComputeUnits * (tiles16 == 8 && dim_pad <= 128 ? 2 : 1);
     p.direct = direct;
     // Row tiles of all sequences: every sequence's last may be part-filled.
     const int64_t items = kv_heads * ((tokens * share >> p.row_shift) + std::min(sequences, tokens));
@@ -388,6 +398,14 @@ void place(Phase& p, void* workspace) {
     }
 }
 
+void launch_phase(const AttentionArgs& a, const Phase& p, int32_t dtype, int tiles16, void* stream) {
+    if (tiles16 < 8) {
+        launch_narrow(a, p, dtype, tiles16, stream);
+    } else {
+        launch_wide(a, p, dtype, stream);
+    }
+}
+
 int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, uint64_t bytes, void* stream) {
     if (bytes < plan.bytes) {
         throw std::invalid_argument("the attention needs " + std::to_string(plan.bytes) + " workspace bytes, got " +
@@ -404,9 +422,9 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
     if (plan.prefix_tiles16 != 0) {
         place(plan.prefix, workspace);
         fit_units(plan.prefix, a.prefix_most);
-        launch_narrow(a, plan.prefix, dtype, plan.prefix_tiles16, stream);
+        launch_phase(a, plan.prefix, dtype, plan.prefix_tiles16, stream);
     }
-    launch_narrow(a, plan.own, dtype, plan.tiles16, stream);
+    launch_phase(a, plan.own, dtype, plan.tiles16, stream);
     const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.kv_heads));
     if (dtype == EKV_BFLOAT16) {
         merge_kernel<Bf16><<<grid, kMergeThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);

@@ -28,8 +28,9 @@ struct Rows {
     // LDS bytes of a V row, a power of two so that its 16-byte pieces can be permuted by exclusive or.
     static constexpr int kBytes = kDim <= 64 ? 128 : (kDim <= 128 ? 256 : 512);
     static __device__ __forceinline__ int place(int key, int piece) {
-        // Rows are permuted so that 16 lanes with 16 keys and one piece meet 16 different 16-byte columns.
-        const int swap = kBytes == 128 ? (key >> 1) & 7 : key & 15;
+        // The pieces of a row are permuted so that 16 lanes with 16 keys and one piece (the write) and the eight rows of
+        // 32 bytes that a transposed read takes at a time each meet every bank once.
+        const int swap = kBytes == 128 ? (((key >> 1) & 3) << 1) | ((key >> 3) & 1) : ((key & 7) << 1) | ((key >> 3) & 1);
         return key * kBytes + ((piece ^ swap) << 4);
     }
 };

@@ -322,4 +322,7 @@ __device__ __forceinline__ void for_segments(const AttentionArgs& a, const Phase
 int narrow_unit_shift(int tiles16, int32_t dim_pad);
 void launch_narrow(const AttentionArgs& a, const Phase& p, int32_t dtype, int tiles16, void* stream);
 
+// attention_wide.hip: row tiles of 128 (row_shift 7) or 256 rows, units of at least 64 keys.
+void launch_wide(const AttentionArgs& a, const Phase& p, int32_t dtype, void* stream);
+
 }  // namespace ekv
