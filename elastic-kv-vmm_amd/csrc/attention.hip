@@ -278,7 +278,9 @@ AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, i
         a.lse = static_cast<float*>(lse.data);
         a.l_token = lse.stride[0], a.l_head = lse.stride[1];
     }
-    a.scale = static_cast<float>(scale * 1.4426950408889634);   // log2 e: the kernels' exponentials have base two
+    // Log2 e: the kernels' exponentials have base two. A negative scale changes the queries' signs.
+    a.scale = static_cast<float>(std::fabs(scale) * 1.4426950408889634);
+    a.flip = scale < 0 ? 0x80008000u : 0;
     return a;
 }
 
@@ -293,8 +295,8 @@ struct Plan {
 
 int32_t padded_dim(int64_t dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : (dim <= 128 ? 128 : 256)); }
 
-// 16-row tiles that hold `rows` rows: 1, 2 or 4 of the kernel for few rows (2 at most at 256 columns, whose registers
-// hold no more), 8 or 16 of the one for many.
+// 16-row tiles that hold `rows` rows: 1, 2 or 4 of the kernel for few rows, 8 or 16 of the one for many (2 and 8 at most
+// at 256 columns, where the registers hold no more).
 int tiles_for(int64_t rows, int32_t dim_pad) {
     if (rows <= 32) {
         return rows <= 16 ? 1 : 2;
@@ -302,7 +304,7 @@ int tiles_for(int64_t rows, int32_t dim_pad) {
     if (rows <= 64 && dim_pad <= 128) {
         return 4;
     }
-    return rows <= 128 ? 8 : 16;
+    return rows <= 128 || dim_pad > 128 ? 8 : 16;
 }
 
 // A phase's cut and its place in the workspace.

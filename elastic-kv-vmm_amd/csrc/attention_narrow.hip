@@ -92,6 +92,7 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
     char* const values = s_data + wave * (kKeys * Rows<kDim>::kBytes);
     const char* const zeros = reinterpret_cast<const char*>(zero_row);
     const int pieces = a.dim >> 3;
+    const float slack = kSlack / fmaxf(a.scale, 1e-30f);     // in raw scores
 
     for_segments(a, p, s_line, [&](const Segment& g) {
         // Query rows: row col of each 16, elements 32 c + 8 quad .. + 7.
@@ -107,6 +108,7 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
                 const int piece = c * 4 + quad;
                 const bool live = row < g.rows && (c < kWholeSteps || piece < pieces);
                 q[m][c] = *reinterpret_cast<const words4*>(live ? at + piece * 16 : zeros);
+                q[m][c] ^= a.flip;
             }
             visible[m] = seen_by(g.q, token);
         }
@@ -242,7 +244,7 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
                     float x[8], most = -INFINITY;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        x[j] = s[m][j >> 2][j & 3] * a.scale;
+                        x[j] = s[m][j >> 2][j & 3];
                     }
                     if (ragged || now != 0xffffffffu) {
                         const int32_t left = own ? visible[m] - base : kKeys;
@@ -256,21 +258,24 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
                     for (int j = 0; j < 8; ++j) {
                         most = fmaxf(most, x[j]);
                     }
-                    most = fmaxf(top[m], over_groups_max(most));
-                    const float safe = most == -INFINITY ? 0.0f : most;
-                    if (__ballot(most > top[m]) != 0) {
-                        const float keep = __builtin_amdgcn_exp2f(top[m] - safe);
+                    most = over_groups_max(most);
+                    // The reference score follows the largest only when that has passed it by 2^kSlack: until then the
+                    // weights are larger than 1, which their type holds, and nothing has to be scaled again.
+                    if (__ballot(most > top[m] + slack) != 0) {
+                        const float to = fmaxf(top[m], most);
+                        const float keep = to == top[m] ? 1.0f : __builtin_amdgcn_exp2f((top[m] - to) * a.scale);
                         sum[m] *= keep;
 #pragma unroll
                         for (int c = 0; c < kCols; ++c) {
                             o[m][c] *= keep;
                         }
-                        top[m] = most;
+                        top[m] = to;
                     }
+                    const float shift = (top[m] == -INFINITY ? 0.0f : top[m] * a.scale) - T::kShift;
                     float w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        w[j] = __builtin_amdgcn_exp2f(x[j] - safe + T::kShift);
+                        w[j] = __builtin_amdgcn_exp2f(x[j] * a.scale - shift);
                         sum[m] += w[j];
                     }
                     weights[m] =
@@ -283,36 +288,34 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
                     const words2 high = read_transposed(values + Rows<kDim>::place(16 + key, piece) + half);
                     return words4{low[0], low[1], high[0], high[1]};
                 };
-                if (!spoiled) {
-#pragma unroll
-                    for (int c = 0; c < kCols; ++c) {
-                        const words4 column_c = column(c);
-#pragma unroll
-                        for (int m = 0; m < kTiles; ++m) {
-                            o[m][c] = T::mfma16(column_c, weights[m], o[m][c]);
-                        }
-                    }
-                } else {
-                    // One query token at a time: its rows take the product with the values that it sees.
-                    const int32_t last = min(g.row_begin + 16 * kTiles, g.rows) - 1;
+                if (spoiled) {
+                    // A key that only some rows see has weight 0 for the others, and 0 * infinity is not 0: the infinities
+                    // and NaN are added to the rows that see them (a weight is positive), then cleared.
 #pragma unroll 1
-                    for (int32_t token = g.row_begin / a.share; token <= last / a.share; ++token) {
-                        const int32_t left = seen_by(g.q, token) - base;
+                    for (int key = 0; key < kKeys; ++key) {
 #pragma unroll
                         for (int c = 0; c < kCols; ++c) {
-                            words4 column_c = column(c);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int key = (j >> 2) * 16 + quad * 4 + (j & 3);
-                                column_c[j >> 1] &= key < left ? 0xffffffffu : ((j & 1) != 0 ? 0x0000ffffu : 0xffff0000u);
-                            }
+                            words2* const at = reinterpret_cast<words2*>(
+                                values + Rows<kDim>::place(key, c * 2 + (quad >> 1)) + (quad & 1) * 8);
+                            const words2 x = *at;
 #pragma unroll
                             for (int m = 0; m < kTiles; ++m) {
-                                const f32x4 x = T::mfma16(column_c, weights[m], o[m][c]);
-                                const int32_t row = g.row_begin + m * 16 + col;
-                                o[m][c] = static_cast<int32_t>(a.share_div.div(row)) == token ? x : o[m][c];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    o[m][c][e] +=
+                                        key < visible[m] - base ? T::unbounded(x[e >> 1] >> (16 * (e & 1))) : 0.0f;
+                                }
                             }
+                            *at = words2{bounded<T>(x[0]), bounded<T>(x[1])};
                         }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    const words4 column_c = column(c);
+#pragma unroll
+                    for (int m = 0; m < kTiles; ++m) {
+                        o[m][c] = T::mfma16(column_c, weights[m], o[m][c]);
                     }
                 }
             }
@@ -323,6 +326,7 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) {
             sum[m] = over_groups_sum(sum[m]);
+            top[m] = top[m] == -INFINITY ? top[m] : top[m] * a.scale;
             if (quad == 0) {
                 s_max[wave][m * 16 + col] = top[m];
                 s_sum[wave][m * 16 + col] = sum[m];

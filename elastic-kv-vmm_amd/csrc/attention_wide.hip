@@ -27,6 +27,7 @@ struct Tile {
     static constexpr int kSize = kTile * kBytes;
     // The 16-byte pieces of a row are permuted by exclusive or so that 16 lanes with 16 keys and one piece (K) and the
     // four rows of 64 bytes that a transposed read takes at a time (V) each meet every bank once.
+    // The permutation depends on key % 16 alone, so other keys and pieces are offsets and exclusive ors of one address.
     static __device__ __forceinline__ int place(int key, int piece) {
         const int swap = kBytes == 128 ? (((key >> 1) & 1) << 2) | ((key >> 2) & 3) : ((key & 3) << 2) | ((key >> 2) & 3);
         return key * kBytes + ((piece ^ swap) << 4);
@@ -51,13 +52,23 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
     constexpr int kKeysAtOnce = kWaves * 64 / kRowThreads;
     constexpr int kLoads = kTile / kKeysAtOnce;    // 16-byte pieces of K, and of V, that a thread loads a tile
     static_assert(kLoads >= 1, "a tile has at least one piece for every thread");
-    __shared__ __align__(16) char s_data[2][2][Tile<kDim>::kSize];     // [buffer][K, V]
+    static_assert(kKeysAtOnce % 8 == 0, "8 keys on, a row's permutation differs by 2");
+    constexpr int kBytes = Tile<kDim>::kBytes;
+    __shared__ __align__(16) char s_data[4 * Tile<kDim>::kSize];       // two buffers of K and V
     __shared__ LineCells<kWaves> s_line;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(tid >> 6));
     const int load_key = tid / kRowThreads, load_piece = tid % kRowThreads;
+    const int write_at = Tile<kDim>::place(load_key, load_piece);
+    // K of key col, piece half; V^T of 16 keys and 32 columns: lane (half, 16-column piece, i) names row 4 half + i / 4
+    // (and + 8), the (i % 4)-th 8 bytes of its 32.
+    const int read_k = Tile<kDim>::place(col, half);
+    const int v_key = half * 4 + ((lane & 15) >> 2), v_piece = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    const int read_v = Tile<kDim>::kSize + Tile<kDim>::place(v_key, v_piece) + (lane & 1) * 8;
+    const int read_v8 = Tile<kDim>::kSize + Tile<kDim>::place(v_key + 8, v_piece) + (lane & 1) * 8;
     const char* const zeros = reinterpret_cast<const char*>(zero_row);
     const int pieces = a.dim >> 3;
+    const float slack = kSlack / fmaxf(a.scale, 1e-30f);     // in raw scores
 
     for_segments(a, p, s_line, [&](const Segment& g) {
         const int32_t row = g.row_begin + wave * 32 + col;     // the lane's query row
@@ -69,6 +80,7 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
             for (int c = 0; c < kSteps; ++c) {
                 const int piece = c * 2 + half;
                 q[c] = *reinterpret_cast<const words4*>(row < g.rows && piece < pieces ? at + piece * 16 : zeros);
+                q[c] ^= a.flip;
             }
         }
         const int32_t visible = seen_by(g.q, token);
@@ -133,12 +145,22 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
             const auto store = [&](int buffer) {
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const int at = Tile<kDim>::place(i * kKeysAtOnce + load_key, load_piece);
+                    char* const to = s_data + buffer + i * kKeysAtOnce * kBytes + (write_at ^ ((i * kKeysAtOnce & 8) << 2));
                     // K past the head size meets zeros of q and must not be an infinity; V's columns are not stored.
                     const words4 kept = load_piece < pieces ? k[i] : words4{0, 0, 0, 0};
-                    *reinterpret_cast<words4*>(&s_data[buffer][0][at]) = kept;
-                    *reinterpret_cast<words4*>(&s_data[buffer][1][at]) = v[i];
+                    *reinterpret_cast<words4*>(to) = kept;
+                    *reinterpret_cast<words4*>(to + Tile<kDim>::kSize) = v[i];
                 }
+            };
+
+            const auto any_not_finite = [&](const char* tile, int first) {
+                bool found = false;
+#pragma unroll 1
+                for (int at = first * 16; at < Tile<kDim>::kSize; at += 64 * 16) {
+                    const words4 x = *reinterpret_cast<const words4*>(tile + Tile<kDim>::kSize + at);
+                    found |= not_finite<T>(x[0]) || not_finite<T>(x[1]) || not_finite<T>(x[2]) || not_finite<T>(x[3]);
+                }
+                return __ballot(found) != 0;
             };
 
             int32_t base = from << p.unit_shift;
@@ -151,14 +173,13 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
             __syncthreads();
             int buffer = 0;
 #pragma unroll 1
-            for (; base < keys; base += kTile, buffer ^= 1) {
-                store(buffer ^ 1);
+            for (; base < keys; base += kTile, buffer ^= 2 * Tile<kDim>::kSize) {
+                store(buffer ^ (2 * Tile<kDim>::kSize));
                 const uint64_t seen = now;
                 now = next;
                 next = fetch(base + 2 * kTile, ids);
                 ids = ids_of(base + 3 * kTile);
-                const char* const k_tile = s_data[buffer][0];
-                const char* const v_tile = s_data[buffer][1];
+                const char* const tile = s_data + buffer;
                 f32x16 s[2];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -168,14 +189,12 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
                     }
 #pragma unroll
                     for (int c = 0; c < kSteps; ++c) {
-                        const words4 x =
-                            *reinterpret_cast<const words4*>(k_tile + Tile<kDim>::place(b * 32 + col, c * 2 + half));
+                        const words4 x = *reinterpret_cast<const words4*>(tile + (read_k ^ (c << 5)) + b * 32 * kBytes);
                         s[b] = T::mfma32(x, q[c], s[b]);
                     }
                 }
                 // Whether some row sees fewer keys of this tile than it holds.
                 const bool ragged = own && base + kTile > first_visible;
-                float most = -INFINITY;
                 if (ragged || seen != ~uint64_t{0}) {
                     const int32_t left = own ? visible - base : kTile;
 #pragma unroll
@@ -184,15 +203,11 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int key = half * 4 + (i & 3) + 8 * (i >> 2);
-                            s[b][i] = ((bits >> key) & 1) != 0 && b * 32 + key < left ? s[b][i] * a.scale : -INFINITY;
+                            s[b][i] = ((bits >> key) & 1) != 0 && b * 32 + key < left ? s[b][i] : -INFINITY;
                         }
                     }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        s[b] *= a.scale;
-                    }
                 }
+                float most = -INFINITY;
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -200,80 +215,72 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
                         most = fmaxf(most, s[b][i]);
                     }
                 }
-                most = fmaxf(top, over_halves_max(most));
-                const float safe = most == -INFINITY ? 0.0f : most;
-                if (__ballot(most > top) != 0) {
-                    const float keep = __builtin_amdgcn_exp2f(top - safe);
+                most = over_halves_max(most);
+                // The reference score follows the largest only when that has passed it by 2^kSlack: until then the
+                // weights are larger than 1, which their type holds, and nothing has to be scaled again.
+                if (__ballot(most > top + slack) != 0) {
+                    const float to_top = fmaxf(top, most);
+                    const float keep = to_top == top ? 1.0f : __builtin_amdgcn_exp2f((top - to_top) * a.scale);
                     sum *= keep;
 #pragma unroll
                     for (int c = 0; c < kCols; ++c) {
                         o[c] *= keep;
                     }
-                    top = most;
+                    top = to_top;
                 }
-                const float shift = safe - T::kShift;
-                words4 weights[4];                    // 16 keys each
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                const float shift = (top == -INFINITY ? 0.0f : top * a.scale) - T::kShift;
+                const auto weights_of = [&](int u) {
                     float w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        w[j] = __builtin_amdgcn_exp2f(s[u >> 1][(u & 1) * 8 + j] - shift);
+                        w[j] = __builtin_amdgcn_exp2f(s[u >> 1][(u & 1) * 8 + j] * a.scale - shift);
                         sum += w[j];
                     }
-                    weights[u] =
-                        words4{T::pack(w[0], w[1]), T::pack(w[2], w[3]), T::pack(w[4], w[5]), T::pack(w[6], w[7])};
-                }
-                // V^T of 16 keys and 32 columns: lane (half, 16-column piece, i) names row 4 half + i / 4 (+ 8).
+                    return words4{T::pack(w[0], w[1]), T::pack(w[2], w[3]), T::pack(w[4], w[5]), T::pack(w[6], w[7])};
+                };
                 const auto column = [&](int u, int c) {
-                    const int i = lane & 15, key = u * 16 + half * 4 + (i >> 2);
-                    const int piece = c * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1), byte = (i & 1) * 8;
-                    const words2 low = read_transposed(v_tile + Tile<kDim>::place(key, piece) + byte);
-                    const words2 high = read_transposed(v_tile + Tile<kDim>::place(key + 8, piece) + byte);
+                    const words2 low = read_transposed(tile + (read_v ^ (c << 6)) + u * 16 * kBytes);
+                    const words2 high = read_transposed(tile + (read_v8 ^ (c << 6)) + u * 16 * kBytes);
                     return words4{low[0], low[1], high[0], high[1]};
                 };
-                bool spoiled = false;
-                if (ragged) {
-                    // A key that only some rows see has weight 0 for the others, and 0 * infinity is not 0.
+                if (ragged && any_not_finite(tile, lane)) {
+                    // A key that only some rows see has weight 0 for the others, and 0 * infinity is not 0: the infinities
+                    // and NaN are added to the rows that see them (a weight is positive), then cleared.
+                    const int32_t left = visible - base;
 #pragma unroll 1
-                    for (int at = lane * 16; at < Tile<kDim>::kSize; at += 64 * 16) {
-                        const words4 x = *reinterpret_cast<const words4*>(v_tile + at);
-                        spoiled |= not_finite<T>(x[0]) || not_finite<T>(x[1]) || not_finite<T>(x[2]) ||
-                                   not_finite<T>(x[3]);
-                    }
-                    spoiled = __ballot(spoiled) != 0;
-                }
-                if (!spoiled) {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
+                    for (int key = 0; key < kTile; ++key) {
 #pragma unroll
                         for (int c = 0; c < kCols; ++c) {
-                            o[c] = T::mfma32(column(u, c), weights[u], o[c]);
-                        }
-                    }
-                } else {
-                    // One query token at a time: its rows take the product with the values that it sees.
-                    const int32_t last = min(g.row_begin + wave * 32 + 32, g.rows) - 1;
-#pragma unroll 1
-                    for (int32_t t = (g.row_begin + wave * 32) / a.share; t <= last / a.share; ++t) {
-                        const int32_t left = seen_by(g.q, t) - base;
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
+                            for (int i = 0; i < 16; i += 4) {
+                                const words2 x = *reinterpret_cast<const words2*>(
+                                    tile + Tile<kDim>::kSize + Tile<kDim>::place(key, c * 4 + (i >> 2)) + half * 8);
 #pragma unroll
-                            for (int c = 0; c < kCols; ++c) {
-                                words4 x = column(u, c);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const int key = u * 16 + half * 4 + (j & 3) + 8 * (j >> 2);
-                                    x[j >> 1] &= key < left ? 0xffffffffu : ((j & 1) != 0 ? 0x0000ffffu : 0xffff0000u);
-                                }
-                                const f32x16 sums = T::mfma32(x, weights[u], o[c]);
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    o[c][i] = token == t ? sums[i] : o[c][i];
+                                for (int e = 0; e < 4; ++e) {
+                                    o[c][i + e] += key < left ? T::unbounded(x[e >> 1] >> (16 * (e & 1))) : 0.0f;
                                 }
                             }
                         }
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int at = tid * 16; at < Tile<kDim>::kSize; at += kWaves * 64 * 16) {
+                        words4* const to = reinterpret_cast<words4*>(s_data + buffer + Tile<kDim>::kSize + at);
+                        words4 x = *to;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[e] = bounded<T>(x[e]);
+                        }
+                        *to = x;
+                    }
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const words4 weights = weights_of(u);
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        o[c] = T::mfma32(column(u, c), weights, o[c]);
                     }
                 }
                 __syncthreads();
@@ -301,7 +308,7 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
                 }
                 if (half == 0 && a.lse != nullptr) {
                     a.lse[(g.q.first + token) * a.l_token + head * a.l_head] =
-                        sum == 0 ? -INFINITY : (top - T::kShift + log2f(sum)) * kLn2;
+                        sum == 0 ? -INFINITY : (top * a.scale - T::kShift + log2f(sum)) * kLn2;
                 }
             } else if (g.slot < p.slots) {
                 float* const part = p.parts + static_cast<int64_t>(g.slot) * kRows * (kDim + 2);
@@ -315,7 +322,7 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
                     }
                 }
                 if (half == 0) {
-                    part[kRows * kDim + inside] = top;
+                    part[kRows * kDim + inside] = top == -INFINITY ? top : top * a.scale;
                     part[kRows * kDim + kRows + inside] = sum;
                 }
             }
@@ -328,7 +335,7 @@ void launch_dim(const AttentionArgs& a, const Phase& p, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(p.workgroups));
     if (p.row_shift == 7) {
         wide_kernel<T, kDim, 4><<<grid, 256, 0, stream>>>(a, p);
-    } else {
+    } else if constexpr (kDim <= 128) {
         wide_kernel<T, kDim, 8><<<grid, 512, 0, stream>>>(a, p);
     }
     check_hip(hipGetLastError(), "launch attention");

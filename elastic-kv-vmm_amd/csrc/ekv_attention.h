@@ -51,7 +51,8 @@ struct AttentionArgs {
     int32_t tokens, batch, groups;
     int32_t heads, kv_heads, share, dim;   // share: query heads of a KV head
     FastDiv share_div;
-    float scale;                  // of the scores, times log2 e
+    float scale;                  // of the scores, times log2 e; not negative
+    uint32_t flip;                // the sign bits of two elements where the scale given was negative
 };
 
 enum PhaseMode : int32_t {
@@ -77,6 +78,7 @@ struct Phase {
 
 constexpr int kSeqChunk = 1024;      // sequences whose sums a workgroup holds at a time
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.0f;       // bits by which a weight may pass 1 before its row is scaled again
 
 #if defined(__HIPCC__)
 
