@@ -78,7 +78,7 @@ struct Ids {
 
 template <typename T, int kDim, int kTiles>
 __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kTiles>() / 4)) void narrow_kernel(
-    const AttentionArgs a, const Phase p) {
+    const Launch) {
     constexpr int kWaves = waves_of<kDim, kTiles>();
     constexpr int kSteps = kDim / 32;      // matrix steps of the first product
     constexpr int kCols = kDim / 16;       // 16-column pieces of the output
@@ -91,10 +91,11 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     char* const values = s_data + wave * (kKeys * Rows<kDim>::kBytes);
     const char* const zeros = reinterpret_cast<const char*>(zero_row);
-    const int pieces = a.dim >> 3;
-    const float slack = kSlack / fmaxf(a.scale, 1e-30f);     // in raw scores
 
-    for_segments(a, p, s_line, [&](const Segment& g) {
+    for_segments(s_line, [&](const Segment& g) {
+        const AttentionArgs& a = fresh().a;
+        const int pieces = a.dim >> 3;
+        const float slack = kSlack / fmaxf(a.scale, 1e-30f);     // in raw scores
         // Query rows: row col of each 16, elements 32 c + 8 quad .. + 7.
         words4 q[kTiles][kSteps];
         int32_t visible[kTiles];           // own keys that the lane's rows see
@@ -125,7 +126,8 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
             }
         }
 
-        const int32_t prefix_end = prefix_units(g.q, p);
+        const int32_t unit_shift = fresh().p.unit_shift;
+        const int32_t prefix_end = (g.q.prefix + (1 << unit_shift) - 1) >> unit_shift;
 #pragma unroll 1
         for (int side = 0; side < 2; ++side) {
             // Tiles [first, last) of this source; a wave takes every kWaves-th.
@@ -139,7 +141,7 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
             src.table = own ? a.tables + g.q.request * a.table_row : a.prefix_tables + g.q.group * a.prefix_row;
             src.step = own ? a.table_col : a.prefix_col;
             src.wide = (own ? a.table64 : a.prefix64) != 0 ? 4 : 0;
-            src.keys = min(own ? g.q.own : g.q.prefix, to << p.unit_shift);
+            src.keys = min(own ? g.q.own : g.q.prefix, to << unit_shift);
             const char* const k_head = a.cache.k + static_cast<uint64_t>(a.cache.head_stride) * g.head + quad * 16;
             const char* const v_head = k_head + a.cache.kv_stride;
 
@@ -183,7 +185,7 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
             };
 
             constexpr int kStride = kWaves * kKeys;
-            int32_t base = (from << p.unit_shift) + wave * kKeys;
+            int32_t base = (from << unit_shift) + wave * kKeys;
             Ids ids = ids_of(base);
             fetch(base, ids);
             ids = ids_of(base + kStride);
@@ -333,6 +335,9 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
             }
         }
         __syncthreads();
+        const Launch& last = fresh();
+        const AttentionArgs& z = last.a;
+        const Phase& p = last.p;
         const bool whole = p.direct != 0 && g.begin == 0 && g.end == g.units;
         const int32_t row_tile = 16 * kTiles;
         float* const part = p.parts + static_cast<int64_t>(g.slot) * row_tile * (kDim + 2);
@@ -364,9 +369,9 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
                         part[row_tile * kDim + m * 16 + col] = most;
                         part[row_tile * kDim + row_tile + m * 16 + col] = total;
                     }
-                } else if (a.lse != nullptr) {
-                    const int32_t token = a.share_div.div(row);
-                    a.lse[(g.q.first + token) * a.l_token + ((g.head - token) * a.share + row) * a.l_head] =
+                } else if (z.lse != nullptr) {
+                    const int32_t token = z.share_div.div(row);
+                    z.lse[(g.q.first + token) * z.l_token + ((g.head - token) * z.share + row) * z.l_head] =
                         total == 0 ? -INFINITY : (most - T::kShift + log2f(total)) * kLn2;
                 }
             }
@@ -389,9 +394,9 @@ __global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kT
                         if (room) {
                             *reinterpret_cast<f32x4*>(part + (m * 16 + col) * kDim + element) = x;
                         }
-                    } else if (element < a.dim) {
-                        const int32_t token = a.share_div.div(row), head = (g.head - token) * a.share + row;
-                        *reinterpret_cast<words2*>(a.out + (g.q.first + token) * a.o_token + head * a.o_head +
+                    } else if (element < z.dim) {
+                        const int32_t token = z.share_div.div(row), head = (g.head - token) * z.share + row;
+                        *reinterpret_cast<words2*>(z.out + (g.q.first + token) * z.o_token + head * z.o_head +
                                                    element * 2) = words2{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
                     }
                 }
@@ -405,11 +410,11 @@ template <typename T, int kDim>
 void launch_dim(const AttentionArgs& a, const Phase& p, int tiles16, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(p.workgroups));
     if (tiles16 == 1) {
-        narrow_kernel<T, kDim, 1><<<grid, waves_of<kDim, 1>() * 64, 0, stream>>>(a, p);
+        narrow_kernel<T, kDim, 1><<<grid, waves_of<kDim, 1>() * 64, 0, stream>>>(Launch{a, p});
     } else if (tiles16 == 2) {
-        narrow_kernel<T, kDim, 2><<<grid, waves_of<kDim, 2>() * 64, 0, stream>>>(a, p);
+        narrow_kernel<T, kDim, 2><<<grid, waves_of<kDim, 2>() * 64, 0, stream>>>(Launch{a, p});
     } else if constexpr (kDim <= 128) {
-        narrow_kernel<T, kDim, 4><<<grid, waves_of<kDim, 4>() * 64, 0, stream>>>(a, p);
+        narrow_kernel<T, kDim, 4><<<grid, waves_of<kDim, 4>() * 64, 0, stream>>>(Launch{a, p});
     }
     check_hip(hipGetLastError(), "launch attention");
 }

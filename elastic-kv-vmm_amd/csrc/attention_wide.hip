@@ -45,7 +45,7 @@ __device__ __forceinline__ float over_halves_sum(float x) {
 }
 
 template <typename T, int kDim, int kWaves>
-__global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(const AttentionArgs a, const Phase p) {
+__global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(const Launch) {
     constexpr int kSteps = kDim / 16;              // matrix steps of the first product
     constexpr int kCols = kDim / 32;               // 32-column pieces of the output
     constexpr int kRowThreads = Tile<kDim>::kBytes / 16;               // threads that load a key's row
@@ -67,10 +67,11 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
     const int read_v = Tile<kDim>::kSize + Tile<kDim>::place(v_key, v_piece) + (lane & 1) * 8;
     const int read_v8 = Tile<kDim>::kSize + Tile<kDim>::place(v_key + 8, v_piece) + (lane & 1) * 8;
     const char* const zeros = reinterpret_cast<const char*>(zero_row);
-    const int pieces = a.dim >> 3;
-    const float slack = kSlack / fmaxf(a.scale, 1e-30f);     // in raw scores
 
-    for_segments(a, p, s_line, [&](const Segment& g) {
+    for_segments(s_line, [&](const Segment& g) {
+        const AttentionArgs& a = fresh().a;
+        const int pieces = a.dim >> 3;
+        const float slack = kSlack / fmaxf(a.scale, 1e-30f);     // in raw scores
         const int32_t row = g.row_begin + wave * 32 + col;     // the lane's query row
         const int32_t token = a.share_div.div(row), head = (g.head - token) * a.share + row;
         words4 q[kSteps];
@@ -98,7 +99,8 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
             }
         }
 
-        const int32_t prefix_end = prefix_units(g.q, p);
+        const int32_t unit_shift = fresh().p.unit_shift;
+        const int32_t prefix_end = (g.q.prefix + (1 << unit_shift) - 1) >> unit_shift;
 #pragma unroll 1
         for (int side = 0; side < 2; ++side) {
             const bool own = side == 1;
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
             const uint32_t step = own ? a.table_col : a.prefix_col;
             const uint32_t wide = (own ? a.table64 : a.prefix64) != 0 ? 4 : 0;
             // Keys past the last that any row sees are nobody's.
-            const int32_t keys = min(own ? last_visible : g.q.prefix, to << p.unit_shift);
+            const int32_t keys = min(own ? last_visible : g.q.prefix, to << unit_shift);
             const char* const k_head = a.cache.k + static_cast<uint64_t>(a.cache.head_stride) * g.head +
                                        (load_piece < pieces ? load_piece : 0) * 16;
 
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
                 return __ballot(found) != 0;
             };
 
-            int32_t base = from << p.unit_shift;
+            int32_t base = from << unit_shift;
             uint64_t now = fetch(base, ids_of(base));
             uint32_t ids = ids_of(base + kTile);
             __syncthreads();     // the buffers' last use
@@ -289,26 +291,29 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
 
         sum = over_halves_sum(sum);
         if (row < g.rows) {
+            const Launch& last = fresh();
+            const AttentionArgs& z = last.a;
+            const Phase& p = last.p;
             const bool whole = p.direct != 0 && g.begin == 0 && g.end == g.units;
             constexpr int kRows = 32 * kWaves;
             if (whole) {
                 const float inverse = sum == 0 ? 0.0f : 1.0f / sum;
-                char* const to = a.out + (g.q.first + token) * a.o_token + head * a.o_head;
+                char* const to = z.out + (g.q.first + token) * z.o_token + head * z.o_head;
 #pragma unroll
                 for (int c = 0; c < kCols; ++c) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         const int element = c * 32 + half * 4 + 2 * i;
-                        if (element < a.dim) {
+                        if (element < z.dim) {
                             *reinterpret_cast<words2*>(to + element * 2) =
                                 words2{T::pack(o[c][i] * inverse, o[c][i + 1] * inverse),
                                        T::pack(o[c][i + 2] * inverse, o[c][i + 3] * inverse)};
                         }
                     }
                 }
-                if (half == 0 && a.lse != nullptr) {
-                    a.lse[(g.q.first + token) * a.l_token + head * a.l_head] =
-                        sum == 0 ? -INFINITY : (top * a.scale - T::kShift + log2f(sum)) * kLn2;
+                if (half == 0 && z.lse != nullptr) {
+                    z.lse[(g.q.first + token) * z.l_token + head * z.l_head] =
+                        sum == 0 ? -INFINITY : (top * z.scale - T::kShift + log2f(sum)) * kLn2;
                 }
             } else if (g.slot < p.slots) {
                 float* const part = p.parts + static_cast<int64_t>(g.slot) * kRows * (kDim + 2);
@@ -322,7 +327,7 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(
                     }
                 }
                 if (half == 0) {
-                    part[kRows * kDim + inside] = top == -INFINITY ? top : top * a.scale;
+                    part[kRows * kDim + inside] = top == -INFINITY ? top : top * z.scale;
                     part[kRows * kDim + kRows + inside] = sum;
                 }
             }
@@ -334,9 +339,9 @@ template <typename T, int kDim>
 void launch_dim(const AttentionArgs& a, const Phase& p, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(p.workgroups));
     if (p.row_shift == 7) {
-        wide_kernel<T, kDim, 4><<<grid, 256, 0, stream>>>(a, p);
+        wide_kernel<T, kDim, 4><<<grid, 256, 0, stream>>>(Launch{a, p});
     } else if constexpr (kDim <= 128) {
-        wide_kernel<T, kDim, 8><<<grid, 512, 0, stream>>>(a, p);
+        wide_kernel<T, kDim, 8><<<grid, 512, 0, stream>>>(Launch{a, p});
     }
     check_hip(hipGetLastError(), "launch attention");
 }

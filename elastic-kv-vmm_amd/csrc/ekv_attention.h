@@ -76,6 +76,14 @@ struct Phase {
     uint32_t* item_starts;           // [sequences + 1]
 };
 
+// The arguments of a kernel. They are more words than a wave has scalar registers, and the compiler loads all of them
+// first and spills what does not fit into vector registers; fresh() hides where they come from, so that each part of a
+// kernel loads what it needs where it needs it.
+struct Launch {
+    AttentionArgs a;
+    Phase p;
+};
+
 constexpr int kSeqChunk = 1024;      // sequences whose sums a workgroup holds at a time
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;       // bits by which a weight may pass 1 before its row is scaled again
@@ -88,6 +96,12 @@ struct Sequence {
     int32_t newest;             // position of the last query token among the own tokens
     int32_t group, request;     // table rows (-1: none)
 };
+
+__device__ __forceinline__ const Launch& fresh() {
+    auto at = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const Launch*)(at);
+}
 
 __device__ __forceinline__ int32_t clamped(int64_t v, int64_t low, int64_t high) {
     return static_cast<int32_t>(v < low ? low : (v > high ? high : v));
@@ -244,8 +258,9 @@ struct Segment {
 
 // Calls body(segment) for every segment of this workgroup, in order; all threads take part.
 template <int kWaves, typename Body>
-__device__ __forceinline__ void for_segments(const AttentionArgs& a, const Phase& p, LineCells<kWaves>& cells,
-                                             Body&& body) {
+__device__ __forceinline__ void for_segments(LineCells<kWaves>& cells, Body&& body) {
+    const AttentionArgs& a = fresh().a;
+    const Phase& p = fresh().p;
     const uint32_t w = blockIdx.x;
     const bool alike = p.mode == kSlots;   // every sequence is as long: places are divided, not searched
     uint32_t total = 0, alike_items = 0, alike_units = 1;
@@ -303,16 +318,19 @@ __device__ __forceinline__ void for_segments(const AttentionArgs& a, const Phase
             before = __builtin_amdgcn_readfirstlane(cells.items[low]);
         }
         Segment g;
-        g.q = sequence_of(a, p.mode, s);
-        g.units = units_of(g.q, p);
-        const uint32_t item = local / g.units;
-        const uint32_t row_tiles = row_tiles_of(a, g.q, p);
-        g.head = item / row_tiles;
-        g.row_begin = (item - g.head * row_tiles) << p.row_shift;
-        g.rows = g.q.count * a.share;
-        g.begin = local - item * g.units;
-        g.end = min(static_cast<uint32_t>(g.units), g.begin + (end - at));
-        g.slot = w + before + item;
+        {
+            const Launch& l = fresh();
+            g.q = sequence_of(l.a, l.p.mode, s);
+            g.units = units_of(g.q, l.p);
+            const uint32_t item = local / g.units;
+            const uint32_t row_tiles = row_tiles_of(l.a, g.q, l.p);
+            g.head = item / row_tiles;
+            g.row_begin = (item - g.head * row_tiles) << l.p.row_shift;
+            g.rows = g.q.count * l.a.share;
+            g.begin = local - item * g.units;
+            g.end = min(static_cast<uint32_t>(g.units), g.begin + (end - at));
+            g.slot = w + before + item;
+        }
         body(g);
         at += g.end - g.begin;
     }
