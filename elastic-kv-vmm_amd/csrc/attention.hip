@@ -23,7 +23,7 @@ constexpr int kMergeThreads = 256;
 struct Parts {
     const float* base;          // first part's row of values
     const float* stats;         // first part's largest score of the row; its sum is row_tile later
-    int64_t step;               // to the next part
+    int32_t step;               // to the next part
     int32_t row_tile;
     int32_t count;              // -1: the output is written already
 };
@@ -32,11 +32,11 @@ struct Parts {
 __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p, int32_t s, int32_t head, int32_t row) {
     uint32_t begin, total, item, units, row_tiles;
     if (p.mode == kSlots) {
-        const Sequence any = sequence_of(a, kSlots, 0);
-        units = units_of(any, p), row_tiles = row_tiles_of(a, any, p);
-        item = s * a.kv_heads * row_tiles;
+        units = p.alike_units.divisor;
+        item = s * p.alike_items.divisor;
+        row_tiles = row_tiles_of(a, sequence_of(a, kSlots, 0), p);
         begin = item * units;
-        total = p.sequences * a.kv_heads * row_tiles * units;
+        total = p.alike_total;
     } else {
         begin = p.unit_starts[s];
         item = p.item_starts[s];
@@ -50,29 +50,43 @@ __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p
     }
     const uint32_t local = head * row_tiles + (row >> p.row_shift);
     begin += local * units;
+    // Who has it: a long item everyone with a place of it, a short one the one whose moved cuts enclose it.
     const uint32_t quota = quota_of(p, total);
-    const uint32_t first = begin / quota, last = (begin + units - 1) / quota;
+    uint32_t first = begin / quota, count = 1;
+    const uint32_t cut = (first + 1) * quota;
+    if (cut < begin + units) {
+        if (keeps_cuts(units, quota)) {
+            count = (begin + units - 1) / quota - first + 1;
+        } else if (moved_cut(cut, begin, units, quota) == begin) {
+            ++first;
+        }
+    }
     Parts r;
     r.row_tile = 1 << p.row_shift;
-    r.step = static_cast<int64_t>(r.row_tile) * (p.dim_pad + 2);
+    r.step = r.row_tile * (p.dim_pad + 2);
     const uint32_t slot = first + item + local, inside = row & (r.row_tile - 1);
-    const float* part = p.parts + slot * r.step;
+    const float* part = p.parts + static_cast<int64_t>(slot) * r.step;
     r.base = part + inside * p.dim_pad;
     r.stats = part + r.row_tile * p.dim_pad + inside;
-    r.count = static_cast<int32_t>(last - first + 1);
-    if (p.direct != 0 && r.count == 1) {
+    r.count = static_cast<int32_t>(count);
+    if (p.direct != 0 && count == 1) {
         r.count = -1;
-    } else if (slot + r.count > static_cast<uint32_t>(p.slots)) {
+    } else if (slot + count > static_cast<uint32_t>(p.slots)) {
         r.count = 0;            // only if the starts were not in order
     }
     return r;
 }
 
-// One workgroup per (query token, KV head): a thread joins four elements of one row over all parts, own first, then the
-// prefix's, each in the order of the workgroups.
+// One workgroup per (query token, KV head). A thread joins four elements of a row over parts i, i + splits, ..., the own
+// parts first and then the prefix's, eight parts' loads in flight; the splits of a unit are joined through LDS. What
+// bounds it is the latency of those loads (a row has as many parts as workgroups shared its keys), so a small row's parts
+// are spread over the threads that it leaves idle.
 template <typename T>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArgs a, const Phase own,
                                                                   const Phase prefix) {
+    constexpr int kBatch = 8;
+    __shared__ f32x4 s_value[kMergeThreads];
+    __shared__ float s_top[kMergeThreads], s_sum[kMergeThreads];
     const int32_t token = blockIdx.x, head = blockIdx.y;
     int32_t b = token;
     if (own.mode != kSlots && a.query_starts.data != nullptr) {
@@ -90,47 +104,90 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
     const int32_t group = b >= 0 && prefix.sequences > 0 ? group_of(a, b) : -1;
     const int32_t own_first = b >= 0 && own.mode != kSlots ? first_token(a, b) : token;
     const int32_t prefix_first = group >= 0 ? first_token(a, first_row(a, group)) : 0;
-    const int32_t quads = (a.dim + 3) >> 2;
-    for (int32_t unit = threadIdx.x; unit < a.share * quads; unit += kMergeThreads) {
-        const int32_t sub = unit / quads, element = (unit % quads) * 4;
-        Parts part[2] = {};
+    const int32_t quads = (a.dim + 3) >> 2, units = a.share * quads;
+    const int32_t splits = units < kMergeThreads ? kMergeThreads / units : 1;
+    for (int32_t begin = 0; begin < units; begin += kMergeThreads) {
+        const int32_t split = splits > 1 ? threadIdx.x / units : 0;
+        const int32_t unit = begin + threadIdx.x - split * units;
+        const bool live = unit < units && split < splits;
+        const int32_t sub = live ? unit / quads : 0, element = live ? (unit - sub * quads) * 4 : 0;
+        Parts mine{}, theirs{};
         if (b >= 0) {
-            part[0] = parts_of(a, own, b, head, (token - own_first) * a.share + sub);
+            mine = parts_of(a, own, b, head, (token - own_first) * a.share + sub);
         }
         if (group >= 0) {
-            part[1] = parts_of(a, prefix, group, head, (token - prefix_first) * a.share + sub);
+            theirs = parts_of(a, prefix, group, head, (token - prefix_first) * a.share + sub);
         }
-        if (part[0].count < 0) {
+        const bool written = mine.count < 0;
+        const int32_t own_count = max(mine.count, 0), count = live && !written ? own_count + theirs.count : 0;
+        float top = -INFINITY, sum = 0;
+        f32x4 value = {0, 0, 0, 0};
+        for (int32_t i = split; i < count; i += splits * kBatch) {
+            float part_top[kBatch], part_sum[kBatch];
+            f32x4 part_value[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int32_t at = i + k * splits;
+                const bool there = at < count;
+                const bool first = at < own_count;
+                const int64_t place = there ? (first ? at : at - own_count) : 0;
+                const bool from_own = there ? first : own_count > 0;
+                const float* stats = (from_own ? mine.stats : theirs.stats) + place * (from_own ? mine.step : theirs.step);
+                const float* base = (from_own ? mine.base : theirs.base) + place * (from_own ? mine.step : theirs.step);
+                part_top[k] = stats[0];
+                part_sum[k] = stats[from_own ? mine.row_tile : theirs.row_tile];
+                part_value[k] = *reinterpret_cast<const f32x4*>(base + element);
+                part_top[k] = there ? part_top[k] : -INFINITY;
+            }
+            float most = top;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                most = fmaxf(most, part_top[k]);
+            }
+            const float safe = most == -INFINITY ? 0.0f : most;
+            const float keep = exp2f(top - safe);
+            sum *= keep;
+            value *= keep;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                // A part that saw nothing holds zeros, or NaN where its scores were; only one that is not there is left out.
+                const float factor = exp2f(part_top[k] - safe);
+                const bool there = i + k * splits < count;
+                sum += there ? part_sum[k] * factor : 0.0f;
+                value += there ? part_value[k] * factor : f32x4{0, 0, 0, 0};
+            }
+            top = most;
+        }
+        if (splits > 1) {
+            s_top[threadIdx.x] = top, s_sum[threadIdx.x] = sum, s_value[threadIdx.x] = value;
+            __syncthreads();
+            if (split == 0) {
+                float most = top;
+                for (int32_t k = 1; k < splits; ++k) {
+                    most = fmaxf(most, s_top[threadIdx.x + k * units]);
+                }
+                const float safe = most == -INFINITY ? 0.0f : most;
+                const float keep = exp2f(top - safe);
+                sum *= keep;
+                value *= keep;
+                for (int32_t k = 1; k < splits; ++k) {
+                    const float factor = exp2f(s_top[threadIdx.x + k * units] - safe);
+                    sum += s_sum[threadIdx.x + k * units] * factor;
+                    value += s_value[threadIdx.x + k * units] * factor;
+                }
+                top = most;
+            }
+        }
+        if (!live || written || split > 0) {
             continue;
         }
-        float most = -INFINITY;
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-#pragma unroll 4
-            for (int32_t i = 0; i < part[side].count; ++i) {
-                most = fmaxf(most, part[side].stats[i * part[side].step]);
-            }
-        }
-        const float safe = most == -INFINITY ? 0.0f : most;
-        float total = 0;
-        f32x4 value = {0, 0, 0, 0};
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-#pragma unroll 4
-            for (int32_t i = 0; i < part[side].count; ++i) {
-                const float* stats = part[side].stats + i * part[side].step;
-                const float keep = exp2f(stats[0] - safe);
-                total += stats[part[side].row_tile] * keep;
-                value += *reinterpret_cast<const f32x4*>(part[side].base + i * part[side].step + element) * keep;
-            }
-        }
         const int32_t row_head = head * a.share + sub;
-        const float inverse = total == 0 ? 0.0f : 1.0f / total;
+        const float inverse = sum == 0 ? 0.0f : 1.0f / sum;
         *reinterpret_cast<words2*>(a.out + token * a.o_token + row_head * a.o_head + element * 2) =
             words2{T::pack(value[0] * inverse, value[1] * inverse), T::pack(value[2] * inverse, value[3] * inverse)};
         if (element == 0 && a.lse != nullptr) {
             a.lse[token * a.l_token + row_head * a.l_head] =
-                total == 0 ? -INFINITY : (most - T::kShift + log2f(total)) * kLn2;
+                sum == 0 ? -INFINITY : (top - T::kShift + log2f(sum)) * kLn2;
         }
     }
 }
@@ -316,9 +373,9 @@ void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, i
     while ((1 << p.row_shift) < 16 * tiles16) {
         ++p.row_shift;
     }
-    p.unit_shift = tiles16 < 8 ? narrow_unit_shift(tiles16, dim_pad) : 6;
+    p.unit_shift = tiles16 < 8 ? narrow_unit_shift() : 6;
     p.dim_pad = dim_pad;
-    p.workgroups = kComputeUnits * (tiles16 == 8 && dim_pad <= 128 ? 2 : 1);
+    p.workgroups = kComputeUnits * (tiles16 < 8 ? narrow_groups(tiles16, dim_pad) : (tiles16 == 8 && dim_pad <= 128 ? 2 : 1));
     p.direct = direct;
     // Row tiles of all sequences: every sequence's last may be part-filled.
     const int64_t items = kv_heads * ((tokens * share >> p.row_shift) + std::min(sequences, tokens));
@@ -421,6 +478,14 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
     }
     place(plan.own, workspace);
     fit_units(plan.own, int64_t{a.own_most} + a.prefix_most);
+    if (plan.own.mode == kSlots) {
+        Phase& p = plan.own;
+        const int64_t units = std::max<int64_t>((int64_t{a.own_most} + (1 << p.unit_shift) - 1) >> p.unit_shift, 1);
+        const int64_t items = int64_t{a.kv_heads} * ((a.share + (1 << p.row_shift) - 1) >> p.row_shift);
+        p.alike_units = FastDiv(static_cast<uint32_t>(units));
+        p.alike_items = FastDiv(static_cast<uint32_t>(items));
+        p.alike_total = static_cast<uint32_t>(units * items * a.tokens);
+    }
     if (plan.prefix_tiles16 != 0) {
         place(plan.prefix, workspace);
         fit_units(plan.prefix, a.prefix_most);

@@ -19,6 +19,7 @@ namespace ekv {
 namespace {
 
 constexpr int kKeys = 32;   // keys of a tile
+constexpr int kWaves = 4;
 
 // What a key that is not seen reads: weight 0 must meet a finite V.
 __device__ __align__(256) const uint32_t zero_row[128] = {};
@@ -35,16 +36,17 @@ struct Rows {
     }
 };
 
-// Waves of a workgroup: as many as share a compute unit at the registers that the row tiles take.
+// Two workgroups share a compute unit where the row tile's registers leave room: one's start and end of an item overlap
+// the other's reading.
 template <int kDim, int kTiles>
-constexpr int waves_of() {
-    return kTiles == 1 && kDim <= 128 ? 8 : 4;
+constexpr int groups_of() {
+    return (kTiles == 1 && kDim <= 128) || (kTiles == 2 && kDim == 64) ? 2 : 1;
 }
 
 template <int kDim, int kTiles>
 constexpr int lds_bytes() {
-    const int values = waves_of<kDim, kTiles>() * kKeys * Rows<kDim>::kBytes;       // V of each wave's tile
-    const int join = waves_of<kDim, kTiles>() * (kDim / 16) * kTiles * 64 * 16;     // each wave's weighted values
+    const int values = kWaves * kKeys * Rows<kDim>::kBytes;       // V of each wave's tile
+    const int join = kWaves * (kDim / 16) * kTiles * 64 * 16;     // each wave's weighted values
     return values > join ? values : join;
 }
 
@@ -77,9 +79,8 @@ struct Ids {
 };
 
 template <typename T, int kDim, int kTiles>
-__global__ __launch_bounds__((waves_of<kDim, kTiles>() * 64), (waves_of<kDim, kTiles>() / 4)) void narrow_kernel(
+__global__ __launch_bounds__(kWaves * 64, (groups_of<kDim, kTiles>())) void narrow_kernel(
     const Launch) {
-    constexpr int kWaves = waves_of<kDim, kTiles>();
     constexpr int kSteps = kDim / 32;      // matrix steps of the first product
     constexpr int kCols = kDim / 16;       // 16-column pieces of the output
     // Head sizes between kDim and the next smaller class end in one of the last steps.
@@ -410,11 +411,11 @@ template <typename T, int kDim>
 void launch_dim(const AttentionArgs& a, const Phase& p, int tiles16, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(p.workgroups));
     if (tiles16 == 1) {
-        narrow_kernel<T, kDim, 1><<<grid, waves_of<kDim, 1>() * 64, 0, stream>>>(Launch{a, p});
+        narrow_kernel<T, kDim, 1><<<grid, kWaves * 64, 0, stream>>>(Launch{a, p});
     } else if (tiles16 == 2) {
-        narrow_kernel<T, kDim, 2><<<grid, waves_of<kDim, 2>() * 64, 0, stream>>>(Launch{a, p});
+        narrow_kernel<T, kDim, 2><<<grid, kWaves * 64, 0, stream>>>(Launch{a, p});
     } else if constexpr (kDim <= 128) {
-        narrow_kernel<T, kDim, 4><<<grid, waves_of<kDim, 4>() * 64, 0, stream>>>(Launch{a, p});
+        narrow_kernel<T, kDim, 4><<<grid, kWaves * 64, 0, stream>>>(Launch{a, p});
     }
     check_hip(hipGetLastError(), "launch attention");
 }
@@ -431,7 +432,11 @@ void launch_type(const AttentionArgs& a, const Phase& p, int tiles16, hipStream_
 
 }  // namespace
 
-int narrow_unit_shift(int tiles16, int32_t dim_pad) { return tiles16 == 1 && dim_pad <= 128 ? 8 : 7; }
+int narrow_unit_shift() { return 7; }
+
+int narrow_groups(int tiles16, int32_t dim_pad) {
+    return (tiles16 == 1 && dim_pad <= 128) || (tiles16 == 2 && dim_pad == 64) ? 2 : 1;
+}
 
 void launch_narrow(const AttentionArgs& a, const Phase& p, int32_t dtype, int tiles16, void* stream) {
     if (dtype == EKV_BFLOAT16) {

@@ -4,9 +4,10 @@
 // one query token's to its slots. A sequence has `rows` rows (query tokens x query heads of one KV head) in tiles of
 // row_tile, and keys in units of unit; an item is one (sequence, KV head, row tile), and its key units are counted in one
 // line over all items. Workgroup w takes places [w * quota, (w + 1) * quota) of that line, whatever the lengths are, so
-// every workgroup has as many keys to read; an item cut between workgroups is joined by the merge kernel from the parts
-// that each left (weighted values, largest score, sum). Places fit 31 bits: the host makes the unit larger where the
-// tables' widths could pass them.
+// every workgroup has as many keys to read; but a cut inside an item of one or two units moves to the item's nearer end:
+// starting and ending an item costs a workgroup about as much as reading a unit, so that cutting it would save nothing. An item cut between workgroups is joined by the merge kernel from the parts that
+// each left (weighted values, largest score, sum). Places fit 31 bits: the host makes the unit larger where the tables'
+// widths could pass them.
 #pragma once
 
 #include "../../include/ekv_kernels.h"
@@ -71,6 +72,8 @@ struct Phase {
     int32_t direct;                  // an item that one workgroup has whole is written to the output
     int32_t dim_pad;
     int32_t slots;
+    uint32_t alike_total;            // kSlots: places, and the items of a sequence and units of an item
+    FastDiv alike_items, alike_units;
     float* parts;                    // slots of row_tile x dim_pad values, then row_tile largest scores and sums
     uint32_t* unit_starts;           // [sequences + 1] of the line, written for the merge
     uint32_t* item_starts;           // [sequences + 1]
@@ -181,6 +184,14 @@ __device__ __forceinline__ uint32_t quota_of(const Phase& p, uint32_t total) {
     return max((total + p.workgroups - 1) / p.workgroups, 1u);
 }
 
+// Whether an item keeps its cuts, and where the cut at place c goes that lies in the item of places
+// [begin, begin + units). An item that moves its cuts has one at most.
+__device__ __forceinline__ bool keeps_cuts(uint32_t units, uint32_t quota) { return units > min(quota, 2u); }
+
+__device__ __forceinline__ uint32_t moved_cut(uint32_t c, uint32_t begin, uint32_t units, uint32_t quota) {
+    return keeps_cuts(units, quota) ? c : (c - begin < begin + units - c ? begin : begin + units);
+}
+
 // How many own tokens a row of query token i (of the sequence's count) sees.
 __device__ __forceinline__ int32_t seen_by(const Sequence& q, int32_t i) {
     return min(max(q.newest - q.count + i + 2, 0), q.own);
@@ -256,6 +267,16 @@ struct Segment {
     int32_t slot;
 };
 
+// The item at a place of the line.
+struct Item {
+    int32_t s;                          // sequence
+    uint32_t local;                     // item within the sequence
+    uint32_t before;                    // items before the sequence
+    uint32_t begin, units;              // its places
+};
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Calls body(segment) for every segment of this workgroup, in order; all threads take part.
 template <int kWaves, typename Body>
 __device__ __forceinline__ void for_segments(LineCells<kWaves>& cells, Body&& body) {
@@ -263,12 +284,9 @@ __device__ __forceinline__ void for_segments(LineCells<kWaves>& cells, Body&& bo
     const Phase& p = fresh().p;
     const uint32_t w = blockIdx.x;
     const bool alike = p.mode == kSlots;   // every sequence is as long: places are divided, not searched
-    uint32_t total = 0, alike_items = 0, alike_units = 1;
+    uint32_t total = 0;
     if (alike) {
-        const Sequence any = sequence_of(a, kSlots, 0);
-        alike_units = units_of(any, p);
-        alike_items = a.kv_heads * row_tiles_of(a, any, p);
-        total = p.sequences * alike_items * alike_units;
+        total = p.alike_total;
     } else {
         uint32_t items = 0;
         for (int32_t chunk = 0; chunk < p.sequences; chunk += kSeqChunk) {
@@ -277,69 +295,105 @@ __device__ __forceinline__ void for_segments(LineCells<kWaves>& cells, Body&& bo
             total = cells.units[count];
             items = cells.items[count];
         }
-        total = __builtin_amdgcn_readfirstlane(total);
+        total = uniform(total);
     }
     const uint32_t quota = quota_of(p, total);
     uint32_t at = w * quota;
-    const uint32_t end = min(at + quota, total);
-    if (at >= end) {
+    if (at >= total) {
         return;
     }
     int32_t chunk = 0, count = min(kSeqChunk, p.sequences);
     if (!alike && p.sequences > kSeqChunk) {
         line_chunk(a, p, 0, 0, 0, cells);
     }
-#pragma unroll 1
-    while (at < end) {
-        int32_t s;
-        uint32_t local, before;           // place within the sequence; items before it
+    // The item at `place`, which does not go back from call to call.
+    const auto item_at = [&](uint32_t place) {
+        Item i;
         if (alike) {
-            s = at / (alike_items * alike_units);
-            local = at - s * (alike_items * alike_units);
-            before = s * alike_items;
-        } else {
-            while (cells.units[count] <= at) {
-                const uint32_t units_before = cells.units[count], items_before = cells.items[count];
-                chunk += kSeqChunk;
-                count = min(kSeqChunk, p.sequences - chunk);
-                line_chunk(a, p, chunk, units_before, items_before, cells);
+            const uint32_t item = p.alike_units.div(place);
+            i.units = p.alike_units.divisor;
+            i.begin = item * i.units;
+            i.s = p.alike_items.div(item);
+            i.before = i.s * p.alike_items.divisor;
+            i.local = item - i.before;
+            return i;
+        }
+        while (cells.units[count] <= place) {
+            const uint32_t units_before = cells.units[count], items_before = cells.items[count];
+            chunk += kSeqChunk;
+            count = min(kSeqChunk, p.sequences - chunk);
+            line_chunk(a, p, chunk, units_before, items_before, cells);
+        }
+        int32_t low = 0, high = count;
+        while (high - low > 1) {
+            const int32_t mid = (low + high) >> 1;
+            if (cells.units[mid] <= place) {
+                low = mid;
+            } else {
+                high = mid;
             }
-            int32_t low = 0, high = count;
-            while (high - low > 1) {
-                const int32_t mid = (low + high) >> 1;
-                if (cells.units[mid] <= at) {
-                    low = mid;
-                } else {
-                    high = mid;
-                }
-            }
-            s = __builtin_amdgcn_readfirstlane(chunk + low);
-            local = __builtin_amdgcn_readfirstlane(at - cells.units[low]);
-            before = __builtin_amdgcn_readfirstlane(cells.items[low]);
+        }
+        const uint32_t begin = uniform(cells.units[low]), all = uniform(cells.units[low + 1]) - begin;
+        i.before = uniform(cells.items[low]);
+        const uint32_t items = uniform(cells.items[low + 1]) - i.before;
+        i.s = uniform(chunk + low);
+        i.units = all, i.local = 0;
+        if (items > 1) {
+            i.units = all / items;
+            i.local = (place - begin) / i.units;
+        }
+        i.begin = begin + i.local * i.units;
+        return i;
+    };
+    Item i = item_at(at);
+    at = moved_cut(at, i.begin, i.units, quota);
+    uint32_t end = w * quota + quota;
+    if (at == i.begin + i.units && at < min(end, total)) {
+        i = item_at(at);
+    }
+    bool last = false;
+#pragma unroll 1
+    while (at < total) {
+        // The workgroup's end: its cut, moved if it lies in this item.
+        if (end < i.begin + i.units) {
+            end = moved_cut(end, i.begin, i.units, quota);
+            last = true;
+        }
+        const uint32_t stop = min(end, i.begin + i.units);
+        if (at >= stop) {
+            break;
         }
         Segment g;
         {
             const Launch& l = fresh();
-            g.q = sequence_of(l.a, l.p.mode, s);
-            g.units = units_of(g.q, l.p);
-            const uint32_t item = local / g.units;
+            g.q = sequence_of(l.a, l.p.mode, i.s);
+            g.units = i.units;
+            g.head = i.local, g.row_begin = 0;
             const uint32_t row_tiles = row_tiles_of(l.a, g.q, l.p);
-            g.head = item / row_tiles;
-            g.row_begin = (item - g.head * row_tiles) << l.p.row_shift;
+            if (row_tiles > 1) {
+                g.head = i.local / row_tiles;
+                g.row_begin = (i.local - g.head * row_tiles) << l.p.row_shift;
+            }
             g.rows = g.q.count * l.a.share;
-            g.begin = local - item * g.units;
-            g.end = min(static_cast<uint32_t>(g.units), g.begin + (end - at));
-            g.slot = w + before + item;
+            g.begin = at - i.begin;
+            g.end = stop - i.begin;
+            g.slot = w + i.before + i.local;
         }
         body(g);
-        at += g.end - g.begin;
+        at = stop;
+        if (last || at >= total || at >= end) {
+            break;
+        }
+        i = item_at(at);
     }
 }
 
 #endif
 
-// attention_narrow.hip: row tiles of 16 * tiles16 rows, units of at least narrow_unit_shift's size.
-int narrow_unit_shift(int tiles16, int32_t dim_pad);
+// attention_narrow.hip: row tiles of 16 * tiles16 rows, units of at least 2^narrow_unit_shift keys, and the workgroups
+// that share a compute unit.
+int narrow_unit_shift();
+int narrow_groups(int tiles16, int32_t dim_pad);
 void launch_narrow(const AttentionArgs& a, const Phase& p, int32_t dtype, int tiles16, void* stream);
 
 // attention_wide.hip: row tiles of 128 (row_shift 7) or 256 rows, units of at least 64 keys.
