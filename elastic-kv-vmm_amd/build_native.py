@@ -28,7 +28,7 @@ LAUNCHER = PACKAGE_ROOT / "lib" / ("_ekv_launch" + sysconfig.get_config_var("EXT
 LAUNCHER_SOURCE = "py_launch.cpp"
 SOURCES = ("vmm_backing.hip", "lookup.hip", "gather.hip", "swap_in.hip", "compare.hip", "hisparse_swap.hip",
            "stream_probe.hip", "decode_step.hip", "block_tables.hip", "attention.hip", "attention_narrow.hip",
-           "attention_wide.hip", "build_info.hip")
+           "attention_wide.hip", "attention_pair.hip", "build_info.hip")
 OFFLOAD_ARCH = "gfx950"
 
 COMMON_FLAGS = [

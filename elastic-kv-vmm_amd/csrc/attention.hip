@@ -21,11 +21,17 @@ constexpr int kMergeThreads = 256;
 
 // The workgroups that hold a token's parts of one phase, and where.
 struct Parts {
-    const float* base;          // first part's row of values
+    const float* base;          // first part
     const float* stats;         // first part's largest score of the row; its sum is row_tile later
     int32_t step;               // to the next part
     int32_t row_tile;
     int32_t count;              // -1: the output is written already
+    uint32_t inside;            // the row's place in its tile
+    int32_t wide, dim_pad, row_shift;
+
+    __device__ __forceinline__ uint32_t place(uint32_t quad) const {
+        return (wide ? wide_place(dim_pad, inside, quad) : narrow_place(row_shift, inside, quad)) * 4;
+    }
 };
 
 // The parts of row `row` (of one KV head) of sequence s: none when the sequence was nobody's work.
@@ -66,7 +72,10 @@ __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p
     r.step = r.row_tile * (p.dim_pad + 2);
     const uint32_t slot = first + item + local, inside = row & (r.row_tile - 1);
     const float* part = p.parts + static_cast<int64_t>(slot) * r.step;
-    r.base = part + inside * p.dim_pad;
+    r.base = part;
+    r.inside = inside;
+    r.wide = p.row_shift > 6;
+    r.dim_pad = p.dim_pad, r.row_shift = p.row_shift;
     r.stats = part + r.row_tile * p.dim_pad + inside;
     r.count = static_cast<int32_t>(count);
     if (p.direct != 0 && count == 1) {
@@ -110,7 +119,8 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
         const int32_t split = splits > 1 ? threadIdx.x / units : 0;
         const int32_t unit = begin + threadIdx.x - split * units;
         const bool live = unit < units && split < splits;
-        const int32_t sub = live ? unit / quads : 0, element = live ? (unit - sub * quads) * 4 : 0;
+        // Rows first: their values lie side by side.
+        const int32_t quad = live ? a.share_div.div(unit) : 0, sub = live ? unit - quad * a.share : 0, element = quad * 4;
         Parts mine{}, theirs{};
         if (b >= 0) {
             mine = parts_of(a, own, b, head, (token - own_first) * a.share + sub);
@@ -118,6 +128,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
         if (group >= 0) {
             theirs = parts_of(a, prefix, group, head, (token - prefix_first) * a.share + sub);
         }
+        const uint32_t my_place = mine.place(quad), their_place = theirs.place(quad);
         const bool written = mine.count < 0;
         const int32_t own_count = max(mine.count, 0), count = live && !written ? own_count + theirs.count : 0;
         float top = -INFINITY, sum = 0;
@@ -136,7 +147,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
                 const float* base = (from_own ? mine.base : theirs.base) + place * (from_own ? mine.step : theirs.step);
                 part_top[k] = stats[0];
                 part_sum[k] = stats[from_own ? mine.row_tile : theirs.row_tile];
-                part_value[k] = *reinterpret_cast<const f32x4*>(base + element);
+                part_value[k] = *reinterpret_cast<const f32x4*>(base + (from_own ? my_place : their_place));
                 part_top[k] = there ? part_top[k] : -INFINITY;
             }
             float most = top;
@@ -343,9 +354,10 @@ AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, i
 
 uint64_t aligned(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// The launches of a call and the workspace they use.
+// The launch of a call and the workspace it uses.
 struct Plan {
-    int tiles16 = 0, prefix_tiles16 = 0;   // 16-row tiles of each launch (0: no such launch)
+    int tiles16 = 0;           // 16-row tiles of the own tokens' kernel
+    bool pair = false;         // own tokens and prefixes as two phases of one launch
     Phase own{}, prefix{};
     uint64_t bytes = 0;
 };
@@ -373,7 +385,7 @@ void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, i
     while ((1 << p.row_shift) < 16 * tiles16) {
         ++p.row_shift;
     }
-    p.unit_shift = tiles16 < 8 ? narrow_unit_shift() : 6;
+    p.unit_shift = tiles16 < 8 ? kNarrowUnit : kWideUnit;
     p.dim_pad = dim_pad;
     p.workgroups = kComputeUnits * (tiles16 < 8 ? narrow_groups(tiles16, dim_pad) : (tiles16 == 8 && dim_pad <= 128 ? 2 : 1));
     p.direct = direct;
@@ -420,13 +432,13 @@ Plan prefix_plan(int64_t tokens, int64_t batch, int64_t groups, int64_t heads, i
     Plan plan;
     const int64_t share = heads / kv_heads, row_rows = std::min(max_query, tokens) * share;
     const int32_t dim_pad = padded_dim(dim);
-    // Rows of a group fill tiles that a batch row's alone leave part-empty: then the prefix is a launch of its own.
+    // Rows of a group fill tiles that a batch row's alone leave part-empty: then the prefix is a phase of its own.
     const int64_t group_rows = groups > 0 ? tokens * share / groups : 0;
     if (groups > 0 && group_rows > row_rows && row_rows < 64) {
-        plan.prefix_tiles16 = tiles_for(group_rows, dim_pad);
-        cut(plan, plan.prefix, kPrefixes, groups, plan.prefix_tiles16, tokens, share, kv_heads, dim_pad, false);
-        plan.tiles16 = tiles_for(row_rows, dim_pad);
+        plan.pair = true;
+        plan.tiles16 = row_rows <= 16 ? 1 : 8;
         cut(plan, plan.own, kOwn, batch, plan.tiles16, tokens, share, kv_heads, dim_pad, false);
+        cut(plan, plan.prefix, kPrefixes, groups, 8, tokens, share, kv_heads, dim_pad, false);
     } else {
         plan.tiles16 = tiles_for(row_rows, dim_pad);
         cut(plan, plan.own, groups > 0 ? kWhole : kOwn, batch, plan.tiles16, tokens, share, kv_heads, dim_pad, true);
@@ -457,14 +469,6 @@ void place(Phase& p, void* workspace) {
     }
 }
 
-void launch_phase(const AttentionArgs& a, const Phase& p, int32_t dtype, int tiles16, void* stream) {
-    if (tiles16 < 8) {
-        launch_narrow(a, p, dtype, tiles16, stream);
-    } else {
-        launch_wide(a, p, dtype, stream);
-    }
-}
-
 int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, uint64_t bytes, void* stream) {
     if (bytes < plan.bytes) {
         throw std::invalid_argument("the attention needs " + std::to_string(plan.bytes) + " workspace bytes, got " +
@@ -486,12 +490,15 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
         p.alike_items = FastDiv(static_cast<uint32_t>(items));
         p.alike_total = static_cast<uint32_t>(units * items * a.tokens);
     }
-    if (plan.prefix_tiles16 != 0) {
+    if (plan.pair) {
         place(plan.prefix, workspace);
         fit_units(plan.prefix, a.prefix_most);
-        launch_phase(a, plan.prefix, dtype, plan.prefix_tiles16, stream);
+        launch_pair(Launch{a, {plan.own, plan.prefix}}, dtype, stream);
+    } else if (plan.tiles16 < 8) {
+        launch_narrow(Launch{a, {plan.own, {}}}, dtype, plan.tiles16, stream);
+    } else {
+        launch_wide(Launch{a, {plan.own, {}}}, dtype, stream);
     }
-    launch_phase(a, plan.own, dtype, plan.tiles16, stream);
     const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.kv_heads));
     if (dtype == EKV_BFLOAT16) {
         merge_kernel<Bf16><<<grid, kMergeThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);

@@ -1,0 +1,69 @@
+// Attention of a batch behind shared prefixes in one launch: own tokens and prefixes are two lines of work, and every
+// workgroup has its share of both (gfx950).
+//
+// Reading own tokens is bound by HBM, the product with a prefix by the matrix pipes once a group has enough rows. The two
+// workgroups of a compute unit take their shares in opposite order, so that at any time one of them reads while the other
+// multiplies. The first and second half of the grid are dealt to the compute units in turn, which pairs them.
+#include "ekv_attention_narrow.h"
+#include "ekv_attention_wide.h"
+
+namespace ekv {
+namespace {
+
+constexpr int kWaves = 4;
+static_assert(kWaves == narrow::kWaves, "one workgroup runs both");
+
+template <int kDim>
+constexpr int data_bytes() {
+    return wide::lds_bytes<kDim>() > narrow::lds_bytes<kDim, 1>() ? wide::lds_bytes<kDim>() : narrow::lds_bytes<kDim, 1>();
+}
+
+template <typename T, int kDim, bool kFew>
+__global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void pair_kernel(const Launch) {
+    __shared__ __align__(16) char s_data[data_bytes<kDim>()];
+    __shared__ __align__(16) char s_stats[narrow::stats_bytes<1>()];
+    __shared__ LineCells<kWaves> s_line;
+    const int first = (blockIdx.x >> 3) & 1;
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {
+        const int which = first ^ turn;
+        if (kFew && which == 0) {
+            narrow::run<T, kDim, 1>(0, s_data, s_stats, s_line);
+        } else {
+            wide::run<T, kDim, kWaves>(which, s_data, s_line);
+        }
+    }
+}
+
+template <typename T, int kDim>
+void launch_dim(const Launch& l, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>(l.p[0].workgroups));
+    if (l.p[0].row_shift == 4) {
+        pair_kernel<T, kDim, true><<<grid, kWaves * 64, 0, stream>>>(l);
+    } else {
+        pair_kernel<T, kDim, false><<<grid, kWaves * 64, 0, stream>>>(l);
+    }
+    check_hip(hipGetLastError(), "launch attention");
+}
+
+template <typename T>
+void launch_type(const Launch& l, hipStream_t stream) {
+    switch (l.p[0].dim_pad) {
+        case 64: launch_dim<T, 64>(l, stream); break;
+        case 96: launch_dim<T, 96>(l, stream); break;
+        case 128: launch_dim<T, 128>(l, stream); break;
+        default: launch_dim<T, 256>(l, stream); break;
+    }
+}
+
+}  // namespace
+
+void launch_pair(const Launch& l, int32_t dtype, void* stream) {
+    if (dtype == EKV_BFLOAT16) {
+        launch_type<Bf16>(l, static_cast<hipStream_t>(stream));
+    } else {
+        launch_type<F16>(l, static_cast<hipStream_t>(stream));
+    }
+}
+
+}  // namespace ekv

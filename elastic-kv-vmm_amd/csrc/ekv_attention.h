@@ -84,14 +84,17 @@ struct Phase {
 // kernel loads what it needs where it needs it.
 struct Launch {
     AttentionArgs a;
-    Phase p;
+    Phase p[2];        // own tokens (or all), prefixes
 };
 
-constexpr int kSeqChunk = 1024;      // sequences whose sums a workgroup holds at a time
+constexpr int kSeqChunk = 256;       // sequences that a workgroup holds at a time
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;       // bits by which a weight may pass 1 before its row is scaled again
 
 #if defined(__HIPCC__)
+
+// What a key that is not seen reads: weight 0 must meet a finite V.
+__device__ __align__(256) static const uint32_t zero_row[128] = {};
 
 struct Sequence {
     int32_t first, count;       // query tokens
@@ -104,6 +107,13 @@ __device__ __forceinline__ const Launch& fresh() {
     auto at = __builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(at));
     return *(const Launch*)(at);
+}
+
+// A lane's number, hidden likewise: what follows from it is computed where it is used, not once at the kernel's start
+// and spilled until then.
+__device__ __forceinline__ int hidden(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 __device__ __forceinline__ int32_t clamped(int64_t v, int64_t low, int64_t high) {
@@ -202,27 +212,23 @@ struct LineCells {
     uint32_t units[kSeqChunk + 1];     // first place of each sequence of the chunk
     uint32_t items[kSeqChunk + 1];
     uint32_t sums[2][kWaves];
+    Sequence sequences[kSeqChunk];
 };
 
-// The places and items of the sequences of one chunk, given what lies before it. All threads call it.
+// The sequences of one chunk, a thread each, and their places and items, given what lies before them. All threads call
+// it.
 template <int kWaves>
 __device__ __forceinline__ void line_chunk(const AttentionArgs& a, const Phase& p, int32_t chunk, uint32_t units_before,
                                            uint32_t items_before, LineCells<kWaves>& cells) {
-    constexpr int kThreads = kWaves * 64;
     const int tid = threadIdx.x, wave = tid >> 6;
     const int32_t count = min(kSeqChunk, p.sequences - chunk);
-    const int32_t per = (count + kThreads - 1) / kThreads;
-    const int32_t first = min(tid * per, count), last = min(first + per, count);
     uint32_t units = 0, items = 0;
     __syncthreads();   // the cells' last use
-#pragma unroll 1
-    for (int32_t at = first; at < last; ++at) {
-        const Sequence q = sequence_of(a, p.mode, chunk + at);
-        const uint32_t mine = a.kv_heads * row_tiles_of(a, q, p);
-        cells.units[at] = mine * units_of(q, p);
-        cells.items[at] = mine;
-        units += cells.units[at];
-        items += mine;
+    if (tid < count) {
+        const Sequence q = sequence_of(a, p.mode, chunk + tid);
+        cells.sequences[tid] = q;
+        items = a.kv_heads * row_tiles_of(a, q, p);
+        units = items * units_of(q, p);
     }
     const uint32_t unit_sum = wave_scan<kAdd>(units), item_sum = wave_scan<kAdd>(items);
     if ((tid & 63) == 63) {
@@ -235,25 +241,19 @@ __device__ __forceinline__ void line_chunk(const AttentionArgs& a, const Phase& 
         unit_at += w < wave ? cells.sums[0][w] : 0;
         item_at += w < wave ? cells.sums[1][w] : 0;
     }
-    const bool publish = blockIdx.x == 0 && p.unit_starts != nullptr;
-#pragma unroll 1
-    for (int32_t at = first; at < last; ++at) {
-        const uint32_t my_units = cells.units[at], my_items = cells.items[at];
-        cells.units[at] = unit_at;
-        cells.items[at] = item_at;
-        if (publish) {
-            p.unit_starts[chunk + at] = unit_at;
-            p.item_starts[chunk + at] = item_at;
+    // The first thread past the last sequence (or the last one) leaves the end.
+    if (tid <= count && tid < kSeqChunk) {
+        cells.units[tid] = unit_at, cells.items[tid] = item_at;
+    }
+    if (tid == kSeqChunk - 1) {
+        cells.units[kSeqChunk] = unit_at + units, cells.items[kSeqChunk] = item_at + items;
+    }
+    if (blockIdx.x == 0 && p.unit_starts != nullptr) {
+        if (tid < count) {
+            p.unit_starts[chunk + tid] = unit_at, p.item_starts[chunk + tid] = item_at;
         }
-        unit_at += my_units;
-        item_at += my_items;
-        if (at == count - 1) {
-            cells.units[count] = unit_at;
-            cells.items[count] = item_at;
-            if (publish && chunk + count == p.sequences) {
-                p.unit_starts[p.sequences] = unit_at;
-                p.item_starts[p.sequences] = item_at;
-            }
+        if (tid == count - 1) {      // overwritten by the next chunk's first, or the end
+            p.unit_starts[chunk + count] = unit_at + units, p.item_starts[chunk + count] = item_at + items;
         }
     }
     __syncthreads();
@@ -267,136 +267,145 @@ struct Segment {
     int32_t slot;
 };
 
-// The item at a place of the line.
-struct Item {
-    int32_t s;                          // sequence
-    uint32_t local;                     // item within the sequence
-    uint32_t before;                    // items before the sequence
-    uint32_t begin, units;              // its places
-};
-
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Calls body(segment) for every segment of this workgroup, in order; all threads take part.
+__device__ __forceinline__ Sequence uniform(const Sequence& q) {
+    Sequence r;
+    r.first = uniform(q.first), r.count = uniform(q.count);
+    r.prefix = uniform(q.prefix), r.own = uniform(q.own), r.newest = uniform(q.newest);
+    r.group = uniform(q.group), r.request = uniform(q.request);
+    return r;
+}
+
+// Calls body(segment) for every segment of phase `which` that this workgroup has, in order; all threads take part.
+//
+// What runs once per workgroup or item costs as much as its instructions' way from memory, so this is kept short:
+// sequences are read once and wait in LDS, and one copy of each step serves all cases.
 template <int kWaves, typename Body>
-__device__ __forceinline__ void for_segments(LineCells<kWaves>& cells, Body&& body) {
+__device__ __forceinline__ void for_segments(int which, LineCells<kWaves>& cells, Body&& body) {
     const AttentionArgs& a = fresh().a;
-    const Phase& p = fresh().p;
-    const uint32_t w = blockIdx.x;
+    const Phase& p = fresh().p[which];
     const bool alike = p.mode == kSlots;   // every sequence is as long: places are divided, not searched
-    uint32_t total = 0;
-    if (alike) {
-        total = p.alike_total;
-    } else {
-        uint32_t items = 0;
-        for (int32_t chunk = 0; chunk < p.sequences; chunk += kSeqChunk) {
-            line_chunk(a, p, chunk, total, items, cells);
-            const int32_t count = min(kSeqChunk, p.sequences - chunk);
-            total = cells.units[count];
-            items = cells.items[count];
-        }
-        total = uniform(total);
-    }
-    const uint32_t quota = quota_of(p, total);
-    uint32_t at = w * quota;
-    if (at >= total) {
-        return;
-    }
-    int32_t chunk = 0, count = min(kSeqChunk, p.sequences);
-    if (!alike && p.sequences > kSeqChunk) {
-        line_chunk(a, p, 0, 0, 0, cells);
-    }
-    // The item at `place`, which does not go back from call to call.
-    const auto item_at = [&](uint32_t place) {
-        Item i;
-        if (alike) {
-            const uint32_t item = p.alike_units.div(place);
-            i.units = p.alike_units.divisor;
-            i.begin = item * i.units;
-            i.s = p.alike_items.div(item);
-            i.before = i.s * p.alike_items.divisor;
-            i.local = item - i.before;
-            return i;
-        }
-        while (cells.units[count] <= place) {
-            const uint32_t units_before = cells.units[count], items_before = cells.items[count];
-            chunk += kSeqChunk;
-            count = min(kSeqChunk, p.sequences - chunk);
-            line_chunk(a, p, chunk, units_before, items_before, cells);
-        }
-        int32_t low = 0, high = count;
-        while (high - low > 1) {
-            const int32_t mid = (low + high) >> 1;
-            if (cells.units[mid] <= place) {
-                low = mid;
-            } else {
-                high = mid;
-            }
-        }
-        const uint32_t begin = uniform(cells.units[low]), all = uniform(cells.units[low + 1]) - begin;
-        i.before = uniform(cells.items[low]);
-        const uint32_t items = uniform(cells.items[low + 1]) - i.before;
-        i.s = uniform(chunk + low);
-        i.units = all, i.local = 0;
-        if (items > 1) {
-            i.units = all / items;
-            i.local = (place - begin) / i.units;
-        }
-        i.begin = begin + i.local * i.units;
-        return i;
-    };
-    Item i = item_at(at);
-    at = moved_cut(at, i.begin, i.units, quota);
-    uint32_t end = w * quota + quota;
-    if (at == i.begin + i.units && at < min(end, total)) {
-        i = item_at(at);
-    }
-    bool last = false;
+    const uint32_t w = blockIdx.x;
+    uint32_t total = p.alike_total, quota = 0, at = 0, end = 0, units_before = 0, items_before = 0;
+    int32_t chunk = 0;
+    bool known = false, starting = true;
 #pragma unroll 1
-    while (at < total) {
-        // The workgroup's end: its cut, moved if it lies in this item.
-        if (end < i.begin + i.units) {
-            end = moved_cut(end, i.begin, i.units, quota);
-            last = true;
+    while (true) {
+        const int32_t count = min(kSeqChunk, p.sequences - chunk);
+        if (!alike) {
+            line_chunk(a, p, chunk, units_before, items_before, cells);
+            units_before = uniform(cells.units[count]), items_before = uniform(cells.items[count]);
         }
-        const uint32_t stop = min(end, i.begin + i.units);
-        if (at >= stop) {
-            break;
-        }
-        Segment g;
-        {
-            const Launch& l = fresh();
-            g.q = sequence_of(l.a, l.p.mode, i.s);
-            g.units = i.units;
-            g.head = i.local, g.row_begin = 0;
-            const uint32_t row_tiles = row_tiles_of(l.a, g.q, l.p);
-            if (row_tiles > 1) {
-                g.head = i.local / row_tiles;
-                g.row_begin = (i.local - g.head * row_tiles) << l.p.row_shift;
+        if (!known) {
+            if (!alike && chunk + kSeqChunk < p.sequences) {
+                chunk += kSeqChunk;
+                continue;
             }
-            g.rows = g.q.count * l.a.share;
-            g.begin = at - i.begin;
-            g.end = stop - i.begin;
-            g.slot = w + i.before + i.local;
+            total = alike ? total : units_before;
+            quota = quota_of(p, total);
+            at = w * quota, end = at + quota;
+            known = true;
+            if (at >= total) {
+                return;
+            }
+            if (chunk > 0) {
+                chunk = 0, units_before = 0, items_before = 0;
+                continue;
+            }
         }
-        body(g);
-        at = stop;
-        if (last || at >= total || at >= end) {
-            break;
+#pragma unroll 1
+        while (alike || at < units_before) {
+            // The item at `at`: its sequence, which of the sequence's items it is, its places.
+            uint32_t s, local = 0, before, begin, units;
+            if (alike) {
+                units = p.alike_units.divisor;
+                const uint32_t item = p.alike_units.div(at);
+                begin = item * units;
+                s = p.alike_items.div(item);
+                before = s * p.alike_items.divisor;
+                local = item - before;
+            } else {
+                int32_t low = 0, high = count;
+                while (high - low > 1) {
+                    const int32_t mid = (low + high) >> 1;
+                    const bool here = cells.units[mid] <= at;
+                    low = here ? mid : low;
+                    high = here ? high : mid;
+                }
+                s = uniform(low);
+                begin = uniform(cells.units[s]);
+                units = uniform(cells.units[s + 1]) - begin;
+                before = uniform(cells.items[s]);
+                const uint32_t items = uniform(cells.items[s + 1]) - before;
+                if (items > 1) {
+                    units = units / items;
+                    local = (at - begin) / units;
+                    begin += local * units;
+                }
+            }
+            if (starting) {
+                starting = false;
+                at = moved_cut(at, begin, units, quota);
+                if (at == begin + units) {
+                    if (at >= total) {
+                        return;
+                    }
+                    continue;
+                }
+            }
+            uint32_t stop = begin + units;
+            const bool last = end < stop;
+            stop = last ? moved_cut(end, begin, units, quota) : stop;
+            if (at >= stop) {
+                return;
+            }
+            Segment g;
+            g.q = alike ? sequence_of(a, kSlots, s) : uniform(cells.sequences[s]);
+            g.units = units;
+            g.head = local, g.row_begin = 0;
+            const uint32_t row_tiles = row_tiles_of(a, g.q, p);
+            if (row_tiles > 1) {
+                g.head = local / row_tiles;
+                g.row_begin = (local - g.head * row_tiles) << p.row_shift;
+            }
+            g.rows = g.q.count * a.share;
+            g.begin = at - begin;
+            g.end = stop - begin;
+            g.slot = w + before + local;
+            body(g);
+            at = stop;
+            if (last || at >= end || at >= total) {
+                return;
+            }
         }
-        i = item_at(at);
+        chunk += kSeqChunk;
     }
+}
+
+// Where a part holds four values, elements 4 quad .. 4 quad + 3 of row `row` of its tile, in 16-byte units: in the order
+// of the registers that they come from, so that a wave's store is one run of memory.
+__device__ __forceinline__ uint32_t narrow_place(int32_t row_shift, uint32_t row, uint32_t quad) {
+    return ((((quad >> 2) << (row_shift - 4)) + (row >> 4)) << 6) + ((quad & 3) << 4) + (row & 15);
+}
+
+__device__ __forceinline__ uint32_t wide_place(int32_t dim_pad, uint32_t row, uint32_t quad) {
+    return (((row >> 5) * (dim_pad >> 3) + (quad >> 1)) << 6) + ((quad & 1) << 5) + (row & 31);
 }
 
 #endif
 
-// attention_narrow.hip: row tiles of 16 * tiles16 rows, units of at least 2^narrow_unit_shift keys, and the workgroups
-// that share a compute unit.
-int narrow_unit_shift();
+// attention_narrow.hip: row tiles of 16 * tiles16 rows, units of at least 2^kNarrowUnit keys, and the workgroups that
+// share a compute unit.
+constexpr int kNarrowUnit = 7;
 int narrow_groups(int tiles16, int32_t dim_pad);
-void launch_narrow(const AttentionArgs& a, const Phase& p, int32_t dtype, int tiles16, void* stream);
+void launch_narrow(const Launch& l, int32_t dtype, int tiles16, void* stream);
 
-// attention_wide.hip: row tiles of 128 (row_shift 7) or 256 rows, units of at least 64 keys.
-void launch_wide(const AttentionArgs& a, const Phase& p, int32_t dtype, void* stream);
+// attention_wide.hip: row tiles of 128 (row_shift 7) or 256 rows, units of at least 2^kWideUnit keys.
+constexpr int kWideUnit = 6;
+void launch_wide(const Launch& l, int32_t dtype, void* stream);
+
+// attention_pair.hip: own tokens by the kernel for few rows (16) or for many (128), prefixes by the one for many.
+void launch_pair(const Launch& l, int32_t dtype, void* stream);
 
 }  // namespace ekv
