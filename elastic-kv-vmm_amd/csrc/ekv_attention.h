@@ -116,6 +116,17 @@ __device__ __forceinline__ int hidden(int x) {
     return x;
 }
 
+// A barrier for what is in LDS. __syncthreads() also waits for every load from memory that is under way, and would end
+// each prefetch at the next barrier.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Keeps what stands beside it under its branch: without it the compiler computes a rare branch's selects every time.
+__device__ __forceinline__ void rarely() { asm volatile(""); }
+
 __device__ __forceinline__ int32_t clamped(int64_t v, int64_t low, int64_t high) {
     return static_cast<int32_t>(v < low ? low : (v > high ? high : v));
 }

@@ -222,6 +222,7 @@ __device__ __forceinline__ void run(int which, char* s_data, char* stats, LineCe
                 }
                 bool spoiled = false;
                 if (ragged) {
+                    rarely();
                     // A key that only some rows see has weight 0 for the others, and 0 * infinity is not 0.
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -253,6 +254,7 @@ __device__ __forceinline__ void run(int which, char* s_data, char* stats, LineCe
                         x[j] = s[m][j >> 2][j & 3];
                     }
                     if (ragged || now != 0xffffffffu) {
+                        rarely();
                         const int32_t left = own ? visible[m] - base : kKeys;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -340,7 +342,7 @@ __device__ __forceinline__ void run(int which, char* s_data, char* stats, LineCe
                 s_sum[wave][m * 16 + end_col] = sum[m];
             }
         }
-        __syncthreads();
+        lds_barrier();
         const Launch& last = fresh();
         const AttentionArgs& z = last.a;
         const Phase& p = last.p[which];
@@ -382,7 +384,7 @@ __device__ __forceinline__ void run(int which, char* s_data, char* stats, LineCe
                 }
             }
         }
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int c = wave; c < kCols; c += kWaves) {
 #pragma unroll
@@ -409,7 +411,7 @@ __device__ __forceinline__ void run(int which, char* s_data, char* stats, LineCe
                 }
             }
         }
-        __syncthreads();
+        lds_barrier();
     });
 }
 

@@ -169,25 +169,137 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
                 return __ballot(found) != 0;
             };
 
+            // Scores of 32 keys of the tile at `tile`: its first or second half.
+            const auto scores = [&](const char* tile, int b) {
+                f32x16 s;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = 0;
+                }
+#pragma unroll
+                for (int c = 0; c < kSteps; ++c) {
+                    const words4 x = *reinterpret_cast<const words4*>(tile + (read_k ^ (c << 5)) + b * 32 * kBytes);
+                    s = T::mfma32(x, q[c], s);
+                }
+                return s;
+            };
+            // Scores of the keys that a row does not see become -infinity; `left` keys of the 32 are before its end.
+            const auto cut_scores = [&](f32x16& s, uint32_t bits, int32_t left) {
+                rarely();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = half * 4 + (i & 3) + 8 * (i >> 2);
+                    s[i] = ((bits >> key) & 1) != 0 && key < left ? s[i] : -INFINITY;
+                }
+            };
+            const auto largest = [&](const f32x16& s) {
+                float most = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) {
+                    most = fmaxf(most, s[i]);
+                }
+                return over_halves_max(most);
+            };
+            // The reference score follows the largest only when that has passed it by 2^kSlack: until then the weights are
+            // larger than 1, which their type holds, and nothing has to be scaled again.
+            const auto follow = [&](float most) {
+                if (__ballot(most > top + slack) != 0) {
+                    const float to_top = fmaxf(top, most);
+                    const float keep = to_top == top ? 1.0f : __builtin_amdgcn_exp2f((top - to_top) * a.scale);
+                    sum *= keep;
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        o[c] *= keep;
+                    }
+                    top = to_top;
+                }
+            };
+            // One step: the weights of s (32 keys, half b of `tile`) and their values, while the next step's scores, of
+            // half `next_b` of `next_tile`, are multiplied: s becomes them. The matrix and the vector instructions are
+            // dealt in turn, so that a wave's softmax runs beside its own products.
+            const auto step_on = [&](f32x16& s, const char* tile, int b, const char* next_tile, int next_b, bool whole,
+                                     uint32_t bits, int32_t left) {
+                const float shift = (top == -INFINITY ? 0.0f : top * a.scale) - T::kShift;
+                f32x16 n;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    n[i] = 0;
+                }
+                const auto key_piece = [&](int c) {
+                    return *reinterpret_cast<const words4*>(next_tile + (read_k ^ (c << 5)) + next_b * 32 * kBytes);
+                };
+                const auto column = [&](int j) {          // of 16-key group j / kCols, columns j % kCols
+                    const int at = (b * 2 + j / kCols) * 16 * kBytes;
+                    const words2 low = read_transposed(tile + (read_v ^ (j % kCols << 6)) + at);
+                    const words2 high = read_transposed(tile + (read_v8 ^ (j % kCols << 6)) + at);
+                    return words4{low[0], low[1], high[0], high[1]};
+                };
+                float w[16];
+                words4 weights[2];
+                words4 ahead[2] = {key_piece(0), key_piece(1)};
+                words4 columns[2];
+#pragma unroll
+                for (int c = 0; c < kSteps; ++c) {
+                    const words4 x = ahead[c & 1];
+                    if (c + 2 < kSteps) {
+                        ahead[c & 1] = key_piece(c + 2);
+                    } else {
+                        columns[c + 2 - kSteps] = column(c + 2 - kSteps);
+                    }
+                    n = T::mfma32(x, q[c], n);
+#pragma unroll
+                    for (int i = c * 16 / kSteps; i < (c + 1) * 16 / kSteps; ++i) {
+                        w[i] = __builtin_amdgcn_exp2f(s[i] * a.scale - shift);
+                        sum += w[i];
+                        if (i & 1) {
+                            weights[i >> 3][(i & 7) >> 1] = T::pack(w[i - 1], w[i]);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                float most = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 2 * kCols; ++j) {
+                    const words4 x = columns[j & 1];
+                    if (j + 2 < 2 * kCols) {
+                        columns[j & 1] = column(j + 2);
+                    }
+                    o[j % kCols] = T::mfma32(x, weights[j / kCols], o[j % kCols]);
+#pragma unroll
+                    for (int i = j * 8 / kCols; i < (j + 1) * 8 / kCols; ++i) {
+                        most = fmaxf(most, n[i]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                most = over_halves_max(most);
+                if (!whole) {
+                    cut_scores(n, bits, left);
+                    most = largest(n);
+                }
+                follow(most);
+                s = n;
+            };
+
             int32_t base = from << unit_shift;
             uint64_t now = fetch(base, ids_of(base));
             uint32_t ids = ids_of(base + kTile);
-            __syncthreads();     // the buffers' last use
+            lds_barrier();     // the buffers' last use
             store(0);
             uint64_t next = fetch(base + kTile, ids);
             ids = ids_of(base + 2 * kTile);
-            __syncthreads();
+            lds_barrier();
             int buffer = 0;
+            f32x16 s = scores(s_data, 0);
+            // Whether some row sees fewer keys of the tile at `base` than it holds.
+            bool ragged = own && base + kTile > first_visible;
+            if (ragged || static_cast<uint32_t>(now) != 0xffffffffu) {
+                cut_scores(s, static_cast<uint32_t>(now), own ? visible - base : 32);
+            }
+            follow(largest(s));
 #pragma unroll 1
             for (; base < keys; base += kTile, buffer ^= 2 * Tile<kDim>::kSize) {
-                store(buffer ^ (2 * Tile<kDim>::kSize));
-                const uint64_t seen = now;
-                now = next;
-                next = fetch(base + 2 * kTile, ids);
-                ids = ids_of(base + 3 * kTile);
                 const char* const tile = s_data + buffer;
-                // Whether some row sees fewer keys of this tile than it holds.
-                const bool ragged = own && base + kTile > first_visible;
+                const char* const other = s_data + (buffer ^ (2 * Tile<kDim>::kSize));
                 if (ragged && any_not_finite(tile, hidden(lane))) {
                     // A key that only some rows see has weight 0 for the others, and 0 * infinity is not 0: the infinities
                     // and NaN are added to the rows that see them (a weight is positive), then cleared.
@@ -208,7 +320,7 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
                             }
                         }
                     }
-                    __syncthreads();
+                    lds_barrier();
 #pragma unroll 1
                     for (int at = hidden(tid) * 16; at < Tile<kDim>::kSize; at += kWaves * 64 * 16) {
                         words4* const to = reinterpret_cast<words4*>(s_data + buffer + Tile<kDim>::kSize + at);
@@ -219,70 +331,20 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
                         }
                         *to = x;
                     }
-                    __syncthreads();
+                    lds_barrier();
                 }
-                const auto column = [&](int u, int c) {
-                    const words2 low = read_transposed(tile + (read_v ^ (c << 6)) + u * 16 * kBytes);
-                    const words2 high = read_transposed(tile + (read_v8 ^ (c << 6)) + u * 16 * kBytes);
-                    return words4{low[0], low[1], high[0], high[1]};
-                };
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    f32x16 s;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[i] = 0;
-                    }
-#pragma unroll
-                    for (int c = 0; c < kSteps; ++c) {
-                        const words4 x = *reinterpret_cast<const words4*>(tile + (read_k ^ (c << 5)) + b * 32 * kBytes);
-                        s = T::mfma32(x, q[c], s);
-                    }
-                    const uint32_t bits = static_cast<uint32_t>(seen >> (32 * b));
-                    if (ragged || bits != 0xffffffffu) {
-                        const int32_t left = own ? visible - base - b * 32 : 32;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int key = half * 4 + (i & 3) + 8 * (i >> 2);
-                            s[i] = ((bits >> key) & 1) != 0 && key < left ? s[i] : -INFINITY;
-                        }
-                    }
-                    float most = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        most = fmaxf(most, s[i]);
-                    }
-                    most = over_halves_max(most);
-                    // The reference score follows the largest only when that has passed it by 2^kSlack: until then the
-                    // weights are larger than 1, which their type holds, and nothing has to be scaled again.
-                    if (__ballot(most > top + slack) != 0) {
-                        const float to_top = fmaxf(top, most);
-                        const float keep = to_top == top ? 1.0f : __builtin_amdgcn_exp2f((top - to_top) * a.scale);
-                        sum *= keep;
-#pragma unroll
-                        for (int c = 0; c < kCols; ++c) {
-                            o[c] *= keep;
-                        }
-                        top = to_top;
-                    }
-                    const float shift = (top == -INFINITY ? 0.0f : top * a.scale) - T::kShift;
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        float w[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            w[j] = __builtin_amdgcn_exp2f(s[u * 8 + j] * a.scale - shift);
-                            sum += w[j];
-                        }
-                        const words4 weights = words4{T::pack(w[0], w[1]), T::pack(w[2], w[3]), T::pack(w[4], w[5]),
-                                                      T::pack(w[6], w[7])};
-#pragma unroll
-                        for (int c = 0; c < kCols; ++c) {
-                            o[c] = T::mfma32(column(b * 2 + u, c), weights, o[c]);
-                        }
-                    }
-                }
-                __syncthreads();
+                store(buffer ^ (2 * Tile<kDim>::kSize));
+                const uint32_t bits = static_cast<uint32_t>(now >> 32);
+                const int32_t left = own ? visible - base : kTile;
+                now = next;
+                next = fetch(base + 2 * kTile, ids);
+                ids = ids_of(base + 3 * kTile);
+                step_on(s, tile, 0, tile, 1, !ragged && bits == 0xffffffffu, bits, left - 32);
+                lds_barrier();      // the other buffer holds the next tile
+                ragged = own && base + 2 * kTile > first_visible;
+                step_on(s, tile, 1, other, 0, !ragged && static_cast<uint32_t>(now) == 0xffffffffu,
+                        static_cast<uint32_t>(now), left - kTile + (own ? 0 : kTile));
+                lds_barrier();      // nobody reads this buffer any more
             }
         }
 
