@@ -149,12 +149,13 @@ __device__ __forceinline__ void run(int which, char* s_data, char* stats, LineCe
             const char* const k_head = a.cache.k + static_cast<uint64_t>(a.cache.head_stride) * g.head + quad * 16;
             const char* const v_head = k_head + a.cache.kv_stride;
 
+            const Cache cache = a.cache;
             const auto ids_of = [&](int32_t base) {
                 Ids e;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int32_t key = base + h * 16 + col;
-                    const char* at = src.table + static_cast<uint64_t>(a.cache.page.div(key)) * src.step;
+                    const char* at = src.table + static_cast<uint64_t>(cache.page.div(key)) * src.step;
                     at = key < src.keys ? at : zeros;
                     e.low[h] = *reinterpret_cast<const uint32_t*>(at);
                     e.high[h] = *reinterpret_cast<const uint32_t*>(at + src.wide);
@@ -169,13 +170,15 @@ __device__ __forceinline__ void run(int which, char* s_data, char* stats, LineCe
                 for (int h = 0; h < 2; ++h) {
                     const int32_t key = base + h * 16 + col;
                     const uint32_t id = e.low[h];
-                    const bool good = key < src.keys && id >= a.cache.zero_below && id < a.cache.pages &&
+                    const bool good = key < src.keys && id >= cache.zero_below && id < cache.pages &&
                                       (src.wide == 0 || e.high[h] == 0);
-                    const uint32_t inside = key - a.cache.page.div(key) * a.cache.page.divisor;
-                    const uint64_t offset = static_cast<uint64_t>(id) * a.cache.page_stride +
-                                            static_cast<uint64_t>(inside) * a.cache.token_stride;
-                    const char* k_at = good ? k_head + offset : zeros;
-                    const char* v_at = good ? v_head + offset : zeros;
+                    const uint32_t inside = key - cache.page.div(key) * cache.page.divisor;
+                    const uint64_t offset = static_cast<uint64_t>(id) * cache.page_stride +
+                                            static_cast<uint64_t>(inside) * cache.token_stride;
+                    const char* k_at = k_head + offset;
+                    const char* v_at = v_head + offset;
+                    k_at = good ? k_at : zeros;
+                    v_at = good ? v_at : zeros;
 #pragma unroll
                     for (int c = 0; c < kSteps; ++c) {
                         // Past the head size: any piece of the row; K meets zeros of q once it is cleared, V's columns

@@ -122,43 +122,60 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
             const char* const k_head = a.cache.k + static_cast<uint64_t>(a.cache.head_stride) * g.head +
                                        (load_piece < pieces ? load_piece : 0) * 16;
 
-            // Page id of key base + lane, or 0xffffffff; every wave holds all of a tile's.
+            const Cache cache = a.cache;
+
+            // Page id of key base + lane, as words (an int64 id whose high word is not zero names no page): every wave
+            // holds all of a tile's, and looks at them one tile later.
+            struct Ids {
+                uint32_t low, high;
+            };
             const auto ids_of = [&](int32_t base) {
                 const int32_t key = base + lane;
-                const char* at = table + static_cast<uint64_t>(a.cache.page.div(key)) * step;
+                const char* at = table + static_cast<uint64_t>(cache.page.div(key)) * step;
                 at = key < keys ? at : zeros;
-                const uint32_t low = *reinterpret_cast<const uint32_t*>(at);
-                const uint32_t high = *reinterpret_cast<const uint32_t*>(at + wide);
-                return key < keys && (wide == 0 || high == 0) ? low : 0xffffffffu;
+                return Ids{*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + wide)};
             };
             words4 k[kLoads], v[kLoads];
-            const auto fetch = [&](int32_t base, uint32_t ids) {
-                const bool good = ids >= a.cache.zero_below && ids < a.cache.pages;
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    const int32_t inside_tile = i * kKeysAtOnce + load_key;
-                    const uint32_t id = __shfl(ids, inside_tile);
-                    const int32_t key = base + inside_tile;
-                    const bool live = id >= a.cache.zero_below && id < a.cache.pages;
-                    const uint32_t inside = key - a.cache.page.div(key) * a.cache.page.divisor;
-                    const uint64_t offset = static_cast<uint64_t>(id) * a.cache.page_stride +
-                                            static_cast<uint64_t>(inside) * a.cache.token_stride;
-                    k[i] = *reinterpret_cast<const words4*>(live ? k_head + offset : zeros);
-                    v[i] = *reinterpret_cast<const words4*>(live ? k_head + offset + a.cache.kv_stride : zeros);
-                }
+            // A tile's rows in three parts: whose keys are seen, then piece i of its loads, then piece i of its stores.
+            uint32_t mine = 0;
+            const auto look = [&](int32_t base, const Ids& ids) {
+                const bool good = base + lane < keys && ids.low >= cache.zero_below && ids.low < cache.pages &&
+                                  (wide == 0 || ids.high == 0);
+                mine = good ? ids.low : 0xffffffffu;
                 return __ballot(good);
             };
-            const auto store = [&](int buffer) {
+            const auto load = [&](int32_t base, int i) {
+                const int32_t inside_tile = i * kKeysAtOnce + load_key;
+                const uint32_t id = __shfl(mine, inside_tile);
+                const int32_t key = base + inside_tile;
+                const uint32_t inside = key - cache.page.div(key) * cache.page.divisor;
+                const char* at = k_head + static_cast<uint64_t>(id) * cache.page_stride +
+                                 static_cast<uint64_t>(inside) * cache.token_stride;
+                const char* v_at = at + cache.kv_stride;
+                at = id != 0xffffffffu ? at : zeros;
+                v_at = id != 0xffffffffu ? v_at : zeros;
+                k[i] = *reinterpret_cast<const words4*>(at);
+                v[i] = *reinterpret_cast<const words4*>(v_at);
+            };
+            const auto store = [&](int buffer, int i) {
+                char* const to = s_data + buffer + i * kKeysAtOnce * kBytes + (write_at ^ ((i * kKeysAtOnce & 8) << 2));
+                // K past the head size meets zeros of q and must not be an infinity; V's columns are not stored.
+                const words4 kept = load_piece < pieces ? k[i] : words4{0, 0, 0, 0};
+                *reinterpret_cast<words4*>(to) = kept;
+                *reinterpret_cast<words4*>(to + Tile<kDim>::kSize) = v[i];
+            };
+            const auto load_all = [&](int32_t base) {
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    char* const to = s_data + buffer + i * kKeysAtOnce * kBytes + (write_at ^ ((i * kKeysAtOnce & 8) << 2));
-                    // K past the head size meets zeros of q and must not be an infinity; V's columns are not stored.
-                    const words4 kept = load_piece < pieces ? k[i] : words4{0, 0, 0, 0};
-                    *reinterpret_cast<words4*>(to) = kept;
-                    *reinterpret_cast<words4*>(to + Tile<kDim>::kSize) = v[i];
+                    load(base, i);
                 }
             };
-
+            const auto store_all = [&](int buffer) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    store(buffer, i);
+                }
+            };
             const auto any_not_finite = [&](const char* tile, int first) {
                 bool found = false;
 #pragma unroll 1
@@ -218,7 +235,7 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
             // half `next_b` of `next_tile`, are multiplied: s becomes them. The matrix and the vector instructions are
             // dealt in turn, so that a wave's softmax runs beside its own products.
             const auto step_on = [&](f32x16& s, const char* tile, int b, const char* next_tile, int next_b, bool whole,
-                                     uint32_t bits, int32_t left) {
+                                     uint32_t bits, int32_t left, auto&& beside) {
                 const float shift = (top == -INFINITY ? 0.0f : top * a.scale) - T::kShift;
                 f32x16 n;
 #pragma unroll
@@ -236,6 +253,13 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
                 };
                 float w[16];
                 words4 weights[2];
+                const auto weigh = [&](int i) {
+                    w[i] = __builtin_amdgcn_exp2f(s[i] * a.scale - shift);
+                    sum += w[i];
+                    if (i & 1) {
+                        weights[i >> 3][(i & 7) >> 1] = T::pack(w[i - 1], w[i]);
+                    }
+                };
                 words4 ahead[2] = {key_piece(0), key_piece(1)};
                 words4 columns[2];
 #pragma unroll
@@ -248,12 +272,8 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
                     }
                     n = T::mfma32(x, q[c], n);
 #pragma unroll
-                    for (int i = c * 16 / kSteps; i < (c + 1) * 16 / kSteps; ++i) {
-                        w[i] = __builtin_amdgcn_exp2f(s[i] * a.scale - shift);
-                        sum += w[i];
-                        if (i & 1) {
-                            weights[i >> 3][(i & 7) >> 1] = T::pack(w[i - 1], w[i]);
-                        }
+                    for (int i = c * 12 / kSteps; i < (c + 1) * 12 / kSteps; ++i) {
+                        weigh(i);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -265,6 +285,13 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
                         columns[j & 1] = column(j + 2);
                     }
                     o[j % kCols] = T::mfma32(x, weights[j / kCols], o[j % kCols]);
+                    if (j < kCols) {
+#pragma unroll
+                        for (int i = 12 + j * 4 / kCols; i < 12 + (j + 1) * 4 / kCols; ++i) {
+                            weigh(i);
+                        }
+                    }
+                    beside(j);
 #pragma unroll
                     for (int i = j * 8 / kCols; i < (j + 1) * 8 / kCols; ++i) {
                         most = fmaxf(most, n[i]);
@@ -281,11 +308,13 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
             };
 
             int32_t base = from << unit_shift;
-            uint64_t now = fetch(base, ids_of(base));
-            uint32_t ids = ids_of(base + kTile);
+            uint64_t now = look(base, ids_of(base));
+            load_all(base);
+            Ids ids = ids_of(base + kTile);
             lds_barrier();     // the buffers' last use
-            store(0);
-            uint64_t next = fetch(base + kTile, ids);
+            store_all(0);
+            uint64_t next = look(base + kTile, ids);
+            load_all(base + kTile);
             ids = ids_of(base + 2 * kTile);
             lds_barrier();
             int buffer = 0;
@@ -333,17 +362,27 @@ __device__ __forceinline__ void run(int which, char* s_data, LineCells<kWaves>& 
                     }
                     lds_barrier();
                 }
-                store(buffer ^ (2 * Tile<kDim>::kSize));
                 const uint32_t bits = static_cast<uint32_t>(now >> 32);
                 const int32_t left = own ? visible - base : kTile;
                 now = next;
-                next = fetch(base + 2 * kTile, ids);
+                next = look(base + 2 * kTile, ids);
                 ids = ids_of(base + 3 * kTile);
-                step_on(s, tile, 0, tile, 1, !ragged && bits == 0xffffffffu, bits, left - 32);
+                step_on(s, tile, 0, tile, 1, !ragged && bits == 0xffffffffu, bits, left - 32, [&](int j) {
+                    // The next tile's rows leave their registers for the one after's.
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i) {
+                        if (i * kCols / kLoads == j) {
+                            store(buffer ^ (2 * Tile<kDim>::kSize), i);
+                        }
+                        if (kCols + i * kCols / kLoads == j) {
+                            load(base + 2 * kTile, i);
+                        }
+                    }
+                });
                 lds_barrier();      // the other buffer holds the next tile
                 ragged = own && base + 2 * kTile > first_visible;
                 step_on(s, tile, 1, other, 0, !ragged && static_cast<uint32_t>(now) == 0xffffffffu,
-                        static_cast<uint32_t>(now), left - kTile + (own ? 0 : kTile));
+                        static_cast<uint32_t>(now), left - kTile + (own ? 0 : kTile), [](int) {});
                 lds_barrier();      // nobody reads this buffer any more
             }
         }
