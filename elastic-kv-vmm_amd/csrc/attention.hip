@@ -35,7 +35,8 @@ struct Parts {
 };
 
 // The parts of row `row` (of one KV head) of sequence s: none when the sequence was nobody's work.
-__device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p, int32_t s, int32_t head, int32_t row) {
+__device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p, uint32_t workgroups, int32_t s, int32_t head,
+                                          int32_t row) {
     uint32_t begin, total, item, units, row_tiles;
     if (p.mode == kSlots) {
         units = p.alike_units.divisor;
@@ -57,7 +58,7 @@ __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p
     const uint32_t local = head * row_tiles + (row >> p.row_shift);
     begin += local * units;
     // Who has it: a long item everyone with a place of it, a short one the one whose moved cuts enclose it.
-    const uint32_t quota = quota_of(p, total);
+    const uint32_t quota = quota_of(total, workgroups);
     uint32_t first = begin / quota, count = 1;
     const uint32_t cut = (first + 1) * quota;
     if (cut < begin + units) {
@@ -113,6 +114,11 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
     const int32_t group = b >= 0 && prefix.sequences > 0 ? group_of(a, b) : -1;
     const int32_t own_first = b >= 0 && own.mode != kSlots ? first_token(a, b) : token;
     const int32_t prefix_first = group >= 0 ? first_token(a, first_row(a, group)) : 0;
+    uint32_t own_workgroups = own.workgroups, shared = 0;
+    if (prefix.sequences > 0) {
+        shared = prefix_workgroups(own, prefix, own.unit_starts[own.sequences], prefix.unit_starts[prefix.sequences]);
+        own_workgroups -= shared;
+    }
     const int32_t quads = (a.dim + 3) >> 2, units = a.share * quads;
     const int32_t splits = units < kMergeThreads ? kMergeThreads / units : 1;
     for (int32_t begin = 0; begin < units; begin += kMergeThreads) {
@@ -123,10 +129,10 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
         const int32_t quad = live ? a.share_div.div(unit) : 0, sub = live ? unit - quad * a.share : 0, element = quad * 4;
         Parts mine{}, theirs{};
         if (b >= 0) {
-            mine = parts_of(a, own, b, head, (token - own_first) * a.share + sub);
+            mine = parts_of(a, own, own_workgroups, b, head, (token - own_first) * a.share + sub);
         }
         if (group >= 0) {
-            theirs = parts_of(a, prefix, group, head, (token - prefix_first) * a.share + sub);
+            theirs = parts_of(a, prefix, shared, group, head, (token - prefix_first) * a.share + sub);
         }
         const uint32_t my_place = mine.place(quad), their_place = theirs.place(quad);
         const bool written = mine.count < 0;
@@ -388,6 +394,9 @@ void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, i
     p.unit_shift = tiles16 < 8 ? kNarrowUnit : kWideUnit;
     p.dim_pad = dim_pad;
     p.workgroups = kComputeUnits * (tiles16 < 8 ? narrow_groups(tiles16, dim_pad) : (tiles16 == 8 && dim_pad <= 128 ? 2 : 1));
+    // A unit of the kernel for few rows is 128 keys read at the card's rate, one of the kernel for many 64 keys'
+    // products: about 4 us and 2.4 us of a workgroup at a head size of 128.
+    p.weight = tiles16 < 8 ? 5 : 3;
     p.direct = direct;
     // Row tiles of all sequences: every sequence's last may be part-filled.
     const int64_t items = kv_heads * ((tokens * share >> p.row_shift) + std::min(sequences, tokens));

@@ -1,9 +1,9 @@
-// Attention of a batch behind shared prefixes in one launch: own tokens and prefixes are two lines of work, and every
-// workgroup has its share of both (gfx950).
+// Attention of a batch behind shared prefixes in one launch: own tokens and prefixes are two lines of work, and the
+// workgroups are shared between them by what the lines cost (gfx950).
 //
-// Reading own tokens is bound by HBM, the product with a prefix by the matrix pipes once a group has enough rows. The two
-// workgroups of a compute unit take their shares in opposite order, so that at any time one of them reads while the other
-// multiplies. The first and second half of the grid are dealt to the compute units in turn, which pairs them.
+// Reading own tokens is bound by HBM, the product with a prefix by the matrix pipes once a group has enough rows. The first
+// workgroups of the grid work on prefixes, the others on own tokens; the first and the second half of the grid are dealt to
+// the compute units in turn, so that as long as both have work most units hold one of each.
 #include "ekv_attention_narrow.h"
 #include "ekv_attention_wide.h"
 
@@ -23,15 +23,15 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void pair_kernel(
     __shared__ __align__(16) char s_data[data_bytes<kDim>()];
     __shared__ __align__(16) char s_stats[narrow::stats_bytes<1>()];
     __shared__ LineCells<kWaves> s_line;
-    const int first = (blockIdx.x >> 3) & 1;
-#pragma unroll 1
-    for (int turn = 0; turn < 2; ++turn) {
-        const int which = first ^ turn;
-        if (kFew && which == 0) {
-            narrow::run<T, kDim, 1>(0, s_data, s_stats, s_line);
-        } else {
-            wide::run<T, kDim, kWaves>(which, s_data, s_line);
-        }
+    const uint32_t prefix_total = line_total(1, s_line), own_total = line_total(0, s_line);
+    const Launch& l = fresh();
+    const uint32_t share = prefix_workgroups(l.p[0], l.p[1], own_total, prefix_total), b = blockIdx.x;
+    if (kFew && b >= share) {
+        narrow::run<T, kDim, 1>(0, b - share, gridDim.x - share, s_data, s_stats, s_line);
+    } else {
+        const int which = b < share ? 1 : 0;
+        wide::run<T, kDim, kWaves>(which, which == 1 ? b : b - share, which == 1 ? share : gridDim.x - share, s_data,
+                                   s_line);
     }
 }
 

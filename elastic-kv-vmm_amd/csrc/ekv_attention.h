@@ -68,7 +68,8 @@ struct Phase {
     PhaseMode mode;
     int32_t sequences;
     int32_t row_shift, unit_shift;   // row_tile and unit as powers of two
-    int32_t workgroups;              // the most that take part
+    int32_t workgroups;              // that take part; of a launch of two phases, that both share
+    int32_t weight;                  // cost of a unit, as the phases of a launch share its workgroups
     int32_t direct;                  // an item that one workgroup has whole is written to the output
     int32_t dim_pad;
     int32_t slots;
@@ -201,8 +202,23 @@ __device__ __forceinline__ int32_t row_tiles_of(const AttentionArgs& a, const Se
 }
 
 // Places of the line per workgroup.
-__device__ __forceinline__ uint32_t quota_of(const Phase& p, uint32_t total) {
-    return max((total + p.workgroups - 1) / p.workgroups, 1u);
+__device__ __forceinline__ uint32_t quota_of(uint32_t total, uint32_t workgroups) {
+    return max((total + workgroups - 1) / workgroups, 1u);
+}
+
+// How many workgroups of a launch of two phases work on prefixes; the others work on own tokens. A prefix unit leaves as
+// many bytes of parts as four hold of keys, so that a workgroup takes no fewer than two of them; beyond that the phases
+// share the workgroups by their units' costs.
+__device__ __forceinline__ uint32_t prefix_workgroups(const Phase& own, const Phase& prefix, uint32_t own_total,
+                                                      uint32_t prefix_total) {
+    const uint32_t all = own.workgroups, most = (prefix_total + 1) / 2;
+    if (most + own_total <= all) {
+        return most;
+    }
+    const int down = max(0, 15 - __builtin_clz(max(own_total, prefix_total) | 1));   // 17 bits of each are kept
+    const uint32_t a = (prefix_total >> down) * prefix.weight, b = (own_total >> down) * own.weight;
+    const uint32_t share = (all * a + (a + b) / 2) / max(a + b, 1u);
+    return min(min(max(share, 1u), all - 1), most);
 }
 
 // Whether an item keeps its cuts, and where the cut at place c goes that lies in the item of places
@@ -288,16 +304,31 @@ __device__ __forceinline__ Sequence uniform(const Sequence& q) {
     return r;
 }
 
-// Calls body(segment) for every segment of phase `which` that this workgroup has, in order; all threads take part.
+// The places of a phase's line. All threads call it; the cells hold its last chunk then.
+template <int kWaves>
+__device__ __forceinline__ uint32_t line_total(int which, LineCells<kWaves>& cells) {
+    const Launch& l = fresh();
+    uint32_t units = 0, items = 0;
+#pragma unroll 1
+    for (int32_t chunk = 0; chunk < l.p[which].sequences; chunk += kSeqChunk) {
+        line_chunk(l.a, l.p[which], chunk, units, items, cells);
+        const int32_t count = min(kSeqChunk, l.p[which].sequences - chunk);
+        units = uniform(cells.units[count]), items = uniform(cells.items[count]);
+    }
+    return units;
+}
+
+// Calls body(segment) for every segment of phase `which` that workgroup w of those that share it has, in order; all
+// threads take part.
 //
 // What runs once per workgroup or item costs as much as its instructions' way from memory, so this is kept short:
 // sequences are read once and wait in LDS, and one copy of each step serves all cases.
 template <int kWaves, typename Body>
-__device__ __forceinline__ void for_segments(int which, LineCells<kWaves>& cells, Body&& body) {
+__device__ __forceinline__ void for_segments(int which, uint32_t w, uint32_t workgroups, LineCells<kWaves>& cells,
+                                             Body&& body) {
     const AttentionArgs& a = fresh().a;
     const Phase& p = fresh().p[which];
     const bool alike = p.mode == kSlots;   // every sequence is as long: places are divided, not searched
-    const uint32_t w = blockIdx.x;
     uint32_t total = p.alike_total, quota = 0, at = 0, end = 0, units_before = 0, items_before = 0;
     int32_t chunk = 0;
     bool known = false, starting = true;
@@ -314,7 +345,7 @@ __device__ __forceinline__ void for_segments(int which, LineCells<kWaves>& cells
                 continue;
             }
             total = alike ? total : units_before;
-            quota = quota_of(p, total);
+            quota = quota_of(total, workgroups);
             at = w * quota, end = at + quota;
             known = true;
             if (at >= total) {
