@@ -9,8 +9,8 @@ template <typename T, int kDim, int kTiles>
 __global__ __launch_bounds__(narrow::kWaves * 64, (narrow::groups_of<kDim, kTiles>())) void narrow_kernel(const Launch) {
     __shared__ __align__(16) char s_data[narrow::lds_bytes<kDim, kTiles>()];
     __shared__ __align__(16) char s_stats[narrow::stats_bytes<kTiles>()];
-    __shared__ LineCells<narrow::kWaves> s_line;
-    narrow::run<T, kDim, kTiles>(0, blockIdx.x, gridDim.x, s_data, s_stats, s_line);
+    __shared__ LineCells<narrow::kWaves, 255> s_line;
+    narrow::run<T, kDim, kTiles>(0, blockIdx.x, gridDim.x, false, 0, s_data, s_stats, s_line);
 }
 
 template <typename T, int kDim>

@@ -22,16 +22,17 @@ template <typename T, int kDim, bool kFew>
 __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void pair_kernel(const Launch) {
     __shared__ __align__(16) char s_data[data_bytes<kDim>()];
     __shared__ __align__(16) char s_stats[narrow::stats_bytes<1>()];
-    __shared__ LineCells<kWaves> s_line;
-    const uint32_t prefix_total = line_total(1, s_line), own_total = line_total(0, s_line);
+    __shared__ LineCells<kWaves, 128> s_line[2];
+    uint32_t totals[2];
+    line_totals(totals, s_line);
     const Launch& l = fresh();
-    const uint32_t share = prefix_workgroups(l.p[0], l.p[1], own_total, prefix_total), b = blockIdx.x;
+    const uint32_t share = prefix_workgroups(l.p[0], l.p[1], totals[0], totals[1]), b = blockIdx.x;
     if (kFew && b >= share) {
-        narrow::run<T, kDim, 1>(0, b - share, gridDim.x - share, s_data, s_stats, s_line);
+        narrow::run<T, kDim, 1>(0, b - share, gridDim.x - share, true, totals[0], s_data, s_stats, s_line[0]);
     } else {
         const int which = b < share ? 1 : 0;
-        wide::run<T, kDim, kWaves>(which, which == 1 ? b : b - share, which == 1 ? share : gridDim.x - share, s_data,
-                                   s_line);
+        wide::run<T, kDim, kWaves>(which, which == 1 ? b : b - share, which == 1 ? share : gridDim.x - share, true,
+                                   totals[which], s_data, s_line[which]);
     }
 }
 

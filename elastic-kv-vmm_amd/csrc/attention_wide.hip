@@ -7,8 +7,8 @@ namespace {
 template <typename T, int kDim, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void wide_kernel(const Launch) {
     __shared__ __align__(16) char s_data[wide::lds_bytes<kDim>()];
-    __shared__ LineCells<kWaves> s_line;
-    wide::run<T, kDim, kWaves>(0, blockIdx.x, gridDim.x, s_data, s_line);
+    __shared__ LineCells<kWaves, 255> s_line;
+    wide::run<T, kDim, kWaves>(0, blockIdx.x, gridDim.x, false, 0, s_data, s_line);
 }
 
 template <typename T, int kDim>

@@ -88,7 +88,6 @@ struct Launch {
     Phase p[2];        // own tokens (or all), prefixes
 };
 
-constexpr int kSeqChunk = 256;       // sequences that a workgroup holds at a time
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;       // bits by which a weight may pass 1 before its row is scaled again
 
@@ -234,56 +233,76 @@ __device__ __forceinline__ int32_t seen_by(const Sequence& q, int32_t i) {
     return min(max(q.newest - q.count + i + 2, 0), q.own);
 }
 
-template <int kWaves>
+// A line's sequences, kChunk at a time.
+template <int kWaves, int kChunk>
 struct LineCells {
-    uint32_t units[kSeqChunk + 1];     // first place of each sequence of the chunk
-    uint32_t items[kSeqChunk + 1];
+    uint32_t units[kChunk + 1];        // first place of each sequence of the chunk
+    uint32_t items[kChunk + 1];
     uint32_t sums[2][kWaves];
-    Sequence sequences[kSeqChunk];
+    Sequence sequences[kChunk];
 };
 
-// The sequences of one chunk, a thread each, and their places and items, given what lies before them. All threads call
-// it.
-template <int kWaves>
-__device__ __forceinline__ void line_chunk(const AttentionArgs& a, const Phase& p, int32_t chunk, uint32_t units_before,
-                                           uint32_t items_before, LineCells<kWaves>& cells) {
-    const int tid = threadIdx.x, wave = tid >> 6;
-    const int32_t count = min(kSeqChunk, p.sequences - chunk);
+// The sequence that this thread has of a chunk, left in the cells, with its places and items.
+struct Share {
     uint32_t units = 0, items = 0;
-    __syncthreads();   // the cells' last use
-    if (tid < count) {
+    uint32_t unit_sum = 0, item_sum = 0;   // inclusive over the wave
+};
+
+template <int kWaves, int kChunk>
+__device__ __forceinline__ Share line_read(const AttentionArgs& a, const Phase& p, int32_t chunk,
+                                           LineCells<kWaves, kChunk>& cells) {
+    Share r;
+    const int tid = threadIdx.x;
+    if (tid < min(kChunk, p.sequences - chunk)) {
         const Sequence q = sequence_of(a, p.mode, chunk + tid);
         cells.sequences[tid] = q;
-        items = a.kv_heads * row_tiles_of(a, q, p);
-        units = items * units_of(q, p);
+        r.items = a.kv_heads * row_tiles_of(a, q, p);
+        r.units = r.items * units_of(q, p);
     }
-    const uint32_t unit_sum = wave_scan<kAdd>(units), item_sum = wave_scan<kAdd>(items);
-    if ((tid & 63) == 63) {
-        cells.sums[0][wave] = unit_sum, cells.sums[1][wave] = item_sum;
+    return r;
+}
+
+template <int kWaves, int kChunk>
+__device__ __forceinline__ void line_scan(Share& r, LineCells<kWaves, kChunk>& cells) {
+    r.unit_sum = wave_scan<kAdd>(r.units), r.item_sum = wave_scan<kAdd>(r.items);
+    if ((threadIdx.x & 63) == 63) {
+        cells.sums[0][threadIdx.x >> 6] = r.unit_sum, cells.sums[1][threadIdx.x >> 6] = r.item_sum;
     }
-    __syncthreads();
-    uint32_t unit_at = units_before + unit_sum - units, item_at = items_before + item_sum - items;
+}
+
+// After a barrier: the chunk's first places, given what lies before it.
+template <int kWaves, int kChunk>
+__device__ __forceinline__ void line_write(const Phase& p, int32_t chunk, const Share& r, uint32_t units_before,
+                                           uint32_t items_before, LineCells<kWaves, kChunk>& cells) {
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int32_t count = min(kChunk, p.sequences - chunk);
+    uint32_t unit_at = units_before + r.unit_sum - r.units, item_at = items_before + r.item_sum - r.items;
 #pragma unroll
     for (int w = 0; w < kWaves - 1; ++w) {
         unit_at += w < wave ? cells.sums[0][w] : 0;
         item_at += w < wave ? cells.sums[1][w] : 0;
     }
-    // The first thread past the last sequence (or the last one) leaves the end.
-    if (tid <= count && tid < kSeqChunk) {
+    // The thread after the last sequence's leaves the end (there is one: a chunk has fewer sequences than threads).
+    static_assert(kChunk < kWaves * 64, "a thread past the chunk's last sequence");
+    if (tid <= count) {
         cells.units[tid] = unit_at, cells.items[tid] = item_at;
-    }
-    if (tid == kSeqChunk - 1) {
-        cells.units[kSeqChunk] = unit_at + units, cells.items[kSeqChunk] = item_at + items;
-    }
-    if (blockIdx.x == 0 && p.unit_starts != nullptr) {
-        if (tid < count) {
+        if (blockIdx.x == 0 && p.unit_starts != nullptr) {
+            // The end is written over by the next chunk's first.
             p.unit_starts[chunk + tid] = unit_at, p.item_starts[chunk + tid] = item_at;
         }
-        if (tid == count - 1) {      // overwritten by the next chunk's first, or the end
-            p.unit_starts[chunk + count] = unit_at + units, p.item_starts[chunk + count] = item_at + items;
-        }
     }
-    __syncthreads();
+}
+
+// The sequences of one chunk and their places. All threads call it.
+template <int kWaves, int kChunk>
+__device__ __forceinline__ void line_chunk(const AttentionArgs& a, const Phase& p, int32_t chunk, uint32_t units_before,
+                                           uint32_t items_before, LineCells<kWaves, kChunk>& cells) {
+    lds_barrier();   // the cells' last use
+    Share r = line_read(a, p, chunk, cells);
+    line_scan(r, cells);
+    lds_barrier();
+    line_write(p, chunk, r, units_before, items_before, cells);
+    lds_barrier();
 }
 
 // What a workgroup does next: key units [begin, end) of the `units` of one item.
@@ -304,47 +323,67 @@ __device__ __forceinline__ Sequence uniform(const Sequence& q) {
     return r;
 }
 
-// The places of a phase's line. All threads call it; the cells hold its last chunk then.
-template <int kWaves>
-__device__ __forceinline__ uint32_t line_total(int which, LineCells<kWaves>& cells) {
+// The places of both phases' lines; the cells hold their first chunks where the lines have no more. All threads call it.
+template <int kWaves, int kChunk>
+__device__ __forceinline__ void line_totals(uint32_t (&totals)[2], LineCells<kWaves, kChunk> (&cells)[2]) {
     const Launch& l = fresh();
-    uint32_t units = 0, items = 0;
+    uint32_t items[2] = {0, 0};
+    totals[0] = totals[1] = 0;
+    const int32_t longest = max(l.p[0].sequences, l.p[1].sequences);
 #pragma unroll 1
-    for (int32_t chunk = 0; chunk < l.p[which].sequences; chunk += kSeqChunk) {
-        line_chunk(l.a, l.p[which], chunk, units, items, cells);
-        const int32_t count = min(kSeqChunk, l.p[which].sequences - chunk);
-        units = uniform(cells.units[count]), items = uniform(cells.items[count]);
+    for (int32_t chunk = 0; chunk < longest; chunk += kChunk) {
+        // Both lines' loads are under way together.
+        lds_barrier();
+        Share own = line_read(l.a, l.p[0], chunk, cells[0]), prefix = line_read(l.a, l.p[1], chunk, cells[1]);
+        line_scan(own, cells[0]);
+        line_scan(prefix, cells[1]);
+        lds_barrier();
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            if (chunk < l.p[side].sequences) {
+                line_write(l.p[side], chunk, side == 0 ? own : prefix, totals[side], items[side], cells[side]);
+            }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const int32_t count = min(kChunk, l.p[side].sequences - chunk);
+            if (count > 0) {
+                totals[side] = uniform(cells[side].units[count]), items[side] = uniform(cells[side].items[count]);
+            }
+        }
     }
-    return units;
 }
 
 // Calls body(segment) for every segment of phase `which` that workgroup w of those that share it has, in order; all
-// threads take part.
+// threads take part. A phase whose sequences are one chunk may have its total and cells from line_totals.
 //
 // What runs once per workgroup or item costs as much as its instructions' way from memory, so this is kept short:
 // sequences are read once and wait in LDS, and one copy of each step serves all cases.
-template <int kWaves, typename Body>
-__device__ __forceinline__ void for_segments(int which, uint32_t w, uint32_t workgroups, LineCells<kWaves>& cells,
-                                             Body&& body) {
+template <int kWaves, int kChunk, typename Body>
+__device__ __forceinline__ void for_segments(int which, uint32_t w, uint32_t workgroups, bool read, uint32_t total_read,
+                                             LineCells<kWaves, kChunk>& cells, Body&& body) {
     const AttentionArgs& a = fresh().a;
     const Phase& p = fresh().p[which];
     const bool alike = p.mode == kSlots;   // every sequence is as long: places are divided, not searched
-    uint32_t total = p.alike_total, quota = 0, at = 0, end = 0, units_before = 0, items_before = 0;
+    const bool ready = alike || (read && p.sequences <= kChunk);
+    uint32_t total = alike ? p.alike_total : total_read, quota = 0, at = 0, end = 0, units_before = 0, items_before = 0;
     int32_t chunk = 0;
     bool known = false, starting = true;
 #pragma unroll 1
     while (true) {
-        const int32_t count = min(kSeqChunk, p.sequences - chunk);
-        if (!alike) {
+        const int32_t count = min(kChunk, p.sequences - chunk);
+        if (!ready) {
             line_chunk(a, p, chunk, units_before, items_before, cells);
             units_before = uniform(cells.units[count]), items_before = uniform(cells.items[count]);
         }
         if (!known) {
-            if (!alike && chunk + kSeqChunk < p.sequences) {
-                chunk += kSeqChunk;
+            if (!ready && chunk + kChunk < p.sequences) {
+                chunk += kChunk;
                 continue;
             }
-            total = alike ? total : units_before;
+            total = ready ? total : units_before;
+            units_before = total;
             quota = quota_of(total, workgroups);
             at = w * quota, end = at + quota;
             known = true;
@@ -421,7 +460,7 @@ __device__ __forceinline__ void for_segments(int which, uint32_t w, uint32_t wor
                 return;
             }
         }
-        chunk += kSeqChunk;
+        chunk += kChunk;
     }
 }
 

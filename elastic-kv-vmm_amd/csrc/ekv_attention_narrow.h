@@ -83,8 +83,9 @@ constexpr int stats_bytes() {
     return 2 * kWaves * kTiles * 16 * static_cast<int>(sizeof(float));
 }
 
-template <typename T, int kDim, int kTiles>
-__device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, char* s_data, char* stats, LineCells<kWaves>& cells) {
+template <typename T, int kDim, int kTiles, int kChunk>
+__device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, bool read, uint32_t total,
+                                    char* s_data, char* stats, LineCells<kWaves, kChunk>& cells) {
     constexpr int kSteps = kDim / 32;      // matrix steps of the first product
     constexpr int kCols = kDim / 16;       // 16-column pieces of the output
     // Head sizes between kDim and the next smaller class end in one of the last steps.
@@ -95,7 +96,7 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
     char* const values = s_data + wave * (kKeys * Rows<kDim>::kBytes);
     const char* const zeros = reinterpret_cast<const char*>(zero_row);
 
-    for_segments(which, w, workgroups, cells, [&](const Segment& g) {
+    for_segments(which, w, workgroups, read, total, cells, [&](const Segment& g) {
         const int lane = hidden(threadIdx.x) & 63, col = lane & 15, quad = lane >> 4;
         const AttentionArgs& a = fresh().a;
         const int pieces = a.dim >> 3;

@@ -50,8 +50,9 @@ constexpr int lds_bytes() {
 }
 
 // Workgroup w's part of phase `which` of the launch. s_data: lds_bytes() of LDS.
-template <typename T, int kDim, int kWaves>
-__device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, char* s_data, LineCells<kWaves>& cells) {
+template <typename T, int kDim, int kWaves, int kChunk>
+__device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, bool read, uint32_t total,
+                                    char* s_data, LineCells<kWaves, kChunk>& cells) {
     constexpr int kSteps = kDim / 16;              // matrix steps of the first product
     constexpr int kCols = kDim / 32;               // 32-column pieces of the output
     constexpr int kRowThreads = Tile<kDim>::kBytes / 16;               // threads that load a key's row
@@ -63,7 +64,7 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
     const char* const zeros = reinterpret_cast<const char*>(zero_row);
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
 
-    for_segments(which, w, workgroups, cells, [&](const Segment& g) {
+    for_segments(which, w, workgroups, read, total, cells, [&](const Segment& g) {
         const int tid = hidden(threadIdx.x), lane = tid & 63, col = lane & 31, half = lane >> 5;
         const int load_key = tid / kRowThreads, load_piece = tid % kRowThreads;
         const int write_at = Tile<kDim>::place(load_key, load_piece);
