@@ -80,9 +80,24 @@ __device__ __forceinline__ int64_t workgroup_before(int64_t value, uint32_t (*ce
     return before + static_cast<int64_t>(low_sum - low) + (static_cast<int64_t>(high_sum - high) << 20);
 }
 
-// The last of the first `count` entries that is at most `value` (entry 0 is).
-__device__ __forceinline__ int last_not_above(const int64_t* entries, int count, int64_t value) {
-    int low = 0, high = count;
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+// The first slot of a row's page `column`, -1 for none: a page that the row had is in its table, a new one in the list.
+__device__ __forceinline__ int64_t page_slot(const TableArgs& a, int64_t head, int64_t row, int64_t base, uint32_t column,
+                                             uint32_t held) {
+    int64_t id;
+    if (column < held) {
+        const int64_t entry = row * a.table_row + int64_t{column} * a.table_col;
+        id = a.table64 ? static_cast<const int64_t*>(a.table)[entry] : static_cast<const int32_t*>(a.table)[entry];
+    } else {
+        const int64_t from = head + base + (column - held);
+        id = from >= 0 && from < a.free_count ? a.free_pages[from] : 0;
+    }
+    return id >= 1 ? id * a.page_size : -1;
+}
+
+// The last of entries low .. high - 1 that is at most `value` (entry `low` is).
+__device__ __forceinline__ int last_not_above(const int64_t* entries, int low, int high, int64_t value) {
     while (high - low > 1) {
         const int mid = (low + high) >> 1;
         if (entries[mid] <= value) {
@@ -94,20 +109,39 @@ __device__ __forceinline__ int last_not_above(const int64_t* entries, int count,
     return low;
 }
 
-__global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs a) {
+// The same among the first `count` entries for a value that a wave shares: its lanes look at 64 entries at a time.
+__device__ __forceinline__ int wave_last_not_above(const int64_t* entries, int count, int64_t value) {
+    const int lane = threadIdx.x & 63, step = (count + 63) >> 6;
+    const int coarse = lane * step;
+    const int base = (__popcll(__ballot(coarse < count && entries[min(coarse, count - 1)] <= value)) - 1) * step;
+    const int fine = base + lane;
+    return base + __popcll(__ballot(lane < step && fine < count && entries[min(fine, count - 1)] <= value)) - 1;
+}
+
+// The kernel's arguments. They are more words than a wave has scalar registers: hidden from the compiler where they come
+// from, each part of the kernel loads what it needs, instead of one load of all and spills.
+__device__ __forceinline__ const TableArgs& arguments() {
+    auto at = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const TableArgs*)(at);
+}
+
+__global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs) {
     __shared__ int64_t s_start[kChunk];    // first token of each row of the chunk
     __shared__ int64_t s_base[kChunk];     // first new page of each row
     __shared__ int32_t s_length[kChunk], s_row[kChunk];
     __shared__ uint32_t s_cells[2][kWaves];
     const int tid = threadIdx.x;
     const bool first = blockIdx.x == 0;
-    const int64_t head = a.free_head[0];
-    const int64_t room = a.columns * a.page_size;
+    const int64_t head = arguments().free_head.fetch(0);
+    const int64_t batch = arguments().batch;
     int64_t token_base = 0, page_base = 0;
     int32_t flags = 0;
 
-    for (int64_t chunk = 0; chunk < a.batch; chunk += kChunk) {
-        const int count = static_cast<int>(min(static_cast<int64_t>(kChunk), a.batch - chunk));
+    for (int64_t chunk = 0; chunk < batch; chunk += kChunk) {
+        const int count = static_cast<int>(min(static_cast<int64_t>(kChunk), batch - chunk));
+        const TableArgs& a = arguments();
+        const int64_t room = a.columns * a.page_size;
         // Thread t sums rows t * kPer .. + kPer - 1 of the chunk; what it knows of each waits in its places in LDS.
         int64_t token_sum = 0, page_sum = 0;
 #pragma unroll
@@ -116,7 +150,8 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
             const bool live = at < count;
             const int64_t b = chunk + (live ? at : 0);
             const int64_t length = a.lengths.fetch(b), added = a.added.fetch(b);
-            const int64_t row = a.rows.data != nullptr ? a.rows.fetch(b) : b;
+            const int64_t given = (a.rows.data != nullptr ? a.rows : a.lengths).fetch(b);   // in flight with the others
+            const int64_t row = a.rows.data != nullptr ? given : b;
             const bool good = row >= 0 && row < a.requests && length >= 0 && length <= room && added >= 0;
             const int64_t held = live ? min(max(length, int64_t{0}), room) : 0;
             const int64_t fits = live && good ? min(added, room - held) : 0;
@@ -154,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
         const int64_t page_end = page_base + page_total;
         for (int64_t u = page_base + int64_t{blockIdx.x} * kThreads + tid; u < page_end;
              u += int64_t{gridDim.x} * kThreads) {
-            const int r = last_not_above(s_base, count, u);
+            const int r = last_not_above(s_base, 0, count, u);
             const int64_t from = head + u;
             const int64_t id = from >= 0 && from < a.free_count ? a.free_pages[from] : 0;
             const uint32_t held = a.page.div(static_cast<uint32_t>(s_length[r]) + a.page.divisor - 1);
@@ -172,9 +207,47 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
         tile += (int64_t{blockIdx.x} + gridDim.x - tile % gridDim.x) % gridDim.x;
         for (; tile * kTile < token_end; tile += gridDim.x) {
             const int64_t t = tile * kTile + tid * kTokens;
-            int r = t >= token_base && t < token_end ? last_not_above(s_start, count, t) : 0;
+            // Rows of the wave's first and last token: long rows leave each lane little to search.
+            const int64_t wave_first = max(tile * kTile + (tid & ~63) * kTokens, token_base);
+            const int64_t wave_last = min(tile * kTile + (tid | 63) * kTokens + kTokens, token_end) - 1;
+            if (wave_first > wave_last) {
+                continue;
+            }
+            const int row_first = wave_last_not_above(s_start, count, wave_first);
+            const int row_last = wave_last_not_above(s_start, count, wave_last);
+            int r = t >= token_base && t < token_end ? last_not_above(s_start, row_first, row_last + 1, t) : 0;
+            const bool whole = t >= token_base && t + kTokens <= token_end;
+            if (a.vector && whole && a.page_size >= kTokens &&
+                (r + 1 < count ? s_start[r + 1] : token_end) >= t + kTokens) {
+                // Four tokens of one row, on one page or two.
+                const uint32_t length = static_cast<uint32_t>(s_length[r]);
+                const uint32_t position = length + static_cast<uint32_t>(t - s_start[r]);
+                const uint32_t column = a.page.div(position), offset = position - column * a.page.divisor;
+                const bool crosses = offset + kTokens > a.page.divisor;
+                const uint32_t held = a.page.div(length + a.page.divisor - 1);
+                const int64_t page = page_slot(a, head, s_row[r], s_base[r], column, held);
+                int64_t next = page;
+                if (crosses) {
+                    next = page_slot(a, head, s_row[r], s_base[r], column + 1, held);
+                }
+                i32x4 slot, place;
+#pragma unroll
+                for (int k = 0; k < kTokens; ++k) {
+                    const bool here = offset + k < a.page.divisor;
+                    const int64_t first_slot = here ? page : next;
+                    const int64_t value = first_slot + (here ? offset + k : offset + k - a.page.divisor);
+                    const bool fits = value <= 0x7fffffff;
+                    flags |= first_slot >= 0 && !fits ? EKV_TABLES_SLOT_RANGE : 0;
+                    slot[k] = first_slot >= 0 && fits ? static_cast<int32_t>(value) : -1;
+                    place[k] = static_cast<int32_t>(position + k);
+                }
+                *reinterpret_cast<i32x4*>(static_cast<int32_t*>(a.slots.data) + t) = slot;
+                if (a.has_positions) {
+                    *reinterpret_cast<i32x4*>(static_cast<int32_t*>(a.positions.data) + t) = place;
+                }
+                continue;
+            }
             int32_t slot32[kTokens], position32[kTokens];
-            bool whole = t >= token_base && t + kTokens <= token_end;
 #pragma unroll
             for (int k = 0; k < kTokens; ++k) {
                 const int64_t at = t + k;
@@ -188,16 +261,8 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
                 const uint32_t position = length + static_cast<uint32_t>(at - s_start[r]);
                 const uint32_t column = a.page.div(position);
                 const uint32_t held = a.page.div(length + a.page.divisor - 1);
-                int64_t id;
-                if (column < held) {
-                    const int64_t entry = s_row[r] * a.table_row + int64_t{column} * a.table_col;
-                    id = a.table64 ? static_cast<const int64_t*>(a.table)[entry]
-                                   : static_cast<const int32_t*>(a.table)[entry];
-                } else {
-                    const int64_t from = head + s_base[r] + (column - held);
-                    id = from >= 0 && from < a.free_count ? a.free_pages[from] : 0;
-                }
-                int64_t slot = id >= 1 ? id * a.page_size + (position - column * a.page.divisor) : -1;
+                const int64_t page = page_slot(a, head, s_row[r], s_base[r], column, held);
+                int64_t slot = page >= 0 ? page + (position - column * a.page.divisor) : -1;
                 if (!a.slots.is64 && slot > 0x7fffffff) {
                     flags |= EKV_TABLES_SLOT_RANGE;
                     slot = -1;
@@ -214,7 +279,6 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
                 }
             }
             if (a.vector && whole) {
-                typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
                 *reinterpret_cast<i32x4*>(static_cast<int32_t*>(a.slots.data) + t) =
                     i32x4{slot32[0], slot32[1], slot32[2], slot32[3]};
                 if (a.has_positions) {
@@ -228,6 +292,7 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
         __syncthreads();   // the chunk's sums are read before the next chunk's replace them
     }
 
+    const TableArgs& a = arguments();
     // Places of the map that no token has.
     for (int64_t t = token_base + int64_t{blockIdx.x} * kThreads + tid; t < a.capacity;
          t += int64_t{gridDim.x} * kThreads) {
