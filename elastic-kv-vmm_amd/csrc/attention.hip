@@ -17,7 +17,8 @@
 namespace ekv {
 namespace {
 
-constexpr int kMergeThreads = 256;
+constexpr int kMergeThreads = 256, kMergeColumns = 8;
+constexpr int kMergeByToken = 16;    // workgroups per compute unit up to which the merge goes by tokens
 
 // The workgroups that hold a token's parts of one phase, and where.
 struct Parts {
@@ -81,20 +82,85 @@ __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p
     r.count = static_cast<int32_t>(count);
     if (p.direct != 0 && count == 1) {
         r.count = -1;
-    } else if (slot + count > static_cast<uint32_t>(p.slots)) {
+    } else if (count > static_cast<uint32_t>(p.slots) || slot > static_cast<uint32_t>(p.slots) - count) {
         r.count = 0;            // only if the starts were not in order
     }
     return r;
 }
 
-// One workgroup per (query token, KV head). A thread joins four elements of a row over parts i, i + splits, ..., the own
-// parts first and then the prefix's, eight parts' loads in flight; the splits of a unit are joined through LDS. What
-// bounds it is the latency of those loads (a row has as many parts as workgroups shared its keys), so a small row's parts
-// are spread over the threads that it leaves idle.
+// Four elements of a row, joined over some of its parts.
+struct Joined {
+    float top = -INFINITY, sum = 0;
+    f32x4 value = {0, 0, 0, 0};
+
+    // Parts split, split + splits, ... of `count`, the own ones first and then the prefix's, the loads of kBatch parts in
+    // flight.
+    template <int kBatch>
+    __device__ __forceinline__ void join(const Parts& mine, const Parts& theirs, int32_t own_count, int32_t count,
+                                         uint32_t quad, int32_t split, int32_t splits) {
+        const uint32_t my_place = mine.place(quad), their_place = theirs.place(quad);
+        for (int32_t i = split; i < count; i += splits * kBatch) {
+            float part_top[kBatch], part_sum[kBatch];
+            f32x4 part_value[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int32_t at = i + k * splits;
+                const bool there = at < count;
+                const bool first = at < own_count;
+                const int64_t place = there ? (first ? at : at - own_count) : 0;
+                const bool from_own = there ? first : own_count > 0;
+                const float* stats = (from_own ? mine.stats : theirs.stats) + place * (from_own ? mine.step : theirs.step);
+                const float* base = (from_own ? mine.base : theirs.base) + place * (from_own ? mine.step : theirs.step);
+                part_top[k] = stats[0];
+                part_sum[k] = stats[from_own ? mine.row_tile : theirs.row_tile];
+                part_value[k] = *reinterpret_cast<const f32x4*>(base + (from_own ? my_place : their_place));
+                part_top[k] = there ? part_top[k] : -INFINITY;
+            }
+            float most = top;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                most = fmaxf(most, part_top[k]);
+            }
+            const float safe = rescale(most);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                // A part that saw nothing holds zeros, or NaN where its scores were; only one that is not there is left out.
+                const float factor = exp2f(part_top[k] - safe);
+                const bool there = i + k * splits < count;
+                sum += there ? part_sum[k] * factor : 0.0f;
+                value += there ? part_value[k] * factor : f32x4{0, 0, 0, 0};
+            }
+        }
+    }
+
+    // Makes `most` the score that the sums are relative to; the score to subtract (0 where no key was seen).
+    __device__ __forceinline__ float rescale(float most) {
+        const float safe = most == -INFINITY ? 0.0f : most;
+        const float keep = exp2f(top - safe);
+        sum *= keep;
+        value *= keep;
+        top = most;
+        return safe;
+    }
+
+    template <typename T>
+    __device__ __forceinline__ void write(const AttentionArgs& a, int32_t token, int32_t row_head, int32_t quad) const {
+        const float inverse = sum == 0 ? 0.0f : 1.0f / sum;
+        *reinterpret_cast<words2*>(a.out + token * a.o_token + row_head * a.o_head + quad * 8) =
+            words2{T::pack(value[0] * inverse, value[1] * inverse), T::pack(value[2] * inverse, value[3] * inverse)};
+        if (quad == 0 && a.lse != nullptr) {
+            a.lse[token * a.l_token + row_head * a.l_head] =
+                sum == 0 ? -INFINITY : (top - T::kShift + log2f(sum)) * kLn2;
+        }
+    }
+};
+
+// One workgroup per (query token, KV head), for launches whose every row has parts and for those of few tokens. What
+// bounds it is the latency of its loads (a row has as many parts as workgroups shared its keys), so a small row's parts
+// are spread over the threads that it leaves idle, and joined through LDS.
 template <typename T>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArgs a, const Phase own,
                                                                   const Phase prefix) {
-    constexpr int kBatch = 8;
     __shared__ f32x4 s_value[kMergeThreads];
     __shared__ float s_top[kMergeThreads], s_sum[kMergeThreads];
     const int32_t token = blockIdx.x, head = blockIdx.y;
@@ -126,7 +192,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
         const int32_t unit = begin + threadIdx.x - split * units;
         const bool live = unit < units && split < splits;
         // Rows first: their values lie side by side.
-        const int32_t quad = live ? a.share_div.div(unit) : 0, sub = live ? unit - quad * a.share : 0, element = quad * 4;
+        const int32_t quad = live ? a.share_div.div(unit) : 0, sub = live ? unit - quad * a.share : 0;
         Parts mine{}, theirs{};
         if (b >= 0) {
             mine = parts_of(a, own, own_workgroups, b, head, (token - own_first) * a.share + sub);
@@ -134,78 +200,109 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
         if (group >= 0) {
             theirs = parts_of(a, prefix, shared, group, head, (token - prefix_first) * a.share + sub);
         }
-        const uint32_t my_place = mine.place(quad), their_place = theirs.place(quad);
         const bool written = mine.count < 0;
         const int32_t own_count = max(mine.count, 0), count = live && !written ? own_count + theirs.count : 0;
-        float top = -INFINITY, sum = 0;
-        f32x4 value = {0, 0, 0, 0};
-        for (int32_t i = split; i < count; i += splits * kBatch) {
-            float part_top[kBatch], part_sum[kBatch];
-            f32x4 part_value[kBatch];
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                const int32_t at = i + k * splits;
-                const bool there = at < count;
-                const bool first = at < own_count;
-                const int64_t place = there ? (first ? at : at - own_count) : 0;
-                const bool from_own = there ? first : own_count > 0;
-                const float* stats = (from_own ? mine.stats : theirs.stats) + place * (from_own ? mine.step : theirs.step);
-                const float* base = (from_own ? mine.base : theirs.base) + place * (from_own ? mine.step : theirs.step);
-                part_top[k] = stats[0];
-                part_sum[k] = stats[from_own ? mine.row_tile : theirs.row_tile];
-                part_value[k] = *reinterpret_cast<const f32x4*>(base + (from_own ? my_place : their_place));
-                part_top[k] = there ? part_top[k] : -INFINITY;
-            }
-            float most = top;
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                most = fmaxf(most, part_top[k]);
-            }
-            const float safe = most == -INFINITY ? 0.0f : most;
-            const float keep = exp2f(top - safe);
-            sum *= keep;
-            value *= keep;
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                // A part that saw nothing holds zeros, or NaN where its scores were; only one that is not there is left out.
-                const float factor = exp2f(part_top[k] - safe);
-                const bool there = i + k * splits < count;
-                sum += there ? part_sum[k] * factor : 0.0f;
-                value += there ? part_value[k] * factor : f32x4{0, 0, 0, 0};
-            }
-            top = most;
-        }
+        Joined joined;
+        joined.template join<8>(mine, theirs, own_count, count, quad, split, splits);
         if (splits > 1) {
-            s_top[threadIdx.x] = top, s_sum[threadIdx.x] = sum, s_value[threadIdx.x] = value;
+            s_top[threadIdx.x] = joined.top, s_sum[threadIdx.x] = joined.sum, s_value[threadIdx.x] = joined.value;
             __syncthreads();
             if (split == 0) {
-                float most = top;
+                float most = joined.top;
                 for (int32_t k = 1; k < splits; ++k) {
                     most = fmaxf(most, s_top[threadIdx.x + k * units]);
                 }
-                const float safe = most == -INFINITY ? 0.0f : most;
-                const float keep = exp2f(top - safe);
-                sum *= keep;
-                value *= keep;
+                const float safe = joined.rescale(most);
                 for (int32_t k = 1; k < splits; ++k) {
                     const float factor = exp2f(s_top[threadIdx.x + k * units] - safe);
-                    sum += s_sum[threadIdx.x + k * units] * factor;
-                    value += s_value[threadIdx.x + k * units] * factor;
+                    joined.sum += s_sum[threadIdx.x + k * units] * factor;
+                    joined.value += s_value[threadIdx.x + k * units] * factor;
                 }
-                top = most;
             }
         }
-        if (!live || written || split > 0) {
+        if (live && !written && split == 0) {
+            joined.write<T>(a, token, head * a.share + sub, quad);
+        }
+    }
+}
+
+// The cuts of a launch of one phase: the column of workgroups w joins the item that workgroup w begins and others go on
+// with, if there is one; all other items are written already. The rows of tokens that belong to no batch row are zeroed
+// here.
+template <typename T>
+__global__ __launch_bounds__(kMergeThreads) void cuts_kernel(const AttentionArgs a, const Phase p) {
+    const uint32_t total = p.mode == kSlots ? p.alike_total : p.unit_starts[p.sequences];
+    const uint32_t quota = quota_of(total, p.workgroups), cut = (blockIdx.x + 1) * quota;
+    const int32_t columns = gridDim.y * kMergeThreads, column = blockIdx.y * kMergeThreads + threadIdx.x;
+    if (p.mode != kSlots && a.query_starts.data != nullptr) {
+        // The batch rows' tokens lie side by side: the others are in front of them and behind.
+        const int32_t front = a.batch > 0 ? first_token(a, 0) : 0, behind = a.batch > 0 ? first_token(a, a.batch) : 0;
+        const int32_t gap = front + a.tokens - behind, quads = a.dim >> 2;
+        for (int32_t i = blockIdx.x; i < gap; i += gridDim.x) {
+            const int32_t token = i < front ? i : behind + i - front;
+            for (int32_t unit = column; unit < a.heads * quads; unit += columns) {
+                const int32_t head = unit / quads;
+                Joined{}.write<T>(a, token, head, unit - head * quads);
+            }
+        }
+    }
+    if (cut >= total) {
+        return;
+    }
+    int32_t s;
+    uint32_t begin, units, items, local;
+    if (p.mode == kSlots) {
+        const uint32_t item = p.alike_units.div(cut);
+        s = p.alike_items.div(item);
+        items = p.alike_items.divisor, units = p.alike_units.divisor;
+        begin = item * units, local = item - s * items;
+    } else {
+        int32_t low = 0, high = p.sequences;
+        while (high - low > 1) {
+            const int32_t mid = (low + high) >> 1;
+            if (p.unit_starts[mid] <= cut) {
+                low = mid;
+            } else {
+                high = mid;
+            }
+        }
+        s = low;
+        items = p.item_starts[s + 1] - p.item_starts[s];
+        if (items == 0) {
+            return;
+        }
+        begin = p.unit_starts[s];
+        units = max((p.unit_starts[s + 1] - begin) / items, 1u);
+        local = (cut - begin) / units;
+        begin += local * units;
+    }
+    if (begin == cut || begin < cut - quota || !keeps_cuts(units, quota)) {
+        return;
+    }
+    const Sequence q = sequence_of(a, p.mode, s);
+    const int32_t row_tiles = max(items / a.kv_heads, 1u), head = local / row_tiles;
+    const int32_t row_begin = (local - head * row_tiles) << p.row_shift, rows = q.count * a.share - row_begin;
+    Parts parts = parts_of(a, p, p.workgroups, s, head, row_begin);
+    const float* stats = parts.stats;
+    const int32_t quads = a.dim >> 2, count = parts.count;
+    if (count < 1) {
+        return;
+    }
+    for (int32_t unit = column; unit < quads << p.row_shift; unit += columns) {
+        // Four rows of all quads: a wave reads pieces of 64 bytes and writes pieces of a row.
+        const int32_t four = (unit >> 2) / quads, quad = (unit >> 2) - four * quads, row = four * 4 + (unit & 3);
+        if (row >= rows) {
             continue;
         }
-        const int32_t row_head = head * a.share + sub;
-        const float inverse = sum == 0 ? 0.0f : 1.0f / sum;
-        *reinterpret_cast<words2*>(a.out + token * a.o_token + row_head * a.o_head + element * 2) =
-            words2{T::pack(value[0] * inverse, value[1] * inverse), T::pack(value[2] * inverse, value[3] * inverse)};
-        if (element == 0 && a.lse != nullptr) {
-            a.lse[token * a.l_token + row_head * a.l_head] =
-                sum == 0 ? -INFINITY : (top - T::kShift + log2f(sum)) * kLn2;
+        parts.inside = row, parts.stats = stats + row;
+        Joined joined;
+        if (count <= 2) {
+            joined.join<2>(parts, parts, count, count, quad, 0, 1);
+        } else {
+            joined.join<8>(parts, parts, count, count, quad, 0, 1);
         }
+        const int32_t at = row_begin + row, token = a.share_div.div(at);
+        joined.write<T>(a, q.first + token, head * a.share + at - token * a.share, quad);
     }
 }
 
@@ -508,11 +605,21 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
     } else {
         launch_wide(Launch{a, {plan.own, {}}}, dtype, stream);
     }
-    const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.kv_heads));
+    const auto merge = [&]<typename T>(T) {
+        const auto on = static_cast<hipStream_t>(stream);
+        // By tokens the time goes with the rows, by cuts with the workgroups.
+        if (!plan.pair && int64_t{a.tokens} * a.kv_heads > kComputeUnits * kMergeByToken) {
+            const dim3 grid(plan.own.workgroups, kMergeColumns);
+            cuts_kernel<T><<<grid, kMergeThreads, 0, on>>>(a, plan.own);
+        } else {
+            const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.kv_heads));
+            merge_kernel<T><<<grid, kMergeThreads, 0, on>>>(a, plan.own, plan.prefix);
+        }
+    };
     if (dtype == EKV_BFLOAT16) {
-        merge_kernel<Bf16><<<grid, kMergeThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);
+        merge(Bf16{});
     } else {
-        merge_kernel<F16><<<grid, kMergeThreads, 0, static_cast<hipStream_t>(stream)>>>(a, plan.own, plan.prefix);
+        merge(F16{});
     }
     check_hip(hipGetLastError(), "launch attention merge");
     return 0;
