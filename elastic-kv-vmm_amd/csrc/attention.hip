@@ -13,6 +13,7 @@
 #include "ekv_mfma.h"
 
 #include <algorithm>
+#include <limits>
 
 namespace ekv {
 namespace {
@@ -381,9 +382,6 @@ AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, i
     a.kv_heads = static_cast<int32_t>(kv_heads);
     a.share = a.heads / a.kv_heads;
     a.share_div = FastDiv(static_cast<uint32_t>(a.share));
-    if (!std::isfinite(scale)) {
-        throw std::invalid_argument("scale must be finite");
-    }
     if (planes == nullptr) {
         throw std::invalid_argument("planes are required");
     }
@@ -449,8 +447,12 @@ AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, i
         a.lse = static_cast<float*>(lse.data);
         a.l_token = lse.stride[0], a.l_head = lse.stride[1];
     }
-    // Log2 e: the kernels' exponentials have base two. A negative scale changes the queries' signs.
-    a.scale = static_cast<float>(std::fabs(scale) * 1.4426950408889634);
+    // Log2 e: the kernels' exponentials have base two. A negative scale changes the queries' signs; zero is taken as the
+    // smallest number, since an unseen key's score is minus infinity, which zero would make NaN.
+    a.scale = std::fmax(static_cast<float>(std::fabs(scale) * 1.4426950408889634), std::numeric_limits<float>::min());
+    if (!std::isfinite(a.scale)) {
+        throw std::invalid_argument("scale must be finite");
+    }
     a.flip = scale < 0 ? 0x80008000u : 0;
     return a;
 }
