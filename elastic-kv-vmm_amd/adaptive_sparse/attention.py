@@ -35,11 +35,13 @@ def topk_workspace(tokens, lanes, query_heads, kv_heads, head_dim):
     return _size("ekv_topk_workspace_bytes", tokens, lanes, query_heads, kv_heads, head_dim)
 
 
-def _check(query, planes):
+def _check(query, planes, workspace):
     if not isinstance(planes, KVPlanes):
         raise TypeError("planes must be a KVPlanes")
     if query.dim() != 3:
         raise ValueError("query must be shaped [tokens, heads, head_dim]")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
 
 
 @profile_range("native/prefix_attention")
@@ -68,7 +70,7 @@ def shared_prefix_attention(query, planes, block_tables, rows, lengths, prefix_t
     shared_prefix_workspace(...) bytes (None: one from torch's allocator); calls
     on several streams need one each.
     """
-    _check(query, planes)
+    _check(query, planes, workspace)
     tokens, heads, dim = query.shape
     if workspace is None:
         groups = prefix_tables.shape[0] if prefix_tables is not None else 0
@@ -95,7 +97,7 @@ def topk_attention(query, planes, slots, output, *, kv_heads, layer=0, scale=Non
     that sees nothing gets zeros and lse -inf. lse, scale and workspace
     (topk_workspace(...) bytes) as in shared_prefix_attention.
     """
-    _check(query, planes)
+    _check(query, planes, workspace)
     tokens, heads, dim = query.shape
     if slots.dim() != 2:
         raise ValueError("slots must be shaped [tokens, K]")

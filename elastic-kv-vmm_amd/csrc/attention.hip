@@ -449,10 +449,11 @@ AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, i
     }
     // Log2 e: the kernels' exponentials have base two. A negative scale changes the queries' signs; zero is taken as the
     // smallest number, since an unseen key's score is minus infinity, which zero would make NaN.
-    a.scale = std::fmax(static_cast<float>(std::fabs(scale) * 1.4426950408889634), std::numeric_limits<float>::min());
+    a.scale = static_cast<float>(std::fabs(scale) * 1.4426950408889634);
     if (!std::isfinite(a.scale)) {
         throw std::invalid_argument("scale must be finite");
     }
+    a.scale = std::max(a.scale, std::numeric_limits<float>::min());
     a.flip = scale < 0 ? 0x80008000u : 0;
     return a;
 }

@@ -2,12 +2,12 @@
 //
 // A launch attends for sequences: a group's query tokens to its prefix, a batch row's to its own tokens or to both, or
 // one query token's to its slots. A sequence has `rows` rows (query tokens x query heads of one KV head) in tiles of
-// row_tile, and keys in units of unit; an item is one (sequence, KV head, row tile), and its key units are counted in one
-// line over all items. Workgroup w takes places [w * quota, (w + 1) * quota) of that line, whatever the lengths are, so
-// every workgroup has as many keys to read; but a cut inside an item of one or two units moves to the item's nearer end:
-// starting and ending an item costs a workgroup about as much as reading a unit, so that cutting it would save nothing. An item cut between workgroups is joined by the merge kernel from the parts that
-// each left (weighted values, largest score, sum). Places fit 31 bits: the host makes the unit larger where the tables'
-// widths could pass them.
+// row_tile, and keys in units of unit; an item is one (sequence, KV head, row tile), and its key units are counted in
+// one line over all items. Workgroup w takes places [w * quota, (w + 1) * quota) of that line, whatever the lengths
+// are, so every workgroup has as many keys to read. But a cut inside an item of one or two units moves to the item's
+// nearer end: starting and ending an item costs a workgroup about as much as reading a unit, so that cutting it would
+// save nothing. An item cut between workgroups is joined from the parts that each left (weighted values, largest score,
+// sum). Places fit 31 bits: the host makes the unit larger where the tables' widths could pass them.
 #pragma once
 
 #include "../../include/ekv_kernels.h"
