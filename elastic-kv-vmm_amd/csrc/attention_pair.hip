@@ -28,7 +28,7 @@ __global__ __launch_bounds__(kWaves * 64, kDim <= 128 ? 2 : 1) void pair_kernel(
     const Launch& l = fresh();
     const uint32_t share = prefix_workgroups(l.p[0], l.p[1], totals[0], totals[1]), b = blockIdx.x;
     if (kFew && b >= share) {
-        narrow::run<T, kDim, 1>(0, b - share, gridDim.x - share, true, totals[0], s_data, s_stats, s_line[0]);
+        narrow::run<T, kDim, 1>(0, on_die(b - share, gridDim.x - share), gridDim.x - share, true, totals[0], s_data, s_stats, s_line[0]);
     } else {
         const int which = b < share ? 1 : 0;
         wide::run<T, kDim, kWaves>(which, which == 1 ? b : b - share, which == 1 ? share : gridDim.x - share, true,

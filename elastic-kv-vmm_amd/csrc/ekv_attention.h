@@ -116,6 +116,13 @@ __device__ __forceinline__ int hidden(int x) {
     return x;
 }
 
+// A load of memory that is not LDS. The compiler cannot tell for an address that a select chose, and its load for either
+// kind returns in no order, so that a wait for one would wait for all that are under way.
+template <typename V>
+__device__ __forceinline__ V load_global(const char* at) {
+    return *(const __attribute__((address_space(1))) V*)(at);
+}
+
 // A barrier for what is in LDS. __syncthreads() also waits for every load from memory that is under way, and would end
 // each prefetch at the next barrier.
 __device__ __forceinline__ void lds_barrier() {
@@ -353,6 +360,13 @@ __device__ __forceinline__ void line_totals(uint32_t (&totals)[2], LineCells<kWa
             }
         }
     }
+}
+
+// The place in the line's order of the b-th of `count` workgroups. Workgroups are dealt to the eight dies in turn: each
+// die gets a run of the line, so that items that read the same keys meet in one L2.
+__device__ __forceinline__ uint32_t on_die(uint32_t b, uint32_t count) {
+    const uint32_t die = b & 7, each = count >> 3, more = count & 7;
+    return die * each + min(die, more) + (b >> 3);
 }
 
 // Calls body(segment) for every segment of phase `which` that workgroup w of those that share it has, in order; all

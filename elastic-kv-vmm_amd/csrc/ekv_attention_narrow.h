@@ -113,7 +113,7 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
             for (int c = 0; c < kSteps; ++c) {
                 const int piece = c * 4 + quad;
                 const bool live = row < g.rows && (c < kWholeSteps || piece < pieces);
-                q[m][c] = *reinterpret_cast<const words4*>(live ? at + piece * 16 : zeros);
+                q[m][c] = load_global<words4>(live ? at + piece * 16 : zeros);
                 q[m][c] ^= a.flip;
             }
             visible[m] = seen_by(g.q, token);
@@ -158,13 +158,13 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
                     const int32_t key = base + h * 16 + col;
                     const char* at = src.table + static_cast<uint64_t>(cache.page.div(key)) * src.step;
                     at = key < src.keys ? at : zeros;
-                    e.low[h] = *reinterpret_cast<const uint32_t*>(at);
-                    e.high[h] = *reinterpret_cast<const uint32_t*>(at + src.wide);
+                    e.low[h] = load_global<uint32_t>(at);
+                    e.high[h] = load_global<uint32_t>(at + src.wide);
                 }
                 return e;
             };
             words4 k[2][kSteps], v[2][kSteps];
-            uint32_t seen = 0;                // bit per key of the tile
+            uint32_t seen;                    // bit per key of the tile
             const auto fetch = [&](int32_t base, const Ids& e) {
                 seen = 0;
 #pragma unroll
@@ -185,20 +185,19 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
                         // Past the head size: any piece of the row; K meets zeros of q once it is cleared, V's columns
                         // are not stored.
                         const int piece = c < kWholeSteps || c * 4 + quad < pieces ? c * 64 : -quad * 16;
-                        k[h][c] = *reinterpret_cast<const words4*>(k_at + (good || c < kWholeSteps ? piece : 0));
-                        v[h][c] = *reinterpret_cast<const words4*>(v_at + (good || c < kWholeSteps ? piece : 0));
+                        k[h][c] = load_global<words4>(k_at + (good || c < kWholeSteps ? piece : 0));
+                        v[h][c] = load_global<words4>(v_at + (good || c < kWholeSteps ? piece : 0));
                     }
                     seen |= (static_cast<uint32_t>(__ballot(good)) & 0xffffu) << (16 * h);
                 }
             };
 
             constexpr int kStride = kWaves * kKeys;
-            int32_t base = (from << unit_shift) + wave * kKeys;
-            Ids ids = ids_of(base);
-            fetch(base, ids);
-            ids = ids_of(base + kStride);
-#pragma unroll 1
-            for (; base < src.keys; base += kStride) {
+            const int32_t start = (from << unit_shift) + wave * kKeys;
+            Ids ids = ids_of(start);
+            fetch(start, ids);
+            ids = ids_of(start + kStride);
+            const auto tile = [&](int32_t base) {
                 const Ids later = ids_of(base + 2 * kStride);
                 const uint32_t now = seen;
                 // Whether some row sees fewer keys of this tile than it holds.
@@ -331,6 +330,10 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
                         o[m][c] = T::mfma16(column_c, weights[m], o[m][c]);
                     }
                 }
+            };
+#pragma unroll 1
+            for (int32_t base = start; base < src.keys; base += kStride) {
+                tile(base);
             }
         }
 

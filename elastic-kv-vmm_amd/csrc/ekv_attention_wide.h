@@ -85,7 +85,7 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
 #pragma unroll
             for (int c = 0; c < kSteps; ++c) {
                 const int piece = c * 2 + half;
-                q[c] = *reinterpret_cast<const words4*>(row < g.rows && piece < pieces ? at + piece * 16 : zeros);
+                q[c] = load_global<words4>(row < g.rows && piece < pieces ? at + piece * 16 : zeros);
                 q[c] ^= a.flip;
             }
         }
@@ -134,7 +134,7 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
                 const int32_t key = base + lane;
                 const char* at = table + static_cast<uint64_t>(cache.page.div(key)) * step;
                 at = key < keys ? at : zeros;
-                return Ids{*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + wide)};
+                return Ids{load_global<uint32_t>(at), load_global<uint32_t>(at + wide)};
             };
             words4 k[kLoads], v[kLoads];
             // A tile's rows in three parts: whose keys are seen, then piece i of its loads, then piece i of its stores.
@@ -155,8 +155,8 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
                 const char* v_at = at + cache.kv_stride;
                 at = id != 0xffffffffu ? at : zeros;
                 v_at = id != 0xffffffffu ? v_at : zeros;
-                k[i] = *reinterpret_cast<const words4*>(at);
-                v[i] = *reinterpret_cast<const words4*>(v_at);
+                k[i] = load_global<words4>(at);
+                v[i] = load_global<words4>(v_at);
             };
             const auto store = [&](int buffer, int i) {
                 char* const to = s_data + buffer + i * kKeysAtOnce * kBytes + (write_at ^ ((i * kKeysAtOnce & 8) << 2));
