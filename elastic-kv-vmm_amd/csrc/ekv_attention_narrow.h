@@ -194,9 +194,9 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
 
             constexpr int kStride = kWaves * kKeys;
             const int32_t start = (from << unit_shift) + wave * kKeys;
-            Ids ids = ids_of(start);
-            fetch(start, ids);
-            ids = ids_of(start + kStride);
+            const Ids first = ids_of(start);
+            Ids ids = ids_of(start + kStride);
+            fetch(start, first);
             const auto tile = [&](int32_t base) {
                 const Ids later = ids_of(base + 2 * kStride);
                 const uint32_t now = seen;

@@ -309,14 +309,16 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
             };
 
             int32_t base = from << unit_shift;
-            uint64_t now = look(base, ids_of(base));
-            load_all(base);
+            // Ids before rows, as in the loop: its first wait would otherwise be for the rows as well.
+            const Ids first = ids_of(base);
             Ids ids = ids_of(base + kTile);
+            uint64_t now = look(base, first);
+            load_all(base);
             lds_barrier();     // the buffers' last use
             store_all(0);
             uint64_t next = look(base + kTile, ids);
-            load_all(base + kTile);
             ids = ids_of(base + 2 * kTile);
+            load_all(base + kTile);
             lds_barrier();
             int buffer = 0;
             f32x16 s = scores(s_data, 0);
