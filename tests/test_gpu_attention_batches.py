@@ -123,3 +123,15 @@ def test_topk_of_more_tokens_than_are_joined_by_token(gpu, heads, lanes):
         at = torch.where(seen, at, 0)
         parts.append(attend(query[t], pool.keys[at, 0], pool.values[at, 0], dim ** -0.5, seen))
     check(out, lse, answer_of(parts), dim)
+
+
+@pytest.mark.parametrize("tokens", [5, 3000])
+@pytest.mark.parametrize("prefixes", [None, [50]])
+def test_a_batch_of_no_rows(gpu, tokens, prefixes):
+    problem = make_problem(gpu, heads=4, kv_heads=2, dim=64, lengths=[30], prefixes=prefixes, permute=False)
+    problem.query = torch.randn((tokens, 4, 64), device=gpu).to(BF16)
+    problem.lengths, problem.counts = [], []
+    if prefixes is not None:
+        problem.group_starts = [0, 0]
+    out, lse = run(problem)
+    assert not out.any() and (lse == -math.inf).all()
