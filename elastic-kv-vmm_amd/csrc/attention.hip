@@ -7,8 +7,9 @@
 // weighted values a = sum exp(s_j - m) v_j, two parts of the keys join as m = max(m1, m2),
 // l = l1 e^(m1 - m) + l2 e^(m2 - m), a likewise, and o = a / l; statistics and sums are held in 32 bits.
 //
-// The kernels that read K and V are in attention_narrow.hip; here are the checks, the choice of a launch, and the merge
-// of the parts that a launch's workgroups leave of one item (ekv_attention.h).
+// The kernels that read K and V are in attention_narrow.hip, attention_wide.hip and attention_pair.hip; here are the
+// checks, the choice of a launch, and the merge of the parts that a launch's workgroups leave of one item
+// (ekv_attention.h).
 #include "ekv_attention.h"
 #include "ekv_mfma.h"
 
@@ -19,7 +20,7 @@ namespace ekv {
 namespace {
 
 constexpr int kMergeThreads = 256, kMergeColumns = 8;
-constexpr int kMergeByToken = 16;    // workgroups per compute unit up to which the merge goes by tokens
+constexpr int kMergeByToken = 8;        // workgroups per compute unit up to which the merge goes by tokens
 
 // The workgroups that hold a token's parts of one phase, and where.
 struct Parts {
@@ -37,8 +38,8 @@ struct Parts {
 };
 
 // The parts of row `row` (of one KV head) of sequence s: none when the sequence was nobody's work.
-__device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p, uint32_t workgroups, int32_t s, int32_t head,
-                                          int32_t row) {
+__device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p, uint32_t workgroups, int32_t s,
+                                          int32_t head, int32_t row) {
     uint32_t begin, total, item, units, row_tiles;
     if (p.mode == kSlots) {
         units = p.alike_units.divisor;
@@ -156,9 +157,12 @@ struct Joined {
     }
 };
 
-// One workgroup per (query token, KV head), for launches whose every row has parts and for those of few tokens. What
-// bounds it is the latency of its loads (a row has as many parts as workgroups shared its keys), so a small row's parts
-// are spread over the threads that it leaves idle, and joined through LDS.
+// One workgroup per (query token, KV head) and 256 pieces of four elements of its rows, for launches whose every row has
+// parts and for those of few tokens. What bounds it is the latency of its loads (a row has as many parts as workgroups
+// shared its keys), so a small row's parts are spread over the threads that it leaves idle, and joined through LDS, and
+// a large share's pieces over workgroups: with one for all of 256 query heads a call took 114 us instead of 46.
+// Measured: 4.4 us behind a Top-K step of 4 tokens, 10.8 us behind 32 tokens of 32 heads with 8192 keys of prefix (22 MB
+// of parts).
 template <typename T>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArgs a, const Phase own,
                                                                   const Phase prefix) {
@@ -188,7 +192,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
     }
     const int32_t quads = (a.dim + 3) >> 2, units = a.share * quads;
     const int32_t splits = units < kMergeThreads ? kMergeThreads / units : 1;
-    for (int32_t begin = 0; begin < units; begin += kMergeThreads) {
+    for (int32_t begin = blockIdx.z * kMergeThreads; begin < units; begin += gridDim.z * kMergeThreads) {
         const int32_t split = splits > 1 ? threadIdx.x / units : 0;
         const int32_t unit = begin + threadIdx.x - split * units;
         const bool live = unit < units && split < splits;
@@ -229,7 +233,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const AttentionArg
 
 // The cuts of a launch of one phase: the column of workgroups w joins the item that workgroup w begins and others go on
 // with, if there is one; all other items are written already. The rows of tokens that belong to no batch row are zeroed
-// here.
+// here. What bounds it: the parts of 256 cut items of 256 rows, 68 MB in 22 us at a head size of 128.
 template <typename T>
 __global__ __launch_bounds__(kMergeThreads) void cuts_kernel(const AttentionArgs a, const Phase p) {
     const uint32_t total = p.mode == kSlots ? p.alike_total : p.unit_starts[p.sequences];
@@ -471,7 +475,12 @@ struct Plan {
 int32_t padded_dim(int64_t dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : (dim <= 128 ? 128 : 256)); }
 
 // 16-row tiles that hold `rows` rows: 1, 2 or 4 of the kernel for few rows, 8 or 16 of the one for many (2 and 8 at most
-// at 256 columns, where the registers hold no more).
+// at 256 columns, where the registers hold no more). A tile that rows fill in part costs its whole products, several tiles
+// read the keys several times. Calls of 32 requests of 2000 tokens, head size 128, us with tiles of 1, 2, 4, 8, 16:
+//   16 rows, 8 KV heads   55  55  57  62  75        64 rows, 2 KV heads    53  36  31  36  34
+//   32 rows, 8 KV heads   96  58  59  65  76       128 rows, 2 KV heads    92  54  42  41  38
+//                                                  256 rows, 2 KV heads   173  99  60  53  46
+// and at a head size of 256 with 1, 2, 8: 106 152 176 for 16 rows, 200 156 181 for 32, 94 83 71 for 64.
 int tiles_for(int64_t rows, int32_t dim_pad) {
     if (rows <= 32) {
         return rows <= 16 ? 1 : 2;
@@ -495,7 +504,8 @@ void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, i
     p.dim_pad = dim_pad;
     p.workgroups = kComputeUnits * (tiles16 < 8 ? narrow_groups(tiles16, dim_pad) : (tiles16 == 8 && dim_pad <= 128 ? 2 : 1));
     // A unit of the kernel for few rows is 128 keys read at the card's rate, one of the kernel for many 64 keys'
-    // products: about 4 us and 2.4 us of a workgroup at a head size of 128.
+    // products. Weights of 3, 4, 5, 6 and 8 against 3 took 47, 46, 43, 41 and 46 us for 32 requests behind 8192 tokens,
+    // 126, 122, 110, 124 and 130 for 128 requests behind 32768, 73, 68, 69, 69 and 69 for seven groups of 13.
     p.weight = tiles16 < 8 ? 5 : 3;
     p.direct = direct;
     // Row tiles of all sequences: every sequence's last may be part-filled.
@@ -541,9 +551,13 @@ Plan prefix_plan(int64_t tokens, int64_t batch, int64_t groups, int64_t heads, i
     Plan plan;
     const int64_t share = heads / kv_heads, row_rows = std::min(max_query, tokens) * share;
     const int32_t dim_pad = padded_dim(dim);
-    // Rows of a group fill tiles that a batch row's alone leave part-empty: then the prefix is a phase of its own.
+    // Rows of a group fill tiles that a batch row's alone leave part-empty: then the prefix is a phase of its own. Where a
+    // batch row has 64 rows both ways are even: 32 requests of 500 tokens behind 8192, head size 128, 8 KV heads, by
+    // rows of a batch row 8, 16, 32, 64, 96: as phases 43, 63, 103, 159, 226 us, as one 134, 138, 142, 166, 199. Own
+    // tokens of 17 rows and more go to the kernel for many rows: in tiles of 16 they are read once per tile, 32 rows of
+    // 4000 tokens 242 us against 164 (of 500 tokens 92 against 100; 16 rows of 4000 tokens 142 against 149).
     const int64_t group_rows = groups > 0 ? tokens * share / groups : 0;
-    if (groups > 0 && group_rows > row_rows && row_rows < 64) {
+    if (groups > 0 && group_rows > row_rows && row_rows <= 64) {
         plan.pair = true;
         plan.tiles16 = row_rows <= 16 ? 1 : 8;
         cut(plan, plan.own, kOwn, batch, plan.tiles16, tokens, share, kv_heads, dim_pad, false);
@@ -610,12 +624,16 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
     }
     const auto merge = [&]<typename T>(T) {
         const auto on = static_cast<hipStream_t>(stream);
-        // By tokens the time goes with the rows, by cuts with the workgroups.
+        // By tokens the time goes with the rows, by cuts with the workgroups: a whole call of 64, 256, 512 and 2048
+        // tokens of 8 KV heads takes 25, 80, 155 and 583 us by tokens and 29, 81, 153 and 550 by cuts; eight prompts'
+        // pieces of up to 1024 tokens take 62 us more by tokens and 22 by cuts.
         if (!plan.pair && int64_t{a.tokens} * a.kv_heads > kComputeUnits * kMergeByToken) {
             const dim3 grid(plan.own.workgroups, kMergeColumns);
             cuts_kernel<T><<<grid, kMergeThreads, 0, on>>>(a, plan.own);
         } else {
-            const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.kv_heads));
+            const uint32_t pieces = (a.share * ((a.dim + 3) / 4) + kMergeThreads - 1) / kMergeThreads;
+            const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.kv_heads),
+                            std::min(pieces, uint32_t{64}));
             merge_kernel<T><<<grid, kMergeThreads, 0, on>>>(a, plan.own, plan.prefix);
         }
     };

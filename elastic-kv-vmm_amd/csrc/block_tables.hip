@@ -8,6 +8,11 @@
 // Both sums are taken by every workgroup for itself (a few loads and two DPP scans per 1024 rows), so one launch does
 // it all with no workgroup waiting for another: a new page's id is read from the free list, never from the table that
 // another workgroup may be writing, and table entries below have_b are written by nobody.
+//
+// What bounds it: for a decode step the chain of launch, lengths, sums, table entry, store, 9.5 us for 128 requests (a
+// launch of an empty kernel and four dependent memory levels); for long prompts the stores behind that chain, 38 MB of
+// slots and positions of 251 requests in 21 us. There a thread's four tokens share one lookup (24 us when each had its
+// own), and 1024 workgroups take tiles of 1024 tokens in turn: 256, 512, 768 and 1536 take 37, 26, 22 and 25 us.
 #include "../../include/ekv_kernels.h"
 #include "ekv_common.h"
 #include "ekv_fastdiv.h"
@@ -26,7 +31,7 @@ constexpr int kPer = 4;                        // rows per thread of a chunk
 constexpr int kChunk = kThreads * kPer;        // rows whose sums a workgroup holds at a time
 constexpr int kTokens = 4;                     // tokens per thread and step: one 16-byte store of int32 slots
 constexpr int kTile = kThreads * kTokens;
-constexpr int64_t kMaxGroups = 1024;
+constexpr int64_t kMaxGroups = 1024;           // four a compute unit
 
 // An int32 or int64 array that is written.
 struct IndexOut {

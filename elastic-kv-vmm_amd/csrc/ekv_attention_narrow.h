@@ -10,8 +10,13 @@
 // What bounds it: the K and V rows from HBM. Every wave reads its own keys (each every kWaves-th tile of the segment), K
 // straight into the registers of the first product, V by way of LDS. A tile's registers are free once the first
 // product and the LDS write have taken them, so the next tile's rows are in flight during the rest of a tile, and the
-// page ids of the one after before them: 16 KB a wave at a head size of 128. Each row of 16 * kTiles rows is held by
-// every wave and joined at the end of an item in a fixed order.
+// page ids of the one after before them: 16 KB a wave at a head size of 128. Two tiles in flight at a head size of 64
+// gained nothing (71 us against 69), nor did non-temporal loads or transposed reads ahead of the products. Each row of
+// 16 * kTiles rows is held by every wave and joined at the end of an item in a fixed order.
+//
+// Measured: a Top-K step of 128 tokens, 2048 slots each, 2 KV heads of 128, bfloat16: 271 MB in 55 us, 4.9 TB/s with the
+// launch, its lines of work and its last items (a streaming copy reaches 6.5 TB/s). A step of 4 tokens and 256 slots
+// takes 8.9 us, the latency of slots, rows, join and store one after the other.
 #pragma once
 
 #include "ekv_attention.h"

@@ -77,7 +77,8 @@ PREFIX = [
     (dict(output=tensor((4, 6, 64), BF16)), "output dimension 0 is 4, expected 5"),
     (dict(kv_heads=4), "kv_heads must divide"),
     (dict(kv_heads=0), "kv_heads must divide"),
-    (dict(query=tensor((5, 6, 60), BF16, (384, 64, 1)), output=tensor((5, 6, 60), BF16, (384, 64, 1))), "multiple of 8 from 8 to 256"),
+    (dict(query=tensor((5, 6, 60), BF16, (384, 64, 1)), output=tensor((5, 6, 60), BF16, (384, 64, 1))),
+     "multiple of 8 from 8 to 256"),
     (dict(query=tensor((5, 6, 264), BF16), output=tensor((5, 6, 264), BF16)), "multiple of 8 from 8 to 256"),
     (dict(scale=float("nan")), "scale must be finite"),
     (dict(scale=1e39), "scale must be finite"),
