@@ -82,12 +82,12 @@ struct Ids {
     uint32_t low[2], high[2];
 };
 
-// Workgroup w's part of phase `which` of the launch. s_data: lds_bytes(), stats: stats_bytes() of LDS.
 template <int kTiles>
 constexpr int stats_bytes() {
     return 2 * kWaves * kTiles * 16 * static_cast<int>(sizeof(float));
 }
 
+// Workgroup w's part of phase `which` of the launch. s_data: lds_bytes(), stats: stats_bytes() of LDS.
 template <typename T, int kDim, int kTiles, int kChunk>
 __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, bool read, uint32_t total,
                                     char* s_data, char* stats, LineCells<kWaves, kChunk>& cells) {
