@@ -273,11 +273,12 @@ __global__ __launch_bounds__(kMergeThreads) void cuts_kernel(const AttentionArgs
         }
         s = low;
         items = p.item_starts[s + 1] - p.item_starts[s];
-        if (items == 0) {
-            return;
-        }
         begin = p.unit_starts[s];
-        units = max((p.unit_starts[s + 1] - begin) / items, 1u);
+        units = p.unit_starts[s + 1] - begin;
+        if (items == 0 || cut - begin >= units) {
+            return;             // the latter only if the starts were not in order
+        }
+        units = max(units / items, 1u);
         local = (cut - begin) / units;
         begin += local * units;
     }

@@ -361,7 +361,7 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
         const bool whole = p.direct != 0 && g.begin == 0 && g.end == g.units;
         const int32_t row_tile = 16 * kTiles;
         float* const part = p.parts + static_cast<int64_t>(g.slot) * row_tile * (kDim + 2);
-        const bool room = g.slot < p.slots;
+        const bool room = static_cast<uint32_t>(g.slot) < static_cast<uint32_t>(p.slots);
         f32x4* const joined = reinterpret_cast<f32x4*>(s_data);   // [wave][column][row tile][end_lane]
         float factor[kTiles];
 #pragma unroll

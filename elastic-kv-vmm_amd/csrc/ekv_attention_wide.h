@@ -425,7 +425,7 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
                     z.lse[(g.q.first + token) * z.l_token + head * z.l_head] =
                         sum == 0 ? -INFINITY : (top * z.scale - T::kShift + log2f(sum)) * kLn2;
                 }
-            } else if (g.slot < p.slots) {
+            } else if (static_cast<uint32_t>(g.slot) < static_cast<uint32_t>(p.slots)) {
                 float* const part = p.parts + static_cast<int64_t>(g.slot) * kRows * (kDim + 2);
                 const int inside = wave * 32 + (end_lane & 31);
 #pragma unroll

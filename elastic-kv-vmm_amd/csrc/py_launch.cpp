@@ -5,10 +5,10 @@
 // (ekv_residency_summary), the batch-token swap-in (ekv_swap_in*), the
 // per-layer SGLang-convention swap-in (ekv_hisparse_swap_in), the one-call
 // decode step (ekv_decode_step), the block tables (ekv_extend_block_tables) and
-// both attentions (ekv_shared_prefix_attention, ekv_topk_attention). Their GPU work can be a few microseconds at
-// small shapes, so
-// describing the tensors for the C ABI from Python (attribute reads and
-// struct packing, about 1 us per tensor) set the call rate. Here the
+// both attentions (ekv_shared_prefix_attention, ekv_topk_attention). Their
+// GPU work can be a few microseconds at small shapes, so describing the
+// tensors for the C ABI from Python (attribute reads and struct packing,
+// about 1 us per tensor) set the call rate. Here the
 // descriptors are read straight from the tensors, the device and stream come
 // from torch's current HIP stream, and the entry point, passed in by address
 // from the loaded libelastic_vmm.so, is called with the GIL released.

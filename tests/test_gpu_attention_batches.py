@@ -135,3 +135,19 @@ def test_a_batch_of_no_rows(gpu, tokens, prefixes):
         problem.group_starts = [0, 0]
     out, lse = run(problem)
     assert not out.any() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_starts_out_of_order_stay_in_bounds(gpu, most):
+    """What such starts give is not defined, but a later call finds its inputs and the memory around as they were."""
+    problem = make_problem(gpu, heads=8, kv_heads=2, dim=64, lengths=[40, 40, 40], counts=[4, 4, 4],
+                           prefixes=[100, 30], groups=[0, 2, 3], seed=41)
+    want = problem.answer()
+    memory = torch.full((14, 8, 64), 7.0, dtype=BF16, device=gpu)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=gpu)  # noqa: E731
+    problem.call(shared_prefix_attention, memory[1:13], None, query_starts=ints([0, 9, 3, 12]),
+                 group_starts=ints([0, 3, 1]), max_query=most)
+    torch.cuda.synchronize()
+    assert (memory[0] == 7).all() and (memory[13] == 7).all()
+    out, lse = run(problem)
+    check(out, lse, want, 64)
