@@ -18,6 +18,7 @@ TABLES_ROW_FULL = 2    # EKV_TABLES_ROW_FULL
 TABLES_NO_PAGES = 4    # EKV_TABLES_NO_PAGES
 TABLES_MAP_FULL = 8    # EKV_TABLES_MAP_FULL
 TABLES_SLOT_RANGE = 16  # EKV_TABLES_SLOT_RANGE
+TABLES_ID_RANGE = 32   # EKV_TABLES_ID_RANGE
 
 _REASONS = (
     (TABLES_BAD_ROW, "a row names no request, or its length or new tokens are negative or past its table"),
@@ -25,6 +26,7 @@ _REASONS = (
     (TABLES_NO_PAGES, "the free list ran out of pages"),
     (TABLES_MAP_FULL, "more new tokens than the slot map holds"),
     (TABLES_SLOT_RANGE, "a slot does not fit the int32 slot map"),
+    (TABLES_ID_RANGE, "a page id does not fit the int32 block table"),
 )
 
 

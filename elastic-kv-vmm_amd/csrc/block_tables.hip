@@ -87,16 +87,24 @@ __device__ __forceinline__ int64_t workgroup_before(int64_t value, uint32_t (*ce
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
+// The page id at place `from` of the free list: 0, the sink, past the list's ends and for an id that the table's type
+// cannot hold (its low half could name another page).
+__device__ __forceinline__ int64_t new_page(const TableArgs& a, int64_t from, int32_t& flags) {
+    const int64_t id = from >= 0 && from < a.free_count ? a.free_pages[from] : 0;
+    const bool fits = a.table64 || id == static_cast<int32_t>(id);
+    flags |= fits ? 0 : EKV_TABLES_ID_RANGE;
+    return fits ? id : 0;
+}
+
 // The first slot of a row's page `column`, -1 for none: a page that the row had is in its table, a new one in the list.
 __device__ __forceinline__ int64_t page_slot(const TableArgs& a, int64_t head, int64_t row, int64_t base, uint32_t column,
-                                             uint32_t held) {
+                                             uint32_t held, int32_t& flags) {
     int64_t id;
     if (column < held) {
         const int64_t entry = row * a.table_row + int64_t{column} * a.table_col;
         id = a.table64 ? static_cast<const int64_t*>(a.table)[entry] : static_cast<const int32_t*>(a.table)[entry];
     } else {
-        const int64_t from = head + base + (column - held);
-        id = from >= 0 && from < a.free_count ? a.free_pages[from] : 0;
+        id = new_page(a, head + base + (column - held), flags);
     }
     return id >= 1 ? id * a.page_size : -1;
 }
@@ -195,8 +203,7 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
         for (int64_t u = page_base + int64_t{blockIdx.x} * kThreads + tid; u < page_end;
              u += int64_t{gridDim.x} * kThreads) {
             const int r = last_not_above(s_base, 0, count, u);
-            const int64_t from = head + u;
-            const int64_t id = from >= 0 && from < a.free_count ? a.free_pages[from] : 0;
+            const int64_t id = new_page(a, head + u, flags);
             const uint32_t held = a.page.div(static_cast<uint32_t>(s_length[r]) + a.page.divisor - 1);
             const int64_t at = s_row[r] * a.table_row + (held + (u - s_base[r])) * a.table_col;
             if (a.table64) {
@@ -230,10 +237,10 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
                 const uint32_t column = a.page.div(position), offset = position - column * a.page.divisor;
                 const bool crosses = offset + kTokens > a.page.divisor;
                 const uint32_t held = a.page.div(length + a.page.divisor - 1);
-                const int64_t page = page_slot(a, head, s_row[r], s_base[r], column, held);
+                const int64_t page = page_slot(a, head, s_row[r], s_base[r], column, held, flags);
                 int64_t next = page;
                 if (crosses) {
-                    next = page_slot(a, head, s_row[r], s_base[r], column + 1, held);
+                    next = page_slot(a, head, s_row[r], s_base[r], column + 1, held, flags);
                 }
                 i32x4 slot, place;
 #pragma unroll
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
                 const uint32_t position = length + static_cast<uint32_t>(at - s_start[r]);
                 const uint32_t column = a.page.div(position);
                 const uint32_t held = a.page.div(length + a.page.divisor - 1);
-                const int64_t page = page_slot(a, head, s_row[r], s_base[r], column, held);
+                const int64_t page = page_slot(a, head, s_row[r], s_base[r], column, held, flags);
                 int64_t slot = page >= 0 ? page + (position - column * a.page.divisor) : -1;
                 if (!a.slots.is64 && slot > 0x7fffffff) {
                     flags |= EKV_TABLES_SLOT_RANGE;

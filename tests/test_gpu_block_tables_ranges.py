@@ -1,0 +1,48 @@
+"""extend_block_tables where a number does not fit the type that it is written in."""
+
+import pytest
+import torch
+
+from adaptive_sparse import block_tables
+from adaptive_sparse.block_tables import check_table_status, extend_block_tables
+
+pytestmark = pytest.mark.gpu
+
+I32, I64 = torch.int32, torch.int64
+
+
+def call(gpu, table, lengths, added, free, page, *, table_type=I32, slot_type=I64, head=0):
+    """One call whose free list and head are int64: table, slots, next head, status."""
+    total = sum(added)
+    tensor = lambda v, kind: torch.tensor(v, dtype=kind, device=gpu)  # noqa: E731
+    table = tensor(table, table_type)
+    slots = torch.full((total,), -77, dtype=slot_type, device=gpu)
+    starts, grown = tensor([0] * (len(lengths) + 1), I32), tensor([0] * len(lengths), I32)
+    next_head, status = tensor([0], I64), tensor([0], I32)
+    print(f"[tables] page {page} head {head} ids {free[:6]}", flush=True)
+    extend_block_tables(table, None, tensor(lengths, I32), tensor(added, I32), tensor(free, I64), tensor([head], I64),
+                        page, slots=slots, starts=starts, new_lengths=grown, new_head=next_head, status=status)
+    assert grown.tolist() == [n + a for n, a in zip(lengths, added)]
+    return table.tolist(), slots.tolist(), int(next_head), status
+
+
+# 2^32 + 6 and 5 - 2^32 keep a page's number in their low words.
+@pytest.mark.parametrize("wrong", [1 << 31, (1 << 32) + 6, 5 - (1 << 32), -(1 << 31) - 1, (1 << 62) + 3])
+@pytest.mark.parametrize("slot_type", [I32, I64])
+def test_a_page_id_that_an_int32_table_cannot_hold(gpu, wrong, slot_type):
+    table, slots, head, status = call(gpu, [[9, 0, 0, 0]], [3], [10], [4, wrong, 7], 4, slot_type=slot_type)
+    assert table == [[9, 4, 0, 7]]                      # the sink in its place
+    assert slots == [39, 16, 17, 18, 19, -1, -1, -1, -1, 28]
+    assert head == 3
+    assert int(status) == block_tables.TABLES_ID_RANGE
+    with pytest.raises(RuntimeError, match="a page id does not fit the int32 block table"):
+        check_table_status(status)
+    check_table_status(status)
+
+
+def test_the_same_ids_in_an_int64_table(gpu):
+    wide = (1 << 32) + 6
+    table, slots, head, status = call(gpu, [[9, 0, 0, 0]], [3], [10], [4, wide, 7], 4, table_type=I64)
+    assert table == [[9, 4, wide, 7]]
+    assert slots == [39, 16, 17, 18, 19, *(wide * 4 + i for i in range(4)), 28]
+    assert int(status) == 0
