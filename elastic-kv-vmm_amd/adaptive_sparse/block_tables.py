@@ -25,7 +25,7 @@ _REASONS = (
     (TABLES_ROW_FULL, "a row's new tokens pass its table's columns"),
     (TABLES_NO_PAGES, "the free list ran out of pages"),
     (TABLES_MAP_FULL, "more new tokens than the slot map holds"),
-    (TABLES_SLOT_RANGE, "a slot does not fit the int32 slot map"),
+    (TABLES_SLOT_RANGE, "a slot does not fit the slot map's type"),
     (TABLES_ID_RANGE, "a page id does not fit the int32 block table"),
 )
 

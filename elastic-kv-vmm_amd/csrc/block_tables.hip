@@ -21,6 +21,7 @@
 #include "ekv_wave.h"
 
 #include <algorithm>
+#include <limits>
 
 namespace ekv {
 namespace {
@@ -57,6 +58,7 @@ struct TableArgs {
     IndexOut slots, positions, starts, new_lengths, new_head;
     int32_t has_positions, vector;
     int64_t batch, capacity, free_count, page_size;
+    int64_t most_id;              // the largest page id whose slots are below 2^63
     FastDiv page;
     int32_t* status;
 };
@@ -106,7 +108,8 @@ __device__ __forceinline__ int64_t page_slot(const TableArgs& a, int64_t head, i
     } else {
         id = new_page(a, head + base + (column - held), flags);
     }
-    return id >= 1 ? id * a.page_size : -1;
+    flags |= id > a.most_id ? EKV_TABLES_SLOT_RANGE : 0;
+    return id >= 1 && id <= a.most_id ? id * a.page_size : -1;
 }
 
 // The last of entries low .. high - 1 that is at most `value` (entry `low` is).
@@ -428,6 +431,7 @@ int extend_block_tables(const ekv_tensor* table_p, const ekv_tensor* rows_p, con
     a.batch = batch;
     a.free_count = free_pages.shape[0];
     a.page_size = page_size;
+    a.most_id = (std::numeric_limits<int64_t>::max() - (page_size - 1)) / page_size;
     a.page = FastDiv(static_cast<uint32_t>(page_size));
     const int64_t groups = std::min(std::max<int64_t>((a.capacity + kTile - 1) / kTile, 1), kMaxGroups);
     extend_tables_kernel<<<static_cast<uint32_t>(groups), kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);

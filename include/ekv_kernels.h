@@ -453,7 +453,7 @@ int ekv_decode_step_static(const ekv_step_args* args, void* stream);
 #define EKV_TABLES_ROW_FULL 2   /* a row's new tokens pass its table's columns: the ones that do not fit are left out */
 #define EKV_TABLES_NO_PAGES 4   /* the free list ran out: entry 0 (the sink) was written, those tokens' slots are -1 */
 #define EKV_TABLES_MAP_FULL 8   /* more new tokens than the slot map holds: the ones past it are left out */
-#define EKV_TABLES_SLOT_RANGE 16 /* a slot does not fit the int32 slot map: -1 */
+#define EKV_TABLES_SLOT_RANGE 16 /* a slot does not fit the slot map's type: -1 */
 #define EKV_TABLES_ID_RANGE 32  /* a page id does not fit the int32 table: as if there were no page */
 
 /*

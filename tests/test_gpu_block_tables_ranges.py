@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from adaptive_sparse import block_tables
-from adaptive_sparse.block_tables import check_table_status, extend_block_tables
+from adaptive_sparse.block_tables import TABLES_SLOT_RANGE, check_table_status, extend_block_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -45,4 +45,20 @@ def test_the_same_ids_in_an_int64_table(gpu):
     table, slots, head, status = call(gpu, [[9, 0, 0, 0]], [3], [10], [4, wide, 7], 4, table_type=I64)
     assert table == [[9, 4, wide, 7]]
     assert slots == [39, 16, 17, 18, 19, *(wide * 4 + i for i in range(4)), 28]
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("wrong", [(1 << 61), (1 << 62) + 1, (1 << 63) - 1])
+def test_a_slot_that_64_bits_cannot_hold(gpu, wrong):
+    # 2^61 * 4 = 2^63; (2^62 + 1) * 4 would be 4 again.
+    table, slots, head, status = call(gpu, [[wrong, 0, 0]], [3], [6], [4, wrong], 4, table_type=I64)
+    assert table == [[wrong, 4, wrong]]
+    assert slots == [-1, 16, 17, 18, 19, -1]
+    assert int(status) == TABLES_SLOT_RANGE
+
+
+def test_the_largest_slot_of_64_bits(gpu):
+    most = ((1 << 63) - 4) // 4
+    table, slots, head, status = call(gpu, [[0]], [0], [4], [most], 4, table_type=I64)
+    assert table == [[most]] and slots == [most * 4 + i for i in range(4)] and slots[-1] == (1 << 63) - 1
     assert int(status) == 0
