@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(const TableArgs
         if (token_base > a.capacity) {
             flags |= EKV_TABLES_MAP_FULL;
         }
-        if (head < 0 || (page_base > 0 && head + page_base > a.free_count)) {
+        if (head < 0 || (page_base > 0 && head > a.free_count - page_base)) {
             flags |= EKV_TABLES_NO_PAGES;
         }
     }

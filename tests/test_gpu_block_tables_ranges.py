@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from adaptive_sparse import block_tables
-from adaptive_sparse.block_tables import TABLES_SLOT_RANGE, check_table_status, extend_block_tables
+from adaptive_sparse.block_tables import TABLES_NO_PAGES, TABLES_SLOT_RANGE, check_table_status, extend_block_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,12 @@ def test_the_largest_slot_of_64_bits(gpu):
     table, slots, head, status = call(gpu, [[0]], [0], [4], [most], 4, table_type=I64)
     assert table == [[most]] and slots == [most * 4 + i for i in range(4)] and slots[-1] == (1 << 63) - 1
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("head", [(1 << 63) - 1, (1 << 63) - 2, 1 << 40, -1, -(1 << 63)])
+def test_heads_far_outside_the_list(gpu, head):
+    table, slots, _, status = call(gpu, [[0, 0, 0]], [0], [9], [4, 5, 6], 4, head=head)
+    assert int(status) == TABLES_NO_PAGES
+    inside = [4, 5] if head == -1 else [0, 0]
+    assert table == [[0, *inside]]
+    assert slots == [-1] * 4 + ([16, 17, 18, 19, 20] if head == -1 else [-1] * 5)
