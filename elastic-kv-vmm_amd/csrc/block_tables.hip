@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <limits>
+#include <numeric>
 
 namespace ekv {
 namespace {
@@ -350,14 +351,31 @@ IndexOut index_out(const ekv_tensor& t) {
     return out;
 }
 
+// Whether two arrays may share a byte. Their elements lie at whole multiples of the strides' greatest common divisor from
+// each other, so arrays that lie in one another without a shared element, as columns of one tensor, are told apart.
 bool overlap(const ekv_tensor& a, const ekv_tensor& b) {
-    const auto range = [](const ekv_tensor& t) {
-        const auto begin = reinterpret_cast<uintptr_t>(t.data);
-        const auto last = t.shape[0] > 0 ? static_cast<uintptr_t>((t.shape[0] - 1) * t.stride[0]) : 0;
-        return std::pair<uintptr_t, uintptr_t>(begin, begin + (last + 1) * static_cast<uintptr_t>(itemsize(t.dtype)));
+    struct Bytes {
+        int64_t begin, end, step, item;
     };
-    const auto x = range(a), y = range(b);
-    return x.first < y.second && y.first < x.second;
+    const auto bytes = [](const ekv_tensor& t) {
+        const int64_t item = itemsize(t.dtype), step = t.shape[0] > 1 ? t.stride[0] * item : 0;
+        const int64_t first = static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.data));
+        const int64_t last = first + (t.shape[0] - 1) * step;
+        return Bytes{std::min(first, last), std::max(first, last) + item, step, item};
+    };
+    if (a.shape[0] == 0 || b.shape[0] == 0) {
+        return false;
+    }
+    const Bytes x = bytes(a), y = bytes(b);
+    if (x.begin >= y.end || y.begin >= x.end) {
+        return false;
+    }
+    const int64_t step = std::gcd(x.step, y.step);
+    if (step == 0) {
+        return true;
+    }
+    const int64_t apart = ((y.begin - x.begin) % step + step) % step;
+    return apart < x.item || step - apart < y.item;
 }
 
 int extend_block_tables(const ekv_tensor* table_p, const ekv_tensor* rows_p, const ekv_tensor* lengths_p,
@@ -386,7 +404,7 @@ int extend_block_tables(const ekv_tensor* table_p, const ekv_tensor* rows_p, con
     const ekv_tensor& starts = need_vector(starts_p, batch + 1, "starts");
     const ekv_tensor& new_lengths = need_vector(new_lengths_p, batch, "new_lengths");
     const ekv_tensor& new_head = need_vector(new_head_p, 1, "new_head");
-    if (batch > 0 && overlap(lengths, new_lengths)) {
+    if (overlap(lengths, new_lengths)) {
         throw std::invalid_argument("new_lengths must not share memory with lengths");
     }
     if (overlap(head, new_head)) {

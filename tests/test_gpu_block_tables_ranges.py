@@ -1,4 +1,4 @@
-"""extend_block_tables where a number does not fit the type that it is written in."""
+"""extend_block_tables where a number does not fit the type that it is written in, and where tensors lie in one another."""
 
 import pytest
 import torch
@@ -71,3 +71,19 @@ def test_heads_far_outside_the_list(gpu, head):
     inside = [4, 5] if head == -1 else [0, 0]
     assert table == [[0, *inside]]
     assert slots == [-1] * 4 + ([16, 17, 18, 19, 20] if head == -1 else [-1] * 5)
+
+
+def test_columns_of_one_tensor_do_not_share_memory(gpu):
+    """Lengths, new lengths, heads and starts side by side in the rows of one tensor: no element is another's."""
+    state = torch.tensor([[3, -77, 1, 0], [0, -77, 5, 1], [6, -77, 2, 2]], dtype=I32, device=gpu)
+    heads = torch.tensor([1, -77], dtype=I32, device=gpu)
+    table = torch.tensor([[9, 0, 0], [0, 0, 0], [7, 8, 0]], dtype=I32, device=gpu)
+    slots, starts = torch.zeros(8, dtype=I32, device=gpu), torch.zeros(4, dtype=I32, device=gpu)
+    status = torch.zeros(1, dtype=I32, device=gpu)
+    extend_block_tables(table, state[:, 3], state[:, 0], state[:, 2], torch.tensor([1, 2, 3, 4], dtype=I32, device=gpu),
+                        heads[:1], 4, slots=slots, starts=starts, new_lengths=state[:, 1], new_head=heads[1:],
+                        status=status)
+    assert state.tolist() == [[3, 4, 1, 0], [0, 5, 5, 1], [6, 8, 2, 2]]
+    assert table.tolist() == [[9, 0, 0], [2, 3, 0], [7, 8, 0]]
+    assert heads.tolist() == [1, 3] and starts.tolist() == [0, 1, 6, 8] and int(status) == 0
+    assert slots.tolist() == [39, 8, 9, 10, 11, 12, 34, 35]
