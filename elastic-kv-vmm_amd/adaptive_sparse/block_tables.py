@@ -42,10 +42,11 @@ def extend_block_tables(block_tables, rows, lengths, added, free_pages, free_hea
     slots [N] gets page * page_size + offset of every new token, batch row
     after batch row, positions [N] its position; starts [B + 1] the rows'
     first tokens there, new_lengths [B] = lengths + added, new_head [1] the
-    next unused entry of the free list (neither may share memory with what it
-    follows, so a call can be repeated or replayed). Places past the last token
-    are -1. Index tensors are int32 or int64. What does not fit is left out and
-    sets bits in status ([1] int32, OR-ed; check_table_status raises for them).
+    next unused entry of the free list. No output may share memory with an input
+    or another output, so a call can be repeated or replayed. Places past the
+    last token are -1. Index tensors are int32 or int64. What does not fit is
+    left out and sets bits in status ([1] int32, OR-ed; check_table_status
+    raises for them).
     """
     helper, entries = _native.launch_helper()
     result = helper.extend_tables(entries["ekv_extend_block_tables"], block_tables, rows, lengths, added, free_pages,

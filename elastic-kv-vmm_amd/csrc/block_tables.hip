@@ -404,12 +404,6 @@ int extend_block_tables(const ekv_tensor* table_p, const ekv_tensor* rows_p, con
     const ekv_tensor& starts = need_vector(starts_p, batch + 1, "starts");
     const ekv_tensor& new_lengths = need_vector(new_lengths_p, batch, "new_lengths");
     const ekv_tensor& new_head = need_vector(new_head_p, 1, "new_head");
-    if (overlap(lengths, new_lengths)) {
-        throw std::invalid_argument("new_lengths must not share memory with lengths");
-    }
-    if (overlap(head, new_head)) {
-        throw std::invalid_argument("new_head must not share memory with free_head");
-    }
     TableArgs a{};
     a.table = table.data;
     a.table_row = table.stride[0];
@@ -445,6 +439,25 @@ int extend_block_tables(const ekv_tensor* table_p, const ekv_tensor* rows_p, con
             throw std::invalid_argument("status must be int32");
         }
         a.status = static_cast<int32_t*>(status.data);
+    }
+    // Workgroups read the inputs while others write the outputs, and a repeated call reads them again.
+    const std::pair<const ekv_tensor*, const char*> inputs[] = {
+        {&lengths, "lengths"}, {&added, "added"}, {rows_p, "rows"}, {&free_pages, "free_pages"}, {&head, "free_head"}};
+    const std::pair<const ekv_tensor*, const char*> outputs[] = {
+        {&new_lengths, "new_lengths"}, {&new_head, "new_head"}, {&starts, "starts"},
+        {&slots, "slots"},             {positions_p, "positions"}, {status_p, "status"}};
+    for (const auto& out : outputs) {
+        const auto apart = [&](const auto& other) {
+            if (out.first != nullptr && other.first != nullptr && overlap(*out.first, *other.first)) {
+                throw std::invalid_argument(std::string(out.second) + " must not share memory with " + other.second);
+            }
+        };
+        for (const auto& in : inputs) {
+            apart(in);
+        }
+        for (const auto* other = outputs; other != &out; ++other) {
+            apart(*other);
+        }
     }
     a.batch = batch;
     a.free_count = free_pages.shape[0];

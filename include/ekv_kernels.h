@@ -475,8 +475,9 @@ int ekv_decode_step_static(const ekv_step_args* args, void* stream);
  *   int64 each; status NULL or [1] int32. M * page_size < 2^30.
  * What does not fit is left out and sets EKV_TABLES_* bits: a row that names no
  * request, or whose length is negative or past its columns, gets no tokens.
- * Batch rows must name distinct requests; new_lengths and new_head must not
- * share memory with lengths and free_head. One launch.
+ * Batch rows must name distinct requests. new_lengths, new_head, starts,
+ * slots, positions and status must not share memory with one another nor with
+ * rows, lengths, added, free_pages and free_head. One launch.
  * No reference counterpart: the reference extends its tables on the host
  * (adaptive_sparse/request_residency.py:739-790).
  */
