@@ -60,17 +60,9 @@ __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p
     }
     const uint32_t local = head * row_tiles + (row >> p.row_shift);
     begin += local * units;
-    // Who has it: a long item everyone with a place of it, a short one the one whose moved cuts enclose it.
-    const uint32_t quota = quota_of(total, workgroups);
-    uint32_t first = begin / quota, count = 1;
-    const uint32_t cut = (first + 1) * quota;
-    if (cut < begin + units) {
-        if (keeps_cuts(units, quota)) {
-            count = (begin + units - 1) / quota - first + 1;
-        } else if (moved_cut(cut, begin, units, quota) == begin) {
-            ++first;
-        }
-    }
+    // Who has it: everyone with a place of it, or the one with its first place where it is not cut.
+    const uint32_t quota = quota_of(total, workgroups), first = begin / quota;
+    const uint32_t count = keeps_cuts(units, quota) ? (begin + units - 1) / quota - first + 1 : 1;
     Parts r;
     r.row_tile = 1 << p.row_shift;
     r.step = r.row_tile * (p.dim_pad + 2);

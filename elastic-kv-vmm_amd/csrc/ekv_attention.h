@@ -4,10 +4,11 @@
 // one query token's to its slots. A sequence has `rows` rows (query tokens x query heads of one KV head) in tiles of
 // row_tile, and keys in units of unit; an item is one (sequence, KV head, row tile), and its key units are counted in
 // one line over all items. Workgroup w takes places [w * quota, (w + 1) * quota) of that line, whatever the lengths
-// are, so every workgroup has as many keys to read. But a cut inside an item of one or two units moves to the item's
-// nearer end: starting and ending an item costs a workgroup about as much as reading a unit, so that cutting it would
-// save nothing. An item cut between workgroups is joined from the parts that each left (weighted values, largest score,
-// sum). Places fit 31 bits: the host makes the unit larger where the tables' widths could pass them.
+// are, so every workgroup has as many keys to read. But where a run has two places or more, an item of one or two units is
+// not cut, the workgroup in whose run it begins has it whole: starting and ending an item costs a workgroup about as much
+// as reading a unit, so that cutting it would save nothing. An item cut between workgroups is joined from the parts that
+// each left (weighted values, largest score, sum). Places fit 31 bits: the host makes the unit larger where the tables'
+// widths could pass them.
 #pragma once
 
 #include "../../include/ekv_kernels.h"
@@ -228,12 +229,12 @@ __device__ __forceinline__ uint32_t prefix_workgroups(const Phase& own, const Ph
     return min(min(max(share, 1u), all - 1), most);
 }
 
-// Whether an item keeps its cuts, and where the cut at place c goes that lies in the item of places
-// [begin, begin + units). An item that moves its cuts has one at most.
+// Whether an item may be cut, and where the cut at place c goes that lies in the item of places [begin, begin + units):
+// one that is not cut has at most one inside, and that moves to its end.
 __device__ __forceinline__ bool keeps_cuts(uint32_t units, uint32_t quota) { return units > min(quota, 2u); }
 
 __device__ __forceinline__ uint32_t moved_cut(uint32_t c, uint32_t begin, uint32_t units, uint32_t quota) {
-    return keeps_cuts(units, quota) ? c : (c - begin < begin + units - c ? begin : begin + units);
+    return c == begin || keeps_cuts(units, quota) ? c : begin + units;
 }
 
 // How many own tokens a row of query token i (of the sequence's count) sees.

@@ -1,9 +1,9 @@
 """Infinities and NaN in V: the query tokens that see such a key get them, the others do not.
 
 A key in a tile that only some rows see has weight 0 for the others, and 0 times infinity is not 0, so the kernels add
-what is not finite apart from the product. Expected per output element, over the keys that its token sees: NaN if V holds
-NaN or infinities of both signs there, the infinity if it holds one, else the answer without them, within the bounds of
-attention_cases.py. Scores are of standard deviation one, so that no weight is rounded to zero.
+what is not finite apart from the product. Expected per output element, over the keys that its token sees: NaN if V
+holds NaN or infinities of both signs there, the infinity if it holds one, else the answer without them, within the
+bounds of attention_cases.py. Scores are of standard deviation one, so that no weight is rounded to zero.
 """
 
 import math

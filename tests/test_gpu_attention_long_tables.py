@@ -1,8 +1,9 @@
 """Attention with tables so wide that a launch's places would pass 31 bits, and starts out of order whose places do.
 
-Work is cut in units of keys that are counted over all rows, row tiles and KV heads from the tables' widths; where those
-counts could pass 31 bits the unit is made larger. The tables here are 2^30 - 16 tokens wide, their rows overlapping windows
-of one list of page ids, so that they cost one row's memory. The bounds are those of attention_cases.py.
+Work is cut in units of keys that are counted over all rows, row tiles and KV heads from the tables' widths; where
+those counts could pass 31 bits the unit is made larger. The tables here are 2^30 - 16 tokens wide, their rows
+overlapping windows of one list of page ids, so that they cost one row's memory. The bounds are those of
+attention_cases.py.
 """
 
 import pytest
