@@ -66,7 +66,7 @@ __device__ __forceinline__ Parts parts_of(const AttentionArgs& a, const Phase& p
     Parts r;
     r.row_tile = 1 << p.row_shift;
     r.step = r.row_tile * (p.dim_pad + 2);
-    const uint32_t slot = first + item + local, inside = row & (r.row_tile - 1);
+    const uint32_t slot = part_slot(p, first, first, item + local), inside = row & (r.row_tile - 1);
     const float* part = p.parts + static_cast<int64_t>(slot) * r.step;
     r.base = part;
     r.inside = inside;
@@ -506,7 +506,9 @@ void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, i
     if (items > (int64_t{1} << 30)) {
         throw std::invalid_argument("more than 2^30 row tiles");
     }
-    p.slots = static_cast<int32_t>(p.workgroups + items);
+    p.items = static_cast<int32_t>(items);
+    p.by_workgroup = direct && items > p.workgroups;
+    p.slots = static_cast<int32_t>(p.workgroups + (p.by_workgroup ? p.workgroups : items));
     p.parts = reinterpret_cast<float*>(plan.bytes);
     plan.bytes += aligned((static_cast<uint64_t>(p.slots) << p.row_shift) * (dim_pad + 2) * sizeof(float));
     if (mode != kSlots) {
@@ -519,8 +521,7 @@ void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, i
 
 // Makes the unit so large that the line's places fit 31 bits, whatever the lengths on the device are.
 void fit_units(Phase& p, int64_t keys) {
-    const int64_t items = p.slots - p.workgroups;
-    while (items > 0 && (keys >> p.unit_shift) + 2 > 0x7fffffff / items) {
+    while (p.items > 0 && (keys >> p.unit_shift) + 2 > 0x7fffffff / p.items) {
         ++p.unit_shift;
     }
 }

@@ -73,6 +73,8 @@ struct Phase {
     int32_t weight;                  // cost of a unit, as the phases of a launch share its workgroups
     int32_t direct;                  // an item that one workgroup has whole is written to the output
     int32_t dim_pad;
+    int32_t items;                   // at most, whatever the lengths are
+    int32_t by_workgroup;            // how parts are numbered (part_slot)
     int32_t slots;
     uint32_t alike_total;            // kSlots: places, and the items of a sequence and units of an item
     FastDiv alike_items, alike_units;
@@ -235,6 +237,14 @@ __device__ __forceinline__ bool keeps_cuts(uint32_t units, uint32_t quota) { ret
 
 __device__ __forceinline__ uint32_t moved_cut(uint32_t c, uint32_t begin, uint32_t units, uint32_t quota) {
     return c == begin || keeps_cuts(units, quota) ? c : begin + units;
+}
+
+// Where workgroup w leaves its part of an item that begins in the run of workgroup `first`, the `item`-th of the line.
+// Where items that one workgroup has whole are written to the output, the items that leave parts begin in runs of their own
+// and one ends before the next begins: first + w differs from part to part, and there are fewer than two a workgroup.
+// Parts are numbered so where there are more items than workgroups, and else by item and workgroup.
+__device__ __forceinline__ uint32_t part_slot(const Phase& p, uint32_t w, uint32_t first, uint32_t item) {
+    return w + (p.by_workgroup != 0 ? first : item);
 }
 
 // How many own tokens a row of query token i (of the sequence's count) sees.
@@ -474,7 +484,7 @@ __device__ __forceinline__ void for_segments(int which, uint32_t w, uint32_t wor
             g.rows = g.q.count * a.share;
             g.begin = at - begin;
             g.end = stop - begin;
-            g.slot = w + before + local;
+            g.slot = part_slot(p, w, at == begin || p.by_workgroup == 0 ? w : begin / quota, before + local);
             body(g);
             at = stop;
             if (last || at >= end || at >= total) {
