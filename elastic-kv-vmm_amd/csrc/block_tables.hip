@@ -404,6 +404,11 @@ int extend_block_tables(const ekv_tensor* table_p, const ekv_tensor* rows_p, con
     const ekv_tensor& starts = need_vector(starts_p, batch + 1, "starts");
     const ekv_tensor& new_lengths = need_vector(new_lengths_p, batch, "new_lengths");
     const ekv_tensor& new_head = need_vector(new_head_p, 1, "new_head");
+    constexpr int64_t kMost32 = std::numeric_limits<int32_t>::max();
+    if ((starts.dtype == EKV_INT32 && slots.shape[0] > kMost32) ||
+        (new_head.dtype == EKV_INT32 && free_pages.shape[0] > kMost32)) {
+        throw std::invalid_argument("int32 starts and new_head count at most 2^31 - 1 slots and free pages");
+    }
     TableArgs a{};
     a.table = table.data;
     a.table_row = table.stride[0];
