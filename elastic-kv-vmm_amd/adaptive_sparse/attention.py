@@ -44,6 +44,10 @@ def _check(query, planes, workspace):
         raise ValueError("workspace must be contiguous")
 
 
+def _scale(scale, dim):
+    return max(dim, 1) ** -0.5 if scale is None else scale    # a head size of 0 is the entry point's to refuse
+
+
 @profile_range("native/prefix_attention")
 def shared_prefix_attention(query, planes, block_tables, rows, lengths, prefix_tables, prefix_lengths, output, *,
                             page_size, kv_heads, layer=0, group_starts=None, query_starts=None, max_query=1,
@@ -80,7 +84,7 @@ def shared_prefix_attention(query, planes, block_tables, rows, lengths, prefix_t
     status = helper.prefix_attention(entries["ekv_shared_prefix_attention"], query, planes, int(layer), int(kv_heads),
                                      int(page_size), block_tables, rows, lengths, prefix_tables, prefix_lengths,
                                      group_starts, query_starts, int(max_query),
-                                     dim ** -0.5 if scale is None else scale, output, lse, workspace)
+                                     _scale(scale, dim), output, lse, workspace)
     _native.launch_check(status, "shared_prefix_attention")
 
 
@@ -106,5 +110,5 @@ def topk_attention(query, planes, slots, output, *, kv_heads, layer=0, scale=Non
         workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
     helper, entries = _native.launch_helper()
     status = helper.topk_attention(entries["ekv_topk_attention"], query, planes, int(layer), int(kv_heads), slots,
-                                   int(zero_below), dim ** -0.5 if scale is None else scale, output, lse, workspace)
+                                   int(zero_below), _scale(scale, dim), output, lse, workspace)
     _native.launch_check(status, "topk_attention")

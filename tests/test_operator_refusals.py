@@ -240,3 +240,19 @@ def test_the_python_calls_refuse():
                                 workspace=torch.zeros((4, 4), dtype=torch.uint8)[:, :2])
     with pytest.raises(ValueError):
         topk_workspace(3, -1, 6, 2, 64)
+
+
+def test_a_head_size_of_zero_is_refused_as_any_other():
+    from adaptive_sparse.attention import shared_prefix_attention, topk_attention
+    from adaptive_sparse.kv_pool import KVPlanes
+
+    memory = torch.zeros((2, 64, 2, 64), dtype=torch.bfloat16)
+    pool = KVPlanes(base=memory.data_ptr(), device=0, layers=1, kv=2, layer_stride=0, kv_stride=64 * 256,
+                    row_stride=256, row_bytes=256, rows=64, owner=memory)
+    query = torch.zeros((3, 6, 0), dtype=torch.bfloat16)
+    ints, workspace = torch.zeros((3, 10), dtype=torch.int32), torch.zeros(4096, dtype=torch.uint8)
+    with pytest.raises((ValueError, RuntimeError)):
+        topk_attention(query, pool, ints, query, kv_heads=2, workspace=workspace)
+    with pytest.raises((ValueError, RuntimeError)):
+        shared_prefix_attention(query, pool, ints, None, ints[:, 0], None, None, query, page_size=16, kv_heads=2,
+                                workspace=workspace)
