@@ -351,32 +351,37 @@ IndexOut index_out(const ekv_tensor& t) {
     return out;
 }
 
-// Whether two arrays may share a byte. Their elements lie at whole multiples of the strides' greatest common divisor from
-// each other, so arrays that lie in one another without a shared element, as columns of one tensor, are told apart.
-bool overlap(const ekv_tensor& a, const ekv_tensor& b) {
-    struct Bytes {
-        int64_t begin, end, step, item;
-    };
-    const auto bytes = [](const ekv_tensor& t) {
-        const int64_t item = itemsize(t.dtype), step = t.shape[0] > 1 ? t.stride[0] * item : 0;
-        const int64_t first = static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.data));
-        const int64_t last = first + (t.shape[0] - 1) * step;
-        return Bytes{std::min(first, last), std::max(first, last) + item, step, item};
-    };
-    if (a.shape[0] == 0 || b.shape[0] == 0) {
-        return false;
+// The bytes of a one-dimensional array: from `begin` to `end`, elements of `item` bytes `step` apart.
+struct Bytes {
+    int64_t begin = 0, end = 0, step = 0, item = 0;
+
+    explicit Bytes(const ekv_tensor* t) {
+        if (t == nullptr || t->shape[0] == 0) {
+            return;
+        }
+        item = itemsize(t->dtype);
+        step = t->shape[0] > 1 ? t->stride[0] * item : 0;
+        const int64_t first = static_cast<int64_t>(reinterpret_cast<uintptr_t>(t->data));
+        const int64_t last = first + (t->shape[0] - 1) * step;
+        begin = std::min(first, last);
+        end = std::max(first, last) + item;
     }
-    const Bytes x = bytes(a), y = bytes(b);
-    if (x.begin >= y.end || y.begin >= x.end) {
-        return false;
+
+    // Whether the arrays may share a byte. Their elements lie at whole multiples of the strides' greatest common divisor
+    // from each other, so arrays that lie in one another without a shared element, as columns of one tensor, are told
+    // apart.
+    bool meets(const Bytes& other) const {
+        if (item == 0 || other.item == 0 || begin >= other.end || other.begin >= end) {
+            return false;
+        }
+        const int64_t common = std::gcd(step, other.step);
+        if (common == 0) {
+            return true;
+        }
+        const int64_t apart = ((other.begin - begin) % common + common) % common;
+        return apart < item || common - apart < other.item;
     }
-    const int64_t step = std::gcd(x.step, y.step);
-    if (step == 0) {
-        return true;
-    }
-    const int64_t apart = ((y.begin - x.begin) % step + step) % step;
-    return apart < x.item || step - apart < y.item;
-}
+};
 
 int extend_block_tables(const ekv_tensor* table_p, const ekv_tensor* rows_p, const ekv_tensor* lengths_p,
                         const ekv_tensor* added_p, const ekv_tensor* free_p, const ekv_tensor* head_p,
@@ -446,21 +451,25 @@ int extend_block_tables(const ekv_tensor* table_p, const ekv_tensor* rows_p, con
         a.status = static_cast<int32_t*>(status.data);
     }
     // Workgroups read the inputs while others write the outputs, and a repeated call reads them again.
-    const std::pair<const ekv_tensor*, const char*> inputs[] = {
-        {&lengths, "lengths"}, {&added, "added"}, {rows_p, "rows"}, {&free_pages, "free_pages"}, {&head, "free_head"}};
-    const std::pair<const ekv_tensor*, const char*> outputs[] = {
-        {&new_lengths, "new_lengths"}, {&new_head, "new_head"}, {&starts, "starts"},
-        {&slots, "slots"},             {positions_p, "positions"}, {status_p, "status"}};
-    for (const auto& out : outputs) {
-        const auto apart = [&](const auto& other) {
-            if (out.first != nullptr && other.first != nullptr && overlap(*out.first, *other.first)) {
-                throw std::invalid_argument(std::string(out.second) + " must not share memory with " + other.second);
+    struct Array {
+        Bytes bytes;
+        const char* name;
+    };
+    const Array inputs[] = {{Bytes(&lengths), "lengths"}, {Bytes(&added), "added"}, {Bytes(rows_p), "rows"},
+                            {Bytes(&free_pages), "free_pages"}, {Bytes(&head), "free_head"}};
+    const Array outputs[] = {{Bytes(&new_lengths), "new_lengths"}, {Bytes(&new_head), "new_head"},
+                             {Bytes(&starts), "starts"}, {Bytes(&slots), "slots"}, {Bytes(positions_p), "positions"},
+                             {Bytes(status_p), "status"}};
+    for (const Array& out : outputs) {
+        const auto apart = [&](const Array& other) {
+            if (out.bytes.meets(other.bytes)) {
+                throw std::invalid_argument(std::string(out.name) + " must not share memory with " + other.name);
             }
         };
-        for (const auto& in : inputs) {
+        for (const Array& in : inputs) {
             apart(in);
         }
-        for (const auto* other = outputs; other != &out; ++other) {
+        for (const Array* other = outputs; other != &out; ++other) {
             apart(*other);
         }
     }
