@@ -62,11 +62,15 @@ def shared_prefix_attention(query, planes, block_tables, rows, lengths, prefix_t
     are in the pool already) among them. query_starts [B + 1]: first query
     token of each row (None: one token a row); token i of n sees the prefix and
     own tokens 0 .. lengths[b] - n + i. max_query: the most query tokens of a
-    row, as far as known: it picks kernels, never results.
+    row, as far as known: it picks kernels, never which keys are seen.
     prefix_tables [G, P], prefix_lengths [G], group_starts [G + 1]: the groups
     of consecutive batch rows and their prefixes (group_starts None: one group
-    of all rows; prefix_tables None: no prefix). K and V of a prefix are read
-    once for all rows of its group.
+    of all rows; prefix_tables None: no prefix). With query rows = query tokens
+    * Hq // kv_heads: if max_query makes 64 of them at most and a group has more
+    on average, K and V of a prefix are read once per 128 query rows of its
+    group, else once per batch row and tile of its rows. One choice serves the
+    whole call: decode rows and long prompt pieces behind one prefix are faster
+    as two calls.
     A page id below 1 or past the pool is not seen (page 0 is the sink); a
     query token that sees nothing gets zeros and lse -inf. lse [N, Hq] float32:
     log of the sum of exp(scale q.k), which merges outputs of other parts.

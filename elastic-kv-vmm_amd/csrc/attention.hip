@@ -498,7 +498,9 @@ void cut(Plan& plan, Phase& p, PhaseMode mode, int64_t sequences, int tiles16, i
     p.workgroups = kComputeUnits * (tiles16 < 8 ? narrow_groups(tiles16, dim_pad) : (tiles16 == 8 && dim_pad <= 128 ? 2 : 1));
     // A unit of the kernel for few rows is 128 keys read at the card's rate, one of the kernel for many 64 keys'
     // products. Weights of 3, 4, 5, 6 and 8 against 3 took 47, 46, 43, 41 and 46 us for 32 requests behind 8192 tokens,
-    // 126, 122, 110, 124 and 130 for 128 requests behind 32768, 73, 68, 69, 69 and 69 for seven groups of 13.
+    // 126, 122, 110, 124 and 130 for 128 requests behind 32768, 73, 68, 69, 69 and 69 for seven groups of 13: head sizes
+    // 128, 128 and 64, 4, 8 and 4 query heads a KV head, pages of 16, 64 and 1. Other ratios of a unit's bytes to its
+    // products rest on these three.
     p.weight = tiles16 < 8 ? 5 : 3;
     p.direct = direct;
     // Row tiles of all sequences: every sequence's last may be part-filled.
@@ -550,6 +552,10 @@ Plan prefix_plan(int64_t tokens, int64_t batch, int64_t groups, int64_t heads, i
     // rows of a batch row 8, 16, 32, 64, 96: as phases 43, 63, 103, 159, 226 us, as one 134, 138, 142, 166, 199. Own
     // tokens of 17 rows and more go to the kernel for many rows: in tiles of 16 they are read once per tile, 32 rows of
     // 4000 tokens 242 us against 164 (of 500 tokens 92 against 100; 16 rows of 4000 tokens 142 against 149).
+    // These were batches of like rows. The rule goes by the longest row, so a prompt piece makes every decode row beside
+    // it read the prefix by itself: 127 rows of one token and one of 1024 behind 32768 tokens, 8 query heads a KV head,
+    // take 1327 us in one call and 108 + 322 in two; 64 of one and four of 64 behind 8192, 183 and 43 + 58; 30 of one and
+    // two of 512 behind 2048, 86 and 26 + 64. A caller who passes a max_query of 64 rows gets phases: 509, 85 and 93 us.
     const int64_t group_rows = groups > 0 ? tokens * share / groups : 0;
     if (groups > 0 && group_rows > row_rows && row_rows <= 64) {
         plan.pair = true;

@@ -6,7 +6,10 @@
 // dealt to the compute units in turn, so that as long as both have work most units hold one of each. Both phases in
 // every workgroup, one after the other, took 67 us where this takes 52 (with the merge; 32 requests of 32 heads, 8 KV
 // heads of 128, 8192 tokens of prefix and up to 1024 own), 148 where it takes 109 (128 requests of 16 heads, 2 KV heads,
-// 32768 and up to 4096): 112 MB in 41 us of this kernel, 338 MB in 103 us.
+// 32768 and up to 4096): 112 MB in 43 us of this kernel, 338 MB in 101 to 111.
+//
+// At a head size of 128 the kernel for many rows has 25 vector registers more than two workgroups a compute unit leave
+// it and keeps them in scratch (104 bytes a lane); at 256 it is 53 to 86.
 #include "ekv_attention_narrow.h"
 #include "ekv_attention_wide.h"
 

@@ -4,11 +4,11 @@
 // one query token's to its slots. A sequence has `rows` rows (query tokens x query heads of one KV head) in tiles of
 // row_tile, and keys in units of unit; an item is one (sequence, KV head, row tile), and its key units are counted in
 // one line over all items. Workgroup w takes places [w * quota, (w + 1) * quota) of that line, whatever the lengths
-// are, so every workgroup has as many keys to read. But where a run has two places or more, an item of one or two units is
-// not cut, the workgroup in whose run it begins has it whole: starting and ending an item costs a workgroup about as much
-// as reading a unit, so that cutting it would save nothing. An item cut between workgroups is joined from the parts that
-// each left (weighted values, largest score, sum). Places fit 31 bits: the host makes the unit larger where the tables'
-// widths could pass them.
+// are, so every workgroup has as many keys to read. But where a run has two places or more, an item of one or two units
+// is not cut, the workgroup in whose run it begins has it whole: starting and ending an item costs a workgroup about as
+// much as reading a unit, so that cutting it would save nothing. An item cut between workgroups is joined from the parts
+// that each left (weighted values, largest score, sum). Places fit 31 bits: the host makes the unit larger where the
+// tables' widths could pass them.
 #pragma once
 
 #include "../../include/ekv_kernels.h"
@@ -217,8 +217,8 @@ __device__ __forceinline__ uint32_t quota_of(uint32_t total, uint32_t workgroups
 
 // How many workgroups of a launch of two phases work on prefixes; the others work on own tokens. A prefix unit leaves as
 // many bytes of parts as four hold of keys, so that a workgroup takes no fewer than two of them: with two, three, four
-// and six 4 requests behind 1024 tokens take 20, 25, 22 and 28 us, 24 behind 5000 with drafts 35, 35, 35 and 36. Beyond
-// that the phases share the workgroups by their units' costs.
+// and six 4 requests behind 1024 tokens take 20, 25, 22 and 28 us, 24 behind 5000 with drafts 35, 35, 35 and 36
+// (bfloat16, head sizes 128 and 96). Beyond that the phases share the workgroups by their units' costs.
 __device__ __forceinline__ uint32_t prefix_workgroups(const Phase& own, const Phase& prefix, uint32_t own_total,
                                                       uint32_t prefix_total) {
     const uint32_t all = own.workgroups, most = (prefix_total + 1) / 2;

@@ -14,9 +14,14 @@
 // gained nothing (71 us against 69), nor did non-temporal loads or transposed reads ahead of the products. Each row of
 // 16 * kTiles rows is held by every wave and joined at the end of an item in a fixed order.
 //
-// Measured: a Top-K step of 128 tokens, 2048 slots each, 2 KV heads of 128, bfloat16: 271 MB in 55 us, 4.9 TB/s with the
-// launch, its lines of work and its last items (a streaming copy reaches 6.5 TB/s). A step of 4 tokens and 256 slots
-// takes 8.9 us, the latency of slots, rows, join and store one after the other.
+// The weights are rounded once to the inputs' type, which the matrix instructions take: at most 2^-8 (bfloat16) or 2^-11
+// (float16) of a weight, as much as K and V carry themselves. Held as a sum of two such numbers they would cost a second
+// product per tile of V. The sums add the weights as they were before the rounding.
+//
+// Measured: a Top-K step of 128 tokens, 2048 slots each (225 thousand of 262 name a row), 2 KV heads of 128, bfloat16:
+// 230 MB in 54.5 us where passes take four pools of 0.5 GB in turn, 12 us less on one pool, part of which is still in the
+// last-level cache. A step of 4 tokens and 256 slots takes 8.5 us, the latency of slots, rows, join and store one after
+// the other: the rows come at 4.2 TB/s with it and 5.0 without (a streaming copy reaches 6.5).
 #pragma once
 
 #include "ekv_attention.h"

@@ -11,7 +11,9 @@
 // rows are loaded, while a tile is worked on; one barrier a half tile. At a head size of 128 a half tile is 16 KB of LDS
 // reads, 16 matrix instructions (512 cycles) and about as many cycles of vector instructions a wave, dealt in turn.
 //
-// Measured: prompts of 0.96 TFLOP, head size 128, bfloat16, 256 rows a workgroup: 1.08 ms, 0.89 PFLOP/s (a library
+// The weights are rounded once to the inputs' type, as there.
+//
+// Measured: prompts of 0.96 TFLOP, head size 128, bfloat16, 256 rows a workgroup: 1.06 ms, 0.91 PFLOP/s (a library
 // product of 16384^3 reaches 1.33); the matrix pipes are busy 47 % of the cycles at the 1.8 GHz that the card holds
 // under this load, LDS 31 %, with no bank conflicts. Staged between the tiles instead of beside the products it took
 // 1.13 ms. 128 rows a workgroup read the keys twice as often: two workgroups of four waves a compute unit, which

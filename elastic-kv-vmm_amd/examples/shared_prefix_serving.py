@@ -6,7 +6,7 @@ Every step is four calls on the device, with no host round trip between them:
 
     extend_block_tables      pages and slots of the step's new tokens, from the request lengths
     scatter_kv               their K and V rows into the pool
-    shared_prefix_attention  each layer, the prefix's K and V read once for all requests
+    shared_prefix_attention  each layer; a decode step reads the prefix once per 128 query rows of all requests
     topk_attention           each layer, over the slots that resolve_resident finds for selected positions
 
 K, V, queries and selections are random numbers in place of a model's. The reference's counterpart is its serving

@@ -501,7 +501,7 @@ typedef struct ekv_prefix_attention_args {
     const ekv_tensor* prefix_lengths; /* [G] */
     const ekv_tensor* group_starts;   /* NULL (one group of all rows) or [G + 1] first batch row of each group */
     const ekv_tensor* query_starts;   /* NULL (one query token a row) or [B + 1] first query token of each row */
-    int64_t max_query;                /* the most query tokens of a row, or about: picks kernels, never results */
+    int64_t max_query;                /* the most query tokens of a row, or about: picks kernels, not what is seen */
     double scale;                     /* of the scores, e.g. D^-0.5 */
     const ekv_tensor* output;         /* [N, Hq, D], the query's type */
     const ekv_tensor* lse;            /* NULL or [N, Hq] float32 */
@@ -520,8 +520,10 @@ uint64_t ekv_shared_prefix_workspace_bytes(int64_t tokens, int64_t batch, int64_
  * 0 .. prefix_lengths[g] - 1 and its request's own tokens
  * 0 .. lengths[b] - n + i. Over the tokens it sees, per query head h:
  *   output = sum_j softmax_j(scale q . k_j) v_j,  lse = log sum_j exp(scale q . k_j)
- * The prefix's K and V are read once for all rows of a group. Token t of a
- * table row lies in page table[t / page_size]; page ids below 1 or past the
+ * With rows = query tokens * Hq / Hkv: if max_query makes 64 rows at most and a
+ * group has more than that on average, the prefix's K and V are read once per
+ * 128 rows of a group, else once per batch row and tile of its rows. Token t of
+ * a table row lies in page table[t / page_size]; page ids below 1 or past the
  * pool, and tokens past the table's columns, are not seen, and their memory is
  * not read. A query token that sees nothing, or that belongs to no batch row,
  * gets zeros and lse -inf. Rows outside every group have no prefix, rows that
