@@ -69,8 +69,8 @@ def shared_prefix_attention(query, planes, block_tables, rows, lengths, prefix_t
     * Hq // kv_heads: if max_query makes 64 of them at most and a group has more
     on average, K and V of a prefix are read once per 128 query rows of its
     group, else once per batch row and tile of its rows. One choice serves the
-    whole call: decode rows and long prompt pieces behind one prefix are faster
-    as two calls.
+    whole call: many decode rows and a few prompt pieces behind a long prefix
+    are faster as two calls.
     A page id below 1 or past the pool is not seen (page 0 is the sink); a
     query token that sees nothing gets zeros and lse -inf. lse [N, Hq] float32:
     log of the sum of exp(scale q.k), which merges outputs of other parts.
