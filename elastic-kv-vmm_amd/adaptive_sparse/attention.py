@@ -1,4 +1,4 @@
-"""Attention over the paged K/V pool (HIP): behind a shared prefix, and over Top-K slots.
+"""Attention over the paged K/V pool (HIP): behind a shared prefix, over Top-K slots, and over lists of blocks.
 
 The reference resolves which pool rows a decode step reads - a shared
 prefix's blocks (adaptive_sparse/shared_prefix.py:122-204) or the selected
@@ -33,6 +33,11 @@ def shared_prefix_workspace(tokens, batch, groups, query_heads, kv_heads, head_d
 def topk_workspace(tokens, lanes, query_heads, kv_heads, head_dim):
     """Bytes of workspace that topk_attention needs for these sizes."""
     return _size("ekv_topk_workspace_bytes", tokens, lanes, query_heads, kv_heads, head_dim)
+
+
+def block_workspace(tokens, width, block_size, query_heads, kv_heads, head_dim, max_query=1):
+    """Bytes of workspace that block_attention needs for lists of `width` blocks."""
+    return _size("ekv_block_workspace_bytes", tokens, width, block_size, query_heads, kv_heads, head_dim, max_query)
 
 
 def _check(query, planes, workspace):
@@ -116,3 +121,33 @@ def topk_attention(query, planes, slots, output, *, kv_heads, layer=0, scale=Non
     status = helper.topk_attention(entries["ekv_topk_attention"], query, planes, int(layer), int(kv_heads), slots,
                                    int(zero_below), _scale(scale, dim), output, lse, workspace)
     _native.launch_check(status, "topk_attention")
+
+
+@profile_range("native/block_attention")
+def block_attention(query, planes, block_tables, rows, lengths, blocks, output, *, page_size, block_size, kv_heads,
+                    layer=0, query_starts=None, max_query=1, scale=None, lse=None, workspace=None):
+    """Attention of each query token to the tokens of its listed blocks, into `output`: one layer, no gather.
+
+    query, output, planes, block_tables, rows, lengths, query_starts, scale
+    and lse as in shared_prefix_attention (without prefixes); blocks [N, G, K]
+    int32 or int64 of any strides, as select_blocks writes them: KV head h
+    reads list h // (kv_heads // G). Query token i of a row's n is at position
+    p = lengths[b] - n + i and sees, of every block j that it lists, the
+    tokens j * block_size .. (j + 1) * block_size - 1 up to p. Ids below 0 or
+    behind the position name no block; a block listed twice counts twice. A
+    token that sees nothing gets zeros and lse -inf. max_query: the most query
+    tokens of a row, as far as known: it picks kernels, never which keys are
+    seen. workspace: block_workspace(...) bytes, as in shared_prefix_attention.
+    """
+    _check(query, planes, workspace)
+    tokens, heads, dim = query.shape
+    if blocks.dim() != 3:
+        raise ValueError("blocks must be shaped [tokens, lists, K]")
+    if workspace is None:
+        size = block_workspace(tokens, blocks.shape[2], block_size, heads, kv_heads, dim, max_query)
+        workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
+    helper, entries = _native.launch_helper()
+    status = helper.block_attention(entries["ekv_block_attention"], query, planes, layer, kv_heads, page_size,
+                                    block_size, block_tables, rows, lengths, blocks, query_starts, max_query,
+                                    _scale(scale, dim), output, lse, workspace)
+    _native.launch_check(status, "block_attention")

@@ -12,6 +12,7 @@
 // (ekv_attention.h).
 #include "ekv_attention.h"
 #include "ekv_mfma.h"
+#include "ekv_pool.h"
 
 #include <algorithm>
 #include <limits>
@@ -310,49 +311,6 @@ constexpr int64_t kMostHeads = 65535, kMostTokens = 1 << 23, kMostRows = int64_t
                   kMostBatch = 1 << 20;
 constexpr int32_t kComputeUnits = 256;
 
-void need_aligned(int64_t value, const char* what) {
-    if (value % 16 != 0) {
-        throw std::invalid_argument(std::string(what) + " must be a multiple of 16 bytes");
-    }
-}
-
-// A [tokens, heads, dim] tensor of 16-bit floats whose rows are dense and whose pieces of 8 are 16-byte aligned.
-const ekv_tensor& need_rows(const ekv_tensor* p, const char* name) {
-    const ekv_tensor& t = need(p, name);
-    need_ndim(t, 3, name);
-    if (t.dtype != EKV_BFLOAT16 && t.dtype != EKV_FLOAT16) {
-        throw std::invalid_argument(std::string(name) + " must be bfloat16 or float16");
-    }
-    need_data(t, name);
-    if (t.shape[2] > 1 && t.stride[2] != 1) {
-        throw std::invalid_argument(std::string(name) + " must be dense in its last dimension");
-    }
-    if (numel(t) > 0) {
-        need_aligned(reinterpret_cast<int64_t>(t.data), (std::string(name) + " address").c_str());
-        need_aligned(t.shape[0] > 1 ? t.stride[0] * 2 : 0, (std::string(name) + " token stride").c_str());
-        need_aligned(t.shape[1] > 1 ? t.stride[1] * 2 : 0, (std::string(name) + " head stride").c_str());
-    }
-    return t;
-}
-
-const ekv_tensor& need_list(const ekv_tensor* p, int64_t extent, const char* name) {
-    const ekv_tensor& t = need(p, name);
-    need_ndim(t, 1, name);
-    need_index(t, name);
-    need_dim(t, 0, extent, name);
-    need_data(t, name);
-    return t;
-}
-
-// Bytes between the columns of a table of page ids.
-uint32_t column_step(const ekv_tensor& t, const char* name) {
-    const int64_t step = t.shape[1] > 1 ? t.stride[1] * itemsize(t.dtype) : 0;
-    if (step < 0 || step > 0x7fffffff) {
-        throw std::invalid_argument(std::string(name) + ": columns more than 2 GiB apart");
-    }
-    return static_cast<uint32_t>(step);
-}
-
 // Query, output, statistics and cache: what both entry points share.
 AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, int64_t layer, int64_t kv_heads,
                  int64_t page_size, double scale, const ekv_tensor* out_p, const ekv_tensor* lse_p) {
@@ -379,55 +337,16 @@ AttentionArgs common_args(const ekv_tensor* query_p, const ekv_planes* planes, i
     a.kv_heads = static_cast<int32_t>(kv_heads);
     a.share = a.heads / a.kv_heads;
     a.share_div = FastDiv(static_cast<uint32_t>(a.share));
-    if (planes == nullptr) {
-        throw std::invalid_argument("planes are required");
-    }
-    if (planes->kv != 2 || planes->layers < 0 || planes->rows < 0) {
-        throw std::invalid_argument("planes must hold K and V (kv 2)");
-    }
-    if (layer < 0 || layer >= planes->layers) {
-        throw std::invalid_argument("layer " + std::to_string(layer) + " outside the pool's " +
-                                    std::to_string(planes->layers));
-    }
-    if (page_size < 1 || page_size > (int64_t{1} << 30)) {
-        throw std::invalid_argument("page_size must be from 1 to 2^30");
-    }
-    const int64_t row = kv_heads * a.dim * 2;
-    int64_t token_stride, page_stride, pages;
-    constexpr int64_t kMostStride = 0xffffffff;
-    if (planes->row_stride < 0 || planes->row_stride > kMostStride) {
-        throw std::invalid_argument("the plane row stride must be below 4 GiB");
-    }
-    if (planes->row_bytes == row) {                       // a plane row is a token
-        token_stride = planes->row_stride;
-        page_stride = planes->row_stride * page_size;
-        pages = planes->rows / page_size;
-    } else if (planes->row_bytes == row * page_size) {    // a plane row is a page
-        token_stride = row;
-        page_stride = planes->row_stride;
-        pages = planes->rows;
-    } else {
-        throw std::invalid_argument("plane rows hold " + std::to_string(planes->row_bytes) + " bytes: neither a token's " +
-                                    std::to_string(row) + " nor a page's " + std::to_string(row * page_size));
-    }
-    if (planes->base == nullptr && planes->rows > 0) {
-        throw std::invalid_argument("null plane base");
-    }
-    if (page_stride > kMostStride || pages > 0x7fffffff) {
-        throw std::invalid_argument("a page must lie within 4 GiB, and a plane hold fewer than 2^31 pages");
-    }
+    const PlanePages pages = plane_pages(planes, layer, kv_heads * a.dim * 2, page_size, 2);
     Cache& c = a.cache;
-    c.token_stride = static_cast<uint32_t>(token_stride);
-    c.page_stride = static_cast<uint32_t>(page_stride);
-    c.pages = static_cast<uint32_t>(pages);
+    c.token_stride = static_cast<uint32_t>(pages.token_stride);
+    c.page_stride = static_cast<uint32_t>(pages.page_stride);
+    c.pages = static_cast<uint32_t>(pages.pages);
     c.head_stride = static_cast<uint32_t>(dim * 2);
     c.page = FastDiv(static_cast<uint32_t>(page_size));
     c.zero_below = 1;
-    c.k = static_cast<const char*>(planes->base) + layer * planes->layer_stride;
-    c.kv_stride = planes->kv_stride;
-    need_aligned(reinterpret_cast<int64_t>(c.k), "plane address");
-    need_aligned(planes->kv_stride, "kv stride");
-    need_aligned(planes->row_stride, "plane row stride");
+    c.k = pages.at;
+    c.kv_stride = pages.kv_stride;
     a.query = static_cast<const char*>(query.data);
     a.q_token = query.stride[0] * 2, a.q_head = query.stride[1] * 2;
     a.out = static_cast<char*>(out.data);
@@ -580,6 +499,23 @@ Plan topk_plan(int64_t tokens, int64_t lanes, int64_t heads, int64_t kv_heads, i
     return plan;
 }
 
+Plan block_plan(int64_t tokens, int64_t width, int64_t block_size, int64_t heads, int64_t kv_heads, int64_t dim,
+                int64_t max_query) {
+    constexpr int64_t kMost = (int64_t{1} << 30) - 1;
+    if (block_size < 1 || block_size > kMost || width < 0 || width > kMost / block_size) {
+        throw std::invalid_argument("a list of blocks may name at most 2^30 - 1 tokens");
+    }
+    if (max_query < 1) {
+        throw std::invalid_argument("max_query must be positive");
+    }
+    need_sizes(tokens, 0, heads, kv_heads, dim);
+    Plan plan;
+    const int32_t dim_pad = padded_dim(dim);
+    plan.tiles16 = std::min(tiles_for(heads / kv_heads, dim_pad), dim_pad <= 128 ? 4 : 2);
+    cut(plan, plan.own, kSlots, tokens, plan.tiles16, tokens, heads / kv_heads, kv_heads, dim_pad, true);
+    return plan;
+}
+
 void place(Phase& p, void* workspace) {
     const auto at = [&](auto*& pointer) {
         pointer = reinterpret_cast<std::remove_reference_t<decltype(pointer)>>(static_cast<char*>(workspace) +
@@ -592,7 +528,8 @@ void place(Phase& p, void* workspace) {
     }
 }
 
-int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, uint64_t bytes, void* stream) {
+int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, uint64_t bytes, void* stream,
+           const BlockLists* lists = nullptr) {
     if (bytes < plan.bytes) {
         throw std::invalid_argument("the attention needs " + std::to_string(plan.bytes) + " workspace bytes, got " +
                                     std::to_string(bytes));
@@ -616,11 +553,13 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
     if (plan.pair) {
         place(plan.prefix, workspace);
         fit_units(plan.prefix, a.prefix_most);
-        launch_pair(Launch{a, {plan.own, plan.prefix}}, dtype, stream);
+        launch_pair(Launch{a, {plan.own, plan.prefix}, {}}, dtype, stream);
+    } else if (lists != nullptr) {
+        launch_blocks(Launch{a, {plan.own, {}}, *lists}, dtype, plan.tiles16, stream);
     } else if (plan.tiles16 < 8) {
-        launch_narrow(Launch{a, {plan.own, {}}}, dtype, plan.tiles16, stream);
+        launch_narrow(Launch{a, {plan.own, {}}, {}}, dtype, plan.tiles16, stream);
     } else {
-        launch_wide(Launch{a, {plan.own, {}}}, dtype, stream);
+        launch_wide(Launch{a, {plan.own, {}}, {}}, dtype, stream);
     }
     const auto merge = [&]<typename T>(T) {
         const auto on = static_cast<hipStream_t>(stream);
@@ -646,20 +585,22 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
     return 0;
 }
 
-int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t workspace_bytes, void* stream) {
-    AttentionArgs a = common_args(s.query, s.planes, s.layer, s.kv_heads, s.page_size, s.scale, s.output, s.lse);
-    const auto need_table = [&](const ekv_tensor* p, const char* name) -> const ekv_tensor& {
-        const ekv_tensor& t = need(p, name);
-        need_ndim(t, 2, name);
-        need_index(t, name);
-        need_data(t, name);
-        if (t.shape[1] > ((int64_t{1} << 30) - 1) / s.page_size) {
-            throw std::invalid_argument(std::string(name) + " rows may cover at most 2^30 - 1 tokens");
-        }
-        return t;
-    };
-    const ekv_tensor& tables = need_table(s.block_tables, "block_tables");
-    const ekv_tensor& lengths = need(s.lengths, "lengths");
+const ekv_tensor& need_table(const ekv_tensor* p, int64_t page_size, const char* name) {
+    const ekv_tensor& t = need(p, name);
+    need_ndim(t, 2, name);
+    need_index(t, name);
+    need_data(t, name);
+    if (t.shape[1] > ((int64_t{1} << 30) - 1) / page_size) {
+        throw std::invalid_argument(std::string(name) + " rows may cover at most 2^30 - 1 tokens");
+    }
+    return t;
+}
+
+// The batch rows: their pages, lengths and query tokens. Returns how many tokens a table row covers.
+int32_t own_tables(AttentionArgs& a, const ekv_tensor* tables_p, const ekv_tensor* rows, const ekv_tensor* lengths_p,
+                   const ekv_tensor* query_starts, int64_t max_query, int64_t page_size) {
+    const ekv_tensor& tables = need_table(tables_p, page_size, "block_tables");
+    const ekv_tensor& lengths = need(lengths_p, "lengths");
     need_ndim(lengths, 1, "lengths");
     need_index(lengths, "lengths");
     need_data(lengths, "lengths");
@@ -673,24 +614,29 @@ int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t 
     a.table_col = column_step(tables, "block_tables");
     a.table64 = tables.dtype == EKV_INT64;
     a.requests = static_cast<int32_t>(std::min<int64_t>(tables.shape[0], 0x7fffffff));
-    a.own_most = static_cast<int32_t>(tables.shape[1] * s.page_size);
-    if (s.rows != nullptr) {
-        a.rows = index_ref(need_list(s.rows, a.batch, "rows"), 0);
+    if (rows != nullptr) {
+        a.rows = index_ref(need_list(rows, a.batch, "rows"), 0);
     }
-    if (s.max_query < 1) {
+    if (max_query < 1) {
         throw std::invalid_argument("max_query must be positive");
     }
-    if (s.query_starts != nullptr) {
-        a.query_starts = index_ref(need_list(s.query_starts, a.batch + 1, "query_starts"), 0);
+    if (query_starts != nullptr) {
+        a.query_starts = index_ref(need_list(query_starts, a.batch + 1, "query_starts"), 0);
     } else if (a.tokens != a.batch) {
         throw std::invalid_argument("without query_starts every batch row has one query token: got " +
                                     std::to_string(a.tokens) + " for " + std::to_string(a.batch) + " rows");
     }
+    return static_cast<int32_t>(tables.shape[1] * page_size);
+}
+
+int shared_prefix(const ekv_prefix_attention_args& s, void* workspace, uint64_t workspace_bytes, void* stream) {
+    AttentionArgs a = common_args(s.query, s.planes, s.layer, s.kv_heads, s.page_size, s.scale, s.output, s.lse);
+    a.own_most = own_tables(a, s.block_tables, s.rows, s.lengths, s.query_starts, s.max_query, s.page_size);
     if ((s.prefix_tables == nullptr) != (s.prefix_lengths == nullptr)) {
         throw std::invalid_argument("prefix_tables and prefix_lengths are given together");
     }
     if (s.prefix_tables != nullptr) {
-        const ekv_tensor& prefix = need_table(s.prefix_tables, "prefix_tables");
+        const ekv_tensor& prefix = need_table(s.prefix_tables, s.page_size, "prefix_tables");
         if (prefix.shape[0] > kMostBatch) {
             throw std::invalid_argument("more than 2^20 prefixes");
         }
@@ -740,6 +686,29 @@ int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64
     return launch(a, plan, query->dtype, workspace, workspace_bytes, stream);
 }
 
+int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t workspace_bytes, void* stream) {
+    AttentionArgs a = common_args(s.query, s.planes, s.layer, s.kv_heads, s.page_size, s.scale, s.output, s.lse);
+    a.block_most = own_tables(a, s.block_tables, s.rows, s.lengths, s.query_starts, s.max_query, s.page_size);
+    const ekv_tensor& blocks = need(s.blocks, "blocks");
+    need_ndim(blocks, 3, "blocks");
+    need_index(blocks, "blocks");
+    need_dim(blocks, 0, a.tokens, "blocks");
+    need_data(blocks, "blocks");
+    if (blocks.shape[1] < 1 || a.kv_heads % blocks.shape[1] != 0) {
+        throw std::invalid_argument("blocks must have a divisor of kv_heads as lists");
+    }
+    Plan plan = block_plan(a.tokens, blocks.shape[2], s.block_size, a.heads, a.kv_heads, a.dim, s.max_query);
+    a.own_most = static_cast<int32_t>(blocks.shape[2] * s.block_size);
+    BlockLists lists{};
+    lists.lists = static_cast<const char*>(blocks.data);
+    lists.token = blocks.stride[0] * itemsize(blocks.dtype), lists.group = blocks.stride[1] * itemsize(blocks.dtype);
+    lists.column = column_step(blocks, "blocks", 2);
+    lists.wide = blocks.dtype == EKV_INT64 ? 4 : 0;
+    lists.block = FastDiv(static_cast<uint32_t>(s.block_size));
+    lists.heads = FastDiv(static_cast<uint32_t>(a.kv_heads / blocks.shape[1]));
+    return launch(a, plan, s.query->dtype, workspace, workspace_bytes, stream, &lists);
+}
+
 }  // namespace
 }  // namespace ekv
 
@@ -771,5 +740,22 @@ extern "C" int ekv_topk_attention(const ekv_tensor* query, const ekv_planes* pla
     return ekv::guarded(-1, [&] {
         return ekv::topk(query, planes, layer, kv_heads, slots, zero_below, scale, output, lse, workspace,
                          workspace_bytes, stream);
+    });
+}
+
+extern "C" uint64_t ekv_block_workspace_bytes(int64_t tokens, int64_t width, int64_t block_size, int64_t heads,
+                                              int64_t kv_heads, int64_t head_dim, int64_t max_query) {
+    return ekv::guarded(~uint64_t{0}, [&] {
+        return ekv::block_plan(tokens, width, block_size, heads, kv_heads, head_dim, max_query).bytes;
+    });
+}
+
+extern "C" int ekv_block_attention(const ekv_block_attention_args* args, void* workspace, uint64_t workspace_bytes,
+                                   void* stream) {
+    return ekv::guarded(-1, [&] {
+        if (args == nullptr) {
+            throw std::invalid_argument("args is required");
+        }
+        return ekv::block_attention(*args, workspace, workspace_bytes, stream);
     });
 }

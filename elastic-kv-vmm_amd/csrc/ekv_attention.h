@@ -47,7 +47,8 @@ struct AttentionArgs {
     int64_t prefix_row;
     uint32_t table_col, prefix_col;
     int32_t requests;
-    int32_t own_most, prefix_most;   // tokens that a table row covers
+    int32_t own_most, prefix_most;   // tokens that a table row covers; of a list of blocks, its places
+    int32_t block_most;              // with lists of blocks, tokens that a table row covers
     IndexRef rows, lengths, query_starts, prefix_lengths, group_starts;
     int32_t table64, prefix64;
     int32_t tokens, batch, groups;
@@ -61,7 +62,7 @@ enum PhaseMode : int32_t {
     kPrefixes,   // sequences are groups: all their query tokens against their prefix
     kOwn,        // sequences are batch rows against their own tokens
     kWhole,      // sequences are batch rows against prefix and own tokens
-    kSlots,      // sequences are query tokens against their slots
+    kSlots,      // sequences are query tokens against their slots, or the places of their lists of blocks
 };
 
 // One launch's cut and where its parts go.
@@ -86,9 +87,20 @@ struct Phase {
 // The arguments of a kernel. They are more words than a wave has scalar registers, and the compiler loads all of them
 // first and spills what does not fit into vector registers; fresh() hides where they come from, so that each part of a
 // kernel loads what it needs where it needs it.
+// Lists of blocks instead of slots (kSlots): place i of a list is token i % block of the block that its entry i / block
+// names; pages of tokens come from AttentionArgs::tables.
+struct BlockLists {
+    const char* lists;                // [N, G, K]
+    int64_t token, group;             // bytes
+    uint32_t column;
+    int32_t wide;                     // 4 for int64 ids
+    FastDiv block, heads;             // tokens of a block; KV heads of a list
+};
+
 struct Launch {
     AttentionArgs a;
     Phase p[2];        // own tokens (or all), prefixes
+    BlockLists lists;
 };
 
 constexpr float kLn2 = 0.6931471805599453f;
@@ -98,6 +110,9 @@ constexpr float kSlack = 8.0f;       // bits by which a weight may pass 1 before
 
 // What a key that is not seen reads: weight 0 must meet a finite V.
 __device__ __align__(256) static const uint32_t zero_row[128] = {};
+
+// What a place behind a list's end reads: a block that nobody has.
+__device__ static const uint32_t no_entry[2] = {0xffffffffu, 0xffffffffu};
 
 struct Sequence {
     int32_t first, count;       // query tokens
@@ -512,6 +527,9 @@ __device__ __forceinline__ uint32_t wide_place(int32_t dim_pad, uint32_t row, ui
 constexpr int kNarrowUnit = 7;
 int narrow_groups(int tiles16, int32_t dim_pad);
 void launch_narrow(const Launch& l, int32_t dtype, int tiles16, void* stream);
+
+// attention_blocks.hip: the same over lists of blocks, at most 64 rows (32 of 256 columns) a tile.
+void launch_blocks(const Launch& l, int32_t dtype, int tiles16, void* stream);
 
 // attention_wide.hip: row tiles of 128 (row_shift 7) or 256 rows, units of at least 2^kWideUnit keys.
 constexpr int kWideUnit = 6;

@@ -87,13 +87,75 @@ struct Ids {
     uint32_t low[2], high[2];
 };
 
+// The pages behind a list of blocks.
+struct BlockSource {
+    const char* pages;        // the request's row of the page table
+    uint32_t step, wide;      // bytes between columns; 4 for int64 ids
+    uint32_t newest;          // the last block that the query token sees anything of
+    uint32_t seen;            // tokens that it sees: 0 .. seen - 1
+    FastDiv block;
+};
+
+// What query token g.q.first sees; src becomes its list's source.
+__device__ __forceinline__ BlockSource block_source(const AttentionArgs& a, const Segment& g, Source& src) {
+    const BlockLists& lists = fresh().lists;
+    const int32_t token = g.q.first;
+    int32_t b = token, last = token;             // batch row; its last query token
+    if (a.query_starts.data != nullptr) {
+        int32_t low = 0, high = a.batch;
+        while (high - low > 1) {
+            const int32_t mid = (low + high) >> 1;
+            const bool here = first_token(a, mid) <= token;
+            low = here ? mid : low;
+            high = here ? high : mid;
+        }
+        last = a.batch > 0 ? first_token(a, low + 1) - 1 : -1;
+        b = last >= token && first_token(a, low) <= token ? low : -1;
+    }
+    int64_t request = -1, length = 0;
+    if (b >= 0) {
+        length = a.lengths.fetch(b);
+        request = a.rows.data != nullptr ? a.rows.fetch(b) : b;
+    }
+    const bool good = request >= 0 && request < a.requests;
+    const int64_t position = clamped(length, 0, 0x7ffffffe) - 1 - (last - token);
+    const int32_t seen = good ? clamped(position + 1, 0, a.block_most) : 0;
+    BlockSource s;
+    s.block = lists.block;
+    s.seen = seen;
+    s.newest = lists.block.div(max(seen - 1, 0));
+    s.pages = a.tables + (good ? request : 0) * a.table_row;
+    s.step = a.table_col;
+    s.wide = a.table64 != 0 ? 4 : 0;
+    src.table = lists.lists + token * lists.token + static_cast<int64_t>(lists.heads.div(g.head)) * lists.group;
+    src.step = lists.column;
+    src.wide = lists.wide;
+    return s;
+}
+
 template <int kTiles>
 constexpr int stats_bytes() {
     return 2 * kWaves * kTiles * 16 * static_cast<int>(sizeof(float));
 }
 
+// The same of a token that a list of blocks names, and its place in its page (~0: it names no token that is seen).
+struct BlockIds : Ids {
+    uint32_t inside[2];
+};
+
+template <bool kBlocks>
+struct IdsOf {
+    typedef Ids type;
+};
+template <>
+struct IdsOf<true> {
+    typedef BlockIds type;
+};
+
 // Workgroup w's part of phase `which` of the launch. s_data: lds_bytes(), stats: stats_bytes() of LDS.
-template <typename T, int kDim, int kTiles, int kChunk>
+// kBlocks: a sequence's keys are those of the blocks that its list names. Their addresses take two reads one after the
+// other, entry and page id, so the entries are asked for a tile earlier than the page ids.
+template <typename T, int kDim, int kTiles, bool kBlocks = false, int kChunk>
 __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, bool read, uint32_t total,
                                     char* s_data, char* stats, LineCells<kWaves, kChunk>& cells) {
     constexpr int kSteps = kDim / 32;      // matrix steps of the first product
@@ -105,6 +167,7 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
     float (*const s_sum)[kTiles * 16] = s_max + kWaves;
     char* const values = s_data + wave * (kKeys * Rows<kDim>::kBytes);
     const char* const zeros = reinterpret_cast<const char*>(zero_row);
+    [[maybe_unused]] const char* const minus_one = reinterpret_cast<const char*>(no_entry);
 
     for_segments(which, w, workgroups, read, total, cells, [&](const Segment& g) {
         const int lane = hidden(threadIdx.x) & 63, col = lane & 15, quad = lane >> 4;
@@ -157,12 +220,49 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
             src.step = own ? a.table_col : a.prefix_col;
             src.wide = (own ? a.table64 : a.prefix64) != 0 ? 4 : 0;
             src.keys = min(own ? g.q.own : g.q.prefix, to << unit_shift);
+            BlockSource blocks;
+            if constexpr (kBlocks) {
+                blocks = block_source(a, g, src);
+            }
             const char* const k_head = a.cache.k + static_cast<uint64_t>(a.cache.head_stride) * g.head + quad * 16;
             const char* const v_head = k_head + a.cache.kv_stride;
 
             const Cache cache = a.cache;
-            const auto ids_of = [&](int32_t base) {
-                Ids e;
+            typedef typename IdsOf<kBlocks>::type KeyIds;
+            const auto entries_of = [&](int32_t base) {
+                Ids e = {};
+                if constexpr (kBlocks) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int32_t key = base + h * 16 + col;
+                        const char* at = src.table + static_cast<uint64_t>(blocks.block.div(key)) * src.step;
+                        at = key < src.keys ? at : minus_one;
+                        e.low[h] = load_global<uint32_t>(at);
+                        e.high[h] = load_global<uint32_t>(at + src.wide);
+                    }
+                }
+                return e;
+            };
+            const auto ids_of = [&](int32_t base, [[maybe_unused]] const Ids& entries) {
+                KeyIds e;
+                if constexpr (kBlocks) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int32_t key = base + h * 16 + col;
+                        const uint32_t block = entries.low[h];
+                        const uint32_t offset = key - blocks.block.div(key) * blocks.block.divisor;
+                        const uint32_t token = block * blocks.block.divisor + offset;
+                        const bool good = block <= blocks.newest && (src.wide == 0 || entries.high[h] == 0) &&
+                                          token < blocks.seen;
+                        const uint32_t page = cache.page.div(token);
+                        const char* at = blocks.pages + static_cast<uint64_t>(page) * blocks.step;
+                        at = good ? at : zeros;
+                        e.low[h] = load_global<uint32_t>(at);
+                        e.high[h] = load_global<uint32_t>(at + blocks.wide);
+                        e.inside[h] = good ? token - page * cache.page.divisor : ~0u;
+                    }
+                    return e;
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int32_t key = base + h * 16 + col;
@@ -175,15 +275,21 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
             };
             words4 k[2][kSteps], v[2][kSteps];
             uint32_t seen;                    // bit per key of the tile
-            const auto fetch = [&](int32_t base, const Ids& e) {
+            const auto fetch = [&](int32_t base, const KeyIds& e) {
                 seen = 0;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int32_t key = base + h * 16 + col;
                     const uint32_t id = e.low[h];
-                    const bool good = key < src.keys && id >= cache.zero_below && id < cache.pages &&
-                                      (src.wide == 0 || e.high[h] == 0);
-                    const uint32_t inside = key - cache.page.div(key) * cache.page.divisor;
+                    bool good = id >= cache.zero_below && id < cache.pages;
+                    uint32_t inside;
+                    if constexpr (kBlocks) {
+                        inside = e.inside[h];
+                        good = good && inside != ~0u && (blocks.wide == 0 || e.high[h] == 0);
+                    } else {
+                        inside = key - cache.page.div(key) * cache.page.divisor;
+                        good = key < src.keys && good && (src.wide == 0 || e.high[h] == 0);
+                    }
                     const uint64_t offset = static_cast<uint64_t>(id) * cache.page_stride +
                                             static_cast<uint64_t>(inside) * cache.token_stride;
                     const char* k_at = k_head + offset;
@@ -204,11 +310,14 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
 
             constexpr int kStride = kWaves * kKeys;
             const int32_t start = (from << unit_shift) + wave * kKeys;
-            const Ids first = ids_of(start);
-            Ids ids = ids_of(start + kStride);
+            const Ids first_entries = entries_of(start), second_entries = entries_of(start + kStride);
+            Ids entries = entries_of(start + 2 * kStride);
+            const KeyIds first = ids_of(start, first_entries);
+            KeyIds ids = ids_of(start + kStride, second_entries);
             fetch(start, first);
             const auto tile = [&](int32_t base) {
-                const Ids later = ids_of(base + 2 * kStride);
+                const KeyIds later = ids_of(base + 2 * kStride, entries);
+                entries = entries_of(base + 3 * kStride);
                 const uint32_t now = seen;
                 // Whether some row sees fewer keys of this tile than it holds.
                 const bool ragged = own && base + kKeys > first_visible;

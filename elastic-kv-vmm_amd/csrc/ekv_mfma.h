@@ -27,6 +27,9 @@ struct Bf16 {
     static __device__ __forceinline__ uint32_t pack(float low, float high) {
         return __builtin_bit_cast(uint32_t, x2{static_cast<__bf16>(low), static_cast<__bf16>(high)});
     }
+    static __device__ __forceinline__ float value(uint16_t bits) {
+        return __uint_as_float(static_cast<uint32_t>(bits) << 16);
+    }
     // The element in the word's low half if it is an infinity or a NaN, else 0.
     static __device__ __forceinline__ float unbounded(uint32_t word) {
         return (word & 0x7f80u) == 0x7f80u ? __uint_as_float(word << 16) : 0.0f;
@@ -49,6 +52,9 @@ struct F16 {
     }
     static __device__ __forceinline__ uint32_t pack(float low, float high) {
         return __builtin_bit_cast(uint32_t, x2{static_cast<_Float16>(low), static_cast<_Float16>(high)});
+    }
+    static __device__ __forceinline__ float value(uint16_t bits) {
+        return static_cast<float>(__builtin_bit_cast(_Float16, bits));
     }
     static __device__ __forceinline__ float unbounded(uint32_t word) {
         return (word & 0x7c00u) == 0x7c00u

@@ -4,8 +4,10 @@
 // ekv_scatter_kv, ekv_move_kv), the residency summary
 // (ekv_residency_summary), the batch-token swap-in (ekv_swap_in*), the
 // per-layer SGLang-convention swap-in (ekv_hisparse_swap_in), the one-call
-// decode step (ekv_decode_step), the block tables (ekv_extend_block_tables) and
-// both attentions (ekv_shared_prefix_attention, ekv_topk_attention). Their
+// decode step (ekv_decode_step), the block tables (ekv_extend_block_tables), the
+// attentions (ekv_shared_prefix_attention, ekv_topk_attention,
+// ekv_block_attention), the new tokens' rows (ekv_append_rotary,
+// ekv_append_index) and the block selection (ekv_select_blocks). Their
 // GPU work can be a few microseconds at small shapes, so describing the
 // tensors for the C ABI from Python (attribute reads and struct packing,
 // about 1 us per tensor) set the call rate. Here the
@@ -866,6 +868,199 @@ PyObject* topk_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     }
 }
 
+// block_attention(entry, query, planes, layer, kv_heads, page_size,
+//                 block_size, block_tables, rows, lengths, blocks,
+//                 query_starts, max_query, scale, output, lse, workspace)
+// -> status of ekv_block_attention
+PyObject* block_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+    if (argc != 17) {
+        PyErr_SetString(PyExc_TypeError, "block_attention takes 17 arguments");
+        return nullptr;
+    }
+    ekv_block_attention_args call{};
+    int64_t entry = 0;
+    if (!read_int(argv[0], "entry", entry) || !read_int(argv[3], "layer", call.layer) ||
+        !read_int(argv[4], "kv_heads", call.kv_heads) || !read_int(argv[5], "page_size", call.page_size) ||
+        !read_int(argv[6], "block_size", call.block_size) || !read_int(argv[12], "max_query", call.max_query) ||
+        !read_scale(argv[13], call.scale)) {
+        return nullptr;
+    }
+    Arg args[] = {{argv[1], "query"},         {argv[7], "block_tables"}, {argv[8], "rows"},
+                  {argv[9], "lengths"},       {argv[10], "blocks"},      {argv[11], "query_starts"},
+                  {argv[14], "output"},       {argv[15], "lse"},         {argv[16], "workspace", false}};
+    try {
+        const int device = describe_all(args);
+        if (device < 0) {
+            return nullptr;
+        }
+        ekv_planes planes{};
+        if (!read_planes(argv[2], planes) || !planes_on(argv[2], device)) {
+            return nullptr;
+        }
+        call.query = args[0].pointer();
+        call.planes = &planes;
+        call.block_tables = args[1].pointer();
+        call.rows = args[2].pointer();
+        call.lengths = args[3].pointer();
+        call.blocks = args[4].pointer();
+        call.query_starts = args[5].pointer();
+        call.output = args[6].pointer();
+        call.lse = args[7].pointer();
+        const at::Tensor* workspace = args[8].tensor;
+        void* data = workspace != nullptr ? workspace->data_ptr() : nullptr;
+        const uint64_t bytes =
+            workspace != nullptr ? static_cast<uint64_t>(workspace->numel()) * workspace->element_size() : 0;
+        CurrentDevice current(device);
+        void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+        int status = 0;
+        Py_BEGIN_ALLOW_THREADS
+        status = reinterpret_cast<decltype(&ekv_block_attention)>(entry)(&call, data, bytes, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(status);
+    } catch (const std::exception& error) {
+        PyErr_SetString(PyExc_RuntimeError, error.what());
+        return nullptr;
+    }
+}
+
+// append_rotary(entry, query, key, value, planes, layer, page_size, slots,
+//               zero_below, positions, turns, magnitude, interleaved, output)
+// -> status of ekv_append_rotary (planes may be None)
+PyObject* append_rotary(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+    if (argc != 14) {
+        PyErr_SetString(PyExc_TypeError, "append_rotary takes 14 arguments");
+        return nullptr;
+    }
+    ekv_append_args call{};
+    int64_t entry = 0;
+    if (!read_int(argv[0], "entry", entry) || !read_int(argv[5], "layer", call.layer) ||
+        !read_int(argv[6], "page_size", call.page_size) || !read_int(argv[8], "zero_below", call.zero_below) ||
+        !read_scale(argv[11], call.magnitude) || !read_int(argv[12], "interleaved", call.interleaved)) {
+        return nullptr;
+    }
+    Arg args[] = {{argv[1], "query"}, {argv[2], "key"},        {argv[3], "value"}, {argv[7], "slots"},
+                  {argv[9], "positions"}, {argv[10], "turns"}, {argv[13], "output"}};
+    try {
+        const int device = describe_all(args);
+        if (device < 0) {
+            return nullptr;
+        }
+        ekv_planes planes{};
+        if (argv[4] != Py_None) {
+            if (!read_planes(argv[4], planes) || !planes_on(argv[4], device)) {
+                return nullptr;
+            }
+            call.planes = &planes;
+        }
+        call.query = args[0].pointer();
+        call.key = args[1].pointer();
+        call.value = args[2].pointer();
+        call.slots = args[3].pointer();
+        call.positions = args[4].pointer();
+        call.turns = args[5].pointer();
+        call.output = args[6].pointer();
+        CurrentDevice current(device);
+        void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+        int status = 0;
+        Py_BEGIN_ALLOW_THREADS
+        status = reinterpret_cast<decltype(&ekv_append_rotary)>(entry)(&call, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(status);
+    } catch (const std::exception& error) {
+        PyErr_SetString(PyExc_RuntimeError, error.what());
+        return nullptr;
+    }
+}
+
+// append_index(entry, index_key, planes, layer, page_size, scales, slots,
+//              zero_below) -> status of ekv_append_index
+PyObject* append_index(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+    if (argc != 8) {
+        PyErr_SetString(PyExc_TypeError, "append_index takes 8 arguments");
+        return nullptr;
+    }
+    int64_t entry = 0, layer = 0, page_size = 0, zero_below = 0;
+    if (!read_int(argv[0], "entry", entry) || !read_int(argv[3], "layer", layer) ||
+        !read_int(argv[4], "page_size", page_size) || !read_int(argv[7], "zero_below", zero_below)) {
+        return nullptr;
+    }
+    Arg args[] = {{argv[1], "index_key"}, {argv[5], "scales"}, {argv[6], "slots"}};
+    try {
+        const int device = describe_all(args);
+        if (device < 0) {
+            return nullptr;
+        }
+        ekv_planes planes{};
+        if (!read_planes(argv[2], planes) || !planes_on(argv[2], device)) {
+            return nullptr;
+        }
+        CurrentDevice current(device);
+        void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+        int status = 0;
+        Py_BEGIN_ALLOW_THREADS
+        status = reinterpret_cast<decltype(&ekv_append_index)>(entry)(
+            args[0].pointer(), &planes, layer, page_size, args[1].pointer(), args[2].pointer(), zero_below, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(status);
+    } catch (const std::exception& error) {
+        PyErr_SetString(PyExc_RuntimeError, error.what());
+        return nullptr;
+    }
+}
+
+// select_blocks(entry, index_query, planes, layer, page_size, block_size,
+//               scales, block_tables, rows, lengths, query_starts, max_query,
+//               first, last, blocks, workspace) -> status of ekv_select_blocks
+PyObject* select_blocks(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+    if (argc != 16) {
+        PyErr_SetString(PyExc_TypeError, "select_blocks takes 16 arguments");
+        return nullptr;
+    }
+    ekv_select_args call{};
+    int64_t entry = 0;
+    if (!read_int(argv[0], "entry", entry) || !read_int(argv[3], "layer", call.layer) ||
+        !read_int(argv[4], "page_size", call.page_size) || !read_int(argv[5], "block_size", call.block_size) ||
+        !read_int(argv[11], "max_query", call.max_query) || !read_int(argv[12], "first", call.first) ||
+        !read_int(argv[13], "last", call.last)) {
+        return nullptr;
+    }
+    Arg args[] = {{argv[1], "index_query"},  {argv[6], "scales"},  {argv[7], "block_tables"}, {argv[8], "rows"},
+                  {argv[9], "lengths"}, {argv[10], "query_starts"}, {argv[14], "blocks"},
+                  {argv[15], "workspace", false}};
+    try {
+        const int device = describe_all(args);
+        if (device < 0) {
+            return nullptr;
+        }
+        ekv_planes planes{};
+        if (!read_planes(argv[2], planes) || !planes_on(argv[2], device)) {
+            return nullptr;
+        }
+        call.index_query = args[0].pointer();
+        call.planes = &planes;
+        call.scales = args[1].pointer();
+        call.block_tables = args[2].pointer();
+        call.rows = args[3].pointer();
+        call.lengths = args[4].pointer();
+        call.query_starts = args[5].pointer();
+        call.blocks = args[6].pointer();
+        const at::Tensor* workspace = args[7].tensor;
+        void* data = workspace != nullptr ? workspace->data_ptr() : nullptr;
+        const uint64_t bytes =
+            workspace != nullptr ? static_cast<uint64_t>(workspace->numel()) * workspace->element_size() : 0;
+        CurrentDevice current(device);
+        void* stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+        int status = 0;
+        Py_BEGIN_ALLOW_THREADS
+        status = reinterpret_cast<decltype(&ekv_select_blocks)>(entry)(&call, data, bytes, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(status);
+    } catch (const std::exception& error) {
+        PyErr_SetString(PyExc_RuntimeError, error.what());
+        return nullptr;
+    }
+}
+
 PyObject* abi_version(PyObject*, PyObject*) { return PyLong_FromLong(EKV_ABI_VERSION); }
 
 PyObject* source_hash(PyObject*, PyObject*) { return PyUnicode_FromString(EKV_STRINGIFY(EKV_SOURCE_HASH)); }
@@ -893,6 +1088,14 @@ PyMethodDef methods[] = {
      METH_FASTCALL, "Describe the queries, tables and planes and call ekv_shared_prefix_attention."},
     {"topk_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(topk_attention)), METH_FASTCALL,
      "Describe the queries, slots and planes and call ekv_topk_attention."},
+    {"block_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(block_attention)),
+     METH_FASTCALL, "Describe the queries, lists of blocks, tables and planes and call ekv_block_attention."},
+    {"append_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(append_rotary)), METH_FASTCALL,
+     "Describe new tokens, their places and the planes and call ekv_append_rotary."},
+    {"append_index", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(append_index)), METH_FASTCALL,
+     "Describe new tokens' index keys and their places and call ekv_append_index."},
+    {"select_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(select_blocks)), METH_FASTCALL,
+     "Describe the index queries, keys and tables and call ekv_select_blocks."},
     {"abi_version", abi_version, METH_NOARGS, "EKV_ABI_VERSION this module was built against."},
     {"source_hash", source_hash, METH_NOARGS, "Fingerprint of the native sources this module was built from."},
     {nullptr, nullptr, 0, nullptr}};

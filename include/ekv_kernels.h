@@ -557,6 +557,132 @@ int ekv_topk_attention(const ekv_tensor* query, const ekv_planes* planes, int64_
                        const ekv_tensor* slots, int64_t zero_below, double scale, const ekv_tensor* output,
                        const ekv_tensor* lse, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* The arguments of ekv_block_attention. */
+typedef struct ekv_block_attention_args {
+    const ekv_tensor* query;          /* [N, Hq, D] bfloat16 or float16 */
+    const ekv_planes* planes;         /* the pool (kv 2); a plane row is a token or a whole page */
+    int64_t layer;
+    int64_t kv_heads;                 /* Hkv, a divisor of Hq: query head h reads KV head h / (Hq / Hkv) */
+    int64_t page_size;
+    int64_t block_size;               /* tokens of a block */
+    const ekv_tensor* block_tables;   /* [R, M] pages of each request */
+    const ekv_tensor* rows;           /* NULL (r = b) or [B] request of each batch row */
+    const ekv_tensor* lengths;        /* [B] tokens of each batch row, its query tokens among them */
+    const ekv_tensor* blocks;         /* [N, G, K] block ids, G a divisor of Hkv: KV head h reads list h / (Hkv / G) */
+    const ekv_tensor* query_starts;   /* NULL (one query token a row) or [B + 1] first query token of each row */
+    int64_t max_query;                /* the most query tokens of a row, or about: picks kernels, not what is seen */
+    double scale;                     /* of the scores, e.g. D^-0.5 */
+    const ekv_tensor* output;         /* [N, Hq, D], the query's type */
+    const ekv_tensor* lse;            /* NULL or [N, Hq] float32 */
+} ekv_block_attention_args;
+
+/* Workspace bytes of ekv_block_attention over lists of `width` blocks. UINT64_MAX on error. */
+uint64_t ekv_block_workspace_bytes(int64_t tokens, int64_t width, int64_t block_size, int64_t query_heads,
+                                   int64_t kv_heads, int64_t head_dim, int64_t max_query);
+
+/*
+ * Attention of query tokens to the blocks that each lists: query token i of
+ * the n of batch row b, at position p = lengths[b] - n + i, sees the tokens
+ * t <= p of every block j of its list (tokens j * block_size ..
+ * (j + 1) * block_size - 1 of its request). A block listed twice counts twice;
+ * ids below 0 or behind the position name none. Otherwise as
+ * ekv_shared_prefix_attention without prefixes.
+ * Replaces: the sparse attention that the reference leaves to its engine
+ * behind the selected blocks (adaptive_sparse/request_residency.py:792-839).
+ */
+int ekv_block_attention(const ekv_block_attention_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* The arguments of ekv_append_rotary. */
+typedef struct ekv_append_args {
+    const ekv_tensor* query;          /* NULL, or [N, Hq, D] bfloat16 or float16 */
+    const ekv_tensor* key;            /* NULL (no K and V), or [N, Hkv, D] of the query's type */
+    const ekv_tensor* value;          /* [N, Hkv, D] */
+    const ekv_planes* planes;         /* the pool (kv 2); a plane row is a token or a whole page */
+    int64_t layer;
+    int64_t page_size;                /* slot s is token s % page_size of page s / page_size */
+    const ekv_tensor* slots;          /* [N] slot of each token */
+    int64_t zero_below;               /* slots below it name no row */
+    const ekv_tensor* positions;      /* [N] */
+    const ekv_tensor* turns;          /* [R / 2] int64: turns a position of each pair, times 2^64, modulo 2^64 */
+    double magnitude;                 /* factor of the rotated elements */
+    int64_t interleaved;              /* pairs (2i, 2i + 1) instead of (i, i + R / 2) */
+    const ekv_tensor* output;         /* [N, Hq, D]: the rotated queries; may be the query */
+} ekv_append_args;
+
+/*
+ * New tokens' queries and keys rotated by their positions, K and V rows put
+ * into the pool: with angle = 2 pi * turns_i / 2^64 * position, elements
+ * (x_a, x_b) of pair i of the first R elements of a head become
+ *   magnitude * (x_a cos - x_b sin, x_b cos + x_a sin),
+ * rounded once; elements from R on, and V, are copied. Whole turns are dropped
+ * in 64-bit integers, so angles are as exact at far positions as at near ones.
+ * A token with position < 0 is left out: its output and row stay as they are.
+ * Slots below zero_below or past the pool write no row. The slots of live
+ * tokens are distinct. Only query, or only key, value, planes and slots, may be
+ * given. D is a multiple of 8 up to 256; addresses and strides of planes,
+ * query, key, value and output are multiples of 16 bytes. The output, and the
+ * layer's planes, share no memory with the inputs, but the output may be the
+ * query itself. One launch.
+ * Replaces: ekv_scatter_kv behind a rotation (the reference leaves both to its
+ * engine's K/V store, whose writes adaptive_sparse/logical_shadow.py:44-70
+ * records).
+ */
+int ekv_append_rotary(const ekv_append_args* args, void* stream);
+
+/*
+ * Index keys of new tokens, held in 8 bits: of each row x of index_key [N, Di]
+ * (bfloat16 or float16) the scale s = max|x| / 127 goes to scales[slot] and the
+ * whole numbers x / s (rounded to 32 bits, then to whole numbers, halves to
+ * even; 0 where s is 0) to the slot's row of `planes` (kv 1; a plane row is a
+ * token's Di bytes, or a page's). scales [slots of the layer] float32. Slots
+ * below zero_below or past the pool write nothing; slots are distinct. Di is a
+ * multiple of 16 up to 256. One launch. No reference counterpart: the
+ * reference's engine keeps its index keys itself.
+ */
+int ekv_append_index(const ekv_tensor* index_key, const ekv_planes* planes, int64_t layer, int64_t page_size,
+                     const ekv_tensor* scales, const ekv_tensor* slots, int64_t zero_below, void* stream);
+
+/* The arguments of ekv_select_blocks. */
+typedef struct ekv_select_args {
+    const ekv_tensor* index_query;    /* [N, Hi, Di] bfloat16 or float16, finite */
+    const ekv_planes* planes;         /* index keys in 8 bits (kv 1); a plane row is a token or a whole page */
+    int64_t layer;
+    int64_t page_size;
+    int64_t block_size;               /* tokens of a block */
+    const ekv_tensor* scales;         /* [tokens of the layer] float32, finite */
+    const ekv_tensor* block_tables;   /* [R, M] pages of each request */
+    const ekv_tensor* rows;           /* NULL (r = b) or [B] request of each batch row */
+    const ekv_tensor* lengths;        /* [B] tokens of each batch row, its query tokens among them */
+    const ekv_tensor* query_starts;   /* NULL (one query token a row) or [B + 1] first query token of each row */
+    int64_t max_query;                /* the most query tokens of a row, or about: picks kernels, not what is chosen */
+    int64_t first, last;              /* how many of the first and of the newest blocks are always chosen */
+    const ekv_tensor* blocks;         /* out [N, G, K] int32, G a divisor of Hi */
+} ekv_select_args;
+
+/* Workspace bytes of ekv_select_blocks for N x G lists and tables of `columns` pages. UINT64_MAX on error. */
+uint64_t ekv_select_workspace_bytes(int64_t tokens, int64_t groups, int64_t columns, int64_t page_size,
+                                    int64_t block_size);
+
+/*
+ * The K blocks of largest score for every query token and group of index
+ * heads. Query token i of the n of batch row b is at position
+ * p = lengths[b] - n + i. Rows of index_query are rounded to 8 bits and a scale
+ * q_s as ekv_append_index rounds keys. With q.k the whole-number product of
+ * codes, the score of block j is, over the group's heads h,
+ *   max_h  q_s[h] * max_{t in block j, t <= p}  scales[t] * (q_h . k_t)
+ * both products rounded to 32 bits. Tokens whose page id is below 1 or past the
+ * pool are not seen; a block without a seen token is not chosen. Blocks below
+ * `first`, and the last `last` up to the position's own, are chosen whatever
+ * their scores. Ties go to the lower block. A list is in ascending order, -1
+ * behind its last block; the lists of tokens of no batch row are all -1.
+ * At most 128 heads a group; N * G <= 2^22. workspace: 256-byte aligned device
+ * memory of ekv_select_workspace_bytes, its contents of no account; calls that
+ * overlap need one each. Two launches, no memset: it can be captured.
+ * Replaces: the block scores that the reference's engine hands to
+ * adaptive_sparse/request_residency.py:792-839 as selected blocks.
+ */
+int ekv_select_blocks(const ekv_select_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* Modes of ekv_stream_probe. */
 #define EKV_PROBE_READ 0   /* read src (fold, no stores)       */
 #define EKV_PROBE_WRITE 1  /* write zeros to dst                */
