@@ -8,8 +8,8 @@
 // be off by 0.06 at position 10^6), and no table of cosines has to be read. The nearest quarter turn is split off as an
 // integer too, and sine and cosine of the rest, at most pi / 4, are their power series in 32 bits.
 //
-// Index keys. A row's scale is its largest magnitude / 127, its codes are the quotients by that scale, rounded to 32 bits
-// and then to whole numbers, halves to even: a definition without freedom, so that equal keys have equal codes everywhere.
+// Index keys: rows as whole numbers of 8 bits (ekv_codes.h).
+#include "ekv_codes.h"
 #include "ekv_mfma.h"
 #include "ekv_pool.h"
 #include "ekv_vec.h"
@@ -235,20 +235,12 @@ __global__ __launch_bounds__(kThreads) void index_kernel(const IndexArgs a) {
     for (int step = 1; step < kLanes; step *= 2) {
         most = fmaxf(most, __shfl_xor(most, step));
     }
-    const float scale = most / 127.0f, divisor = scale > 0 ? scale : 1.0f;
+    const float scale = code_scale(most);
+    uint32_t words[2];
+    code_words(x, scale, words);
     const int64_t slot = there ? a.slots.fetch(token) : -1, row = a.rows.offset(slot);
     if (!live || row < 0) {
         return;
-    }
-    uint32_t words[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        words[w] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int32_t code = static_cast<int32_t>(rintf(x[4 * w + j] / divisor));
-            words[w] |= (static_cast<uint32_t>(code) & 0xffu) << (8 * j);
-        }
     }
     *reinterpret_cast<u32x2*>(a.plane + row + piece * 8) = u32x2{words[0], words[1]};
     if (piece == 0) {

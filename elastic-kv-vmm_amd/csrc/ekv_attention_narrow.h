@@ -281,14 +281,16 @@ __device__ __forceinline__ void run(int which, uint32_t w, uint32_t workgroups, 
                 for (int h = 0; h < 2; ++h) {
                     const int32_t key = base + h * 16 + col;
                     const uint32_t id = e.low[h];
-                    bool good = id >= cache.zero_below && id < cache.pages;
+                    bool good;
                     uint32_t inside;
                     if constexpr (kBlocks) {
                         inside = e.inside[h];
-                        good = good && inside != ~0u && (blocks.wide == 0 || e.high[h] == 0);
+                        good = inside != ~0u && id >= cache.zero_below && id < cache.pages &&
+                               (blocks.wide == 0 || e.high[h] == 0);
                     } else {
+                        good = key < src.keys && id >= cache.zero_below && id < cache.pages &&
+                               (src.wide == 0 || e.high[h] == 0);
                         inside = key - cache.page.div(key) * cache.page.divisor;
-                        good = key < src.keys && good && (src.wide == 0 || e.high[h] == 0);
                     }
                     const uint64_t offset = static_cast<uint64_t>(id) * cache.page_stride +
                                             static_cast<uint64_t>(inside) * cache.token_stride;

@@ -8,18 +8,23 @@
 // rounded to codes here, as append.hip rounds keys.
 //
 // Two launches: scores of all blocks as ordered 32-bit keys into the workspace, then each (token, group)'s largest.
+#include "ekv_codes.h"
+#include "ekv_memory.h"
 #include "ekv_mfma.h"
 #include "ekv_pool.h"
 #include "ekv_vec.h"
 #include "ekv_wave.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ekv {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
-constexpr int kUnit = 32;                   // keys of a wave's step
+// Keys of a wave's step: 8 KB of them at an index size of 128 or more.
+constexpr int unit_of(int steps) { return steps == 4 ? 32 : 64; }
+
 constexpr int kSegmentKeys = 4096;          // ordered keys of a workgroup's segment in LDS
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
@@ -47,7 +52,7 @@ struct ScoreArgs {
     int32_t groups, share, dim;             // groups of share heads
     FastDiv group_div, share_div;
     FastDiv block;                          // tokens of a block
-    int32_t block_units, sub_shift;         // steps of a block; or blocks of 2^sub_shift < kUnit tokens (-1: not)
+    int32_t block_units, sub_shift;         // steps of a block; or blocks of 2^sub_shift tokens, several a step (-1: not)
     uint32_t* scores;                       // [tokens, groups, score_row]
     int64_t score_row;
     int32_t segment_blocks, segments;       // blocks of a segment; workgroups beside each other that share a tile's
@@ -116,22 +121,25 @@ __device__ __forceinline__ float over_quads_max(float x) {
 
 // Scores of a tile of rows (query heads of one batch row's tokens) against segments of its context. Keys down and rows
 // across in 16x16x64 products, every wave with keys of its own straight from memory, the tile's queries in its registers.
-template <int kSteps, int kTiles>
-__global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
+// kShort: blocks of 2^sub_shift tokens, several a step.
+template <int kSteps, int kTiles, bool kShort>
+__global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_kernel(const ScoreArgs a) {
     constexpr int kRowBytes = kSteps * 64, kPieces = kSteps * 4;
-    __shared__ __align__(16) char s_codes[kTiles * 16 * kRowBytes];
-    __shared__ float s_scale[kTiles * 16];
+    constexpr int kUnit = unit_of(kSteps), kHalves = kUnit / 16;
+    constexpr uint64_t kAll = kUnit == 64 ? ~uint64_t{0} : (uint64_t{1} << (kUnit & 63)) - 1;
+    constexpr int kLanes = kPieces;                    // lanes that read a key's row
+    constexpr int kAtOnce = 64 / kLanes;               // keys of one access
+    constexpr int kLoads = kUnit / kAtOnce;
+    static_assert(kTiles * 16 * kRowBytes <= kWaves * kUnit * kRowBytes, "codes fit where the keys will be");
+    __shared__ __align__(16) char s_data[kWaves * kUnit * kRowBytes];      // the tile's codes, then each wave's keys
+    __shared__ __align__(16) float s_scale[kTiles * 16 > kWaves * kUnit ? kTiles * 16 : kWaves * kUnit];
     extern __shared__ uint32_t s_score[];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // Workgroups are dealt to the eight dies in turn: those of one segment meet behind one L2.
-    int32_t tile, segment;
-    if (a.segments % 8 == 0) {
-        const int32_t each = blockIdx.x >> 3;
-        tile = each % a.tiles, segment = (each / a.tiles) * 8 + (blockIdx.x & 7);
-    } else {
-        tile = blockIdx.x % a.tiles, segment = blockIdx.x / a.tiles;
-    }
+    // Workgroups are dealt to the eight dies in turn, and a context's segments with them: long and short contexts, and the
+    // early segments that all have, are everybody's.
+    int32_t segment = blockIdx.x / a.tiles;
+    const int32_t tile = (blockIdx.x + segment) % a.tiles;
     int32_t b, part;
     if (a.at.query_starts.data == nullptr) {
         b = tile / a.row_tiles, part = tile - b * a.row_tiles;
@@ -169,37 +177,33 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
 
     // Queries as codes.
     {
-        constexpr int kLanes = kSteps * 8;
-        const int piece = tid % kLanes;
-        for (int r = tid / kLanes; r < kTiles * 16; r += kThreads / kLanes) {
+        constexpr int kRowThreads = kSteps * 8;
+        const int piece = tid % kRowThreads;
+        for (int r = tid / kRowThreads; r < kTiles * 16; r += kThreads / kRowThreads) {
             const int32_t pair = a.share_div.div(r), inside = r - pair * a.share;
             float x[8] = {};
             float most = 0;
             if (pair < pair_count && piece * 8 < a.dim) {
                 const int32_t all = pair_begin + pair, token = a.group_div.div(all);
                 const int32_t head = (all - token * a.groups) * a.share + inside;
-                const u32x4 words = *reinterpret_cast<const u32x4*>(
+                const u32x4 given = load_global<u32x4>(
                     a.query + int64_t{row.first + token} * a.q_token + head * a.q_head + piece * 16);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const uint16_t bits = static_cast<uint16_t>(words[j >> 1] >> (16 * (j & 1)));
+                    const uint16_t bits = static_cast<uint16_t>(given[j >> 1] >> (16 * (j & 1)));
                     x[j] = a.f16 != 0 ? F16::value(bits) : Bf16::value(bits);
                     most = fmaxf(most, fabsf(x[j]));
                 }
             }
 #pragma unroll
-            for (int step = 1; step < kLanes; step *= 2) {
+            for (int step = 1; step < kRowThreads; step *= 2) {
                 most = fmaxf(most, __shfl_xor(most, step));
             }
-            const float scale = most / 127.0f, divisor = scale > 0 ? scale : 1.0f;
-            u32x2 words = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int32_t code = static_cast<int32_t>(rintf(x[j] / divisor));
-                words[j >> 2] |= (static_cast<uint32_t>(code) & 0xffu) << (8 * (j & 3));
-            }
+            const float scale = code_scale(most);
+            uint32_t words[2];
+            code_words(x, scale, words);
             const int at = r * kRowBytes + (((piece >> 1) ^ (r & (kPieces - 1))) << 4) + (piece & 1) * 8;
-            *reinterpret_cast<u32x2*>(s_codes + at) = words;
+            *reinterpret_cast<u32x2*>(s_data + at) = u32x2{words[0], words[1]};
             if (piece == 0) {
                 s_scale[r] = scale;
             }
@@ -214,13 +218,14 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
         const int r = m * 16 + col;
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
-            q[m][c] = *reinterpret_cast<const i32x4*>(s_codes + r * kRowBytes + (((c * 4 + quad) ^ (r & (kPieces - 1))) << 4));
+            q[m][c] = *reinterpret_cast<const i32x4*>(s_data + r * kRowBytes + (((c * 4 + quad) ^ (r & (kPieces - 1))) << 4));
         }
         q_scale[m] = s_scale[r];
         const int32_t pair = a.share_div.div(r);
         pair_of[m] = pair < pair_count ? pair : -1;
         sight[m] = row.position + static_cast<int32_t>(a.group_div.div(pair_begin + max(pair_of[m], 0))) + 1;
     }
+    __syncthreads();      // the keys come where the codes are
     const char* const table = a.tables + row.request * a.table_row;
     const char* const nothing = reinterpret_cast<const char*>(no_key);
     const int32_t block_tokens = a.block.divisor, blocks = a.block.div(last_seen - 1) + 1;   // of the context
@@ -233,63 +238,83 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
         __syncthreads();
         const int32_t begin = block_begin * block_tokens;
         // The context's last block may end early: every step begins at a token that somebody sees.
-        const int32_t units = a.sub_shift >= 0
+        const int32_t units = kShort
                                   ? (min(held << a.sub_shift, last_seen - begin) + kUnit - 1) / kUnit
                                   : (held - 1) * a.block_units +
                                         (min(block_tokens, last_seen - begin - (held - 1) * block_tokens) + kUnit - 1) / kUnit;
         const int32_t from = units * wave / kWaves, to = units * (wave + 1) / kWaves;
 
-        // First position of a step, and where its block's tokens end.
-        const auto place = [&](int32_t u, int32_t& base, int32_t& end) {
-            if (a.sub_shift >= 0) {
-                base = begin + u * kUnit;
-                end = min(row.seen, last_seen);
-            } else {
-                const int32_t block = u / a.block_units;
-                base = begin + block * block_tokens + (u - block * a.block_units) * kUnit;
-                end = min(begin + (block + 1) * block_tokens, last_seen);
+        // A wave's steps one after the other: kUnit tokens from `base` on, those before `end`.
+        const int32_t span = kShort ? 0x7fffffff : block_tokens;      // tokens that steps go through in a run
+        struct Step {
+            int32_t left, start, offset, end;      // steps to come; first token of the block, and how far in it
+            __device__ __forceinline__ int32_t base() const { return start + offset; }
+        };
+        const auto end_of = [&](int32_t start) { return last_seen - start > span ? start + span : last_seen; };
+        const auto advance = [&](Step& s) {
+            s.left -= 1;
+            if (s.left <= 0) {
+                s.end = 0;                         // nothing is read behind the last step
+                return;
+            }
+            s.offset += kUnit;
+            if (s.offset >= span) {
+                s.start += span, s.offset = 0;
+                s.end = end_of(s.start);
             }
         };
+        // Page ids of a step: lane l's is that of its l-th key (an int64 id whose high word is not zero names no page).
         struct Ids {
-            uint32_t low[2], high[2];
+            uint32_t low, high, inside;
         };
-        const auto ids_of = [&](int32_t u) {
-            Ids e;
-            int32_t base, end;
-            place(min(u, units - 1), base, end);
+        const auto ids_of = [&](const Step& step) {
+            const int32_t key = step.base() + lane;
+            const bool good = lane < kUnit && key < step.end;
+            const uint32_t page = a.page.div(key);
+            const char* at = good ? table + uint64_t{page} * a.table_col : nothing;
+            return Ids{load_global<uint32_t>(at), load_global<uint32_t>(at + (a.table64 != 0 ? 4 : 0)),
+                       good ? key - page * a.page.divisor : ~0u};
+        };
+        // Rows of a step in registers: every access reads whole rows of kAtOnce keys, 16 bytes a lane. (With the lanes of
+        // the matrix tiles it would read 64 bytes of each of 16 keys, and each 128-byte line twice.)
+        struct Keys {
+            i32x4 row[kLoads];
+            float scale;                   // of key `lane`
+            uint64_t seen;
+        };
+        const int my_piece = lane % kLanes * 16, my_key = lane / kLanes;
+        const char* const from_piece = a.keys + (my_piece < a.dim ? my_piece : 0);     // the others meet codes of 0
+        const auto fetch = [&](const Ids& e, Keys& keys) {
+            const bool good = e.inside != ~0u && e.low >= 1 && e.low < a.pages && (a.table64 == 0 || e.high == 0);
+            const char* scale_at = reinterpret_cast<const char*>(a.scales) +
+                                   (uint64_t{e.low} * a.page.divisor + e.inside) * a.scale_step * 4;
+            keys.scale = load_global<float>(good ? scale_at : nothing);
+            keys.seen = __ballot(good);
+            const uint64_t offset = uint64_t{e.low} * a.page_stride + uint64_t{e.inside} * a.token_stride;
+            const uint32_t low = good ? static_cast<uint32_t>(offset) : ~0u;
+            const uint32_t high = good ? static_cast<uint32_t>(offset >> 32) : ~0u;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int32_t key = base + h * 16 + col;
-                const char* at = key < end ? table + uint64_t{a.page.div(key)} * a.table_col : nothing;
-                e.low[h] = *reinterpret_cast<const uint32_t*>(at);
-                e.high[h] = *reinterpret_cast<const uint32_t*>(at + (a.table64 != 0 ? 4 : 0));
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t l = __shfl(low, i * kAtOnce + my_key), h = __shfl(high, i * kAtOnce + my_key);
+                const char* at = from_piece + (uint64_t{h} << 32 | l);
+                keys.row[i] = load_global<i32x4>(h != ~0u ? at : nothing);
             }
-            return e;
         };
-        i32x4 k[2][kSteps];
-        float scale[2];
-        uint32_t seen = 0;
-        const auto fetch = [&](int32_t u, const Ids& e) {
-            int32_t base, end;
-            place(min(u, units - 1), base, end);
-            seen = 0;
+        // Keys in LDS, their 16-byte pieces permuted by exclusive or so that 16 lanes with 16 keys and one piece meet every
+        // bank once. Nobody but the wave reads them, and its accesses stay in order.
+        char* const my_keys = s_data + wave * (kUnit * kRowBytes);
+        float* const my_scales = s_scale + wave * kUnit;
+        const auto swap_of = [](int key) {
+            return kSteps == 1 ? (key >> 2) & 3 : (kSteps == 2 ? (key >> 1) & 7 : key & 15);
+        };
+        const auto put = [&](const Keys& keys) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int32_t key = base + h * 16 + col;
-                const uint32_t id = e.low[h];
-                const bool good = key < end && id >= 1 && id < a.pages && (a.table64 == 0 || e.high[h] == 0);
-                const uint32_t inside = key - a.page.div(key) * a.page.divisor;
-                const char* at = good ? a.keys + uint64_t{id} * a.page_stride + uint64_t{inside} * a.token_stride : nothing;
-                const float* scale_at =
-                    a.scales + (int64_t{id} * a.page.divisor + inside) * a.scale_step;
-                scale[h] = *(good ? scale_at : reinterpret_cast<const float*>(nothing));
-#pragma unroll
-                for (int c = 0; c < kSteps; ++c) {
-                    // Behind the key's last piece any other of its pieces: it meets codes of 0.
-                    const int piece = (c * 4 + quad) * 16;
-                    k[h][c] = *reinterpret_cast<const i32x4*>(at + (good && piece < a.dim ? piece : 0));
-                }
-                seen |= (static_cast<uint32_t>(__ballot(good)) & 0xffffu) << (16 * h);
+            for (int i = 0; i < kLoads; ++i) {
+                const int key = i * kAtOnce + my_key;
+                *reinterpret_cast<i32x4*>(my_keys + key * kRowBytes + ((lane % kLanes ^ swap_of(key)) << 4)) = keys.row[i];
+            }
+            if (lane < kUnit) {
+                my_scales[lane] = keys.scale;
             }
         };
         float best[kTiles];
@@ -303,99 +328,100 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
                 atomicMax(&s_score[pair_of[m] * held + block], ordered(times));
             }
         };
-        if (from < to) {
-            Ids ids = ids_of(from);
-            fetch(from, ids);
-            ids = ids_of(from + 1);
-#pragma unroll 1
-            for (int32_t u = from; u < to; ++u) {
-                const Ids later = ids_of(u + 2);
-                int32_t base, end;
-                place(u, base, end);
-                const uint32_t now = seen;
-                float key_scale[2][4];
-                i32x4 s[kTiles][2];
+        // The scores of the keys in LDS, 16 of them at a time; kRagged: some are not seen by all rows.
+        const auto score = [&]<bool kRagged>(const Step& now, uint64_t seen, std::bool_constant<kRagged>) {
+            const int32_t base = now.base();
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < kHalves; ++h) {
+            i32x4 k[kSteps];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        key_scale[h][j] = __shfl(scale[h], quad * 4 + j);
+            for (int c = 0; c < kSteps; ++c) {
+                k[c] = *reinterpret_cast<const i32x4*>(my_keys + (h * 16 + col) * kRowBytes +
+                                                       (((c * 4 + quad) ^ swap_of(col)) << 4));
+            }
+            const f32x4 key_scale = *reinterpret_cast<const f32x4*>(my_scales + h * 16 + quad * 4);
+#pragma unroll
+            for (int m = 0; m < kTiles; ++m) {
+                if (kRagged) {
+                    __builtin_amdgcn_sched_barrier(0);     // masks of one tile at a time: scalar registers are few
+                }
+                i32x4 s = {0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < kSteps; ++c) {
+                    s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[c], q[m][c], s, 0, 0, 0);
+                }
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[j] = static_cast<float>(s[j]) * key_scale[j];
+                    if (kRagged) {
+                        const int key = quad * 4 + j;
+                        x[j] = ((seen >> (h * 16)) >> key & 1) != 0 && key < sight[m] - base - h * 16 ? x[j] : -INFINITY;
                     }
                 }
-#pragma unroll
-                for (int m = 0; m < kTiles; ++m) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        s[m][h] = i32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int c = 0; c < kSteps; ++c) {
-                            s[m][h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[h][c], q[m][c], s[m][h], 0, 0, 0);
-                        }
-                    }
-                }
-                fetch(u + 1, ids);
-                ids = later;
-                const bool ragged = now != 0xffffffffu || base + kUnit > first_seen;
-#pragma unroll
-                for (int m = 0; m < kTiles; ++m) {
-                    float x[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                if constexpr (!kShort) {
+                    best[m] = fmaxf(fmaxf(best[m], x[0]), x[1]);
+                    best[m] = fmaxf(fmaxf(best[m], x[2]), x[3]);
+                } else {
+                    const int32_t key = base - begin + h * 16 + quad * 4;      // from the segment's first
+                    if (a.sub_shift == 0) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            x[h][j] = static_cast<float>(s[m][h][j]) * key_scale[h][j];
+                            leave(m, x[j], key + j);
                         }
-                    }
-                    if (ragged) {
-                        const int32_t left = sight[m] - base;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int key = h * 16 + quad * 4 + j;
-                                x[h][j] = ((now >> key) & 1) != 0 && key < left ? x[h][j] : -INFINITY;
-                            }
-                        }
-                    }
-                    if (a.sub_shift < 0) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                best[m] = fmaxf(best[m], x[h][j]);
-                            }
-                        }
+                    } else if (a.sub_shift == 1) {
+                        leave(m, fmaxf(x[0], x[1]), key >> 1);
+                        leave(m, fmaxf(x[2], x[3]), (key >> 1) + 1);
                     } else {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int32_t key = u * kUnit + h * 16 + quad * 4;      // from the segment's first
-                            if (a.sub_shift == 0) {
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    leave(m, x[h][j], key + j);
-                                }
-                            } else if (a.sub_shift == 1) {
-                                leave(m, fmaxf(x[h][0], x[h][1]), key >> 1);
-                                leave(m, fmaxf(x[h][2], x[h][3]), (key >> 1) + 1);
-                            } else {
-                                leave(m, fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3])), key >> a.sub_shift);
-                            }
-                        }
+                        leave(m, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), key >> a.sub_shift);
                     }
                 }
-                if (a.sub_shift < 0) {
-                    const int32_t block = u / a.block_units;
-                    if (u + 1 == to || (u + 1) / a.block_units != block) {
+            }
+            }
+        };
+        const auto work = [&](const Step& now, uint64_t seen) {
+            if (seen == kAll && now.base() + kUnit <= first_seen) {
+                score(now, seen, std::false_type{});
+            } else {
+                rarely();
+                score(now, seen, std::true_type{});
+            }
+            if (!kShort && (now.left == 1 || now.offset + kUnit >= span)) {
+                const int32_t block = a.block.div(now.start - begin);
 #pragma unroll
-                        for (int m = 0; m < kTiles; ++m) {
-                            const float most = over_quads_max(best[m]);
-                            if (quad == 0) {
-                                leave(m, most, block);
-                            }
-                            best[m] = -INFINITY;
-                        }
+                for (int m = 0; m < kTiles; ++m) {
+                    const float most = over_quads_max(best[m]);
+                    if (quad == 0) {
+                        leave(m, most, block);
                     }
+                    best[m] = -INFINITY;
                 }
+            }
+        };
+        if (from < to) {
+            // Page ids are asked for two steps ahead, rows one.
+            Step now;
+            const int32_t block = kShort ? 0 : from / a.block_units;
+            now.left = to - from;
+            now.start = begin + (kShort ? 0 : block * block_tokens);
+            now.offset = (from - (kShort ? 0 : block * a.block_units)) * kUnit;
+            now.end = end_of(now.start);
+            Step ahead = now;
+            const Ids first = ids_of(ahead);
+            advance(ahead);
+            Ids ids = ids_of(ahead);
+            advance(ahead);
+            Keys keys;
+            fetch(first, keys);
+#pragma unroll 1
+            for (; now.left > 0; advance(now)) {
+                const Ids later = ids_of(ahead);
+                advance(ahead);
+                const uint64_t seen = keys.seen;
+                put(keys);
+                fetch(ids, keys);
+                ids = later;
+                work(now, seen);
             }
         }
         __syncthreads();
@@ -404,6 +430,18 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
             a.scores[(int64_t{row.first} * a.groups + pair_begin + pair) * a.score_row + block_begin + block] = s_score[i];
         }
         __syncthreads();
+    }
+}
+
+__device__ __forceinline__ uint32_t uniform_lane(uint32_t scanned) {
+    return __builtin_amdgcn_readlane(scanned, 63);
+}
+
+// Keeps the compiler from making the masks of all of a wave's registers before it counts the first: it has scalar
+// registers for few.
+__device__ __forceinline__ void few_at_once(int r) {
+    if (r % 8 == 7) {
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -439,47 +477,110 @@ __device__ __forceinline__ Candidates candidates_of(const PickArgs& a, int64_t p
         c.count = seen > 0 ? a.block.div(seen - 1) + 1 : 0;
         c.forced_from = position >= 0 ? static_cast<int32_t>(a.block.div(position)) + 1 - a.last : 0;
     }
+    c.count = __builtin_amdgcn_readfirstlane(c.count);
+    c.forced_from = __builtin_amdgcn_readfirstlane(c.forced_from);
     return c;
 }
 
-// One wave a (token, group): block 64 r + lane in register r. The K-th largest key bit by bit, by counting the keys that
-// are not below a bound; then the keys above it and the first of those equal to it, in order of their blocks.
-template <int kRegs>
-__global__ __launch_bounds__(kThreads) void pick_kernel(const PickArgs a) {
+// A workgroup of kWaves waves a (token, group), or a wave each where kWaves is 1; wave w holds the w-th equal run of its
+// blocks, 64 to a register. The K-th largest key bit by bit, by counting the keys that are not below a bound: that takes
+// no order of the keys and no atomics, and stops as soon as exactly K are not below. Then the keys above the bound and the
+// first of those equal to it, in order of their blocks. The bits that all keys share in front are skipped.
+//
+// What bounds it: the reads of the keys and the steps one after the other: kRegs comparisons and, between waves, a barrier
+// a bit.
+template <int kWaves, int kRegs>
+__global__ __launch_bounds__(kWaves == 1 ? kThreads : kWaves * 64) void pick_kernel(const PickArgs a) {
+    constexpr int kCells = kWaves == 1 ? 1 : kWaves;
+    __shared__ uint32_t s_cells[2][2][kCells];
     const int lane = threadIdx.x & 63;
-    const int64_t pair = int64_t{blockIdx.x} * kWaves + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int in_group = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int wave = kWaves == 1 ? 0 : in_group;
+    const int64_t pair = kWaves == 1 ? int64_t{blockIdx.x} * (kThreads / 64) + in_group : blockIdx.x;
     if (pair >= int64_t{a.at.tokens} * a.groups) {
         return;
     }
     const Candidates c = candidates_of(a, pair);
+    const int32_t used = (c.count + kWaves * 64 - 1) / (kWaves * 64);     // registers
+    const int32_t begin = wave * used * 64;
     uint32_t key[kRegs];
+    uint32_t least = 0xffffffffu, most = 0;
 #pragma unroll
     for (int r = 0; r < kRegs; ++r) {
-        key[r] = c.key(r * 64 + lane);
+        const int32_t j = begin + r * 64 + lane;
+        const uint32_t k = r < used ? c.scores[j < c.count ? j : 0] : 0u;
+        key[r] = r < used && j < c.count && k != 0 ? ((j < c.forced_below || j >= c.forced_from) ? 0xffffffffu : k) : 0u;
+        // What is none, or always taken, says nothing of where the K-th largest lies.
+        least = min(least, key[r] != 0 ? key[r] : 0xffffffffu);
+        most = max(most, key[r] != 0xffffffffu ? key[r] : 0u);
     }
+    int parity = 0;
+    // One number of each wave (the same in all its lanes), all of them to everybody.
+    const auto share = [&](uint32_t first, uint32_t second, auto&& each) {
+        if constexpr (kWaves > 1) {
+            if (lane == 0) {
+                s_cells[parity][0][wave] = first, s_cells[parity][1][wave] = second;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                each(w, s_cells[parity][0][w], s_cells[parity][1][w]);
+            }
+            parity ^= 1;     // the next call's barrier stands between these reads and the writes after it
+        } else {
+            each(0, first, second);
+        }
+    };
     const auto not_below = [&](uint32_t bound) {
-        int32_t n = 0;
+        uint32_t n = 0;
 #pragma unroll
         for (int r = 0; r < kRegs; ++r) {
             n += __popcll(__ballot(key[r] >= bound));
+            few_at_once(r);
         }
-        return n;
+        int32_t all = 0;
+        share(n, 0, [&](int, uint32_t x, uint32_t) { all += static_cast<int32_t>(x); });
+        return all;
     };
-    uint32_t bound = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+    {
+        const uint32_t low = ~uniform_lane(wave_scan<kMax>(~least)), high = uniform_lane(wave_scan<kMax>(most));
+        least = 0xffffffffu, most = 0;
+        share(low, high, [&](int, uint32_t x, uint32_t y) { least = min(least, x), most = max(most, y); });
+    }
+    // The K-th largest begins with the bits that the least and the largest share. With fewer than K keys the bound ends not
+    // above the least, with K that are always taken not below the largest of the others: either way those are taken.
+    const uint32_t differ = least ^ most;
+    const int top = differ != 0 ? 31 - __builtin_clz(differ) : -1;
+    uint32_t bound = top >= 31 ? 0u : (top < 0 ? least : least & ~((2u << top) - 1));
+    bool exact = false;
+    for (int bit = top; bit >= 0 && !exact; --bit) {
         const uint32_t tried = bound | (1u << bit);
         const int32_t n = not_below(tried);
-        if (n >= a.chosen) {
-            bound = tried;
-            if (n == a.chosen) {
-                break;
-            }
-        }
+        bound = n >= a.chosen ? tried : bound;
+        exact = n == a.chosen;
     }
-    int32_t equal = a.chosen - (bound == 0xffffffffu ? 0 : not_below(bound + 1));     // how many equal to the bound
+    const int32_t above = bound == 0xffffffffu ? 0 : not_below(bound + 1);
+    int32_t equal = max(a.chosen - above, 0);                            // how many equal to the bound are taken
     const int32_t token = a.group_div.div(static_cast<uint32_t>(pair)), group = static_cast<int32_t>(pair) - token * a.groups;
     int32_t* const out = a.blocks + token * a.b_token + group * a.b_group;
-    int32_t at = 0;
+    int32_t at = 0, taken_all = 0;
+    if constexpr (kWaves > 1) {
+        uint32_t mine_above = 0, mine_same = 0;
+#pragma unroll
+        for (int r = 0; r < kRegs; ++r) {
+            mine_above += __popcll(__ballot(key[r] > bound));
+            mine_same += __popcll(__ballot(bound != 0 && key[r] == bound));
+            few_at_once(r);
+        }
+        int32_t same_before = 0, above_before = 0, same_all = 0;
+        share(mine_above, mine_same, [&](int w, uint32_t x, uint32_t y) {
+            above_before += w < wave ? x : 0, same_before += w < wave ? y : 0;
+            same_all += y;
+        });
+        at = above_before + min(same_before, equal);
+        taken_all = above + min(same_all, equal);
+        equal -= min(same_before, equal);
+    }
 #pragma unroll
     for (int r = 0; r < kRegs; ++r) {
         const uint64_t same = __ballot(bound != 0 && key[r] == bound);
@@ -487,82 +588,179 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const PickArgs a) {
         const bool take = key[r] > bound || ((same & mine) != 0 && __popcll(same & (mine - 1)) < equal);
         const uint64_t taken = __ballot(take);
         if (take) {
-            out[(at + __popcll(taken & (mine - 1))) * a.b_column] = r * 64 + lane;
+            out[(at + __popcll(taken & (mine - 1))) * a.b_column] = begin + r * 64 + lane;
         }
         at += __popcll(taken);
         equal -= min(equal, static_cast<int32_t>(__popcll(same)));
+        few_at_once(r);
     }
-    for (int32_t i = at + lane; i < a.chosen; i += 64) {
+    taken_all = kWaves == 1 ? at : taken_all;
+    for (int32_t i = taken_all + (kWaves == 1 ? lane : static_cast<int32_t>(threadIdx.x)); i < a.chosen;
+         i += kWaves == 1 ? 64 : kWaves * 64) {
         out[i * a.b_column] = -1;
     }
 }
 
-constexpr int kManyThreads = 1024, kManyWaves = 16;
+constexpr int kManyWaves = 16, kManyThreads = kManyWaves * 64;
+constexpr int kDigit = 11, kBins = 1 << kDigit;
 
-// The same by a workgroup, for any number of blocks: they are read again for every bit.
+// The same for many blocks: the K-th largest key digit by digit, 11 bits at a time, from the counts of the digits of those
+// keys that agree with it so far. kRegs: a lane's keys in registers; 0: any number of keys, read again for each digit.
+//
+// What bounds it: the additions to the counts in LDS. The first digit begins at the first bit in which keys differ, so
+// that they spread over many counts. Bit by bit, 40000 keys took 94 us a launch.
+template <int kRegs>
 __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs a) {
-    __shared__ int32_t s_count[2][kManyWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ uint32_t s_bins[kBins];
+    __shared__ uint32_t s_cells[2][kManyWaves];
+    __shared__ uint32_t s_found[2];               // the digit, and how many keys have a larger one
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t pair = blockIdx.x;
     const Candidates c = candidates_of(a, pair);
-    int parity = 0;
-    const auto total = [&](int32_t mine) {
-        // mine: the wave's count, the same in all its lanes.
-        s_count[parity][wave] = mine;
-        __syncthreads();
-        int32_t n = 0;
-        for (int w = 0; w < kManyWaves; ++w) {
-            n += s_count[parity][w];
+    const int32_t used = (c.count + kManyThreads - 1) / kManyThreads;      // a lane's keys
+    const int32_t begin = wave * used * 64;
+    uint32_t held[kRegs > 0 ? kRegs : 1];
+    if constexpr (kRegs > 0) {
+#pragma unroll
+        for (int r = 0; r < kRegs; ++r) {
+            held[r] = r < used ? c.key(begin + r * 64 + lane) : 0u;
         }
-        parity ^= 1;
-        return n;
-    };
-    const auto not_below = [&](uint32_t bound) {
-        int32_t n = 0;
-        for (int32_t j = tid; j - lane < c.count; j += kManyThreads) {
-            n += __popcll(__ballot(c.key(j) >= bound));
-        }
-        return total(n);
-    };
-    uint32_t bound = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t tried = bound | (1u << bit);
-        const int32_t n = not_below(tried);
-        if (n >= a.chosen) {
-            bound = tried;
-            if (n == a.chosen) {
-                break;
+    }
+    // body(r, key) for each of a lane's keys, in order; whole waves take part.
+    const auto for_keys = [&](auto&& body) {
+        if constexpr (kRegs > 0) {
+#pragma unroll
+            for (int r = 0; r < kRegs; ++r) {
+                if (r < used) {
+                    body(r, held[r]);
+                }
+            }
+        } else {
+            for (int r = 0; r < used; ++r) {
+                body(r, c.key(begin + r * 64 + lane));
             }
         }
+    };
+    uint32_t least = 0xffffffffu, most = 0;
+    for_keys([&](int, uint32_t key) {
+        // What is none, or always taken, says nothing of where the K-th largest lies.
+        least = min(least, key != 0 ? key : 0xffffffffu);
+        most = max(most, key != 0xffffffffu ? key : 0u);
+    });
+    least = ~uniform_lane(wave_scan<kMax>(~least)), most = uniform_lane(wave_scan<kMax>(most));
+    if (lane == 0) {
+        s_cells[0][wave] = least, s_cells[1][wave] = most;
     }
-    const int32_t equal = a.chosen - (bound == 0xffffffffu ? 0 : not_below(bound + 1));
+    __syncthreads();
+    for (int w = 0; w < kManyWaves; ++w) {
+        least = min(least, s_cells[0][w]), most = max(most, s_cells[1][w]);
+    }
+    // Keys that are always taken count as the largest of the others, and those that are none fall out: with what the others
+    // share in front, the bound is theirs.
+    const uint32_t differ = least ^ most;
+    int bits = least > most ? 0 : (differ != 0 ? 32 - __builtin_clz(differ) : 0);     // undecided bits of the bound
+    uint32_t bound = bits >= 32 ? 0u : (least >> bits) << bits;
+    uint32_t wanted = a.chosen, forced = 0;
+    for_keys([&](int, uint32_t key) { forced += key == 0xffffffffu; });
+    forced = uniform_lane(wave_scan<kAdd>(forced));
+    __syncthreads();
+    if (lane == 0) {
+        s_cells[0][wave] = forced;
+    }
+    __syncthreads();
+    forced = 0;
+    for (int w = 0; w < kManyWaves; ++w) {
+        forced += s_cells[0][w];
+    }
+    wanted -= min(wanted, forced);
+    if (least > most || wanted == 0) {
+        bound = least > most ? 0u : 0xffffffffu;      // no others; or none of them
+        bits = 0;
+    }
+    bool all = false;                                 // fewer than K are there
+    while (bits > 0 && !all) {
+        const int digit = min(bits, kDigit), shift = bits - digit;
+        for (int i = tid; i < kBins; i += kManyThreads) {
+            s_bins[i] = 0;
+        }
+        __syncthreads();
+        for_keys([&](int, uint32_t key) {
+            if (key != 0 && key != 0xffffffffu && (bits >= 32 || (key ^ bound) >> bits == 0)) {
+                atomicAdd(&s_bins[(key >> shift) & ((1u << digit) - 1)], 1u);
+            }
+        });
+        __syncthreads();
+        // From the largest digit down: two to a thread.
+        const int top = kBins - 1 - 2 * tid;
+        const uint32_t first = s_bins[top], second = s_bins[top - 1];
+        const uint32_t sum = wave_scan<kAdd>(first + second);
+        if (lane == 63) {
+            s_cells[0][wave] = sum;
+        }
+        if (tid == 0) {
+            s_found[0] = kBins;
+        }
+        __syncthreads();
+        uint32_t before = sum - first - second;
+        for (int w = 0; w < wave; ++w) {
+            before += s_cells[0][w];
+        }
+        if (before < wanted && wanted <= before + first + second) {
+            const bool high = wanted <= before + first;
+            s_found[0] = high ? top : top - 1;
+            s_found[1] = high ? before : before + first;
+        }
+        __syncthreads();
+        all = s_found[0] == kBins;
+        if (!all) {
+            bound |= s_found[0] << shift;
+            wanted -= s_found[1];
+            bits = shift;
+        }
+        __syncthreads();
+    }
+    if (all) {
+        bound = 0;                                    // all there are
+    }
+    // How many equal to the bound are taken.
+    const int32_t equal = bound == 0xffffffffu ? a.chosen : static_cast<int32_t>(wanted);
     const int32_t token = a.group_div.div(static_cast<uint32_t>(pair)), group = static_cast<int32_t>(pair) - token * a.groups;
     int32_t* const out = a.blocks + token * a.b_token + group * a.b_group;
-    int32_t at = 0, sames = 0;
-    for (int32_t chunk = 0; chunk < c.count; chunk += kManyThreads) {
-        const uint32_t key = c.key(chunk + tid);
-        const uint64_t mine = uint64_t{1} << lane, below = mine - 1;
-        const uint64_t same = __ballot(bound != 0 && key == bound), above = __ballot(key > bound);
-        __syncthreads();
-        s_count[0][wave] = __popcll(same);
-        s_count[1][wave] = __popcll(above);
-        __syncthreads();
-        int32_t same_before = sames, above_before = 0, above_all = 0, same_all = 0;
-        for (int w = 0; w < kManyWaves; ++w) {
-            same_before += w < wave ? s_count[0][w] : 0;
-            above_before += w < wave ? s_count[1][w] : 0;
-            same_all += s_count[0][w], above_all += s_count[1][w];
-        }
-        const int32_t same_rank = same_before + __popcll(same & below);
-        const int32_t taken_same = min(same_rank, equal) - min(sames, equal);
-        const int32_t place = at + above_before + __popcll(above & below) + taken_same;
-        if ((above & mine) != 0 || ((same & mine) != 0 && same_rank < equal)) {
-            out[place * a.b_column] = chunk + tid;
-        }
-        at += above_all + min(sames + same_all, equal) - min(sames, equal);
-        sames += same_all;
+    uint32_t above = 0, same = 0;
+    for_keys([&](int, uint32_t key) {
+        above += key > bound;
+        same += bound != 0 && key == bound;
+    });
+    above = uniform_lane(wave_scan<kAdd>(above)), same = uniform_lane(wave_scan<kAdd>(same));
+    __syncthreads();
+    if (lane == 0) {
+        s_cells[0][wave] = above, s_cells[1][wave] = same;
     }
-    for (int32_t i = at + tid; i < a.chosen; i += kManyThreads) {
+    __syncthreads();
+    int32_t at = 0, same_before = 0, above_all = 0, same_all = 0;
+    for (int w = 0; w < kManyWaves; ++w) {
+        const int32_t x = s_cells[0][w], y = s_cells[1][w];
+        at += w < wave ? x : 0, same_before += w < wave ? y : 0;
+        above_all += x, same_all += y;
+    }
+    at += min(same_before, equal);
+    int32_t left = max(equal - same_before, 0);              // of those equal to the bound, for this wave and later ones
+    uint32_t limit = __builtin_amdgcn_readfirstlane(bound);
+    asm volatile("" : "+s"(limit));                          // or the masks of both loops would be kept for each other
+    for_keys([&](int r, uint32_t key) {
+        const uint64_t mine = uint64_t{1} << lane;
+        const uint64_t equals = __ballot(limit != 0 && key == limit);
+        const bool take = key > limit || ((equals & mine) != 0 && __popcll(equals & (mine - 1)) < left);
+        const uint64_t taken = __ballot(take);
+        if (take) {
+            out[(at + __popcll(taken & (mine - 1))) * a.b_column] = begin + r * 64 + lane;
+        }
+        at += __popcll(taken);
+        left = max(left - static_cast<int32_t>(__popcll(equals)), 0);
+        __builtin_amdgcn_sched_barrier(0);
+    });
+    for (int32_t i = above_all + min(same_all, equal) + tid; i < a.chosen; i += kManyThreads) {
         out[i * a.b_column] = -1;
     }
 }
@@ -597,15 +795,24 @@ Plan plan_of(int64_t tokens, int64_t groups, int64_t columns, int64_t page_size,
     return p;
 }
 
-template <int kSteps>
-void launch_scores(const ScoreArgs& a, int tiles16, uint32_t grid, uint32_t lds, hipStream_t stream) {
+template <int kSteps, bool kShort>
+void launch_tiles(const ScoreArgs& a, int tiles16, uint32_t grid, uint32_t lds, hipStream_t stream) {
     switch (tiles16) {
-        case 1: score_kernel<kSteps, 1><<<grid, kThreads, lds, stream>>>(a); break;
-        case 2: score_kernel<kSteps, 2><<<grid, kThreads, lds, stream>>>(a); break;
-        case 4: score_kernel<kSteps, 4><<<grid, kThreads, lds, stream>>>(a); break;
-        default: score_kernel<kSteps, 8><<<grid, kThreads, lds, stream>>>(a); break;
+        case 1: score_kernel<kSteps, 1, kShort><<<grid, kThreads, lds, stream>>>(a); break;
+        case 2: score_kernel<kSteps, 2, kShort><<<grid, kThreads, lds, stream>>>(a); break;
+        case 4: score_kernel<kSteps, 4, kShort><<<grid, kThreads, lds, stream>>>(a); break;
+        default: score_kernel<kSteps, 8, kShort><<<grid, kThreads, lds, stream>>>(a); break;
     }
     check_hip(hipGetLastError(), "launch block scores");
+}
+
+template <int kSteps>
+void launch_scores(const ScoreArgs& a, int tiles16, uint32_t grid, uint32_t lds, hipStream_t stream) {
+    if (a.sub_shift >= 0) {
+        launch_tiles<kSteps, true>(a, tiles16, grid, lds, stream);
+    } else {
+        launch_tiles<kSteps, false>(a, tiles16, grid, lds, stream);
+    }
 }
 
 int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_bytes, void* stream) {
@@ -714,13 +921,6 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     a.dim = static_cast<int32_t>(dim);
     a.group_div = FastDiv(static_cast<uint32_t>(a.groups)), a.share_div = FastDiv(static_cast<uint32_t>(a.share));
     a.block = FastDiv(static_cast<uint32_t>(s.block_size));
-    a.block_units = static_cast<int32_t>((s.block_size + kUnit - 1) / kUnit);
-    a.sub_shift = -1;
-    for (int shift = 0; shift < 5; ++shift) {
-        if (s.block_size == 1 << shift) {
-            a.sub_shift = shift;
-        }
-    }
     a.scores = static_cast<uint32_t*>(workspace);
     a.score_row = plan.score_row;
     const int64_t most_rows = std::min(s.max_query, tokens) * heads;
@@ -728,26 +928,32 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     while (16 * tiles16 < a.share) {
         tiles16 *= 2;
     }
+    const int unit = unit_of(dim <= 64 ? 1 : (dim <= 128 ? 2 : 4));
+    a.block_units = static_cast<int32_t>((s.block_size + unit - 1) / unit);
+    a.sub_shift = -1;
+    for (int shift = 0; 1 << shift < unit; ++shift) {
+        if (s.block_size == 1 << shift) {
+            a.sub_shift = shift;
+        }
+    }
     a.pairs = 16 * tiles16 / a.share;
     a.row_tiles = (a.groups + a.pairs - 1) / a.pairs;
     a.tiles = static_cast<int32_t>(s.query_starts != nullptr ? tokens * groups / a.pairs + a.at.batch
                                                              : tokens * a.row_tiles);
-    // Segments of at least 256 tokens, longer where the context makes more than 2048 workgroups, and as many blocks as
-    // there is room for keys.
+    // Segments of at least 256 tokens, longer where the contexts make more workgroups than fill the card a few times over,
+    // and as many blocks as there is room for keys.
     const int64_t capacity = std::max<int64_t>(a.at.own_most, 1);
-    int64_t wanted = std::min<int64_t>(std::max<int64_t>(a.tiles * capacity / 2048, 256), 4096);
-    wanted = (wanted + kUnit - 1) / kUnit * kUnit;
+    int64_t wanted = std::min<int64_t>(std::max<int64_t>(a.tiles * capacity / (tiles16 < 4 ? 8192 : 512), 256), 4096);
     int64_t segment_blocks = std::max<int64_t>(wanted / s.block_size, 1);
     segment_blocks = std::min<int64_t>(segment_blocks, kSegmentKeys / a.pairs);
     if (a.sub_shift >= 0) {
-        segment_blocks = std::max<int64_t>(segment_blocks >> (5 - a.sub_shift), 1) << (5 - a.sub_shift);
+        // Whole steps: as many tokens as kSegmentKeys / 128 pairs leave room for are one at least.
+        const int64_t each = unit >> a.sub_shift;
+        segment_blocks = std::max<int64_t>(segment_blocks / each, 1) * each;
     }
     a.segment_blocks = static_cast<int32_t>(segment_blocks);
-    int64_t segments = std::min<int64_t>((plan.score_row + segment_blocks - 1) / segment_blocks,
+    const int64_t segments = std::min<int64_t>((plan.score_row + segment_blocks - 1) / segment_blocks,
                                          std::max<int64_t>(65536 / a.tiles, 1));
-    if (segments > 8) {
-        segments = (segments + 7) / 8 * 8;
-    }
     a.segments = static_cast<int32_t>(segments);
     const uint32_t lds = static_cast<uint32_t>(a.pairs * segment_blocks * 4);
     const auto on = static_cast<hipStream_t>(stream);
@@ -770,15 +976,19 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     k.first = static_cast<int32_t>(s.first), k.last = static_cast<int32_t>(s.last);
     k.blocks = static_cast<int32_t*>(blocks.data);
     k.b_token = blocks.stride[0], k.b_group = blocks.stride[1], k.b_column = blocks.stride[2];
-    const uint32_t pairs = static_cast<uint32_t>(tokens * groups), grid = (pairs + kWaves - 1) / kWaves;
+    const uint32_t pairs = static_cast<uint32_t>(tokens * groups), grid = (pairs + kThreads / 64 - 1) / (kThreads / 64);
     if (plan.score_row <= 64) {
-        pick_kernel<1><<<grid, kThreads, 0, on>>>(k);
+        pick_kernel<1, 1><<<grid, kThreads, 0, on>>>(k);
     } else if (plan.score_row <= 256) {
-        pick_kernel<4><<<grid, kThreads, 0, on>>>(k);
-    } else if (plan.score_row <= 1024) {
-        pick_kernel<16><<<grid, kThreads, 0, on>>>(k);
+        pick_kernel<1, 4><<<grid, kThreads, 0, on>>>(k);
+    } else if (plan.score_row <= 2048) {
+        pick_kernel<4, 8><<<pairs, 256, 0, on>>>(k);
+    } else if (plan.score_row <= 16384) {
+        pick_many_kernel<16><<<pairs, kManyThreads, 0, on>>>(k);
+    } else if (plan.score_row <= 65536) {
+        pick_many_kernel<64><<<pairs, kManyThreads, 0, on>>>(k);
     } else {
-        pick_many_kernel<<<pairs, kManyThreads, 0, on>>>(k);
+        pick_many_kernel<0><<<pairs, kManyThreads, 0, on>>>(k);
     }
     check_hip(hipGetLastError(), "launch block selection");
     return 0;

@@ -200,3 +200,15 @@ def test_the_resident_lookup_takes_the_lists(gpu):
         tokens = [j * 32 + i for j in want[b].tolist() for i in range(32)]
         expected = [int(table[b, t]) if 0 <= t < length else -1 for t in tokens]
         assert slots[0, b].tolist() == expected
+
+
+@pytest.mark.parametrize("chosen,first,last", [(1, 0, 1), (7, 3, 4), (300, 1, 1), (2500, 1000, 1500), (2100, 0, 0)])
+def test_many_blocks_of_equal_and_forced_scores(gpu, chosen, first, last):
+    """Lists of tokens: scores with few values, lists as long as what is always chosen, longer than the context."""
+    batch = make_batch(gpu, [2400, 130, 2050], None, 64, seed=13)
+    pool = make_index_pool(gpu, batch.pages, 64, 16, seed=13, small=True)
+    query = torch.ones((3, 1, 16), dtype=BF16, device=gpu)
+    want = selection(batch, pool, query, 1, chosen, 1, first, last)
+    assert torch.equal(choose(batch, pool, query, 1, chosen, 1, first, last).cpu(), want)
+    batch.tables = torch.cat([batch.tables, torch.zeros((3, 1100), dtype=torch.int32, device=gpu)], 1)   # > 65536 places
+    assert torch.equal(choose(batch, pool, query, 1, chosen, 1, first, last).cpu(), want)
