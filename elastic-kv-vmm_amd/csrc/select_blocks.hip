@@ -9,6 +9,7 @@
 //
 // Two launches: scores of all blocks as ordered 32-bit keys into the workspace, then each (token, group)'s largest.
 #include "ekv_codes.h"
+#include "ekv_device.h"
 #include "ekv_memory.h"
 #include "ekv_mfma.h"
 #include "ekv_pool.h"
@@ -61,11 +62,19 @@ struct ScoreArgs {
     int32_t tiles;
 };
 
-// Scores in the order of whole numbers, 0 for a block without a token that is seen.
+// Scores in the order of whole numbers: 0 for a block without a token that is seen, kForced for one that is always taken,
+// which no score reaches.
+constexpr uint32_t kForced = 0xff800000u;
+
 __device__ __forceinline__ uint32_t ordered(float score) {
-    const uint32_t bits = __float_as_uint(score + 0.0f);     // -0 counts as 0
+    const uint32_t bits = __float_as_uint(fminf(score, 3.4028235e38f) + 0.0f);     // -0 counts as 0
     const uint32_t key = bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
     return score > -INFINITY ? key : 0u;
+}
+
+// The score of a key: infinity of kForced, NaN of 0.
+__device__ __forceinline__ float score_of(uint32_t key) {
+    return __uint_as_float(key ^ (~static_cast<uint32_t>(static_cast<int32_t>(key) >> 31) | 0x80000000u));
 }
 
 __device__ __forceinline__ int32_t clamped(int64_t v, int64_t low, int64_t high) {
@@ -460,9 +469,19 @@ struct Candidates {
     const uint32_t* scores;
     int32_t count, forced_below, forced_from;
 
-    __device__ __forceinline__ uint32_t key(int32_t j) const {
-        const uint32_t k = j < count ? scores[j] : 0u;
-        return k != 0 && (j < forced_below || j >= forced_from) ? 0xffffffffu : k;
+    // Block j's key, given what is held for it.
+    __device__ __forceinline__ uint32_t key_of(int32_t j, uint32_t k) const {
+        k = j < count ? k : 0u;
+        return k != 0 && (j < forced_below || j >= forced_from) ? kForced : k;
+    }
+
+    __device__ __forceinline__ uint32_t held(int32_t j) const {
+        return load_global<uint32_t>(reinterpret_cast<const char*>(scores + max(min(j, count - 1), 0)));
+    }
+
+    // Whether some of blocks j .. j + 63 are always taken or past the end.
+    __device__ __forceinline__ bool mixed(int32_t j) const {
+        return j < forced_below || j + 63 >= forced_from || j + 63 >= count;
     }
 };
 
@@ -508,11 +527,10 @@ __global__ __launch_bounds__(kWaves == 1 ? kThreads : kWaves * 64) void pick_ker
 #pragma unroll
     for (int r = 0; r < kRegs; ++r) {
         const int32_t j = begin + r * 64 + lane;
-        const uint32_t k = r < used ? c.scores[j < c.count ? j : 0] : 0u;
-        key[r] = r < used && j < c.count && k != 0 ? ((j < c.forced_below || j >= c.forced_from) ? 0xffffffffu : k) : 0u;
+        key[r] = r < used ? c.key_of(j, c.held(j)) : 0u;
         // What is none, or always taken, says nothing of where the K-th largest lies.
         least = min(least, key[r] != 0 ? key[r] : 0xffffffffu);
-        most = max(most, key[r] != 0xffffffffu ? key[r] : 0u);
+        most = max(most, key[r] != kForced ? key[r] : 0u);
     }
     int parity = 0;
     // One number of each wave (the same in all its lanes), all of them to everybody.
@@ -603,17 +621,21 @@ __global__ __launch_bounds__(kWaves == 1 ? kThreads : kWaves * 64) void pick_ker
 
 constexpr int kManyWaves = 16, kManyThreads = kManyWaves * 64;
 constexpr int kDigit = 11, kBins = 1 << kDigit;
+constexpr int kFew = 1024;                    // keys that one wave looks through
 
-// The same for many blocks: the K-th largest key digit by digit, 11 bits at a time, from the counts of the digits of those
-// keys that agree with it so far. kRegs: a lane's keys in registers; 0: any number of keys, read again for each digit.
+// The same for many blocks. The range of the scores in 2047 equal parts, the keys counted in them, the part that holds
+// the K-th largest; its keys, few as a rule, to one wave, which finds the K-th largest bit by bit. (Parts of the range,
+// not leading bits: those are the exponent, and most scores have one of few.) Where a part holds more than kFew, what is
+// left is decided in digits of 11 bits of the key. kRegs: a lane's keys in registers; 0: any number of keys, read again
+// each time.
 //
-// What bounds it: the additions to the counts in LDS. The first digit begins at the first bit in which keys differ, so
-// that they spread over many counts. Bit by bit, 40000 keys took 94 us a launch.
+// What bounds it: a workgroup's instructions, some 30 a key in passes over all keys; rows are few where they are long.
 template <int kRegs>
 __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs a) {
     __shared__ uint32_t s_bins[kBins];
+    __shared__ uint32_t s_few[kFew];
     __shared__ uint32_t s_cells[2][kManyWaves];
-    __shared__ uint32_t s_found[2];               // the digit, and how many keys have a larger one
+    __shared__ uint32_t s_found[3];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t pair = blockIdx.x;
@@ -624,107 +646,195 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
     if constexpr (kRegs > 0) {
 #pragma unroll
         for (int r = 0; r < kRegs; ++r) {
-            held[r] = r < used ? c.key(begin + r * 64 + lane) : 0u;
+            held[r] = c.held(begin + min(r, used) * 64 + lane);
+        }
+#pragma unroll
+        for (int r = 0; r < kRegs; ++r) {
+            if (r >= used) {
+                held[r] = 0;
+            } else if (c.mixed(begin + r * 64)) {
+                held[r] = c.key_of(begin + r * 64 + lane, held[r]);
+            }
         }
     }
-    // body(r, key) for each of a lane's keys, in order; whole waves take part.
+    // body(r, key) for each of a lane's keys, in order, and perhaps for keys of 0 behind them; whole waves take part.
     const auto for_keys = [&](auto&& body) {
         if constexpr (kRegs > 0) {
 #pragma unroll
-            for (int r = 0; r < kRegs; ++r) {
-                if (r < used) {
-                    body(r, held[r]);
+            for (int eight = 0; eight < kRegs; eight += 8) {
+                if (eight < used) {
+#pragma unroll
+                    for (int r = eight; r < eight + 8; ++r) {
+                        body(r, held[r]);
+                        __builtin_amdgcn_sched_barrier(0);     // the masks of all would fill the scalar registers
+                    }
                 }
             }
         } else {
             for (int r = 0; r < used; ++r) {
-                body(r, c.key(begin + r * 64 + lane));
+                const int32_t j = begin + r * 64 + lane;
+                body(r, c.key_of(j, c.held(j)));
             }
         }
     };
-    uint32_t least = 0xffffffffu, most = 0;
-    for_keys([&](int, uint32_t key) {
-        // What is none, or always taken, says nothing of where the K-th largest lies.
-        least = min(least, key != 0 ? key : 0xffffffffu);
-        most = max(most, key != 0xffffffffu ? key : 0u);
-    });
-    least = ~uniform_lane(wave_scan<kMax>(~least)), most = uniform_lane(wave_scan<kMax>(most));
-    if (lane == 0) {
-        s_cells[0][wave] = least, s_cells[1][wave] = most;
-    }
-    __syncthreads();
-    for (int w = 0; w < kManyWaves; ++w) {
-        least = min(least, s_cells[0][w]), most = max(most, s_cells[1][w]);
-    }
-    // Keys that are always taken count as the largest of the others, and those that are none fall out: with what the others
-    // share in front, the bound is theirs.
-    const uint32_t differ = least ^ most;
-    int bits = least > most ? 0 : (differ != 0 ? 32 - __builtin_clz(differ) : 0);     // undecided bits of the bound
-    uint32_t bound = bits >= 32 ? 0u : (least >> bits) << bits;
-    uint32_t wanted = a.chosen, forced = 0;
-    for_keys([&](int, uint32_t key) { forced += key == 0xffffffffu; });
-    forced = uniform_lane(wave_scan<kAdd>(forced));
-    __syncthreads();
-    if (lane == 0) {
-        s_cells[0][wave] = forced;
-    }
-    __syncthreads();
-    forced = 0;
-    for (int w = 0; w < kManyWaves; ++w) {
-        forced += s_cells[0][w];
-    }
-    wanted -= min(wanted, forced);
-    if (least > most || wanted == 0) {
-        bound = least > most ? 0u : 0xffffffffu;      // no others; or none of them
-        bits = 0;
-    }
-    bool all = false;                                 // fewer than K are there
-    while (bits > 0 && !all) {
-        const int digit = min(bits, kDigit), shift = bits - digit;
-        for (int i = tid; i < kBins; i += kManyThreads) {
-            s_bins[i] = 0;
+    // Values of each wave, the same in all its lanes, to all waves.
+    const auto share = [&](uint32_t first, uint32_t second, auto&& each) {
+        __syncthreads();
+        if (lane == 0) {
+            s_cells[0][wave] = first, s_cells[1][wave] = second;
         }
         __syncthreads();
-        for_keys([&](int, uint32_t key) {
-            if (key != 0 && key != 0xffffffffu && (bits >= 32 || (key ^ bound) >> bits == 0)) {
-                atomicAdd(&s_bins[(key >> shift) & ((1u << digit) - 1)], 1u);
-            }
-        });
+#pragma unroll
+        for (int w = 0; w < kManyWaves; ++w) {
+            each(w, s_cells[0][w], s_cells[1][w]);
+        }
+    };
+    // The least and the largest of the keys that are neither none nor always taken: 0 - 1 and kForced - kForced are last.
+    uint32_t least = 0xffffffffu, most = 0;
+    for_keys([&](int, uint32_t key) {
+        least = min(least, key - 1);
+        most = max(most, key == kForced ? 0u : key);
+    });
+    {
+        const uint32_t low = ~uniform_lane(wave_scan<kMax>(~least)), high = uniform_lane(wave_scan<kMax>(most));
+        least = 0xffffffffu, most = 0;
+        share(low, high, [&](int, uint32_t x, uint32_t y) { least = min(least, x), most = max(most, y); });
+        least += 1;
+    }
+    uint32_t wanted = a.chosen;
+    // Where, among the bins that place(key) counts keys in (-1: nowhere), the `wanted`-th largest is, of how many: false
+    // if there are fewer. `wanted` becomes its place among those.
+    const auto find = [&](auto&& place, uint32_t& bin, uint32_t& among) {
         __syncthreads();
-        // From the largest digit down: two to a thread.
-        const int top = kBins - 1 - 2 * tid;
-        const uint32_t first = s_bins[top], second = s_bins[top - 1];
-        const uint32_t sum = wave_scan<kAdd>(first + second);
-        if (lane == 63) {
-            s_cells[0][wave] = sum;
+        for (int i = tid; i < kBins; i += kManyThreads) {
+            s_bins[i] = 0;
         }
         if (tid == 0) {
             s_found[0] = kBins;
         }
         __syncthreads();
+        for_keys([&](int, uint32_t key) {
+            const int at = place(key);
+            if (at >= 0) {
+                atomicAdd(&s_bins[at], 1u);
+            }
+        });
+        __syncthreads();
+        // From the largest down: two to a thread.
+        const int top = kBins - 1 - 2 * tid;
+        const uint32_t first = s_bins[top], second = s_bins[top - 1];
+        const uint32_t sum = wave_scan<kAdd>(first + second);
         uint32_t before = sum - first - second;
-        for (int w = 0; w < wave; ++w) {
-            before += s_cells[0][w];
-        }
+        share(uniform_lane(sum), 0, [&](int w, uint32_t x, uint32_t) { before += w < wave ? x : 0; });
         if (before < wanted && wanted <= before + first + second) {
             const bool high = wanted <= before + first;
             s_found[0] = high ? top : top - 1;
             s_found[1] = high ? before : before + first;
+            s_found[2] = high ? first : second;
         }
         __syncthreads();
-        all = s_found[0] == kBins;
-        if (!all) {
-            bound |= s_found[0] << shift;
-            wanted -= s_found[1];
+        bin = s_found[0];
+        if (bin == kBins) {
+            return false;
+        }
+        wanted -= s_found[1];
+        among = s_found[2];
+        return true;
+    };
+    uint32_t from = 1, to = kForced, among = kFew + 1;       // the K-th largest is the wanted-th of `among` from .. to
+    bool there = true;
+    const float low = score_of(least), scale = (kBins - 2) / (score_of(most) - low);
+    if (least < most && scale > 0 && scale < INFINITY) {
+        // Parts 1 .. kBins - 1.
+        const auto part = [&](uint32_t key) {
+            return min(static_cast<int>(fmaf(score_of(key) - low, scale, 1.0f)), kBins - 1);
+        };
+        uint32_t bin = 0;
+        there = find([&](uint32_t key) { return key != 0 ? part(key) : -1; }, bin, among);
+        if (there) {
+            // Its first and last key, by trying 64 keys at a time.
+            const auto first_of = [&](int wanted_part) {
+                uint32_t below = 0, above = kForced + 1;         // the first key lies above `below`, not above `above`
+                while (above - below > 1) {
+                    const uint32_t step = (above - below + 63) / 64, at = below + min((lane + 1) * step, above - below);
+                    const bool reached = at > kForced || (at != 0 && part(at) >= wanted_part);
+                    const int which = __builtin_ctzll(__ballot(reached));
+                    above = below + min((which + 1) * step, above - below);
+                    below += which * step;
+                }
+                return above;
+            };
+            from = first_of(bin), to = first_of(bin + 1) - 1;
+        }
+    }
+    uint32_t bound = 0;                               // all there are
+    if (there && among <= kFew) {
+        __syncthreads();
+        if (tid == 0) {
+            s_found[0] = 0;
+        }
+        __syncthreads();
+        for_keys([&](int, uint32_t key) {
+            if (key >= from && key <= to) {
+                const uint32_t i = atomicAdd(&s_found[0], 1u);
+                if (i < kFew) {
+                    s_few[i] = key;
+                }
+            }
+        });
+        __syncthreads();
+        if (wave == 0) {
+            uint32_t few[kFew / 64];
+#pragma unroll
+            for (int r = 0; r < kFew / 64; ++r) {
+                const uint32_t i = r * 64 + lane;
+                few[r] = i < among ? s_few[i] : 0u;
+            }
+            const uint32_t differ = from ^ to;
+            const int bits = differ != 0 ? 32 - __builtin_clz(differ) : 0;
+            uint32_t found = bits >= 32 ? 0u : (from >> bits) << bits;
+            for (int bit = bits - 1; bit >= 0; --bit) {
+                const uint32_t tried = found | (1u << bit);
+                uint32_t n = 0;
+#pragma unroll
+                for (int r = 0; r < kFew / 64; ++r) {
+                    if (r * 64 < among) {
+                        n += __popcll(__ballot(few[r] >= tried));
+                    }
+                }
+                found = n >= wanted ? tried : found;
+            }
+            uint32_t larger = 0;
+#pragma unroll
+            for (int r = 0; r < kFew / 64; ++r) {
+                larger += __popcll(__ballot(few[r] > found));
+            }
+            if (lane == 0) {
+                s_found[0] = found, s_found[1] = larger;
+            }
+        }
+        __syncthreads();
+        bound = s_found[0];
+        wanted -= s_found[1];
+    } else if (there) {
+        const uint32_t differ = from ^ to;
+        int bits = differ != 0 ? 32 - __builtin_clz(differ) : 0;
+        bound = bits >= 32 ? 0u : (from >> bits) << bits;
+        while (there && bits > 0) {
+            const int digit = min(bits, kDigit), shift = bits - digit;
+            uint32_t bin = 0;
+            there = find(
+                [&](uint32_t key) {
+                    const bool mine = key >= from && key <= to && (bits >= 32 || (key ^ bound) >> bits == 0);
+                    return mine ? static_cast<int>((key >> shift) & ((1u << digit) - 1)) : -1;
+                },
+                bin, among);
+            bound |= bin << shift;
             bits = shift;
         }
-        __syncthreads();
+        bound = there ? bound : 0u;
     }
-    if (all) {
-        bound = 0;                                    // all there are
-    }
-    // How many equal to the bound are taken.
-    const int32_t equal = bound == 0xffffffffu ? a.chosen : static_cast<int32_t>(wanted);
+    const int32_t equal = static_cast<int32_t>(wanted);      // how many equal to the bound are taken
     const int32_t token = a.group_div.div(static_cast<uint32_t>(pair)), group = static_cast<int32_t>(pair) - token * a.groups;
     int32_t* const out = a.blocks + token * a.b_token + group * a.b_group;
     uint32_t above = 0, same = 0;
@@ -733,33 +843,32 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
         same += bound != 0 && key == bound;
     });
     above = uniform_lane(wave_scan<kAdd>(above)), same = uniform_lane(wave_scan<kAdd>(same));
-    __syncthreads();
-    if (lane == 0) {
-        s_cells[0][wave] = above, s_cells[1][wave] = same;
-    }
-    __syncthreads();
     int32_t at = 0, same_before = 0, above_all = 0, same_all = 0;
-    for (int w = 0; w < kManyWaves; ++w) {
-        const int32_t x = s_cells[0][w], y = s_cells[1][w];
+    share(above, same, [&](int w, uint32_t x, uint32_t y) {
         at += w < wave ? x : 0, same_before += w < wave ? y : 0;
         above_all += x, same_all += y;
-    }
+    });
     at += min(same_before, equal);
     int32_t left = max(equal - same_before, 0);              // of those equal to the bound, for this wave and later ones
-    uint32_t limit = __builtin_amdgcn_readfirstlane(bound);
-    asm volatile("" : "+s"(limit));                          // or the masks of both loops would be kept for each other
-    for_keys([&](int r, uint32_t key) {
-        const uint64_t mine = uint64_t{1} << lane;
-        const uint64_t equals = __ballot(limit != 0 && key == limit);
-        const bool take = key > limit || ((equals & mine) != 0 && __popcll(equals & (mine - 1)) < left);
+    const uint64_t mine = uint64_t{1} << lane;
+    const auto leave = [&](int r, bool take) {
         const uint64_t taken = __ballot(take);
         if (take) {
-            out[(at + __popcll(taken & (mine - 1))) * a.b_column] = begin + r * 64 + lane;
+            out[(at + lanes_below(taken)) * a.b_column] = begin + r * 64 + lane;
         }
         at += __popcll(taken);
-        left = max(left - static_cast<int32_t>(__popcll(equals)), 0);
-        __builtin_amdgcn_sched_barrier(0);
-    });
+    };
+    const uint32_t limit = bound != 0 ? bound : 1u;
+    if (bound == 0 || same_all <= equal) {
+        for_keys([&](int r, uint32_t key) { leave(r, key >= limit); });
+    } else {
+        for_keys([&](int r, uint32_t key) {
+            const uint64_t equals = __ballot(key == limit);
+            const bool take = key > limit || ((equals & mine) != 0 && static_cast<int32_t>(lanes_below(equals)) < left);
+            leave(r, take);
+            left = max(left - static_cast<int32_t>(__popcll(equals)), 0);
+        });
+    }
     for (int32_t i = above_all + min(same_all, equal) + tid; i < a.chosen; i += kManyThreads) {
         out[i * a.b_column] = -1;
     }
