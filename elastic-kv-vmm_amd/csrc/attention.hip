@@ -528,8 +528,7 @@ void place(Phase& p, void* workspace) {
     }
 }
 
-int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, uint64_t bytes, void* stream,
-           const BlockLists* lists = nullptr) {
+void need_workspace(const Plan& plan, const void* workspace, uint64_t bytes) {
     if (bytes < plan.bytes) {
         throw std::invalid_argument("the attention needs " + std::to_string(plan.bytes) + " workspace bytes, got " +
                                     std::to_string(bytes));
@@ -537,6 +536,11 @@ int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, u
     if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) {
         throw std::invalid_argument("the workspace must be a 256-byte aligned device buffer");
     }
+}
+
+int launch(const AttentionArgs& a, Plan& plan, int32_t dtype, void* workspace, uint64_t bytes, void* stream,
+           const BlockLists* lists = nullptr) {
+    need_workspace(plan, workspace, bytes);
     if (a.tokens == 0) {
         return 0;
     }
@@ -686,6 +690,15 @@ int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64
     return launch(a, plan, query->dtype, workspace, workspace_bytes, stream);
 }
 
+// Whether query tokens go through their lists together.
+bool union_pays(const AttentionArgs& a, const BlockLists& lists, int64_t block_size, int64_t max_query, int32_t dim_pad) {
+    const int64_t tile_tokens = std::min<int64_t>(64, 63 / a.share + 2);
+    const bool fits = dim_pad <= 128 && block_size % 32 == 0 && tile_tokens * lists.width <= kUnionEntries &&
+                      a.block_most / block_size < kUnionBlocks &&
+                      (int64_t{a.tokens} * a.share / 64 + a.batch) * a.kv_heads < 1 << 24;   // fewer than 2^32 threads
+    return fits && a.share <= 32 && max_query * a.share >= 64 && int64_t{a.tokens} * a.share * a.kv_heads >= 64 * 128;
+}
+
 int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t workspace_bytes, void* stream) {
     AttentionArgs a = common_args(s.query, s.planes, s.layer, s.kv_heads, s.page_size, s.scale, s.output, s.lse);
     a.block_most = own_tables(a, s.block_tables, s.rows, s.lengths, s.query_starts, s.max_query, s.page_size);
@@ -706,6 +719,16 @@ int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t
     lists.wide = blocks.dtype == EKV_INT64 ? 4 : 0;
     lists.block = FastDiv(static_cast<uint32_t>(s.block_size));
     lists.heads = FastDiv(static_cast<uint32_t>(a.kv_heads / blocks.shape[1]));
+    lists.width = static_cast<int32_t>(blocks.shape[2]);
+    if (s.query_starts != nullptr && union_pays(a, lists, s.block_size, s.max_query, plan.own.dim_pad)) {
+        need_workspace(plan, workspace, workspace_bytes);
+        if (a.tokens > 0) {
+            lists.halves = FastDiv(static_cast<uint32_t>(s.block_size / 32));
+            lists.tiles = static_cast<int32_t>(int64_t{a.tokens} * a.share / 64 + a.batch);
+            launch_union(Launch{a, {plan.own, {}}, lists}, s.query->dtype, stream);
+        }
+        return 0;
+    }
     return launch(a, plan, s.query->dtype, workspace, workspace_bytes, stream, &lists);
 }
 

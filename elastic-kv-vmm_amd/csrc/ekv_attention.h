@@ -96,6 +96,9 @@ struct BlockLists {
     uint32_t column;
     int32_t wide;                     // 4 for int64 ids
     FastDiv block, heads;             // tokens of a block; KV heads of a list
+    // attention_union.hip
+    int32_t width, tiles;             // entries of a list; tiles of 64 rows of a KV head
+    FastDiv halves;                   // runs of 32 tokens of a block
 };
 
 struct Launch {
@@ -513,6 +516,11 @@ void launch_narrow(const Launch& l, int32_t dtype, int tiles16, void* stream);
 
 // attention_blocks.hip: the same over lists of blocks, at most 64 rows (32 of 256 columns) a tile.
 void launch_blocks(const Launch& l, int32_t dtype, int tiles16, void* stream);
+
+// attention_union.hip: tiles of 64 rows over all blocks that their tokens list, at most kUnionEntries entries in those
+// lists, of a context of at most kUnionBlocks blocks; blocks of whole runs of 32 tokens, head sizes up to 128.
+constexpr int kUnionEntries = 1024, kUnionBlocks = 4096;
+void launch_union(const Launch& l, int32_t dtype, void* stream);
 
 // attention_wide.hip: row tiles of 128 (row_shift 7) or 256 rows, units of at least 2^kWideUnit keys.
 constexpr int kWideUnit = 6;
