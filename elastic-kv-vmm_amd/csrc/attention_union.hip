@@ -67,7 +67,7 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
         const AttentionArgs& a = l.a;
         // Tiles of a head lie side by side: their blocks meet behind one L2.
         const int32_t item = on_die(blockIdx.x, gridDim.x);
-        head = item / l.lists.tiles;
+        head = uniform(item / l.lists.tiles);
         const int32_t tile = item - head * l.lists.tiles;
         // Batch row b has tiles from starts[b] * share / 64 + b on.
         const auto begin = [&](int32_t b) {
@@ -92,9 +92,10 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
         }
         const int64_t length = a.lengths.fetch(low), given = a.rows.data != nullptr ? a.rows.fetch(low) : low;
         const bool good = given >= 0 && given < a.requests;
-        request = good ? static_cast<int32_t>(given) : 0;
-        seen_most = good ? clamped(length, 0, a.block_most) : 0;
-        position = clamped(length, -1, 0x7ffffffe) - count;
+        request = uniform(good ? static_cast<int32_t>(given) : 0);
+        seen_most = uniform(good ? clamped(length, 0, a.block_most) : 0);
+        position = uniform(clamped(length, -1, 0x7ffffffe) - count);
+        first = uniform(first), rows = uniform(rows), row_begin = uniform(row_begin);
     }
     // Tokens that the batch row's i-th query token sees.
     const auto seen_by_token = [&](int32_t i) { return min(max(position + i + 1, 0), seen_most); };
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
                 __syncthreads();
             }
         } while (__syncthreads_or(again));
-        entries = min(entries, kUnionEntries);
+        entries = uniform(min(entries, kUnionEntries));
     }
 
     const AttentionArgs& a = fresh().a;
@@ -240,30 +241,27 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
             offset_high = good ? static_cast<uint32_t>(offset >> 32) : ~0u;
             return __ballot(good);
         };
-        words4 k[kLoads], v[kLoads];
-        const auto load = [&](int i) {
-            const uint32_t low = __shfl(offset_low, i * kKeysAtOnce + load_key);
-            const uint32_t high = __shfl(offset_high, i * kKeysAtOnce + load_key);
-            const char* at = k_head + (static_cast<uint64_t>(high) << 32 | low);
-            const char* v_at = at + cache.kv_stride;
-            k[i] = load_global<words4>(high != ~0u ? at : zeros);
-            v[i] = load_global<words4>(high != ~0u ? v_at : zeros);
-        };
-        const auto load_all = [&] {
+        words4 k[kLoads], v[kLoads];                               // a tile's rows on their way to LDS
+        const auto load = [&] {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                load(i);
+                const uint32_t low = __shfl(offset_low, i * kKeysAtOnce + load_key);
+                const uint32_t high = __shfl(offset_high, i * kKeysAtOnce + load_key);
+                const char* at = k_head + (static_cast<uint64_t>(high) << 32 | low);
+                const char* v_at = at + cache.kv_stride;
+                k[i] = load_global<words4>(high != ~0u ? at : zeros);
+                v[i] = load_global<words4>(high != ~0u ? v_at : zeros);
             }
         };
-        const auto store_all = [&](int buffer, int32_t tile) {
+        const auto store = [&](int buffer, int32_t tile) {
             typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
             u16x2 most = {0, 0};
+            const int at = hidden(write_at);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                char* const to = s_data + buffer + i * kKeysAtOnce * kBytes + (write_at ^ ((i * kKeysAtOnce & 8) << 2));
+                char* const to = s_data + buffer + i * kKeysAtOnce * kBytes + (at ^ ((i * kKeysAtOnce & 8) << 2));
                 // K past the head size meets zeros of q and must not be an infinity; V's columns are not stored.
-                const words4 kept = load_piece < pieces ? k[i] : words4{0, 0, 0, 0};
-                *reinterpret_cast<words4*>(to) = kept;
+                *reinterpret_cast<words4*>(to) = load_piece < pieces ? k[i] : words4{0, 0, 0, 0};
                 *reinterpret_cast<words4*>(to + Tile<kDim>::kSize) = v[i];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -318,38 +316,49 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
                 top = to_top;
             }
         };
-        const auto key_piece = [&](const char* tile, int c) {
-            return *reinterpret_cast<const words4*>(tile + (read_k ^ (c << 5)) + half_at);
-        };
-
-        const Ids first_ids = ids_of(0), second_ids = ids_of(1);
-        uint64_t now = look(first_ids);
-        load_all();
-        store_all(0, 0);
-        uint64_t next = look(second_ids);
-        Ids ids = ids_of(2);
-        load_all();
-        lds_barrier();
-        f32x16 s;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[i] = 0;
+        // The rows of a tile leave their registers for LDS while the tile before it is worked on, the next one's are then
+        // on their way, and the page ids of the one after that. One barrier a tile; products and softmax of a wave stand
+        // beside those of the other workgroup on the compute unit.
+        uint64_t now, next;
+        Ids ids;
+        {
+            const Ids first_ids = ids_of(0), second_ids = ids_of(1);
+            ids = ids_of(2);
+            now = look(first_ids);
+            load();
+            store(0, 0);
+            next = look(second_ids);
+            load();
         }
-#pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-            s = T::mfma32(key_piece(s_data, c), q[c], s);
-        }
-        if (!sight(0, now)) {
-            cut_scores(s);
-        }
-        follow(largest(s));
         int buffer = 0;
 #pragma unroll 1
         for (int32_t tile = 0; tile < tiles; ++tile, buffer ^= 2 * Tile<kDim>::kSize) {
+            lds_barrier();      // this buffer holds the tile, and nobody reads the other one any more
             const char* const here = s_data + buffer;
-            const char* const other = s_data + (buffer ^ (2 * Tile<kDim>::kSize));
-            store_all(buffer ^ (2 * Tile<kDim>::kSize), tile + 1);
-            lds_barrier();      // the other buffer holds the next tile
+            // Hidden, or what follows from them would be computed once and spilled.
+            const int at_k = hidden(read_k), at_v = hidden(read_v), at_v8 = hidden(read_v8);
+            store(buffer ^ (2 * Tile<kDim>::kSize), tile + 1);
+            const bool whole = sight(tile, now);
+            now = next;
+            {
+                const Ids later = ids_of(tile + 3);      // before the rows: a wait for them would be for the rows as well
+                next = look(ids);
+                load();
+                ids = later;
+            }
+            f32x16 s;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[i] = 0;
+            }
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) {
+                s = T::mfma32(*reinterpret_cast<const words4*>(here + (at_k ^ (c << 5)) + half_at), q[c], s);
+            }
+            if (!whole) {
+                cut_scores(s);
+            }
+            follow(largest(s));
             if (s_spoiled[tile & 1] == static_cast<uint32_t>(tile + 1)) {
                 // A key that only some rows see has weight 0 for the others, and 0 * infinity is not 0: the infinities
                 // and NaN are added to the rows that see them (a weight is positive), then cleared.
@@ -383,84 +392,23 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
                 }
                 lds_barrier();
             }
-            now = next;
-            next = look(ids);
-            ids = ids_of(tile + 3);
-            // The weights of s and their values, while the next tile's scores are multiplied: matrix and vector
-            // instructions are dealt in turn, so that a wave's softmax runs beside its own products.
             const float shift = (top == -INFINITY ? 0.0f : top * scale) - T::kShift;
-            const bool whole = sight(tile + 1, now);
-            f32x16 n;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                n[i] = 0;
-            }
-            const auto column = [&](int j) {          // of 16-key group j / kCols, columns j % kCols
-                const int at = half_at + j / kCols * 16 * kBytes;
-                const words2 low = read_transposed(here + (read_v ^ (j % kCols << 6)) + at);
-                const words2 high = read_transposed(here + (read_v8 ^ (j % kCols << 6)) + at);
-                return words4{low[0], low[1], high[0], high[1]};
-            };
-            float w[16];
             words4 weights[2];
-            const auto weigh = [&](int i) {
-                w[i] = __builtin_amdgcn_exp2f(s[i] * scale - shift);
-                sum += w[i];
-                if (i & 1) {
-                    weights[i >> 3][(i & 7) >> 1] = T::pack(w[i - 1], w[i]);
-                }
-            };
-            words4 ahead[2] = {key_piece(other, 0), key_piece(other, 1)};
-            words4 columns[2];
 #pragma unroll
-            for (int c = 0; c < kSteps; ++c) {
-                const words4 x = ahead[c & 1];
-                if (c + 2 < kSteps) {
-                    ahead[c & 1] = key_piece(other, c + 2);
-                } else {
-                    columns[c + 2 - kSteps] = column(c + 2 - kSteps);
-                }
-                n = T::mfma32(x, q[c], n);
-#pragma unroll
-                for (int i = c * 12 / kSteps; i < (c + 1) * 12 / kSteps; ++i) {
-                    weigh(i);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < 16; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(s[i] * scale - shift);
+                const float y = __builtin_amdgcn_exp2f(s[i + 1] * scale - shift);
+                sum += x;
+                sum += y;
+                weights[i >> 3][(i & 7) >> 1] = T::pack(x, y);
             }
-            float most = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 2 * kCols; ++j) {
-                const words4 x = columns[j & 1];
-                if (j + 2 < 2 * kCols) {
-                    columns[j & 1] = column(j + 2);
-                }
-                o[j % kCols] = T::mfma32(x, weights[j / kCols], o[j % kCols]);
-                if (j < kCols) {
-#pragma unroll
-                    for (int i = 12 + j * 4 / kCols; i < 12 + (j + 1) * 4 / kCols; ++i) {
-                        weigh(i);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    if (i * 2 * kCols / kLoads == j) {
-                        load(i);
-                    }
-                }
-#pragma unroll
-                for (int i = j * 8 / kCols; i < (j + 1) * 8 / kCols; ++i) {
-                    most = fmaxf(most, n[i]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < 2 * kCols; ++j) {     // 16 keys, 32 columns
+                const int at = half_at + j / kCols * 16 * kBytes;
+                const words2 low = read_transposed(here + (at_v ^ (j % kCols << 6)) + at);
+                const words2 high = read_transposed(here + (at_v8 ^ (j % kCols << 6)) + at);
+                o[j % kCols] = T::mfma32(words4{low[0], low[1], high[0], high[1]}, weights[j / kCols], o[j % kCols]);
             }
-            most = over_halves_max(most);
-            if (!whole) {
-                cut_scores(n);
-                most = largest(n);
-            }
-            follow(most);
-            s = n;
-            lds_barrier();      // nobody reads this buffer any more
         }
     }
 
