@@ -56,6 +56,8 @@ struct ScoreArgs {
     int32_t block_units, sub_shift;         // steps of a block; or blocks of 2^sub_shift tokens, several a step (-1: not)
     uint32_t* scores;                       // [tokens, groups, score_row]
     int64_t score_row;
+    char* codes;                            // queries as codes already, [tokens, groups, share] rows, and their scales;
+    float* code_scales;                     // or NULL
     int32_t segment_blocks, segments;       // blocks of a segment; workgroups beside each other that share a tile's
     int32_t pairs;                          // (token, group) pairs of a tile of rows
     int32_t row_tiles;                      // tiles of a batch row with one query token
@@ -102,21 +104,37 @@ __device__ __forceinline__ BatchRow batch_row(const BatchRows& a, int32_t b) {
     return r;
 }
 
-// The batch row whose query tokens hold `token`, or -1.
+// The last batch row whose value is not above `wanted` (-1: none), where values do not decrease from row to row: 64 of them
+// are looked at together, so that a call's first reads are two at most, one after the other, for 4096 rows. All lanes of
+// a wave call it, with the same `wanted`.
+template <typename Value>
+__device__ __forceinline__ int32_t last_row_not_above(int32_t batch, int32_t wanted, Value&& value) {
+    const int32_t lane = threadIdx.x & 63;
+    int32_t low = 0, rows = batch;
+    while (rows > 0) {
+        const int32_t step = (rows + 63) >> 6, at = lane * step;
+        const int32_t below = __popcll(__ballot(at < rows && value(low + min(at, rows - 1)) <= wanted));
+        if (below == 0) {
+            return low - 1;
+        }
+        // Row low + (below - 1) * step is not above it, the next of those looked at is.
+        const int32_t begin = (below - 1) * step;
+        if (step == 1) {
+            return low + begin;
+        }
+        rows = min(step, rows - begin);
+        low += begin;
+    }
+    return -1;
+}
+
+// The batch row whose query tokens hold `token` (a wave's), or -1.
 __device__ __forceinline__ int32_t row_of_token(const BatchRows& a, int32_t token) {
     if (a.query_starts.data == nullptr) {
         return token < a.batch ? token : -1;
     }
-    int32_t low = 0, high = a.batch;
-    while (high - low > 1) {
-        const int32_t mid = (low + high) >> 1;
-        if (first_token(a, mid) <= token) {
-            low = mid;
-        } else {
-            high = mid;
-        }
-    }
-    return a.batch > 0 && first_token(a, low) <= token && token < first_token(a, low + 1) ? low : -1;
+    const int32_t b = last_row_not_above(a.batch, token, [&](int32_t row) { return first_token(a, row); });
+    return b >= 0 && token < first_token(a, b + 1) ? b : -1;
 }
 
 __device__ __align__(256) const uint32_t no_key[64] = {};
@@ -126,6 +144,50 @@ __device__ __forceinline__ float over_quads_max(float x) {
     x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Eight elements of an index query as codes, by the lanes that have its row (kSteps * 8 of them): all of a wave call it.
+template <int kSteps>
+__device__ __forceinline__ float query_codes(const ScoreArgs& a, bool live, int64_t token, int32_t head, int piece,
+                                             uint32_t (&words)[2]) {
+    float x[8] = {};
+    float most = 0;
+    if (live && piece * 8 < a.dim) {
+        const u32x4 given = load_global<u32x4>(a.query + token * a.q_token + head * a.q_head + piece * 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint16_t bits = static_cast<uint16_t>(given[j >> 1] >> (16 * (j & 1)));
+            x[j] = a.f16 != 0 ? F16::value(bits) : Bf16::value(bits);
+            most = fmaxf(most, fabsf(x[j]));
+        }
+    }
+#pragma unroll
+    for (int step = 1; step < kSteps * 8; step *= 2) {
+        most = fmaxf(most, __shfl_xor(most, step));
+    }
+    const float scale = code_scale(most);
+    code_words(x, scale, words);
+    return scale;
+}
+
+// All queries as codes, once, where many workgroups would each make the same ones: their making was 40 % of the
+// instructions of a prompt's scores.
+template <int kSteps>
+__global__ __launch_bounds__(kThreads) void code_kernel(const ScoreArgs a) {
+    constexpr int kRowThreads = kSteps * 8;
+    const int64_t row = (int64_t{blockIdx.x} * kThreads + threadIdx.x) / kRowThreads;
+    const int piece = threadIdx.x % kRowThreads;
+    const bool live = row < int64_t{a.at.tokens} * a.groups * a.share;
+    const int32_t heads = a.groups * a.share;
+    const int64_t token = live ? row / heads : 0;
+    uint32_t words[2];
+    const float scale = query_codes<kSteps>(a, live, token, static_cast<int32_t>(row - token * heads), piece, words);
+    if (live) {
+        *reinterpret_cast<u32x2*>(a.codes + row * (kSteps * 64) + piece * 8) = u32x2{words[0], words[1]};
+        if (piece == 0) {
+            a.code_scales[row] = scale;
+        }
+    }
 }
 
 // Scores of a tile of rows (query heads of one batch row's tokens) against segments of its context. Keys down and rows
@@ -157,18 +219,10 @@ __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_
         const auto begin = [&](int32_t row) {
             return static_cast<int32_t>(int64_t{first_token(a.at, row)} * a.groups / a.pairs) + row;
         };
-        int32_t low = 0, high = a.at.batch;
-        while (high - low > 1) {
-            const int32_t mid = (low + high) >> 1;
-            if (begin(mid) <= tile) {
-                low = mid;
-            } else {
-                high = mid;
-            }
-        }
-        b = low, part = tile - begin(low);
+        b = __builtin_amdgcn_readfirstlane(last_row_not_above(a.at.batch, tile, begin));
+        part = b >= 0 ? tile - begin(b) : -1;
     }
-    if (b >= a.at.batch || part < 0) {
+    if (b < 0 || b >= a.at.batch || part < 0) {
         return;
     }
     const BatchRow row = batch_row(a.at, b);
@@ -184,57 +238,55 @@ __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_
         return;
     }
 
-    // Queries as codes.
-    {
+    i32x4 q[kTiles][kSteps];
+    float q_scale[kTiles];
+    int32_t sight[kTiles], pair_of[kTiles];        // of the lane's row of each 16; pair -1: no row
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+        const int32_t pair = a.share_div.div(m * 16 + col);
+        pair_of[m] = pair < pair_count ? pair : -1;
+        sight[m] = row.position + static_cast<int32_t>(a.group_div.div(pair_begin + max(pair_of[m], 0))) + 1;
+    }
+    if (a.codes != nullptr) {
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) {
+            const int r = m * 16 + col;
+            const int64_t at = (int64_t{row.first} * a.groups + pair_begin) * a.share + r;
+            const char* codes = pair_of[m] >= 0 ? a.codes + at * kRowBytes + quad * 16 : reinterpret_cast<const char*>(no_key);
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) {
+                q[m][c] = load_global<i32x4>(codes + (pair_of[m] >= 0 ? c * 64 : 0));
+            }
+            q_scale[m] = load_global<float>(pair_of[m] >= 0 ? reinterpret_cast<const char*>(a.code_scales + at)
+                                                            : reinterpret_cast<const char*>(no_key));
+        }
+    } else {
         constexpr int kRowThreads = kSteps * 8;
         const int piece = tid % kRowThreads;
         for (int r = tid / kRowThreads; r < kTiles * 16; r += kThreads / kRowThreads) {
-            const int32_t pair = a.share_div.div(r), inside = r - pair * a.share;
-            float x[8] = {};
-            float most = 0;
-            if (pair < pair_count && piece * 8 < a.dim) {
-                const int32_t all = pair_begin + pair, token = a.group_div.div(all);
-                const int32_t head = (all - token * a.groups) * a.share + inside;
-                const u32x4 given = load_global<u32x4>(
-                    a.query + int64_t{row.first + token} * a.q_token + head * a.q_head + piece * 16);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint16_t bits = static_cast<uint16_t>(given[j >> 1] >> (16 * (j & 1)));
-                    x[j] = a.f16 != 0 ? F16::value(bits) : Bf16::value(bits);
-                    most = fmaxf(most, fabsf(x[j]));
-                }
-            }
-#pragma unroll
-            for (int step = 1; step < kRowThreads; step *= 2) {
-                most = fmaxf(most, __shfl_xor(most, step));
-            }
-            const float scale = code_scale(most);
+            const int32_t pair = a.share_div.div(r), all = pair_begin + pair, token = a.group_div.div(all);
+            const int32_t head = (all - token * a.groups) * a.share + r - pair * a.share;
             uint32_t words[2];
-            code_words(x, scale, words);
+            const float scale = query_codes<kSteps>(a, pair < pair_count, row.first + token, head, piece, words);
             const int at = r * kRowBytes + (((piece >> 1) ^ (r & (kPieces - 1))) << 4) + (piece & 1) * 8;
             *reinterpret_cast<u32x2*>(s_data + at) = u32x2{words[0], words[1]};
             if (piece == 0) {
                 s_scale[r] = scale;
             }
         }
-    }
-    __syncthreads();
-    i32x4 q[kTiles][kSteps];
-    float q_scale[kTiles];
-    int32_t sight[kTiles], pair_of[kTiles];        // of the lane's row of each 16; pair -1: no row
+        __syncthreads();
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-        const int r = m * 16 + col;
+        for (int m = 0; m < kTiles; ++m) {
+            const int r = m * 16 + col;
 #pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-            q[m][c] = *reinterpret_cast<const i32x4*>(s_data + r * kRowBytes + (((c * 4 + quad) ^ (r & (kPieces - 1))) << 4));
+            for (int c = 0; c < kSteps; ++c) {
+                q[m][c] = *reinterpret_cast<const i32x4*>(s_data + r * kRowBytes +
+                                                          (((c * 4 + quad) ^ (r & (kPieces - 1))) << 4));
+            }
+            q_scale[m] = s_scale[r];
         }
-        q_scale[m] = s_scale[r];
-        const int32_t pair = a.share_div.div(r);
-        pair_of[m] = pair < pair_count ? pair : -1;
-        sight[m] = row.position + static_cast<int32_t>(a.group_div.div(pair_begin + max(pair_of[m], 0))) + 1;
+        lds_barrier();      // the keys come where the codes are
     }
-    __syncthreads();      // the keys come where the codes are
     const char* const table = a.tables + row.request * a.table_row;
     const char* const nothing = reinterpret_cast<const char*>(no_key);
     const int32_t block_tokens = a.block.divisor, blocks = a.block.div(last_seen - 1) + 1;   // of the context
@@ -244,7 +296,7 @@ __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_
         for (int i = tid; i < pair_count * held; i += kThreads) {
             s_score[i] = 0;
         }
-        __syncthreads();
+        lds_barrier();
         const int32_t begin = block_begin * block_tokens;
         // The context's last block may end early: every step begins at a token that somebody sees.
         const int32_t units = kShort
@@ -433,12 +485,12 @@ __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_
                 work(now, seen);
             }
         }
-        __syncthreads();
+        lds_barrier();
         for (int i = tid; i < pair_count * held; i += kThreads) {
             const int32_t pair = i / held, block = i - pair * held;
             a.scores[(int64_t{row.first} * a.groups + pair_begin + pair) * a.score_row + block_begin + block] = s_score[i];
         }
-        __syncthreads();
+        lds_barrier();
     }
 }
 
@@ -879,8 +931,12 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
 constexpr int64_t kMostTokens = 1 << 23, kMostBatch = 1 << 20, kMostGroups = 1024, kMostShare = 128,
                   kMostPairs = 1 << 22;      // a workgroup each, of 1024 threads: fewer than 2^32 threads
 
+// What the workspace keeps for the codes of a selection's queries: 1 KB of codes and a scale for each of up to 16 heads.
+constexpr int64_t kCodeRoom = 1024, kScaleRoom = 64;
+
 struct Plan {
     int64_t score_row = 0;
+    uint64_t codes = 0, scales = 0;      // places in the workspace, behind the scores
     uint64_t bytes = 0;
 };
 
@@ -900,7 +956,11 @@ Plan plan_of(int64_t tokens, int64_t groups, int64_t columns, int64_t page_size,
     }
     Plan p;
     p.score_row = std::max<int64_t>((columns * page_size + block_size - 1) / block_size, 1);
-    p.bytes = (static_cast<uint64_t>(tokens * groups) * static_cast<uint64_t>(p.score_row) * 4 + 255) / 256 * 256;
+    const auto aligned = [](uint64_t bytes) { return (bytes + 255) / 256 * 256; };
+    const uint64_t lists = static_cast<uint64_t>(tokens * groups);
+    p.codes = aligned(lists * static_cast<uint64_t>(p.score_row) * 4);
+    p.scales = p.codes + lists * kCodeRoom;
+    p.bytes = aligned(p.scales + lists * kScaleRoom);
     return p;
 }
 
@@ -1034,6 +1094,13 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     a.score_row = plan.score_row;
     const int64_t most_rows = std::min(s.max_query, tokens) * heads;
     int tiles16 = most_rows <= 16 ? 1 : (most_rows <= 32 ? 2 : (most_rows <= 64 ? 4 : 8));
+    // Tiles of 128 rows go over the keys half as often as tiles of 64 (19 instead of 25 vector instructions for 16 keys and
+    // 16 rows); where they make few workgroups, 64 rows fill the card better: six pieces of up to 1024 tokens of 4 heads
+    // behind 16384, 82 us with 128 rows and 78 with 64.
+    const int64_t capacity = std::max<int64_t>(a.at.own_most, 1);
+    if (tiles16 == 8 && tokens * heads * capacity < int64_t{1024} * 128 * 4096) {
+        tiles16 = 4;
+    }
     while (16 * tiles16 < a.share) {
         tiles16 *= 2;
     }
@@ -1051,8 +1118,8 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
                                                              : tokens * a.row_tiles);
     // Segments of at least 256 tokens, longer where the contexts make more workgroups than fill the card a few times over,
     // and as many blocks as there is room for keys.
-    const int64_t capacity = std::max<int64_t>(a.at.own_most, 1);
-    int64_t wanted = std::min<int64_t>(std::max<int64_t>(a.tiles * capacity / (tiles16 < 4 ? 8192 : 512), 256), 4096);
+    const int64_t workgroups = tiles16 < 4 ? 8192 : (tiles16 == 4 ? 2048 : 512);
+    int64_t wanted = std::min<int64_t>(std::max<int64_t>(a.tiles * capacity / workgroups, 256), 4096);
     int64_t segment_blocks = std::max<int64_t>(wanted / s.block_size, 1);
     segment_blocks = std::min<int64_t>(segment_blocks, kSegmentKeys / a.pairs);
     if (a.sub_shift >= 0) {
@@ -1066,6 +1133,19 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     a.segments = static_cast<int32_t>(segments);
     const uint32_t lds = static_cast<uint32_t>(a.pairs * segment_blocks * 4);
     const auto on = static_cast<hipStream_t>(stream);
+    // Codes made once, where the rows are many: below that a launch costs more than their making again and again.
+    const int steps = dim <= 64 ? 1 : (dim <= 128 ? 2 : 4);
+    if (tiles16 >= 4 && int64_t{a.share} * steps * 64 <= kCodeRoom && a.at.batch > 0) {
+        a.codes = static_cast<char*>(workspace) + plan.codes;
+        a.code_scales = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.scales);
+        const uint32_t grid = static_cast<uint32_t>((tokens * heads * steps * 8 + kThreads - 1) / kThreads);
+        switch (steps) {
+            case 1: code_kernel<1><<<grid, kThreads, 0, on>>>(a); break;
+            case 2: code_kernel<2><<<grid, kThreads, 0, on>>>(a); break;
+            default: code_kernel<4><<<grid, kThreads, 0, on>>>(a); break;
+        }
+        check_hip(hipGetLastError(), "launch index query codes");
+    }
     if (a.at.batch > 0) {
         const uint32_t grid = static_cast<uint32_t>(a.tiles * segments);
         if (dim <= 64) {
