@@ -214,18 +214,36 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
             }
         }
     };
-    read_batch(tid);
-    for (int i = tid; i < count * a.half; i += kThreads) {
-        const int token = i / a.half, pair = i - token * a.half;
-        const int64_t position = a.positions.fetch(first + token);
-        const CosSin cs = turned(static_cast<uint64_t>(position) * a.turns[pair]);
-        s_cos[token * kMostPairs + pair] = cs.cos * a.magnitude;
-        s_sin[token * kMostPairs + pair] = cs.sin * a.magnitude;
+    // Positions before rows: a wait for what was asked for later would be for the rows as well.
+    constexpr int kAngles = kMostTokens * kMostPairs / kThreads;
+    int32_t token_of[kAngles], pair_of[kAngles];
+    int64_t position[kAngles], mine = 0, slot = 0;
+    uint64_t turn[kAngles];
+#pragma unroll
+    for (int k = 0; k < kAngles; ++k) {
+        const int i = tid + k * kThreads;
+        if (i < count * a.half) {
+            token_of[k] = i / a.half, pair_of[k] = i - token_of[k] * a.half;
+            position[k] = a.positions.fetch(first + token_of[k]);
+            turn[k] = a.turns[pair_of[k]];
+        }
     }
     if (tid < count) {
-        const bool live = a.positions.fetch(first + tid) >= 0;
-        s_live[tid] = live;
-        s_row[tid] = live && a.kv_heads > 0 ? a.rows.offset(a.slots.fetch(first + tid)) : -1;
+        mine = a.positions.fetch(first + tid);
+        slot = a.kv_heads > 0 ? a.slots.fetch(first + tid) : -1;
+    }
+    read_batch(tid);
+#pragma unroll
+    for (int k = 0; k < kAngles; ++k) {
+        if (tid + k * kThreads < count * a.half) {
+            const CosSin cs = turned(static_cast<uint64_t>(position[k]) * turn[k]);
+            s_cos[token_of[k] * kMostPairs + pair_of[k]] = cs.cos * a.magnitude;
+            s_sin[token_of[k] * kMostPairs + pair_of[k]] = cs.sin * a.magnitude;
+        }
+    }
+    if (tid < count) {
+        s_live[tid] = mine >= 0;
+        s_row[tid] = mine >= 0 && a.kv_heads > 0 ? a.rows.offset(slot) : -1;
     }
     lds_barrier();
     for (int32_t base = tid; base < units; base += kBatch * kThreads) {
