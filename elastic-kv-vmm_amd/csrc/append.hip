@@ -408,9 +408,7 @@ int append_rotary(const ekv_append_args& s, void* stream) {
         a.query = rows_of(query);
         a.out = static_cast<char*>(out.data);
         a.o_token = out.stride[0] * 2, a.o_head = out.stride[1] * 2;
-        if ((out.shape[0] > 1 && out.stride[0] == 0) || (out.shape[1] > 1 && out.stride[1] == 0)) {
-            throw std::invalid_argument("output must not repeat its elements");
-        }
+        need_distinct(out, "output");
         const Extent o(&out);
         if (!same_view(query, out)) {
             need_apart(o, "output", Extent(&query), "query, unless it is the query");
@@ -428,6 +426,7 @@ int append_rotary(const ekv_append_args& s, void* stream) {
         a.slots = index_ref(slots, 0);
         const int64_t row = a.kv_heads * dim * 2;
         const PlanePages p = plane_pages(s.planes, s.layer, row, s.page_size, 2);
+        need_distinct_rows(*s.planes);
         a.rows = slot_rows(p, s.page_size, s.planes->rows, s.planes->row_bytes == row, s.zero_below);
         a.plane = p.at;
         a.kv_stride = p.kv_stride;
@@ -528,9 +527,8 @@ int append_index(const ekv_tensor* key_p, const ekv_planes* planes, int64_t laye
         throw std::invalid_argument("scales must have an element for each of the pool's " +
                                     std::to_string(a.rows.slots) + " slots, got " + std::to_string(scales.shape[0]));
     }
-    if (scales.shape[0] > 1 && scales.stride[0] == 0) {
-        throw std::invalid_argument("scales must not repeat their elements");
-    }
+    need_distinct(scales, "scales");
+    need_distinct_rows(*planes);
     const Extent plane(p, *planes, 0), scale_extent(&scales);
     need_apart(Extent(&key), "index_key", plane, "the layer's plane");
     need_apart(Extent(&slots), "slots", plane, "the layer's plane");

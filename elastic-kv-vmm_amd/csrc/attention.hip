@@ -720,6 +720,30 @@ int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t
     lists.block = FastDiv(static_cast<uint32_t>(s.block_size));
     lists.heads = FastDiv(static_cast<uint32_t>(a.kv_heads / blocks.shape[1]));
     lists.width = static_cast<int32_t>(blocks.shape[2]);
+    need_distinct(*s.output, "output");
+    if (!same_view(*s.query, *s.output)) {
+        need_apart(Extent(s.output), "output", Extent(s.query), "query, unless it is the query");
+    }
+    const PlanePages pages = plane_pages(s.planes, s.layer, int64_t{a.kv_heads} * a.dim * 2, s.page_size, 2);
+    const Extent planes[2] = {Extent(pages, *s.planes, 0), Extent(pages, *s.planes, 1)};
+    const auto apart = [&](const ekv_tensor* t, const char* name) {
+        const Extent e(t);
+        for (const Extent& plane : planes) {
+            need_apart(e, name, plane, "the layer's planes");
+        }
+        need_apart(e, name, Extent(s.block_tables), "block_tables");
+        need_apart(e, name, Extent(s.rows), "rows");
+        need_apart(e, name, Extent(s.lengths), "lengths");
+        need_apart(e, name, Extent(&blocks), "blocks");
+        need_apart(e, name, Extent(s.query_starts), "query_starts");
+    };
+    apart(s.output, "output");
+    if (s.lse != nullptr) {
+        need_distinct(*s.lse, "lse");
+        apart(s.lse, "lse");
+        need_apart(Extent(s.lse), "lse", Extent(s.query), "query");
+        need_apart(Extent(s.lse), "lse", Extent(s.output), "output");
+    }
     if (s.query_starts != nullptr && union_pays(a, lists, s.block_size, s.max_query, plan.own.dim_pad)) {
         need_workspace(plan, workspace, workspace_bytes);
         if (a.tokens > 0) {

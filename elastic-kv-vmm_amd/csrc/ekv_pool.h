@@ -6,7 +6,10 @@
 #include "ekv_tensor_util.h"
 
 #include <algorithm>
+#include <array>
+#include <cstdlib>
 #include <numeric>
+#include <utility>
 
 namespace ekv {
 
@@ -171,6 +174,32 @@ struct Extent {
 inline void need_apart(const Extent& a, const char* name, const Extent& b, const char* other) {
     if (a.meets(b)) {
         throw std::invalid_argument(std::string(name) + " must not share memory with " + other);
+    }
+}
+
+// An output whose elements are all different: every dimension steps over the whole of those with smaller strides.
+inline void need_distinct(const ekv_tensor& t, const char* name) {
+    std::array<std::pair<int64_t, int64_t>, 4> dims;      // stride, extent
+    int count = 0;
+    for (int i = 0; i < t.ndim; ++i) {
+        if (t.shape[i] > 1) {
+            dims[count++] = {std::abs(t.stride[i]), t.shape[i]};
+        }
+    }
+    std::sort(dims.begin(), dims.begin() + count);
+    int64_t reach = 0;
+    for (int i = 0; i < count && numel(t) > 0; ++i) {
+        if (dims[i].first <= reach) {
+            throw std::invalid_argument(std::string(name) + " must not repeat its elements");
+        }
+        reach += (dims[i].second - 1) * dims[i].first;
+    }
+}
+
+// Rows of a plane that are written: no two share a byte.
+inline void need_distinct_rows(const ekv_planes& planes) {
+    if (planes.rows > 1 && planes.row_stride < planes.row_bytes) {
+        throw std::invalid_argument("plane rows must not overlap");
     }
 }
 

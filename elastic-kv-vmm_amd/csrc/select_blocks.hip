@@ -997,11 +997,7 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     if (blocks.dtype != EKV_INT32) {
         throw std::invalid_argument("blocks must be int32");
     }
-    for (int d = 0; d < 3; ++d) {
-        if (blocks.shape[d] > 1 && blocks.stride[d] == 0) {
-            throw std::invalid_argument("blocks must not repeat its elements");
-        }
-    }
+    need_distinct(blocks, "blocks");
     const int64_t groups = blocks.shape[1], chosen = blocks.shape[2];
     if (groups < 1 || groups > kMostGroups || heads < 1 || heads % groups != 0 || heads / groups > kMostShare) {
         throw std::invalid_argument("blocks must have a divisor of the index heads as groups, at most 1024 of at most "
