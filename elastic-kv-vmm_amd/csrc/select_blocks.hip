@@ -673,19 +673,18 @@ __global__ __launch_bounds__(kWaves == 1 ? kThreads : kWaves * 64) void pick_ker
 
 constexpr int kManyWaves = 16, kManyThreads = kManyWaves * 64;
 constexpr int kDigit = 11, kBins = 1 << kDigit;
-constexpr int kFew = 1024;                    // keys that one wave looks through
+constexpr int kFew = 256;                     // keys that are compared with each other
 
 // The same for many blocks. The range of the scores in 2047 equal parts, the keys counted in them, the part that holds
-// the K-th largest; its keys, few as a rule, to one wave, which finds the K-th largest bit by bit. (Parts of the range,
-// not leading bits: those are the exponent, and most scores have one of few.) Where a part holds more than kFew, what is
-// left is decided in digits of 11 bits of the key. kRegs: a lane's keys in registers; 0: any number of keys, read again
-// each time.
+// the K-th largest; its keys, few as a rule, are compared with each other. (Parts of the range, not leading bits: those
+// are the exponent, and most scores have one of few.) Where a part holds more than kFew, what is left is decided in digits
+// of 11 bits of the key. kRegs: a lane's keys in registers; 0: any number of keys, read again each time.
 //
 // What bounds it: a workgroup's instructions, some 30 a key in passes over all keys; rows are few where they are long.
 template <int kRegs>
 __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs a) {
     __shared__ uint32_t s_bins[kBins];
-    __shared__ uint32_t s_few[kFew];
+    __shared__ __align__(16) uint32_t s_few[kFew];
     __shared__ uint32_t s_cells[2][kManyWaves];
     __shared__ uint32_t s_found[3];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -795,6 +794,7 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
     };
     uint32_t from = 1, to = kForced, among = kFew + 1;       // the K-th largest is the wanted-th of `among` from .. to
     bool there = true;
+    uint32_t bound = 0;                                      // all there are
     const float low = score_of(least), scale = (kBins - 2) / (score_of(most) - low);
     if (least < most && scale > 0 && scale < INFINITY) {
         // Parts 1 .. kBins - 1.
@@ -803,7 +803,41 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
         };
         uint32_t bin = 0;
         there = find([&](uint32_t key) { return key != 0 ? part(key) : -1; }, bin, among);
-        if (there) {
+        if (there && among <= kFew) {
+            // Each of them to a thread, which counts the larger ones.
+            if (tid < kFew) {
+                s_few[tid] = 0;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                s_found[0] = 0;
+            }
+            __syncthreads();
+            for_keys([&](int, uint32_t key) {
+                if (key != 0 && part(key) == static_cast<int>(bin)) {
+                    s_few[atomicAdd(&s_found[0], 1u)] = key;
+                }
+            });
+            __syncthreads();
+            if (tid < among) {
+                const uint32_t mine = s_few[tid];
+                uint32_t larger = 0, alike = 0;
+                for (uint32_t i = 0; i < among; i += 4) {
+                    const u32x4 some = *reinterpret_cast<const u32x4*>(s_few + i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        larger += some[e] > mine, alike += some[e] == mine;
+                    }
+                }
+                if (larger < wanted && wanted <= larger + alike) {
+                    s_found[1] = mine, s_found[2] = larger;
+                }
+            }
+            __syncthreads();
+            bound = s_found[1];
+            wanted -= s_found[2];
+        }
+        if (there && among > kFew) {
             // Its first and last key, by trying 64 keys at a time.
             const auto first_of = [&](int wanted_part) {
                 uint32_t below = 0, above = kForced + 1;         // the first key lies above `below`, not above `above`
@@ -819,56 +853,7 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
             from = first_of(bin), to = first_of(bin + 1) - 1;
         }
     }
-    uint32_t bound = 0;                               // all there are
-    if (there && among <= kFew) {
-        __syncthreads();
-        if (tid == 0) {
-            s_found[0] = 0;
-        }
-        __syncthreads();
-        for_keys([&](int, uint32_t key) {
-            if (key >= from && key <= to) {
-                const uint32_t i = atomicAdd(&s_found[0], 1u);
-                if (i < kFew) {
-                    s_few[i] = key;
-                }
-            }
-        });
-        __syncthreads();
-        if (wave == 0) {
-            uint32_t few[kFew / 64];
-#pragma unroll
-            for (int r = 0; r < kFew / 64; ++r) {
-                const uint32_t i = r * 64 + lane;
-                few[r] = i < among ? s_few[i] : 0u;
-            }
-            const uint32_t differ = from ^ to;
-            const int bits = differ != 0 ? 32 - __builtin_clz(differ) : 0;
-            uint32_t found = bits >= 32 ? 0u : (from >> bits) << bits;
-            for (int bit = bits - 1; bit >= 0; --bit) {
-                const uint32_t tried = found | (1u << bit);
-                uint32_t n = 0;
-#pragma unroll
-                for (int r = 0; r < kFew / 64; ++r) {
-                    if (r * 64 < among) {
-                        n += __popcll(__ballot(few[r] >= tried));
-                    }
-                }
-                found = n >= wanted ? tried : found;
-            }
-            uint32_t larger = 0;
-#pragma unroll
-            for (int r = 0; r < kFew / 64; ++r) {
-                larger += __popcll(__ballot(few[r] > found));
-            }
-            if (lane == 0) {
-                s_found[0] = found, s_found[1] = larger;
-            }
-        }
-        __syncthreads();
-        bound = s_found[0];
-        wanted -= s_found[1];
-    } else if (there) {
+    if (there && among > kFew) {
         const uint32_t differ = from ^ to;
         int bits = differ != 0 ? 32 - __builtin_clz(differ) : 0;
         bound = bits >= 32 ? 0u : (from >> bits) << bits;
