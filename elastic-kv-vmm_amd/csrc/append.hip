@@ -112,7 +112,8 @@ __device__ __forceinline__ void store_piece(char* at, const Piece<kWidth>& p) {
 // that are only copied, two by two; where neighbours are pairs, pieces 2 i and 2 i + 1.
 //
 // What bounds it: the rows from and to HBM, and for a decode step the chain position -> angle -> store. Sines and cosines
-// are computed once a token for all heads and shared through LDS.
+// are computed once a token for all heads and shared through LDS. 25 thousand tokens of 48 heads of 128, 0.62 GB read and
+// written, take 122 us, 5.1 TB/s (129 when the first rows were asked for behind the angles); 128 tokens 4.0 us.
 template <typename T, int kWidth, bool kNeighbours>
 __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
     __shared__ __align__(16) float s_cos[kMostTokens * kMostPairs], s_sin[kMostTokens * kMostPairs];
@@ -270,7 +271,8 @@ struct IndexArgs {
     int32_t tokens, pieces;           // pieces of 8 elements of a key
 };
 
-// kLanes lanes a token, 8 elements each.
+// kLanes lanes a token, 8 elements each: a row's largest magnitude without LDS. What bounds it: a launch, at the sizes that
+// there are: 128 tokens of 128 take 2.5 us, 12 thousand, 4.6 MB read and written, 8.
 template <typename T, int kLanes>
 __global__ __launch_bounds__(kThreads) void index_kernel(const IndexArgs a) {
     const int64_t token = (int64_t{blockIdx.x} * kThreads + threadIdx.x) / kLanes;

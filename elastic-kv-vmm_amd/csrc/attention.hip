@@ -690,13 +690,19 @@ int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64
     return launch(a, plan, query->dtype, workspace, workspace_bytes, stream);
 }
 
-// Whether query tokens go through their lists together.
+// Whether query tokens go through their lists together: where batch rows fill tiles of 64 rows, and where the kernel for few
+// rows would have so many (token, KV head) pairs that its time passes that of a workgroup's blocks one after the other.
+// Lists of 16 blocks of 64 behind 16384 tokens, neighbours' alike, together and one by one: 16 heads on 2 of 128, four
+// pieces of 256 tokens 78 and 141 us, eight of 64 (1024 pairs) 76 and 76, one of 256 83 and 41; 32 heads on 4 of 128,
+// eight of 64 80 and 142, eight of 32 78 and 76; 8 heads on 8 of 64, eight of 64 (4096 pairs of half the bytes) 67 and 149,
+// eight of 32 67 and 87. The host cannot see whether they are alike: random lists take 178 and 144, 188 and 84, 181 and
+// 42; 219 and 154, 179 and 83; 328 and 154, 288 and 90.
 bool union_pays(const AttentionArgs& a, const BlockLists& lists, int64_t block_size, int64_t max_query, int32_t dim_pad) {
     const int64_t tile_tokens = std::min<int64_t>(64, 63 / a.share + 2);
     const bool fits = dim_pad <= 128 && block_size % 32 == 0 && tile_tokens * lists.width <= kUnionEntries &&
                       a.block_most / block_size < kUnionBlocks &&
                       (int64_t{a.tokens} * a.share / 64 + a.batch) * a.kv_heads < 1 << 24;   // fewer than 2^32 threads
-    return fits && a.share <= 32 && max_query * a.share >= 64 && int64_t{a.tokens} * a.share * a.kv_heads >= 64 * 128;
+    return fits && a.share <= 32 && max_query * a.share >= 64 && int64_t{a.tokens} * a.kv_heads * dim_pad >= 2048 * 128;
 }
 
 int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t workspace_bytes, void* stream) {

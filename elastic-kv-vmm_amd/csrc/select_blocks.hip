@@ -7,7 +7,8 @@
 // terms nor its conversion rounds: scores have no freedom, and a selection is the same wherever it is made. Queries are
 // rounded to codes here, as append.hip rounds keys.
 //
-// Two launches: scores of all blocks as ordered 32-bit keys into the workspace, then each (token, group)'s largest.
+// Two launches: scores of all blocks as ordered 32-bit keys into the workspace, then each (token, group)'s largest. Before
+// them, for many query rows, one that makes the queries' codes.
 #include "ekv_codes.h"
 #include "ekv_device.h"
 #include "ekv_memory.h"
@@ -191,8 +192,15 @@ __global__ __launch_bounds__(kThreads) void code_kernel(const ScoreArgs a) {
 }
 
 // Scores of a tile of rows (query heads of one batch row's tokens) against segments of its context. Keys down and rows
-// across in 16x16x64 products, every wave with keys of its own straight from memory, the tile's queries in its registers.
-// kShort: blocks of 2^sub_shift tokens, several a step.
+// across in 16x16x64 products, the tile's queries in registers, every wave with keys of its own: whole rows into registers
+// while the keys before them are worked on, through LDS to the lanes that the products want. kShort: blocks of
+// 2^sub_shift tokens, several a step.
+//
+// What bounds it: with few rows the reading. 5.2 million keys of 128 and their scales, 0.69 GB, of 128 requests of up to
+// 65536 tokens take 130 us, 5.3 TB/s (lanes that read the products' way, 64 bytes of 16 rows, read each 128-byte line
+// twice: 212). With many rows the instructions on the products, 19 for 16 keys and 16 rows: six pieces of up to 1024
+// tokens of 4 heads behind 16384 take 71 us, 0.78 * 10^15 operations a second. Lists of tokens take longest for their
+// bytes, a maximum in LDS for each key: 24 requests of up to 40000 tokens, 42 MB, 18 us.
 template <int kSteps, int kTiles, bool kShort>
 __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_kernel(const ScoreArgs a) {
     constexpr int kRowBytes = kSteps * 64, kPieces = kSteps * 4;
@@ -559,7 +567,7 @@ __device__ __forceinline__ Candidates candidates_of(const PickArgs& a, int64_t p
 // first of those equal to it, in order of their blocks. The bits that all keys share in front are skipped.
 //
 // What bounds it: the reads of the keys and the steps one after the other: kRegs comparisons and, between waves, a barrier
-// a bit.
+// a bit. 256 lists of up to 1024 blocks take 9.5 us, 4 lists of 64 3.5.
 template <int kWaves, int kRegs>
 __global__ __launch_bounds__(kWaves == 1 ? kThreads : kWaves * 64) void pick_kernel(const PickArgs a) {
     constexpr int kCells = kWaves == 1 ? 1 : kWaves;
@@ -680,7 +688,9 @@ constexpr int kFew = 256;                     // keys that are compared with eac
 // are the exponent, and most scores have one of few.) Where a part holds more than kFew, what is left is decided in digits
 // of 11 bits of the key. kRegs: a lane's keys in registers; 0: any number of keys, read again each time.
 //
-// What bounds it: a workgroup's instructions, some 30 a key in passes over all keys; rows are few where they are long.
+// What bounds it: one compute unit has a list. 24 lists of 2048 out of up to 40000 tokens take 24 us: 6 for reading a
+// list's 160 KB, 4 for counting, 4 for the few, 6 for counting those above and writing them, the rest in the steps between.
+// (The K-th largest bit by bit from all keys took 94 us, by digits of 11 bits 49.)
 template <int kRegs>
 __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs a) {
     __shared__ uint32_t s_bins[kBins];
@@ -1074,14 +1084,10 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     a.scores = static_cast<uint32_t*>(workspace);
     a.score_row = plan.score_row;
     const int64_t most_rows = std::min(s.max_query, tokens) * heads;
+    // Row tiles of 16, 32, 64 and 128: calls of 4 heads of 128 for 32 requests of up to 16384 tokens take, with 4 query
+    // tokens each, 26, 27, 30 and 31 us, with 8 tokens 39, 30, 30 and 32, with 16 tokens 57, 44, 31 and 36, four pieces
+    // of 1024 tokens behind 8192 87, 79, 53 and 44.
     int tiles16 = most_rows <= 16 ? 1 : (most_rows <= 32 ? 2 : (most_rows <= 64 ? 4 : 8));
-    // Tiles of 128 rows go over the keys half as often as tiles of 64 (19 instead of 25 vector instructions for 16 keys and
-    // 16 rows); where they make few workgroups, 64 rows fill the card better: six pieces of up to 1024 tokens of 4 heads
-    // behind 16384, 82 us with 128 rows and 78 with 64.
-    const int64_t capacity = std::max<int64_t>(a.at.own_most, 1);
-    if (tiles16 == 8 && tokens * heads * capacity < int64_t{1024} * 128 * 4096) {
-        tiles16 = 4;
-    }
     while (16 * tiles16 < a.share) {
         tiles16 *= 2;
     }
@@ -1097,10 +1103,15 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     a.row_tiles = (a.groups + a.pairs - 1) / a.pairs;
     a.tiles = static_cast<int32_t>(s.query_starts != nullptr ? tokens * groups / a.pairs + a.at.batch
                                                              : tokens * a.row_tiles);
-    // Segments of at least 256 tokens, longer where the contexts make more workgroups than fill the card a few times over,
-    // and as many blocks as there is room for keys.
+    // Segments of 256 tokens, of 512 where those fill the card twice, and longer where the contexts make more workgroups
+    // than fill it a few times over (one for long tiles, whose start costs most); as many blocks as there is room for keys.
+    // By 256, 512, 1024, 2048 and 4096 tokens: one query token of 4 heads for 4 requests of 8192 tokens 10, 11, 13, 17 and
+    // 25 us, for 32 of 16384 26, 22, 23, 24 and 30, of 8 heads for 128 of 65536 181, 143, 138, 141 and 145; six pieces
+    // of 600 behind 16384 126, 89, 77, 75 and 72 (by this rule 67), four of 1024 behind 8192 77, 57, 50, 44 and 66.
+    const int64_t capacity = std::max<int64_t>(a.at.own_most, 1);
     const int64_t workgroups = tiles16 < 4 ? 8192 : (tiles16 == 4 ? 2048 : 512);
-    int64_t wanted = std::min<int64_t>(std::max<int64_t>(a.tiles * capacity / workgroups, 256), 4096);
+    const int64_t least = a.tiles * capacity / 512 >= 512 ? 512 : 256;
+    const int64_t wanted = std::min<int64_t>(std::max<int64_t>(a.tiles * capacity / workgroups, least), 4096);
     int64_t segment_blocks = std::max<int64_t>(wanted / s.block_size, 1);
     segment_blocks = std::min<int64_t>(segment_blocks, kSegmentKeys / a.pairs);
     if (a.sub_shift >= 0) {
@@ -1114,7 +1125,9 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     a.segments = static_cast<int32_t>(segments);
     const uint32_t lds = static_cast<uint32_t>(a.pairs * segment_blocks * 4);
     const auto on = static_cast<hipStream_t>(stream);
-    // Codes made once, where the rows are many: below that a launch costs more than their making again and again.
+    // Codes made once, by a launch of its own, where the rows are many: four pieces of 256 tokens of 4 heads behind 8192
+    // take 33 instead of 38 us, 32 requests' 16 tokens each behind 16384 31 instead of 33. With few rows there is no
+    // difference: 128 requests of one token behind 32768 take 87 and 88, 32 requests of 4 tokens 27 and 27.
     const int steps = dim <= 64 ? 1 : (dim <= 128 ? 2 : 4);
     if (tiles16 >= 4 && int64_t{a.share} * steps * 64 <= kCodeRoom && a.at.batch > 0) {
         a.codes = static_cast<char*>(workspace) + plan.codes;
@@ -1147,9 +1160,11 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     k.blocks = static_cast<int32_t*>(blocks.data);
     k.b_token = blocks.stride[0], k.b_group = blocks.stride[1], k.b_column = blocks.stride[2];
     const uint32_t pairs = static_cast<uint32_t>(tokens * groups), grid = (pairs + kThreads / 64 - 1) / (kThreads / 64);
-    if (plan.score_row <= 64) {
-        pick_kernel<1, 1><<<grid, kThreads, 0, on>>>(k);
-    } else if (plan.score_row <= 256) {
+    // By a wave, by four, by sixteen, the last with keys in registers or read again each time. 4096 lists of the 256
+    // blocks of 16384 tokens, a whole call: 94 us by a wave and 110 by four (8 lists: 11 and 14); of 2048 blocks 132 by
+    // four and 205 by sixteen (8 lists: 16 and 15); of 16384 tokens 367 with 16 registers, 413 with 64 (8 lists: 19 and
+    // 21); 8 lists of 65536 tokens 43 with 64 registers and 95 without.
+    if (plan.score_row <= 256) {
         pick_kernel<1, 4><<<grid, kThreads, 0, on>>>(k);
     } else if (plan.score_row <= 2048) {
         pick_kernel<4, 8><<<pairs, 256, 0, on>>>(k);
