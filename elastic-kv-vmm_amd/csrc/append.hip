@@ -272,7 +272,7 @@ struct IndexArgs {
 };
 
 // kLanes lanes a token, 8 elements each: a row's largest magnitude without LDS. What bounds it: a launch, at the sizes that
-// there are: 128 tokens of 128 take 2.5 us, 12 thousand, 4.6 MB read and written, 8.
+// there are: 128 tokens of 64 take 2.5 us, 50 thousand of 128, 19 MB read and written, 8.
 template <typename T, int kLanes>
 __global__ __launch_bounds__(kThreads) void index_kernel(const IndexArgs a) {
     const int64_t token = (int64_t{blockIdx.x} * kThreads + threadIdx.x) / kLanes;
@@ -464,7 +464,7 @@ int append_rotary(const ekv_append_args& s, void* stream) {
     const int64_t head_units = (a.pieces + 1) / 2, units = head_units * (a.q_heads + 2 * int64_t{a.kv_heads});
     a.head_units = FastDiv(static_cast<uint32_t>(head_units));
     a.token_units = FastDiv(static_cast<uint32_t>(units));
-    // A workgroup takes one token while there are few, so that more of them share the reads: four prompts' 25 thousand
+    // A workgroup takes one token while there are few, so that more of them share the reads: eight prompts' 25 thousand
     // tokens of 48 heads take 122 us by four, 121 by two and 133 by one, 2549 of 20 heads of 80 7.5, 8.5 and 10.4.
     a.each = tokens <= 1024 ? 1 : kMostTokens;
     const auto on = static_cast<hipStream_t>(stream);
