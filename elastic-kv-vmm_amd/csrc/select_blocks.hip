@@ -924,7 +924,7 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
 // ---------------------------------------------------------------- host
 
 constexpr int64_t kMostTokens = 1 << 23, kMostBatch = 1 << 20, kMostGroups = 1024, kMostShare = 128,
-                  kMostPairs = 1 << 22;      // a workgroup each, of 1024 threads: fewer than 2^32 threads
+                  kMostPairs = (1 << 22) - 1;      // a workgroup each, of 1024 threads: fewer than 2^32 threads
 
 // What the workspace keeps for the codes of a selection's queries: 1 KB of codes and a scale for each of up to 16 heads.
 constexpr int64_t kCodeRoom = 1024, kScaleRoom = 64;
@@ -947,7 +947,7 @@ Plan plan_of(int64_t tokens, int64_t groups, int64_t columns, int64_t page_size,
         throw std::invalid_argument("block_size must be from 1 to 2^30");
     }
     if (tokens * groups > kMostPairs) {
-        throw std::invalid_argument("more than 2^22 selections");
+        throw std::invalid_argument("more than 2^22 - 1 selections");
     }
     Plan p;
     p.score_row = std::max<int64_t>((columns * page_size + block_size - 1) / block_size, 1);

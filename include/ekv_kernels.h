@@ -676,7 +676,7 @@ uint64_t ekv_select_workspace_bytes(int64_t tokens, int64_t groups, int64_t colu
  * `first`, and the last `last` up to the position's own, are chosen whatever
  * their scores. Ties go to the lower block. A list is in ascending order, -1
  * behind its last block; the lists of tokens of no batch row are all -1.
- * At most 128 heads a group; N * G <= 2^22. workspace: 256-byte aligned device
+ * At most 128 heads a group; N * G < 2^22. workspace: 256-byte aligned device
  * memory of ekv_select_workspace_bytes, its contents of no account; calls that
  * overlap need one each. Two or three launches, no memset: it can be captured.
  * Replaces: the block scores that the reference's engine hands to

@@ -305,7 +305,7 @@ def test_no_selections_are_no_launch(lib):  # noqa: F811
 
 @pytest.mark.parametrize("sizes", [(-1, 2, 9, 16, 64), (5, 0, 9, 16, 64), (5, 1025, 9, 16, 64), (5, 2, -1, 16, 64),
                                    (5, 2, 9, 0, 64), (5, 2, 9, 16, 0), (5, 2, 1 << 26, 16, 64), (5, 2, 1, 1 << 31, 64),
-                                   ((1 << 22) + 1, 1, 9, 16, 64), (1 << 20, 8, 9, 16, 64), (1 << 62, 2, 9, 16, 64)])
+                                   (1 << 22, 1, 9, 16, 64), (1 << 20, 8, 9, 16, 64), (1 << 62, 2, 9, 16, 64)])
 def test_selection_workspaces_that_cannot_be(lib, sizes):  # noqa: F811
     from adaptive_sparse.block_selection import selection_workspace
 
@@ -321,7 +321,7 @@ def test_selection_workspaces_hold_a_score_for_each_block(lib):  # noqa: F811
         lists = tokens * groups
         assert selection_workspace(tokens, groups, columns, page, block) >= lists * -(-columns * page // block) * 4
     # The largest that the sizes allow is held in 64 bits.
-    assert selection_workspace(1 << 22, 1, (1 << 30) - 1, 1, 1) > 1 << 53
+    assert selection_workspace((1 << 22) - 1, 1, (1 << 30) - 1, 1, 1) > 1 << 53
 
 
 def blocks_call(lib, workspace=0, size=0, **changes):  # noqa: F811
