@@ -1,6 +1,7 @@
 """block_attention of prompts, whose neighbouring tokens go through their lists together: against a 64-bit answer.
 
-All calls here have more query rows than the rule for that asks for (8192, and 64 of a batch row).
+All calls here have as many query rows and heads as the rule for that asks for: 64 rows of a batch row, and 2048 pairs
+of a token and a KV head of 128, or more of smaller ones.
 """
 
 import math
@@ -18,9 +19,17 @@ pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
 
 
+ENOUGH = 2048 * 128
+
+
+def padded(dim):
+    return 64 if dim <= 64 else 96 if dim <= 96 else 128
+
+
 def run(problem, **extra):
-    rows = problem.query.shape[0] * problem.query.shape[1]
-    assert rows >= 8192 and max(problem.batch.counts) * problem.query.shape[1] // problem.pool.keys.shape[2] >= 64
+    tokens, heads, dim = problem.query.shape
+    kv_heads = problem.pool.keys.shape[2]
+    assert max(problem.batch.counts) * heads // kv_heads >= 64 and tokens * kv_heads * padded(dim) >= ENOUGH
     out = torch.full_like(problem.query, 7.0)
     lse = torch.full(out.shape[:2], 7.0, device=out.device)
     problem.call(block_attention, out, lse, **extra)
@@ -41,11 +50,12 @@ CASES = [
 ]
 
 
-@pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("together", [False, True])
+@pytest.mark.parametrize("dtype,together", [(BF16, True), (F16, False)])
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
 def test_prompts(gpu, dtype, together, case):
     heads, kv_heads, dim, page, layout, lengths, counts, block, chosen, lists = case
+    times = -(-ENOUGH // (sum(counts) * kv_heads * padded(dim)))
+    lengths, counts = lengths * times, counts * times
     print(f"[blocks] {case} {dtype} {together}", flush=True)
     problem = make_block_problem(gpu, dtype=dtype, heads=heads, kv_heads=kv_heads, dim=dim, page=page, layout=layout,
                                  lengths=lengths, counts=counts, block=block, chosen=chosen, lists=lists,
@@ -57,13 +67,13 @@ def test_prompts(gpu, dtype, together, case):
 
 
 def test_empty_lists_tokens_of_no_row_and_requests_that_are_not(gpu):
-    problem = make_block_problem(gpu, heads=64, kv_heads=4, lengths=[300, 0, 450, 200], counts=[90, 0, 3, 42], tail=3,
-                                 lists=2, seed=1, together=True)
+    problem = make_block_problem(gpu, heads=64, kv_heads=4, lengths=[300] * 5 + [0, 450, 200],
+                                 counts=[95] * 5 + [0, 3, 42], tail=3, lists=2, seed=1, together=True)
     problem.blocks[3] = -1
     problem.blocks[5, 1] = 1000                       # behind the position
     problem.batch.rows = problem.batch.rows.clone()
-    problem.batch.rows[3] = 9
-    for most in (90, 5000):
+    problem.batch.rows[7] = 9
+    for most in (95, 5000):
         out, lse = run(problem, max_query=most)
         check(out, lse, problem.answer(), 128)
         assert not bool(out[-45:].any()) and bool((lse[-45:] == -math.inf).all())
@@ -71,22 +81,22 @@ def test_empty_lists_tokens_of_no_row_and_requests_that_are_not(gpu):
 
 
 def test_bad_pages_and_a_length_past_the_table(gpu):
-    problem = make_block_problem(gpu, heads=64, kv_heads=4, lengths=[640], counts=[140], chosen=10, block=32, seed=3,
-                                 together=True)
+    problem = make_block_problem(gpu, heads=64, kv_heads=4, lengths=[640] * 4, counts=[140] * 4, chosen=10, block=32,
+                                 seed=3, together=True)
     place = int(problem.batch.rows[0])
     tables = problem.batch.tables
     tables[place, 0:2], tables[place, 5], tables[place, 39] = 0, problem.batch.pages, -3
     problem.blocks[7, 0] = torch.arange(10, device=gpu)
     out, lse = run(problem)
     check(out, lse, problem.answer(), 128)
-    problem.batch.lengths = [700]                     # more than the table covers
+    problem.batch.lengths = [700] * 4                 # more than the table covers
     out, lse = run(problem)
     check(out, lse, problem.answer(), 128)
 
 
 def test_what_is_not_seen_may_be_anything(gpu):
-    problem = make_block_problem(gpu, heads=64, kv_heads=2, lengths=[300, 77], counts=[140, 2], block=64, chosen=3,
-                                 lists=2, seed=4, together=True)
+    problem = make_block_problem(gpu, heads=64, kv_heads=2, lengths=[300] * 8 + [77], counts=[140] * 8 + [2], block=64,
+                                 chosen=3, lists=2, seed=4, together=True)
     want = problem.answer()
     keys, values = problem.pool.keys, problem.pool.values
     used = torch.zeros(keys.shape[:2], dtype=torch.bool, device=gpu)
@@ -104,7 +114,7 @@ def test_what_is_not_seen_may_be_anything(gpu):
 def test_infinities_reach_the_tokens_that_see_them(gpu, dim):
     """Key i of a row's last tokens has an infinity in column i of V: token i sees its own and earlier ones it lists."""
     count, length, heads = 64, 256, 128
-    problem = make_block_problem(gpu, heads=heads, kv_heads=8, dim=dim, lengths=[length], counts=[count], block=32,
+    problem = make_block_problem(gpu, heads=heads, kv_heads=64, dim=dim, lengths=[length], counts=[count], block=32,
                                  chosen=3, seed=5)
     problem.query = problem.query * 0.25
     listed = torch.tensor([[0, 6, 7]] * count, dtype=torch.int32, device=gpu).unsqueeze(1)
@@ -125,8 +135,8 @@ def test_infinities_reach_the_tokens_that_see_them(gpu, dim):
 
 
 def test_a_block_listed_twice_counts_twice(gpu):
-    problem = make_block_problem(gpu, heads=64, kv_heads=4, lengths=[300, 200], counts=[100, 39], block=32, chosen=5,
-                                 lists=2, seed=6, together=True)
+    problem = make_block_problem(gpu, heads=64, kv_heads=4, lengths=[300, 200] * 4, counts=[100, 39] * 4, block=32,
+                                 chosen=5, lists=2, seed=6, together=True)
     problem.blocks[:, 0, 1] = problem.blocks[:, 0, 0]
     problem.blocks[::2, 1] = problem.blocks[::2, 1, :1]       # five times
     out, lse = run(problem)
@@ -136,12 +146,12 @@ def test_a_block_listed_twice_counts_twice(gpu):
 
 
 def test_a_replay_of_prompts_on_another_stream(gpu):
-    problem = make_block_problem(gpu, heads=64, kv_heads=4, lengths=[300, 200], counts=[100, 39], block=32, chosen=5,
-                                 lists=2, seed=7, together=True)
+    problem = make_block_problem(gpu, heads=64, kv_heads=4, lengths=[300, 200] * 4, counts=[100, 39] * 4, block=32,
+                                 chosen=5, lists=2, seed=7, together=True)
     out, lse = torch.empty_like(problem.query), torch.empty(problem.query.shape[:2], device=gpu)
     lengths, starts = problem.batch.ints(problem.batch.lengths), problem.batch.ints(problem.batch.starts())
     from adaptive_sparse.attention import block_workspace
-    workspace = torch.empty(block_workspace(139, 5, 32, 64, 4, 128, 100), dtype=torch.uint8, device=gpu)
+    workspace = torch.empty(block_workspace(556, 5, 32, 64, 4, 128, 100), dtype=torch.uint8, device=gpu)
     call = lambda: block_attention(problem.query, problem.pool.planes, problem.batch.tables,  # noqa: E731
                                    problem.batch.rows, lengths, problem.blocks, out, page_size=16, block_size=32,
                                    kv_heads=4, layer=problem.pool.layer, query_starts=starts, max_query=100, lse=lse,
@@ -155,7 +165,7 @@ def test_a_replay_of_prompts_on_another_stream(gpu):
             call()
     torch.cuda.synchronize()
     for step in range(3):
-        problem.batch.counts = [100 - 30 * step, 39 + 30 * step]
+        problem.batch.counts = [100 - 30 * step, 39 + 30 * step] * 4
         starts.copy_(problem.batch.ints(problem.batch.starts()))
         out.fill_(7)
         graph.replay()
