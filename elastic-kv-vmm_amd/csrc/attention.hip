@@ -511,7 +511,10 @@ Plan block_plan(int64_t tokens, int64_t width, int64_t block_size, int64_t heads
     need_sizes(tokens, 0, heads, kv_heads, dim);
     Plan plan;
     const int32_t dim_pad = padded_dim(dim);
-    plan.tiles16 = std::min(tiles_for(heads / kv_heads, dim_pad), dim_pad <= 128 ? 4 : 2);
+    // 64 tokens' 32 blocks of 64, one KV head of 128, by 1, 2 and 4 row tiles: 16 query heads 24, 25 and 30 us, 32 heads 34,
+    // 26 and 31, 64 heads 54, 38 and 34; of 256, where two spill 76 registers, by 1 and 2: 32 heads 57 and 59, 64 heads
+    // 97 and 91.
+    plan.tiles16 = dim_pad <= 128 ? std::min(tiles_for(heads / kv_heads, dim_pad), 4) : 1;
     cut(plan, plan.own, kSlots, tokens, plan.tiles16, tokens, heads / kv_heads, kv_heads, dim_pad, true);
     return plan;
 }

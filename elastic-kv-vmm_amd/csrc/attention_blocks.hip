@@ -19,12 +19,14 @@ __global__ __launch_bounds__(narrow::kWaves * 64, (narrow::groups_of<kDim, kTile
 template <typename T, int kDim>
 void launch_dim(const Launch& l, int tiles16, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(l.p[0].workgroups)), block(narrow::kWaves * 64);
-    if (tiles16 == 1) {
+    if constexpr (kDim <= 128) {
+        switch (tiles16) {
+            case 1: blocks_kernel<T, kDim, 1><<<grid, block, 0, stream>>>(l); break;
+            case 2: blocks_kernel<T, kDim, 2><<<grid, block, 0, stream>>>(l); break;
+            default: blocks_kernel<T, kDim, 4><<<grid, block, 0, stream>>>(l); break;
+        }
+    } else {
         blocks_kernel<T, kDim, 1><<<grid, block, 0, stream>>>(l);
-    } else if (tiles16 == 2) {
-        blocks_kernel<T, kDim, 2><<<grid, block, 0, stream>>>(l);
-    } else if constexpr (kDim <= 128) {
-        blocks_kernel<T, kDim, 4><<<grid, block, 0, stream>>>(l);
     }
     check_hip(hipGetLastError(), "launch block attention");
 }
