@@ -809,7 +809,7 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
     if (least < most && scale > 0 && scale < INFINITY) {
         // Parts 1 .. kBins - 1.
         const auto part = [&](uint32_t key) {
-            return min(static_cast<int>(fmaf(score_of(key) - low, scale, 1.0f)), kBins - 1);
+            return static_cast<int>(fminf(fmaf(score_of(key) - low, scale, 1.0f), kBins - 1));
         };
         uint32_t bin = 0;
         there = find([&](uint32_t key) { return key != 0 ? part(key) : -1; }, bin, among);
