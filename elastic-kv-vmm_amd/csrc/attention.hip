@@ -699,13 +699,17 @@ int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64
 // pieces of 256 tokens 78 and 141 us, eight of 64 (1024 pairs) 76 and 76, one of 256 83 and 41; 32 heads on 4 of 128,
 // eight of 64 80 and 142, eight of 32 78 and 76; 8 heads on 8 of 64, eight of 64 (4096 pairs of half the bytes) 67 and 149,
 // eight of 32 67 and 87. The host cannot see whether they are alike: random lists take 178 and 144, 188 and 84, 181 and
-// 42; 219 and 154, 179 and 83; 328 and 154, 288 and 90.
+// 42; 219 and 154, 179 and 83; 328 and 154, 288 and 90. Blocks go in runs of 32 keys, the last part-filled: eight pieces of
+// 128 tokens (2048 pairs) of 16 heads on 2 of 128 with 16 blocks of 100 take 114 and 206 us, with 32 of 20 77 and 100, with
+// 32 of 16 80 and 87. At a head size of 256, eight of 128 take 172 and 305, eight of 64 175 and 157.
 bool union_pays(const AttentionArgs& a, const BlockLists& lists, int64_t block_size, int64_t max_query, int32_t dim_pad) {
     const int64_t tile_tokens = std::min<int64_t>(64, 63 / a.share + 2);
-    const bool fits = dim_pad <= 128 && block_size % 32 == 0 && tile_tokens * lists.width <= kUnionEntries &&
+    const bool fits = block_size >= 16 && tile_tokens * lists.width <= kUnionEntries &&
                       a.block_most / block_size < kUnionBlocks &&
                       (int64_t{a.tokens} * a.share / 64 + a.batch) * a.kv_heads < 1 << 24;   // fewer than 2^32 threads
-    return fits && a.share <= 32 && max_query * a.share >= 64 && int64_t{a.tokens} * a.kv_heads * dim_pad >= 2048 * 128;
+    const int64_t filled = (block_size + 31) / 32 * 32;
+    const int64_t pairs = int64_t{a.tokens} * a.kv_heads * std::min(dim_pad, 128) / 128 * block_size / filled;
+    return fits && a.share <= 32 && max_query * a.share >= 64 && pairs >= 2048;
 }
 
 int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t workspace_bytes, void* stream) {
@@ -756,7 +760,7 @@ int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t
     if (s.query_starts != nullptr && union_pays(a, lists, s.block_size, s.max_query, plan.own.dim_pad)) {
         need_workspace(plan, workspace, workspace_bytes);
         if (a.tokens > 0) {
-            lists.halves = FastDiv(static_cast<uint32_t>(s.block_size / 32));
+            lists.runs_of = FastDiv(static_cast<uint32_t>((s.block_size + 31) / 32));
             lists.tiles = static_cast<int32_t>(int64_t{a.tokens} * a.share / 64 + a.batch);
             launch_union(Launch{a, {plan.own, {}}, lists}, s.query->dtype, stream);
         }

@@ -30,7 +30,7 @@ using wide::Tile;
 constexpr int kThreads = 256, kWaves = 4, kRows = 64;
 
 template <typename T, int kDim>
-__global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
+__global__ __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) void union_kernel(const Launch) {
     constexpr int kSteps = kDim / 16;              // matrix steps of the first product
     constexpr int kCols = kDim / 32;               // 32-column pieces of the output
     constexpr int kBytes = Tile<kDim>::kBytes;
@@ -204,9 +204,9 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
         }
     }
 
-    // Runs of 32 keys: `halves` to a block, two to a tile.
-    const FastDiv halves = fresh().lists.halves;
-    const int32_t runs = entries * static_cast<int32_t>(halves.divisor), tiles = (runs + 1) >> 1;
+    // Runs of 32 keys: `runs_of` to a block, whose last may be part-filled; two to a tile.
+    const FastDiv runs_of = fresh().lists.runs_of;
+    const int32_t runs = entries * static_cast<int32_t>(runs_of.divisor), tiles = (runs + 1) >> 1;
     if (tiles > 0) {
         const Cache cache = a.cache;
         const char* const table = a.tables + request * a.table_row;
@@ -228,10 +228,10 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
         const auto ids_of = [&](int32_t tile) {
             const int32_t run = 2 * tile + half;
             const bool there = run < runs;
-            const int32_t entry = there ? static_cast<int32_t>(halves.div(run)) : 0;
-            const int32_t key = static_cast<int32_t>(s_block[entry] * block.divisor) +
-                                (run - entry * static_cast<int32_t>(halves.divisor)) * 32 + col;
-            const bool good = there && key < last_seen;
+            const int32_t entry = there ? static_cast<int32_t>(runs_of.div(run)) : 0;
+            const int32_t in_block = (run - entry * static_cast<int32_t>(runs_of.divisor)) * 32 + col;
+            const int32_t key = static_cast<int32_t>(s_block[entry] * block.divisor) + in_block;
+            const bool good = there && in_block < static_cast<int32_t>(block.divisor) && key < last_seen;
             const uint32_t page = cache.page.div(key);
             const char* at = good ? table + static_cast<uint64_t>(page) * step : zeros;
             return Ids{load_global<uint32_t>(at), load_global<uint32_t>(at + wide64),
@@ -284,9 +284,9 @@ __global__ __launch_bounds__(kThreads, 2) void union_kernel(const Launch) {
         int32_t left = 0;
         const auto sight = [&](int32_t tile, uint64_t now) {
             const int32_t run = 2 * tile + key_half;
-            const int32_t entry = run < runs ? static_cast<int32_t>(halves.div(run)) : 0;
+            const int32_t entry = run < runs ? static_cast<int32_t>(runs_of.div(run)) : 0;
             const int32_t base = static_cast<int32_t>(s_block[entry] * block.divisor) +
-                                 (run - entry * static_cast<int32_t>(halves.divisor)) * 32;
+                                 (run - entry * static_cast<int32_t>(runs_of.divisor)) * 32;
             const bool listed = !live || ((s_mask[entry] >> place) & 1) != 0;
             left = listed ? min(max(my_seen - base, 0), 32) : 0;
             bits = static_cast<uint32_t>(now >> (32 * key_half));
@@ -473,7 +473,8 @@ void launch_type(const Launch& l, hipStream_t stream) {
     switch (l.p[0].dim_pad) {
         case 64: union_kernel<T, 64><<<grid, kThreads, 0, stream>>>(l); break;
         case 96: union_kernel<T, 96><<<grid, kThreads, 0, stream>>>(l); break;
-        default: union_kernel<T, 128><<<grid, kThreads, 0, stream>>>(l); break;
+        case 128: union_kernel<T, 128><<<grid, kThreads, 0, stream>>>(l); break;
+        default: union_kernel<T, 256><<<grid, kThreads, 0, stream>>>(l); break;
     }
     check_hip(hipGetLastError(), "launch block attention");
 }

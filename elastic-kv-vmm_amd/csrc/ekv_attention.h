@@ -98,7 +98,7 @@ struct BlockLists {
     FastDiv block, heads;             // tokens of a block; KV heads of a list
     // attention_union.hip
     int32_t width, tiles;             // entries of a list; tiles of 64 rows of a KV head
-    FastDiv halves;                   // runs of 32 tokens of a block
+    FastDiv runs_of;                  // runs of up to 32 tokens of a block
 };
 
 struct Launch {

@@ -1,7 +1,7 @@
 """block_attention of prompts, whose neighbouring tokens go through their lists together: against a 64-bit answer.
 
 All calls here have as many query rows and heads as the rule for that asks for: 64 rows of a batch row, and 2048 pairs
-of a token and a KV head of 128, or more of smaller ones.
+of a token and a KV head, or more.
 """
 
 import math
@@ -19,17 +19,17 @@ pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
 
 
-ENOUGH = 2048 * 128
-
-
-def padded(dim):
-    return 64 if dim <= 64 else 96 if dim <= 96 else 128
+def pairs_wanted(dim, block):
+    """(token, KV head) pairs, more where heads are small or blocks end inside 32 keys."""
+    size = 64 if dim <= 64 else 96 if dim <= 96 else 128
+    return 2049 * 128 / size * (-(-block // 32) * 32) / block + 1
 
 
 def run(problem, **extra):
     tokens, heads, dim = problem.query.shape
     kv_heads = problem.pool.keys.shape[2]
-    assert max(problem.batch.counts) * heads // kv_heads >= 64 and tokens * kv_heads * padded(dim) >= ENOUGH
+    assert max(problem.batch.counts) * heads // kv_heads >= 64
+    assert tokens * kv_heads >= pairs_wanted(dim, problem.block)
     out = torch.full_like(problem.query, 7.0)
     lse = torch.full(out.shape[:2], 7.0, device=out.device)
     problem.call(block_attention, out, lse, **extra)
@@ -47,6 +47,11 @@ CASES = [
     (72, 24, 8, 16, "planes", [260], [130], 64, 3, 1),
     (64, 4, 128, 16, "planes", [5000, 77], [100, 77], 128, 16, 2),
     (64, 2, 128, 16, "planes", [5000], [130], 2048, 2, 1),             # blocks longer than most of the context
+    (64, 4, 128, 16, "planes", [300, 90, 450], [100, 90, 3], 16, 9, 4),    # blocks that 32 keys are too many for
+    (64, 4, 128, 16, "planes", [300, 90, 450], [100, 90, 3], 100, 3, 1),
+    (63, 9, 80, 64, "blocks", [150, 330], [110, 40], 20, 6, 3),
+    (32, 4, 256, 16, "planes", [300, 90], [100, 60], 64, 4, 2),
+    (24, 2, 200, 100, "blocks", [300, 90], [100, 60], 33, 5, 1),
 ]
 
 
@@ -54,7 +59,7 @@ CASES = [
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
 def test_prompts(gpu, dtype, together, case):
     heads, kv_heads, dim, page, layout, lengths, counts, block, chosen, lists = case
-    times = -(-ENOUGH // (sum(counts) * kv_heads * padded(dim)))
+    times = math.ceil(pairs_wanted(dim, block) / (sum(counts) * kv_heads))
     lengths, counts = lengths * times, counts * times
     print(f"[blocks] {case} {dtype} {together}", flush=True)
     problem = make_block_problem(gpu, dtype=dtype, heads=heads, kv_heads=kv_heads, dim=dim, page=page, layout=layout,
@@ -110,11 +115,11 @@ def test_what_is_not_seen_may_be_anything(gpu):
         check(out, lse, want, 128)
 
 
-@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dim", [64, 128, 256])
 def test_infinities_reach_the_tokens_that_see_them(gpu, dim):
     """Key i of a row's last tokens has an infinity in column i of V: token i sees its own and earlier ones it lists."""
     count, length, heads = 64, 256, 128
-    problem = make_block_problem(gpu, heads=heads, kv_heads=64, dim=dim, lengths=[length], counts=[count], block=32,
+    problem = make_block_problem(gpu, heads=heads, kv_heads=heads, dim=dim, lengths=[length], counts=[count], block=32,
                                  chosen=3, seed=5)
     problem.query = problem.query * 0.25
     listed = torch.tensor([[0, 6, 7]] * count, dtype=torch.int32, device=gpu).unsqueeze(1)
