@@ -848,12 +848,13 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
             wanted -= s_found[2];
         }
         if (there && among > kFew) {
-            // Its first and last key, by trying 64 keys at a time.
+            // Its first and last key, by trying 64 keys at a time. Not those below the least: the keys of no score, NaN as
+            // numbers, are among them, and parts do not increase from them on.
             const auto first_of = [&](int wanted_part) {
-                uint32_t below = 0, above = kForced + 1;         // the first key lies above `below`, not above `above`
+                uint32_t below = least - 1, above = kForced + 1;         // the first lies above `below`, not above `above`
                 while (above - below > 1) {
                     const uint32_t step = (above - below + 63) / 64, at = below + min((lane + 1) * step, above - below);
-                    const bool reached = at > kForced || (at != 0 && part(at) >= wanted_part);
+                    const bool reached = at > kForced || part(at) >= wanted_part;
                     const int which = __builtin_ctzll(__ballot(reached));
                     above = below + min((which + 1) * step, above - below);
                     below += which * step;
@@ -898,10 +899,12 @@ __global__ __launch_bounds__(kManyThreads) void pick_many_kernel(const PickArgs 
     at += min(same_before, equal);
     int32_t left = max(equal - same_before, 0);              // of those equal to the bound, for this wave and later ones
     const uint64_t mine = uint64_t{1} << lane;
+    // Never behind the list, not even where somebody else writes to the workspace and keys read again are others.
     const auto leave = [&](int r, bool take) {
         const uint64_t taken = __ballot(take);
-        if (take) {
-            out[(at + lanes_below(taken)) * a.b_column] = begin + r * 64 + lane;
+        const int32_t place = at + static_cast<int32_t>(lanes_below(taken));
+        if (take && place < a.chosen) {
+            out[place * a.b_column] = begin + r * 64 + lane;
         }
         at += __popcll(taken);
     };
