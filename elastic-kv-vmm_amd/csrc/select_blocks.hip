@@ -1104,8 +1104,9 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     }
     a.pairs = 16 * tiles16 / a.share;
     a.row_tiles = (a.groups + a.pairs - 1) / a.pairs;
-    a.tiles = static_cast<int32_t>(s.query_starts != nullptr ? tokens * groups / a.pairs + a.at.batch
-                                                             : tokens * a.row_tiles);
+    // Not none where there are no batch rows and nothing is scored.
+    a.tiles = std::max(static_cast<int32_t>(s.query_starts != nullptr ? tokens * groups / a.pairs + a.at.batch
+                                                                      : tokens * a.row_tiles), 1);
     // Segments of 256 tokens, of 512 where those fill the card twice, and longer where the contexts make more workgroups
     // than fill it a few times over (one for long tiles, whose start costs most); as many blocks as there is room for keys.
     // By 256, 512, 1024, 2048 and 4096 tokens: one query token of 4 heads for 4 requests of 8192 tokens 10, 11, 13, 17 and

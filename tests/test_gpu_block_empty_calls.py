@@ -1,0 +1,29 @@
+"""The block-sparse operators where there is nothing to choose from or to attend to: no batch rows, tokens or blocks."""
+
+import pytest
+import torch
+
+from adaptive_sparse.block_selection import select_blocks
+
+from block_cases import make_index_pool
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+@pytest.mark.parametrize("tokens,heads,groups,most", [(1, 8, 2, 1), (3, 4, 4, 1), (70, 2, 1, 64), (300, 4, 2, 300)])
+@pytest.mark.parametrize("columns", [4, 200, 1200, 5000])
+def test_tokens_without_a_batch_row_select_nothing(gpu, tokens, heads, groups, most, columns):
+    print(f"[select] {tokens} tokens of no row, {heads} heads, {groups} groups, {columns} pages", flush=True)
+    pool = make_index_pool(gpu, 8, 16, 64)
+    query = torch.randn((tokens, heads, 64), device=gpu).to(BF16)
+    tables = torch.zeros((2, columns), dtype=torch.int32, device=gpu)
+    none = torch.zeros(0, dtype=torch.int32, device=gpu)
+    starts = torch.zeros(1, dtype=torch.int32, device=gpu)
+    blocks = torch.full((tokens, groups, 5), 77, dtype=torch.int32, device=gpu)
+    for rows in (None, none):
+        blocks.fill_(77)
+        select_blocks(query, pool.planes, pool.scales, tables, rows, none, blocks, page_size=16, block_size=16, layer=1,
+                      query_starts=starts, max_query=most)
+        assert bool((blocks == -1).all())
