@@ -1,10 +1,14 @@
 """The block-sparse operators where there is nothing to choose from or to attend to: no batch rows, tokens or blocks."""
 
+import math
+
 import pytest
 import torch
 
+from adaptive_sparse.attention import block_attention
 from adaptive_sparse.block_selection import select_blocks
 
+from attention_cases import make_pool
 from block_cases import make_index_pool
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +31,21 @@ def test_tokens_without_a_batch_row_select_nothing(gpu, tokens, heads, groups, m
         select_blocks(query, pool.planes, pool.scales, tables, rows, none, blocks, page_size=16, block_size=16, layer=1,
                       query_starts=starts, max_query=most)
         assert bool((blocks == -1).all())
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,most", [(16, 128, 128, 64), (1, 8, 2, 1), (63, 64, 64, 64), (70, 64, 32, 64),
+                                                        (2100, 8, 2, 1000)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_tokens_without_a_batch_row_attend_to_nothing(gpu, tokens, heads, kv_heads, most, dim):
+    print(f"[blocks] {tokens} tokens of no row, {heads} heads, {kv_heads} KV heads of {dim}", flush=True)
+    pool = make_pool(gpu, BF16, 4, 16, kv_heads, dim)
+    query = torch.randn((tokens, heads, dim), device=gpu).to(BF16)
+    tables = torch.ones((2, 40), dtype=torch.int32, device=gpu)
+    none = torch.zeros(0, dtype=torch.int32, device=gpu)
+    starts = torch.zeros(1, dtype=torch.int32, device=gpu)
+    blocks = torch.zeros((tokens, 1, 3), dtype=torch.int32, device=gpu)
+    out = torch.full_like(query, 7.0)
+    lse = torch.full((tokens, heads), 7.0, device=gpu)
+    block_attention(query, pool.planes, tables, None, none, blocks, out, page_size=16, block_size=32, kv_heads=kv_heads,
+                    layer=pool.layer, query_starts=starts, max_query=most, lse=lse)
+    assert not bool(out.any()) and bool((lse == -math.inf).all())
