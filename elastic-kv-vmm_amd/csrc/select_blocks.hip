@@ -1055,15 +1055,15 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     need_apart(out, "blocks", Extent(&lengths), "lengths");
     need_apart(out, "blocks", Extent(s.rows), "rows");
     need_apart(out, "blocks", Extent(s.query_starts), "query_starts");
+    if (tokens == 0) {
+        return 0;          // no workspace either: a tensor of its 0 bytes has no address
+    }
     if (workspace_bytes < plan.bytes) {
         throw std::invalid_argument("the selection needs " + std::to_string(plan.bytes) + " workspace bytes, got " +
                                     std::to_string(workspace_bytes));
     }
     if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) {
         throw std::invalid_argument("the workspace must be a 256-byte aligned device buffer");
-    }
-    if (tokens == 0) {
-        return 0;
     }
     a.query = static_cast<const char*>(query.data);
     a.q_token = query.stride[0] * 2, a.q_head = query.stride[1] * 2;

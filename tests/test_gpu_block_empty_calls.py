@@ -33,6 +33,14 @@ def test_tokens_without_a_batch_row_select_nothing(gpu, tokens, heads, groups, m
         assert bool((blocks == -1).all())
 
 
+@pytest.mark.parametrize("batch", [0, 2])
+def test_no_tokens_select_nothing(gpu, batch):
+    pool = make_index_pool(gpu, 8, 16, 64)
+    ints = lambda n: torch.zeros(n, dtype=torch.int32, device=gpu)  # noqa: E731
+    select_blocks(torch.empty((0, 4, 64), dtype=BF16, device=gpu), pool.planes, pool.scales, ints((2, 4)), None, ints(batch),
+                  ints((0, 2, 5)), page_size=16, block_size=16, layer=1, query_starts=ints(batch + 1), max_query=4)
+
+
 @pytest.mark.parametrize("tokens,heads,kv_heads,most", [(16, 128, 128, 64), (1, 8, 2, 1), (63, 64, 64, 64), (70, 64, 32, 64),
                                                         (2100, 8, 2, 1000)])
 @pytest.mark.parametrize("dim", [64, 256])
