@@ -39,7 +39,8 @@ def select_blocks(index_query, planes, scales, block_tables, rows, lengths, bloc
     most query tokens of a row, as far as known: it picks kernels, never what
     is chosen.
     A block's score is the largest, over a group's heads and the block's seen
-    tokens, of the product of query and key as they are held in 8 bits. The
+    tokens, of the product of query and key as they are held in 8 bits, and one
+    past the largest or the lowest number of 32 bits counts as that. The
     `first` blocks of the context and the `last` up to the position's own are
     chosen whatever their scores; ties go to the lower block. block_size = 1
     chooses tokens. workspace: a uint8 device tensor of selection_workspace(...)

@@ -66,13 +66,22 @@ struct ScoreArgs {
 };
 
 // Scores in the order of whole numbers: 0 for a block without a token that is seen, kForced for one that is always taken,
-// which no score reaches.
+// which no score reaches. What passes the largest or the lowest number counts as that one.
 constexpr uint32_t kForced = 0xff800000u;
 
+// The score of what is not seen: NaN, of no account beside another in a maximum. (-infinity is a score: that of products
+// that pass the lowest number.) The compiler is not to know it: it would make two maxima of three numbers again.
+__device__ __forceinline__ float no_score() {
+    uint32_t bits = 0x7fc00000u;
+    asm("" : "+v"(bits));
+    return __uint_as_float(bits);
+}
+
 __device__ __forceinline__ uint32_t ordered(float score) {
-    const uint32_t bits = __float_as_uint(fminf(score, 3.4028235e38f) + 0.0f);     // -0 counts as 0
+    const float most = 3.4028235e38f, held = __builtin_amdgcn_fmed3f(score, -most, most);
+    const uint32_t bits = __float_as_uint(held + 0.0f);                            // -0 counts as 0
     const uint32_t key = bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
-    return score > -INFINITY ? key : 0u;
+    return score == score ? key : 0u;
 }
 
 // The score of a key: infinity of kForced, NaN of 0.
@@ -386,15 +395,15 @@ __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_
                 my_scales[lane] = keys.scale;
             }
         };
+        const float none = no_score();
         float best[kTiles];
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) {
-            best[m] = -INFINITY;
+            best[m] = none;
         }
         const auto leave = [&](int m, float score, int32_t block) {
-            const float times = score > -INFINITY ? score * q_scale[m] : -INFINITY;
             if (pair_of[m] >= 0 && block < held) {
-                atomicMax(&s_score[pair_of[m] * held + block], ordered(times));
+                atomicMax(&s_score[pair_of[m] * held + block], ordered(score * q_scale[m]));
             }
         };
         // The scores of the keys in LDS, 16 of them at a time; kRagged: some are not seen by all rows.
@@ -425,7 +434,9 @@ __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_
                     x[j] = static_cast<float>(s[j]) * key_scale[j];
                     if (kRagged) {
                         const int key = quad * 4 + j;
-                        x[j] = ((seen >> (h * 16)) >> key & 1) != 0 && key < sight[m] - base - h * 16 ? x[j] : -INFINITY;
+                        // Not &&, which became branches.
+                        const bool there = (((seen >> (h * 16)) >> key & 1) != 0) & (key < sight[m] - base - h * 16);
+                        x[j] = there ? x[j] : none;
                     }
                 }
                 if constexpr (!kShort) {
@@ -463,7 +474,7 @@ __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_
                     if (quad == 0) {
                         leave(m, most, block);
                     }
-                    best[m] = -INFINITY;
+                    best[m] = none;
                 }
             }
         };

@@ -671,7 +671,8 @@ uint64_t ekv_select_workspace_bytes(int64_t tokens, int64_t groups, int64_t colu
  * q_s as ekv_append_index rounds keys. With q.k the whole-number product of
  * codes, the score of block j is, over the group's heads h,
  *   max_h  q_s[h] * max_{t in block j, t <= p}  scales[t] * (q_h . k_t)
- * both products rounded to 32 bits. Tokens whose page id is below 1 or past the
+ * both products rounded to 32 bits; a score past the largest or the lowest
+ * number counts as that one. Tokens whose page id is below 1 or past the
  * pool are not seen; a block without a seen token is not chosen. Blocks below
  * `first`, and the last `last` up to the position's own, are chosen whatever
  * their scores. Ties go to the lower block. A list is in ascending order, -1

@@ -74,3 +74,51 @@ def test_scores_of_all_magnitudes(gpu, places, low, high):
     for chosen in (64, 1500):
         got, want = scored(gpu, rows, chosen, places=places, first=2)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("places", [256, 1024, *PLACES])
+@pytest.mark.parametrize("block", [1, 2, 4, 16, 100])
+def test_scores_past_the_lowest_number_are_scores(gpu, places, block):
+    """Blocks whose products pass the lowest number are the last to be chosen, but are chosen: no block is without a score."""
+    print(f"[select] blocks of {block}, {places} places", flush=True)
+    batch = make_batch(gpu, [240, 33], None, 16, seed=4, permute=False)
+    pool = make_index_pool(gpu, batch.pages, 16, 16, seed=4)
+    wide = max(places // 16 - batch.tables.shape[1], 0)
+    batch.tables = torch.cat([batch.tables, torch.zeros((2, wide), dtype=torch.int32, device=gpu)], 1)
+    pool.keys.zero_()
+    pool.keys[..., 0] = -1
+    pool.scales.fill_(3e38)                                         # 127 times it passes the lowest number
+    # The scores of the first two blocks of the long row do not.
+    for t in range(2 * block):
+        pool.scales[int(batch.tables[0, t // 16]) * 16 + t % 16] = 1.0 + t // block
+    query = torch.zeros((2, 1, 16), dtype=torch.bfloat16, device=gpu)
+    query[:, :, 0] = 127
+    for chosen, first, last in ((1, 0, 1), (3, 0, 1), (3, 0, 0), (4, 2, 1), (300, 0, 0)):
+        blocks = torch.full((2, 1, chosen), 77, dtype=torch.int32, device=gpu)
+        select_blocks(query, pool.planes, pool.scales, batch.tables, None, batch.ints(batch.lengths), blocks,
+                      page_size=16, block_size=block, layer=pool.layer, first=first, last=last)
+        for b, length in enumerate(batch.lengths):
+            count = (length - 1) // block + 1
+            cost = [1.0 + j if b == 0 and j < 2 else float("inf") for j in range(count)]
+            rank = sorted(range(count), key=lambda j: (not (j < first or j >= count - last), cost[j], j))
+            want = sorted(rank[:chosen])
+            assert blocks[b, 0].tolist() == want + [-1] * (chosen - len(want))
+
+
+@pytest.mark.parametrize("counts", [None, [70, 90]])
+def test_scores_past_the_largest_number_go_to_lower_blocks(gpu, counts):
+    batch = make_batch(gpu, [300, 200], counts, 16, seed=5)
+    pool = make_index_pool(gpu, batch.pages, 16, 16, seed=5)
+    pool.keys.zero_()
+    pool.keys[..., 0] = 1
+    pool.scales.fill_(3e38)
+    tokens = sum(batch.counts)
+    query = torch.zeros((tokens, 2, 16), dtype=torch.bfloat16, device=gpu)
+    query[:, 0, 0] = 127                                            # the other head's scores are 0
+    blocks = torch.full((tokens, 1, 3), 77, dtype=torch.int32, device=gpu)
+    for block in (1, 8, 64):
+        select_blocks(query, pool.planes, pool.scales, batch.tables, batch.rows, batch.ints(batch.lengths), blocks,
+                      page_size=16, block_size=block, layer=pool.layer, last=0, **batch.given(tokens))
+        for n, (_, position) in enumerate(batch.places(tokens)):
+            count = min(position // block + 1, 3)
+            assert blocks[n, 0].tolist() == list(range(count)) + [-1] * (3 - count)
