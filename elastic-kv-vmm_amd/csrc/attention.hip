@@ -740,8 +740,7 @@ int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t
     }
     const PlanePages pages = plane_pages(s.planes, s.layer, int64_t{a.kv_heads} * a.dim * 2, s.page_size, 2);
     const Extent planes[2] = {Extent(pages, *s.planes, 0), Extent(pages, *s.planes, 1)};
-    const auto apart = [&](const ekv_tensor* t, const char* name) {
-        const Extent e(t);
+    const auto apart = [&](const Extent& e, const char* name) {
         for (const Extent& plane : planes) {
             need_apart(e, name, plane, "the layer's planes");
         }
@@ -751,15 +750,20 @@ int block_attention(const ekv_block_attention_args& s, void* workspace, uint64_t
         need_apart(e, name, Extent(&blocks), "blocks");
         need_apart(e, name, Extent(s.query_starts), "query_starts");
     };
-    apart(s.output, "output");
+    apart(Extent(s.output), "output");
     if (s.lse != nullptr) {
         need_distinct(*s.lse, "lse");
-        apart(s.lse, "lse");
+        apart(Extent(s.lse), "lse");
         need_apart(Extent(s.lse), "lse", Extent(s.query), "query");
         need_apart(Extent(s.lse), "lse", Extent(s.output), "output");
     }
+    need_workspace(plan, workspace, workspace_bytes);
+    const Extent work(workspace, plan.bytes);
+    apart(work, "the workspace");
+    need_apart(work, "the workspace", Extent(s.query), "query");
+    need_apart(work, "the workspace", Extent(s.output), "output");
+    need_apart(work, "the workspace", Extent(s.lse), "lse");
     if (s.query_starts != nullptr && union_pays(a, lists, s.block_size, s.max_query, plan.own.dim_pad)) {
-        need_workspace(plan, workspace, workspace_bytes);
         if (a.tokens > 0) {
             lists.runs_of = FastDiv(static_cast<uint32_t>((s.block_size + 31) / 32));
             lists.tiles = static_cast<int32_t>(int64_t{a.tokens} * a.share / 64 + a.batch);

@@ -146,6 +146,14 @@ struct Extent {
         }
     }
 
+    Extent(const void* data, uint64_t bytes) {
+        if (bytes > 0) {
+            begin = reinterpret_cast<int64_t>(data);
+            run = static_cast<int64_t>(bytes);
+            end = begin + run;
+        }
+    }
+
     // Plane `kv` of a layer.
     Extent(const PlanePages& p, const ekv_planes& planes, int64_t kv) {
         if (planes.rows > 0) {

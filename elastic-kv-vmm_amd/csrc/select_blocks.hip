@@ -1076,6 +1076,15 @@ int select_blocks(const ekv_select_args& s, void* workspace, uint64_t workspace_
     if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) {
         throw std::invalid_argument("the workspace must be a 256-byte aligned device buffer");
     }
+    const Extent work(workspace, plan.bytes);
+    need_apart(work, "the workspace", out, "blocks");
+    need_apart(work, "the workspace", Extent(&query), "index_query");
+    need_apart(work, "the workspace", Extent(p, *s.planes, 0), "the layer's plane");
+    need_apart(work, "the workspace", Extent(&scales), "scales");
+    need_apart(work, "the workspace", Extent(&tables), "block_tables");
+    need_apart(work, "the workspace", Extent(&lengths), "lengths");
+    need_apart(work, "the workspace", Extent(s.rows), "rows");
+    need_apart(work, "the workspace", Extent(s.query_starts), "query_starts");
     a.query = static_cast<const char*>(query.data);
     a.q_token = query.stride[0] * 2, a.q_head = query.stride[1] * 2;
     a.f16 = query.dtype == EKV_FLOAT16;

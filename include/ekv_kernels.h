@@ -586,7 +586,8 @@ uint64_t ekv_block_workspace_bytes(int64_t tokens, int64_t width, int64_t block_
  * t <= p of every block j of its list (tokens j * block_size ..
  * (j + 1) * block_size - 1 of its request). A block listed twice counts twice;
  * ids below 0 or behind the position name none. The output may be the query
- * itself, and output and lse share no memory with the other inputs. Otherwise
+ * itself, and output, lse and workspace share no memory with one another nor
+ * with the other inputs. Otherwise
  * as ekv_shared_prefix_attention without prefixes.
  * Replaces: the sparse attention that the reference leaves to its engine
  * behind the selected blocks (adaptive_sparse/request_residency.py:792-839).
@@ -679,7 +680,8 @@ uint64_t ekv_select_workspace_bytes(int64_t tokens, int64_t groups, int64_t colu
  * behind its last block; the lists of tokens of no batch row are all -1.
  * At most 128 heads a group; N * G < 2^22. workspace: 256-byte aligned device
  * memory of ekv_select_workspace_bytes, its contents of no account; calls that
- * overlap need one each. Two or three launches, no memset: it can be captured.
+ * overlap need one each. Neither it nor `blocks` shares memory with an input or
+ * with the other. Two or three launches, no memset: it can be captured.
  * Replaces: the block scores that the reference's engine hands to
  * adaptive_sparse/request_residency.py:792-839 as selected blocks.
  */
