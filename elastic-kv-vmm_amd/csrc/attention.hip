@@ -704,9 +704,10 @@ int topk(const ekv_tensor* query, const ekv_planes* planes, int64_t layer, int64
 // 32 of 16 80 and 87. At a head size of 256, eight of 128 take 172 and 305, eight of 64 175 and 157.
 bool union_pays(const AttentionArgs& a, const BlockLists& lists, int64_t block_size, int64_t max_query, int32_t dim_pad) {
     const int64_t tile_tokens = std::min<int64_t>(64, 63 / a.share + 2);
-    // Without batch rows there may be no tile: the other kernel writes the zeros.
-    const bool fits = a.batch > 0 && block_size >= 16 && tile_tokens * lists.width <= kUnionEntries &&
-                      a.block_most / block_size < kUnionBlocks &&
+    // Without batch rows there may be no tile, and lists of no entries have no width to divide by: the other kernel writes
+    // the zeros.
+    const bool fits = a.batch > 0 && lists.width > 0 && block_size >= 16 &&
+                      tile_tokens * lists.width <= kUnionEntries && a.block_most / block_size < kUnionBlocks &&
                       (int64_t{a.tokens} * a.share / 64 + a.batch) * a.kv_heads < 1 << 24;   // fewer than 2^32 threads
     const int64_t filled = (block_size + 31) / 32 * 32;
     const int64_t pairs = int64_t{a.tokens} * a.kv_heads * std::min(dim_pad, 128) / 128 * block_size / filled;

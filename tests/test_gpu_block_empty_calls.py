@@ -57,3 +57,20 @@ def test_tokens_without_a_batch_row_attend_to_nothing(gpu, tokens, heads, kv_hea
     block_attention(query, pool.planes, tables, None, none, blocks, out, page_size=16, block_size=32, kv_heads=kv_heads,
                     layer=pool.layer, query_starts=starts, max_query=most, lse=lse)
     assert not bool(out.any()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("share", [1, 4])
+def test_prompts_with_lists_of_no_entries(gpu, share):
+    """As many tokens as go through their lists together where there are entries."""
+    tokens, kv_heads = 2100, 2
+    pool = make_pool(gpu, BF16, 200, 16, kv_heads, 64)
+    query = torch.randn((tokens, share * kv_heads, 64), device=gpu).to(BF16)
+    ints = lambda values: torch.tensor(values, dtype=torch.int32, device=gpu)  # noqa: E731
+    tables = torch.arange(1, 133, dtype=torch.int32, device=gpu).view(1, -1)
+    out = torch.full_like(query, 7.0)
+    lse = torch.full(out.shape[:2], 7.0, device=gpu)
+    block_attention(query, pool.planes, tables, None, ints([tokens]), torch.empty((tokens, 1, 0), dtype=torch.int32,
+                                                                                  device=gpu),
+                    out, page_size=16, block_size=32, kv_heads=kv_heads, layer=pool.layer, query_starts=ints([0, tokens]),
+                    max_query=tokens, lse=lse)
+    assert not bool(out.any()) and bool((lse == -math.inf).all())
