@@ -129,15 +129,18 @@ def block_attention(query, planes, block_tables, rows, lengths, blocks, output, 
     """Attention of each query token to the tokens of its listed blocks, into `output`: one layer, no gather.
 
     query, output, planes, block_tables, rows, lengths, query_starts, scale
-    and lse as in shared_prefix_attention (without prefixes); blocks [N, G, K]
-    int32 or int64 of any strides, as select_blocks writes them: KV head h
-    reads list h // (kv_heads // G). Query token i of a row's n is at position
-    p = lengths[b] - n + i and sees, of every block j that it lists, the
-    tokens j * block_size .. (j + 1) * block_size - 1 up to p. Ids below 0 or
-    behind the position name no block; a block listed twice counts twice. A
-    token that sees nothing gets zeros and lse -inf. max_query: the most query
-    tokens of a row, as far as known: it picks kernels, never which keys are
-    seen. workspace: block_workspace(...) bytes, as in shared_prefix_attention.
+    and lse as in shared_prefix_attention (without prefixes), but the output
+    may be the query itself; blocks [N, G, K] int32 or int64 of any strides, as
+    select_blocks writes them: KV head h reads list h // (kv_heads // G). Query
+    token i of a row's n is at position p = lengths[b] - n + i and sees, of
+    every block j that it lists, the tokens j * block_size ..
+    (j + 1) * block_size - 1 up to p. Ids below 0 or behind the position name
+    no block; a block listed twice counts twice. A token that sees nothing gets
+    zeros and lse -inf. Scores, their softmax and the sums are held in 32 bits;
+    the weights are rounded once to the query's type for the product with V.
+    max_query: the most query tokens of a row, as far as known: it picks
+    kernels, never which keys are seen. workspace: block_workspace(...) bytes,
+    as in shared_prefix_attention, apart from all other tensors.
     """
     _check(query, planes, workspace)
     tokens, heads, dim = query.shape
