@@ -70,6 +70,10 @@ def make_rotary(rotary_dim, *, device, base=10000.0, scaling=None, factor=1.0, o
     from one to the other between them, with a magnitude of 0.1 ln(factor) + 1
     (Peng et al., "YaRN: Efficient context window extension of large language
     models", 2023). magnitude: another factor of the rotated elements.
+
+    A frequency and its turns are rounded as numbers of 64 bits: where a pair
+    turns a radian a position or less, its angle is off by less than 4e-16
+    radians a position, 4e-7 at position 2^30.
     """
     frequencies, factor_of = rotary_frequencies(rotary_dim, base=base, scaling=scaling, factor=factor,
                                                 original=original, fast=fast, slow=slow)

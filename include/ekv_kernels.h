@@ -617,7 +617,8 @@ typedef struct ekv_append_args {
  * (x_a, x_b) of pair i of the first R elements of a head become
  *   magnitude * (x_a cos - x_b sin, x_b cos + x_a sin),
  * rounded once; elements from R on, and V, are copied. Whole turns are dropped
- * in 64-bit integers, so angles are as exact at far positions as at near ones.
+ * in 64-bit integers, so the product adds no error: an angle is off by the
+ * position times what its turns are off.
  * A token with position < 0 is left out: its output and row stay as they are.
  * Slots below zero_below or past the pool write no row. The slots of live
  * tokens are distinct. Only query, or only key, value, planes and slots, may be
