@@ -85,9 +85,6 @@ struct Phase {
     uint32_t* item_starts;           // [sequences + 1]
 };
 
-// The arguments of a kernel. They are more words than a wave has scalar registers, and the compiler loads all of them
-// first and spills what does not fit into vector registers; fresh() hides where they come from, so that each part of a
-// kernel loads what it needs where it needs it.
 // Lists of blocks instead of slots (kSlots): place i of a list is token i % block of the block that its entry i / block
 // names; pages of tokens come from AttentionArgs::tables.
 struct BlockLists {
@@ -101,6 +98,9 @@ struct BlockLists {
     FastDiv runs_of;                  // runs of up to 32 tokens of a block
 };
 
+// The arguments of a kernel. They are more words than a wave has scalar registers, and the compiler loads all of them
+// first and spills what does not fit into vector registers; fresh() hides where they come from, so that each part of a
+// kernel loads what it needs where it needs it.
 struct Launch {
     AttentionArgs a;
     Phase p[2];        // own tokens (or all), prefixes
@@ -514,11 +514,11 @@ constexpr int kNarrowUnit = 7;
 int narrow_groups(int tiles16, int32_t dim_pad);
 void launch_narrow(const Launch& l, int32_t dtype, int tiles16, void* stream);
 
-// attention_blocks.hip: the same over lists of blocks, at most 64 rows (32 of 256 columns) a tile.
+// attention_blocks.hip: the same over lists of blocks, at most 64 rows (16 of more than 128 columns) a tile.
 void launch_blocks(const Launch& l, int32_t dtype, int tiles16, void* stream);
 
-// attention_union.hip: tiles of 64 rows over all blocks that their tokens list, at most kUnionEntries entries in those
-// lists, of a context of at most kUnionBlocks blocks; blocks of whole runs of 32 tokens, head sizes up to 128.
+// attention_union.hip: tiles of 64 rows over all blocks that their tokens list, from 1 to kUnionEntries entries in those
+// lists, of page tables that cover at most kUnionBlocks blocks of 16 tokens or more.
 constexpr int kUnionEntries = 1024, kUnionBlocks = 4096;
 void launch_union(const Launch& l, int32_t dtype, void* stream);
 

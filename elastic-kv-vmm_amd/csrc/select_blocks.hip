@@ -207,8 +207,9 @@ __global__ __launch_bounds__(kThreads) void code_kernel(const ScoreArgs a) {
 //
 // What bounds it: with few rows the reading. 5.2 million keys of 128 and their scales, 0.69 GB, of 128 requests of up to
 // 65536 tokens take 130 us, 5.3 TB/s (lanes that read the products' way, 64 bytes of 16 rows, read each 128-byte line
-// twice: 212). With many rows the instructions on the products, 19 for 16 keys and 16 rows: six pieces of up to 1024
-// tokens of 4 heads behind 16384 take 71 us, 0.78 * 10^15 operations a second. Lists of tokens take longest for their
+// twice: 212). With many rows nothing alone: six pieces of up to 1024 tokens of 4 heads behind 16384 take 71 us, 0.77 *
+// 10^15 operations a second, with the matrix pipes busy 15 % of the cycles, vector instructions (19 for 16 keys and 16
+// rows) 36 %, and workgroups on the compute units two thirds of the time. Lists of tokens take longest for their
 // bytes, a maximum in LDS for each key: 24 requests of up to 40000 tokens, 42 MB, 18 us.
 template <int kSteps, int kTiles, bool kShort>
 __global__ __launch_bounds__(kThreads, kSteps * kTiles > 16 ? 1 : 2) void score_kernel(const ScoreArgs a) {
