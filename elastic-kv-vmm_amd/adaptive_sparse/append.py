@@ -31,6 +31,19 @@ class Rotary:
     frequencies: tuple = field(repr=False)   # radians a position
 
 
+def _power(base, exponent):
+    try:
+        return base ** exponent
+    except OverflowError:
+        return math.inf
+
+
+def _held(frequencies):
+    if not all(math.isfinite(f) for f in frequencies):
+        raise ValueError("frequencies must be finite")
+    return frequencies
+
+
 def rotary_frequencies(rotary_dim, *, base=10000.0, scaling=None, factor=1.0, original=None, fast=32.0, slow=1.0):
     """(radians a position of every pair, factor of the rotated elements) of make_rotary's arguments."""
     if type(rotary_dim) is not int or rotary_dim < 2 or rotary_dim % 2:
@@ -43,19 +56,21 @@ def rotary_frequencies(rotary_dim, *, base=10000.0, scaling=None, factor=1.0, or
     if scaling == "base":
         if rotary_dim < 4:
             raise ValueError("scaling the base needs a rotary_dim of 4 or more")
-        base *= factor ** (rotary_dim / (rotary_dim - 2))
-    plain = [base ** (-2 * i / rotary_dim) for i in range(rotary_dim // 2)]
+        base *= _power(factor, rotary_dim / (rotary_dim - 2))
+        if not 0 < base < math.inf:
+            raise ValueError("the scaled base must be positive and finite")
+    plain = _held([_power(base, -2 * i / rotary_dim) for i in range(rotary_dim // 2)])
     if scaling == "linear":
-        return [f / factor for f in plain], 1.0
+        return _held([f / factor for f in plain]), 1.0
     if scaling != "ramp":
         return plain, 1.0
-    if original is None or not (original > 0 and fast > slow > 0 and base > 1):
+    if original is None or not (math.inf > original > 0 and math.inf > fast > slow > 0 and base > 1):
         raise ValueError("a ramp needs the original context length, fast > slow > 0 and a base above 1")
     # The place among the pairs of one that turns `turns` times in the original context.
     place = [rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in (fast, slow)]
     low, high = max(math.floor(place[0]), 0), min(math.ceil(place[1]), rotary_dim - 1)
     slowed = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(rotary_dim // 2)]
-    return [f * (1 - s) + f / factor * s for f, s in zip(plain, slowed)], max(0.1 * math.log(factor) + 1.0, 1.0)
+    return _held([f * (1 - s) + f / factor * s for f, s in zip(plain, slowed)]), max(0.1 * math.log(factor) + 1.0, 1.0)
 
 
 def make_rotary(rotary_dim, *, device, base=10000.0, scaling=None, factor=1.0, original=None, fast=32.0, slow=1.0,

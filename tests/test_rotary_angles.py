@@ -58,6 +58,18 @@ def test_turns_are_those_of_the_frequencies(size, base):
         assert off / 2 ** 64 * 2 * PI < Fraction(4, 10 ** 16)
 
 
+@pytest.mark.parametrize("given", [
+    dict(scaling="ramp", original=math.inf), dict(scaling="ramp", original=4096, fast=math.inf),
+    dict(scaling="ramp", original=math.nan), dict(scaling="base", factor=1e308, base=1e300),
+    dict(rotary_dim=4, scaling="base", factor=1e200), dict(rotary_dim=4, scaling="base", factor=1e-200),
+    dict(rotary_dim=256, base=5e-324),
+    dict(scaling="linear", factor=5e-324, base=0.5),
+])
+def test_frequencies_past_the_numbers_are_refused(given):
+    with pytest.raises(ValueError):
+        make_rotary(**{"rotary_dim": 64, "device": "cpu", **given})
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("neighbours", [False, True])
 @pytest.mark.parametrize("base", [10000, 500000])
